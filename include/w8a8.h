@@ -569,6 +569,154 @@ int w8a8_moe_combine(const void* y, uint32_t ldy, uint32_t rows_y, const float* 
                      const int32_t* dst_row, uint32_t tokens, uint32_t topk, uint32_t n,
                      void* out, uint32_t ldo, hipStream_t stream);
 
+/*
+ * The whole expert layer for the few tokens of a decode step, in two launches:
+ * routing, the MoE quantizer, the gate_up GEMM, SiLU(gate) * up, the
+ * requantization, the down GEMM and the weighted combine of the chain above
+ * (w8a8_topk_softmax ... w8a8_moe_combine), without its sort and without an
+ * fp16 rounding between the steps.  Per token t and slot s, with e = the
+ * token's s-th expert and its softmax weight as w8a8_topk_softmax gives them
+ * (a slot without an expert contributes nothing), all in fp32:
+ *   q, r   = quantizer of float(x[t]) * smooth_scale[e]
+ *   g, u   = (float(q . w_gate_up[e]^T) * r) * sb_gate_up[e]   (rows [0, inter), [inter, 2 inter))
+ *   a      = (g / (1 + exp(-g))) * u [* smooth_scale_down[e]]
+ *   q2, r2 = quantizer of a
+ *   y      = (float(q2 . w_down[e]^T) * r2) * sb_down[e]
+ *   out[t] = half(sum over slots s (ascending) of fma(weight[t, s], y, acc))
+ *   x            fp16 [tokens, ldx] (ldx = 0 means hidden), out fp16 [tokens, ldo]
+ *                (ldo = 0 means hidden); out may not overlap x
+ *   logits       fp32 or (logits_f16 = 1) fp16 [tokens, experts]
+ *   smooth_scale fp32 [experts, hidden]; smooth_scale_down fp32 [experts, inter] or NULL
+ *   w_gate_up    int8 [experts, 2 * inter, hidden], sb_gate_up fp32 [experts, 2 * inter]
+ *   w_down       int8 [experts, hidden, inter], sb_down fp32 [experts, hidden]
+ * tokens <= W8A8_MOE_DECODE_MAX_TOKENS, tokens * hidden <= 131072, experts <=
+ * 4096, topk <= 64; hidden, inter multiples of 16 and <= 32768; x, ldx,
+ * smooth scales and weights 16-byte aligned (W8A8_ERROR_NOT_SUPPORTED
+ * otherwise: the chain takes more tokens).  workspace: 256-byte aligned,
+ * w8a8_moe_ffn_decode_workspace_size bytes; needs no clearing.  Calls that
+ * share a workspace must be ordered on one stream.  Results do not depend on
+ * the order in which blocks run.
+ */
+#define W8A8_MOE_DECODE_MAX_TOKENS 16
+size_t w8a8_moe_ffn_decode_workspace_size(uint32_t tokens, uint32_t topk, uint32_t hidden,
+                                          uint32_t inter);
+
+int w8a8_moe_ffn_decode(const void* x, const void* logits, int logits_f16,
+                        const float* smooth_scale, const int8_t* w_gate_up,
+                        const float* sb_gate_up, const float* smooth_scale_down,
+                        const int8_t* w_down, const float* sb_down, void* out, uint32_t tokens,
+                        uint32_t hidden, uint32_t inter, uint32_t experts, uint32_t topk,
+                        float quant_max, uint32_t ldx, uint32_t ldo, void* workspace,
+                        size_t ws_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Attention                                                                  */
+/* ------------------------------------------------------------------------- */
+
+/*
+ * Causal attention of whole prompts, several sequences packed into one row
+ * matrix: token t of a sequence attends to the tokens of that sequence up to
+ * and including itself,
+ *   out[t, h] = sum_j p[j] * v[j, h / (heads / kv_heads)],
+ *   p = softmax over j of scale * (q[t, h] . k[j, h / (heads / kv_heads)])
+ * with the products and sums in fp32, each p rounded to fp16 as the second
+ * product's operand, and one rounding of the result to fp16.
+ *   q   fp16 [tokens, ldq], head h in columns [h * head_dim, (h + 1) * head_dim);
+ *   k, v fp16 [tokens, ldk / ldv] likewise with kv_heads heads; out fp16
+ *       [tokens, ldo].  All three may be columns of one projection's output
+ *       (ldq = ldk = ldv = its width).  out may not overlap q, k or v.
+ *   seq_starts int32 [seqs + 1] on the device, ascending: sequence i is rows
+ *       [seq_starts[i], seq_starts[i + 1]), any length including 0.  Rows
+ *       before the first and behind the last sequence are left as they were;
+ *       values outside [0, tokens] count as the nearer end.
+ * What a token may not see does not reach it, infinities and NaN included.
+ * kv_heads divides heads; head_dim 64 or 128; scale > 0; pointers 16-byte
+ * aligned, row strides multiples of 8 (W8A8_ERROR_NOT_SUPPORTED otherwise).
+ * tokens = 0 or seqs = 0 does nothing.
+ */
+int w8a8_attention(const void* q, const void* k, const void* v, void* out,
+                   const int32_t* seq_starts, uint32_t seqs, uint32_t tokens, uint32_t heads,
+                   uint32_t kv_heads, uint32_t head_dim, uint32_t ldq, uint32_t ldk,
+                   uint32_t ldv, uint32_t ldo, float scale, hipStream_t stream);
+
+/*
+ * A paged cache of keys and values in 4 bits.  Token rows of one page and one
+ * key head lie together:
+ *   k_codes, v_codes   uint8 [pages, kv_heads, page_size, head_dim / 2]: two
+ *                      codes a byte, the even one in the low half.  Rows of
+ *                      v_codes hold the channels in order, rows of k_codes in
+ *                      the order [4][head_dim / 32][8]: channel 32 j + 8 g + i
+ *                      (i < 8, g < 4) is code g * head_dim / 4 + 8 j + i, so
+ *                      that the 16 bytes one lane of a matrix instruction's
+ *                      operand takes are contiguous.
+ *   k_scales, v_scales fp16 [pages, kv_heads, page_size, head_dim / group, 2]:
+ *                      (scale, offset) of each group of consecutive channels
+ * A code n of 0..15 stands for offset + scale * (n - 8).
+ * Buffers are 16-byte aligned; page_size a power of two in 16..1024, head_dim
+ * 64 or 128, group 32, 64 or 128 and at most head_dim.
+ */
+typedef struct w8a8_kv4_cache {
+    uint8_t* k_codes;
+    uint8_t* v_codes;
+    void*    k_scales;
+    void*    v_scales;
+    uint32_t pages, page_size, kv_heads, head_dim, group;
+} w8a8_kv4_cache;
+
+/*
+ * Quantizes the keys and values of `tokens` tokens into the cache: token t into
+ * slot slots[t] = page * page_size + place (int32 on the device; a slot outside
+ * the cache skips its token).  Per group of channels, fp32 arithmetic:
+ *   scale  = half((max - min) / 15),  offset = half(min + 8 * scale)
+ *   code   = clamp(rint((x - offset) / scale) + 8, 0, 15), 8 where scale = 0
+ * A group of equal values is stored exactly (up to the fp16 it came in); one
+ * that holds an infinity or a NaN reads back as NaN.  Two tokens given the same
+ * slot leave in it the codes and scales of either, group by group.
+ *   k, v  fp16 [tokens, ldk / ldv] (0 means kv_heads * head_dim), head h in
+ *         columns [h * head_dim, ...); 16-byte aligned, strides multiples of 8
+ * `cache` is read on the host before the call returns.  tokens = 0 does nothing.
+ */
+int w8a8_kv4_store(const void* k, const void* v, const int32_t* slots, uint32_t tokens,
+                   uint32_t ldk, uint32_t ldv, const w8a8_kv4_cache* cache, hipStream_t stream);
+
+/*
+ * Reads rows of the cache back: k, v fp16 [tokens, ldk / ldv] of the slots
+ * given, half(fma(scale, code - 8, offset)).  Rows of slots outside the cache
+ * are left as they were.
+ */
+int w8a8_kv4_load(void* k, void* v, const int32_t* slots, uint32_t tokens, uint32_t ldk,
+                  uint32_t ldv, const w8a8_kv4_cache* cache, hipStream_t stream);
+
+/*
+ * Attention of one token per sequence over the cache:
+ *   out[s, h] = sum_j p[j] * v[j, h / (heads / kv_heads)], p the softmax of
+ *   scale * (q[s, h] . k[j, ...]) over the first seq_lens[s] tokens j of the
+ *   sequence, token j in page block_table[s, j / page_size] at place
+ *   j % page_size.
+ *   q   fp16 [seqs, ldq], heads as in w8a8_attention; out fp16 [seqs, ldo]
+ *   block_table int32 [seqs, table_ld], its first table_cols columns used;
+ *   seq_lens int32 [seqs]; both on the device.  A length outside [0,
+ *   table_cols * page_size] counts as the nearer end, and the tokens of a page
+ *   number outside [0, pages) are left out.  A sequence of no tokens gives
+ *   zeros.
+ * Codes enter the matrix products as they are, exactly; scores, softmax
+ * statistics and sums are fp32, and p * scale of a value is rounded to fp16 as
+ * the second product's operand.
+ * workspace: 16-byte aligned, w8a8_attention_kv4_workspace_size(seqs, heads,
+ * kv_heads, head_dim, table_cols * page_size) bytes, needs no clearing: long
+ * contexts are cut into pieces that run side by side, and a second launch joins
+ * them in order.  Without one (NULL, or smaller) a sequence's head is one
+ * block's work.  Calls that share a workspace must be ordered on one stream.
+ * 16-byte aligned q, out, ldq and ldo multiples of 8.
+ */
+size_t w8a8_attention_kv4_workspace_size(uint32_t seqs, uint32_t heads, uint32_t kv_heads,
+                                         uint32_t head_dim, uint32_t max_len);
+
+int w8a8_attention_kv4(const void* q, const w8a8_kv4_cache* cache, const int32_t* block_table,
+                       uint32_t table_cols, uint32_t table_ld, const int32_t* seq_lens, void* out,
+                       uint32_t seqs, uint32_t heads, uint32_t ldq, uint32_t ldo, float scale,
+                       void* workspace, size_t ws_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,9 +17,17 @@ The functions mirror the reference kernels this path replaces:
   moe_sort         <- kernel_moe_histogram/prefix_sum/scatter (rocwmma_moe_sorting.cpp:53-125)
   moe_gemm, moe_silu_mul_quant, moe_combine, moe_ffn
                    <- the expert FFN chain (rocwmma_fused_moe.cpp:96-211), gate*up form
+and beside them, without a counterpart there, what a decoder layer needs next to
+its linear layers:
+  moe_ffn_decode   the expert FFN of a few tokens in two launches
+  attention        causal attention of packed prompts
+  KV4Cache, kv4_store, kv4_load, attention_kv4
+                   a paged 4-bit cache of keys and values, and the attention of
+                   single tokens over it
 """
 from __future__ import annotations
 
+import ctypes
 import struct
 
 from . import _lib
@@ -44,7 +52,9 @@ __all__ = [
     "topk_softmax", "moe_sort", "moe_sort_workspace_size", "moe_gemm", "moe_gemm_workspace_size", "moe_silu_mul_quant",
     "moe_interleave_gate_up", "moe_gate_up_silu", "moe_gate_up_silu_workspace_size",
     "moe_combine", "moe_ffn", "add_rmsnorm_smoothquant", "rmsnorm", "add_rmsnorm",
-    "quantize_weights",
+    "quantize_weights", "moe_ffn_decode", "moe_ffn_decode_workspace_size",
+    "attention", "KV4Cache", "kv4_store", "kv4_load", "attention_kv4",
+    "attention_kv4_workspace_size",
 ]
 
 
@@ -277,8 +287,6 @@ def gemm_streamk_status(clear: bool = True) -> int:
     """w8a8_gemm_streamk_status: the current device's sticky stream-K flags
     (STREAMK_WAIT_EXPIRED when a split tile's bounded wait gave up), read after
     a device-wide synchronisation; cleared when `clear`."""
-    import ctypes
-
     flags = ctypes.c_uint32(0)
     _lib.call("w8a8_gemm_streamk_status", ctypes.byref(flags), 1 if clear else 0)
     return int(flags.value)
@@ -690,3 +698,264 @@ def moe_ffn(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_down, top
     y = moe_gemm(q2, w_down, srt["start"], srt["count"], r2, sb_down, workspace=ws)
     out = moe_combine(y, w, srt["dst_row"])
     return out, dict(weights=w, ids=ids, sort=srt, qa=qa, ra=ra, gate_up=gu, q2=q2, r2=r2, y=y)
+
+
+def _call_on(device, name: str, *args) -> None:
+    """_lib.call with `device` current: a launch goes to the current device."""
+    torch = _torch()
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args)
+
+
+def _require_on(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            if not t.is_cuda:
+                raise ValueError("W8A8 kernels take device tensors (got a CPU tensor)")
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _require(name, t, dtype, shape) -> None:
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} "
+                         f"(got {t.dtype}, {tuple(t.shape)}, strides {tuple(t.stride())})")
+
+
+def moe_ffn_decode_workspace_size(tokens: int, topk: int, hidden: int, inter: int) -> int:
+    """Bytes of the workspace moe_ffn_decode needs."""
+    return int(library().w8a8_moe_ffn_decode_workspace_size(tokens, topk, hidden, inter))
+
+
+def moe_ffn_decode(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_down, topk: int,
+                   smooth_scale_down=None, quant_max: float = 127.0, out=None, workspace="auto"):
+    """The expert FFN of moe_ffn for at most 16 tokens, in two launches.
+
+    x fp16 [T, H] (any row stride that is a multiple of 8), logits fp32 or fp16
+    [T, E], smooth_scale fp32 [E, H], w_gate_up int8 [E, 2*I, H] with sb_gate_up
+    fp32 [E, 2*I], w_down int8 [E, H, I] with sb_down fp32 [E, H],
+    smooth_scale_down fp32 [E, I] or None.  Returns out fp16 [T, H].  The
+    intermediate values stay fp32 (moe_ffn rounds the GEMM outputs to fp16), so
+    the result is moe_ffn's up to those roundings.
+    workspace: 'auto' (allocated here) or a device tensor of
+    moe_ffn_decode_workspace_size bytes."""
+    torch = _torch()
+    _require_cuda(x)
+    dev = x.device
+    _require_on(dev, logits=logits, smooth_scale=smooth_scale, w_gate_up=w_gate_up,
+                sb_gate_up=sb_gate_up, w_down=w_down, sb_down=sb_down,
+                smooth_scale_down=smooth_scale_down, out=out)
+    _rows2d("x", x)
+    t, h = x.shape
+    if w_down.dim() != 3:
+        raise ValueError("w_down must be [E, H, I]")
+    e, _, i = w_down.shape
+    if logits.dtype not in (torch.float32, torch.float16):
+        raise ValueError("logits must be fp32 or fp16")
+    _require("logits", logits, logits.dtype, (t, e))
+    _require("smooth_scale", smooth_scale, torch.float32, (e, h))
+    _require("w_gate_up", w_gate_up, torch.int8, (e, 2 * i, h))
+    _require("sb_gate_up", sb_gate_up, torch.float32, (e, 2 * i))
+    _require("w_down", w_down, torch.int8, (e, h, i))
+    _require("sb_down", sb_down, torch.float32, (e, h))
+    if smooth_scale_down is not None:
+        _require("smooth_scale_down", smooth_scale_down, torch.float32, (e, i))
+    if out is None:
+        out = torch.empty((t, h), dtype=torch.float16, device=dev)
+    else:
+        _rows2d("out", out, h)
+        if out.shape[0] != t:
+            raise ValueError(f"out must have {t} rows")
+    if workspace is None:
+        raise ValueError("moe_ffn_decode needs a workspace")
+    ws, ws_bytes = _workspace(workspace, lambda: moe_ffn_decode_workspace_size(t, topk, h, i), dev)
+    _call_on(dev, "w8a8_moe_ffn_decode", x.data_ptr(), logits.data_ptr(),
+             1 if logits.dtype == torch.float16 else 0, smooth_scale.data_ptr(),
+             w_gate_up.data_ptr(), sb_gate_up.data_ptr(), _ptr(smooth_scale_down),
+             w_down.data_ptr(), sb_down.data_ptr(), out.data_ptr(), t, h, i, e, topk,
+             float(quant_max), x.stride(0), out.stride(0), _ptr(ws), ws_bytes, _stream(dev))
+    return out
+
+
+def _heads3d(name, t, heads=None, dim=None) -> int:
+    """Checks fp16 [tokens, heads, dim] whose heads lie side by side; its row stride."""
+    torch = _torch()
+    if t.dim() != 3 or t.dtype != torch.float16:
+        raise ValueError(f"{name} must be a 3-D fp16 tensor [tokens, heads, head_dim]")
+    if (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
+        raise ValueError(f"{name} must have {heads} heads of {dim} channels, "
+                         f"got {tuple(t.shape)}")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError(f"{name}: the heads of a token must lie side by side "
+                         f"(strides {tuple(t.stride())})")
+    # a single row may carry any stride
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def attention(q, k, v, seq_starts, scale: float | None = None, out=None):
+    """Causal attention of whole prompts packed into one row matrix.
+
+    q fp16 [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]:
+    slices of one projection's output are fine (any row stride that is a
+    multiple of 8; the heads of a token side by side).  seq_starts int32
+    [seqs + 1] on the device, ascending: sequence i is rows seq_starts[i] ..
+    seq_starts[i + 1].  scale: 1 / sqrt(head_dim) unless given.  Returns fp16
+    [tokens, heads, head_dim]; rows of no sequence are left as they were in
+    `out` (undefined in a new tensor)."""
+    torch = _torch()
+    _require_cuda(q)
+    dev = q.device
+    _require_on(dev, k=k, v=v, seq_starts=seq_starts, out=out)
+    ldq = _heads3d("q", q)
+    tokens, heads, dim = q.shape
+    ldk, ldv = _heads3d("k", k, None, dim), _heads3d("v", v, None, dim)
+    kv_heads = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != tokens:
+        raise ValueError("k and v must have q's tokens and head_dim, and one number of heads")
+    if seq_starts.dtype != torch.int32 or seq_starts.dim() != 1 or not seq_starts.is_contiguous() \
+            or seq_starts.numel() < 1:
+        raise ValueError("seq_starts must be a contiguous int32 tensor [seqs + 1]")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=torch.float16, device=dev)
+    ldo = _heads3d("out", out, heads, dim)
+    if out.shape[0] != tokens:
+        raise ValueError(f"out must have {tokens} rows")
+    _call_on(dev, "w8a8_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+             seq_starts.data_ptr(), seq_starts.numel() - 1, tokens, heads, kv_heads, dim, ldq, ldk,
+             ldv, ldo, dim ** -0.5 if scale is None else float(scale), _stream(dev))
+    return out
+
+
+class KV4Cache:
+    """A paged cache of keys and values in 4 bits (w8a8_kv4_cache), over four
+    tensors: k_codes, v_codes uint8 [pages, kv_heads, page_size, head_dim / 2]
+    and k_scales, v_scales fp16 [pages, kv_heads, page_size, head_dim / group, 2].
+    KV4Cache.empty allocates them; the cache keeps them alive."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales):
+        torch = _torch()
+        _require_cuda(k_codes)
+        _require_on(k_codes.device, v_codes=v_codes, k_scales=k_scales, v_scales=v_scales)
+        if k_codes.dim() != 4 or k_scales.dim() != 5 or k_scales.shape[3] == 0:
+            raise ValueError("codes must be [pages, kv_heads, page_size, head_dim / 2], scales "
+                             "[pages, kv_heads, page_size, head_dim / group, 2]")
+        pages, kv_heads, page_size, half = k_codes.shape
+        groups = k_scales.shape[3]
+        for name, t in (("k_codes", k_codes), ("v_codes", v_codes)):
+            _require(name, t, torch.uint8, (pages, kv_heads, page_size, half))
+        for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+            _require(name, t, torch.float16, (pages, kv_heads, page_size, groups, 2))
+        if 2 * half % groups != 0:
+            raise ValueError("the groups must divide the channels of a head")
+        self.k_codes, self.v_codes, self.k_scales, self.v_scales = (k_codes, v_codes, k_scales,
+                                                                    v_scales)
+        self.pages, self.kv_heads, self.page_size, self.head_dim = (pages, kv_heads, page_size,
+                                                                    2 * half)
+        self.group = 2 * half // groups
+        self.device = k_codes.device
+        self._desc = _lib.Kv4Cache(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(),
+                                   v_scales.data_ptr(), pages, page_size, kv_heads, 2 * half,
+                                   self.group)
+        self._ref = ctypes.byref(self._desc)
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, group: int = 32,
+              device="cuda"):
+        """A cache of newly allocated pages (contents undefined)."""
+        torch = _torch()
+        codes = (pages, kv_heads, page_size, head_dim // 2)
+        scales = (pages, kv_heads, page_size, head_dim // group, 2)
+        return cls(torch.empty(codes, dtype=torch.uint8, device=device),
+                   torch.empty(codes, dtype=torch.uint8, device=device),
+                   torch.empty(scales, dtype=torch.float16, device=device),
+                   torch.empty(scales, dtype=torch.float16, device=device))
+
+
+def _kv4_slots(slots) -> int:
+    if slots.dtype != _torch().int32 or slots.dim() != 1 or not slots.is_contiguous():
+        raise ValueError("slots must be a contiguous 1-D int32 tensor")
+    return slots.numel()
+
+
+def kv4_store(k, v, slots, cache: KV4Cache) -> None:
+    """Quantize the keys and values of some tokens into the cache: k, v fp16
+    [tokens, kv_heads, head_dim] (any row stride that is a multiple of 8), token
+    t into slot slots[t] = page * page_size + place (int32; a slot outside the
+    cache skips its token; the slots of one call should differ)."""
+    _require_on(cache.device, k=k, v=v, slots=slots)
+    n = _kv4_slots(slots)
+    ldk = _heads3d("k", k, cache.kv_heads, cache.head_dim)
+    ldv = _heads3d("v", v, cache.kv_heads, cache.head_dim)
+    if k.shape[0] != n or v.shape[0] != n:
+        raise ValueError(f"k and v must have {n} tokens, one per slot")
+    _call_on(cache.device, "w8a8_kv4_store", k.data_ptr(), v.data_ptr(), slots.data_ptr(), n, ldk,
+             ldv, cache._ref, _stream(cache.device))
+
+
+def kv4_load(cache: KV4Cache, slots, out=None):
+    """Read slots of the cache back: (k, v) fp16 [n, kv_heads, head_dim].  Rows
+    of slots outside the cache are left as they were in `out`, a (k, v) pair
+    (undefined in new tensors)."""
+    torch = _torch()
+    _require_on(cache.device, slots=slots)
+    n = _kv4_slots(slots)
+    if out is None:
+        shape = (n, cache.kv_heads, cache.head_dim)
+        out = (torch.empty(shape, dtype=torch.float16, device=cache.device),
+               torch.empty(shape, dtype=torch.float16, device=cache.device))
+    k, v = out
+    _require_on(cache.device, k=k, v=v)
+    ldk = _heads3d("k", k, cache.kv_heads, cache.head_dim)
+    ldv = _heads3d("v", v, cache.kv_heads, cache.head_dim)
+    if k.shape[0] != n or v.shape[0] != n:
+        raise ValueError(f"k and v must have {n} rows, one per slot")
+    _call_on(cache.device, "w8a8_kv4_load", k.data_ptr(), v.data_ptr(), slots.data_ptr(), n, ldk,
+             ldv, cache._ref, _stream(cache.device))
+    return k, v
+
+
+def attention_kv4_workspace_size(seqs: int, heads: int, kv_heads: int, head_dim: int,
+                                 max_len: int) -> int:
+    """Bytes of workspace attention_kv4 can use (0: none); max_len is the block
+    table's columns times the page size."""
+    return int(library().w8a8_attention_kv4_workspace_size(seqs, heads, kv_heads, head_dim,
+                                                           max_len))
+
+
+def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None = None, out=None,
+                  workspace="auto"):
+    """Attention of one new token per sequence over the cache.
+
+    q fp16 [seqs, heads, head_dim]; block_table int32 [seqs, columns] (unit
+    column stride): the page of each page_size tokens of a sequence; seq_lens
+    int32 [seqs]: the tokens to attend to, the new one (stored before) among
+    them.  Returns fp16 [seqs, heads, head_dim]; a sequence of no tokens gives
+    zeros.  workspace: 'auto' (allocated here), None (each head of a sequence is
+    one block's work) or a device tensor of attention_kv4_workspace_size bytes."""
+    torch = _torch()
+    dev = cache.device
+    _require_on(dev, q=q, block_table=block_table, seq_lens=seq_lens, out=out)
+    ldq = _heads3d("q", q, None, cache.head_dim)
+    seqs, heads, dim = q.shape
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != seqs \
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be int32 [seqs, columns] with unit column stride")
+    if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (seqs,) \
+            or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be a contiguous int32 tensor [seqs]")
+    cols = block_table.shape[1]
+    table_ld = block_table.stride(0) if seqs > 1 else cols
+    if out is None:
+        out = torch.empty((seqs, heads, dim), dtype=torch.float16, device=dev)
+    ldo = _heads3d("out", out, heads, dim)
+    if out.shape[0] != seqs:
+        raise ValueError(f"out must have {seqs} rows")
+    ws, ws_bytes = _workspace(
+        workspace, lambda: attention_kv4_workspace_size(seqs, heads, cache.kv_heads, dim,
+                                                        cols * cache.page_size), dev)
+    _call_on(dev, "w8a8_attention_kv4", q.data_ptr(), cache._ref, block_table.data_ptr(), cols,
+             table_ld, seq_lens.data_ptr(), out.data_ptr(), seqs, heads, ldq, ldo,
+             dim ** -0.5 if scale is None else float(scale), _ptr(ws), ws_bytes, _stream(dev))
+    return out

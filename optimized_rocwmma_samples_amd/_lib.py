@@ -34,6 +34,7 @@ PLAN_MOE_REQUANT = 6
 PLAN_GROUPED = 7
 
 GROUPED_INLINE_GROUPS = 48  # W8A8_GROUPED_INLINE_GROUPS
+MOE_DECODE_MAX_TOKENS = 16  # W8A8_MOE_DECODE_MAX_TOKENS
 
 FOLD_MULTIPLY = 0
 FOLD_DIVIDE = 1
@@ -53,6 +54,15 @@ class GroupDesc(ctypes.Structure):
                 ("m", ctypes.c_uint32), ("n", ctypes.c_uint32), ("k", ctypes.c_uint32),
                 ("lda", ctypes.c_uint32), ("ldb", ctypes.c_uint32), ("ldc", ctypes.c_uint32),
                 ("tensor_scale_a", ctypes.c_float), ("tensor_scale_b", ctypes.c_float)]
+
+
+class Kv4Cache(ctypes.Structure):
+    """w8a8_kv4_cache (include/w8a8.h)."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+                ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+                ("pages", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("group", ctypes.c_uint32)]
 
 
 # name -> (restype, argtypes); mirrors include/w8a8.h
@@ -107,6 +117,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                      _ptr]),
     "w8a8_moe_combine": (_i32, [_ptr, _u32, _u32, _ptr, _ptr, _u32, _u32, _u32, _ptr, _u32,
                                 _ptr]),
+    "w8a8_moe_ffn_decode_workspace_size": (_size, [_u32, _u32, _u32, _u32]),
+    "w8a8_moe_ffn_decode": (_i32, [_ptr, _ptr, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                   _u32, _u32, _u32, _u32, _u32, _f32, _u32, _u32, _ptr, _size,
+                                   _ptr]),
+    "w8a8_attention": (_i32, [_ptr, _ptr, _ptr, _ptr, _ptr, _u32, _u32, _u32, _u32, _u32, _u32,
+                              _u32, _u32, _u32, _f32, _ptr]),
+    "w8a8_kv4_store": (_i32, [_ptr, _ptr, _ptr, _u32, _u32, _u32, ctypes.POINTER(Kv4Cache),
+                              _ptr]),
+    "w8a8_kv4_load": (_i32, [_ptr, _ptr, _ptr, _u32, _u32, _u32, ctypes.POINTER(Kv4Cache), _ptr]),
+    "w8a8_attention_kv4_workspace_size": (_size, [_u32, _u32, _u32, _u32, _u32]),
+    "w8a8_attention_kv4": (_i32, [_ptr, ctypes.POINTER(Kv4Cache), _ptr, _u32, _u32, _ptr, _ptr,
+                                  _u32, _u32, _u32, _u32, _f32, _ptr, _size, _ptr]),
 }
 
 

@@ -45,6 +45,9 @@ SOURCES = [
     "moe.hip",
     "rmsnorm_sq.hip",
     "weights.hip",
+    "attention.hip",
+    "kv4.hip",
+    "moe_decode.hip",
 ]
 
 # -packed-fp32-ops: keep the compiler from emitting packed fp32 VALU ops.

@@ -3,6 +3,7 @@
 // between the two expert GEMMs, the weighted combine back to token order, and
 // the launchers of the grouped / MoE GEMM kernels.
 #include "gemm_i8_grouped_kernel.hpp"
+#include "moe_route.hpp"
 #include "w8a8_internal.hpp"
 
 #include <algorithm>
@@ -23,24 +24,6 @@ namespace {
 constexpr int kTopkWaves = 4;
 
 template <bool F16>
-__device__ __forceinline__ float load_logit(const void* p, size_t i)
-{
-    if constexpr(F16)
-        return half_bits_to_float(static_cast<const uint16_t*>(p)[i]);
-    else
-        return static_cast<const float*>(p)[i];
-}
-
-// (value, index) of the better of two candidates: larger value, then lower index.
-__device__ __forceinline__ void better(float& v, int& i, float ov, int oi)
-{
-    if(ov > v || (ov == v && oi < i)) {
-        v = ov;
-        i = oi;
-    }
-}
-
-template <bool F16>
 __global__ void __launch_bounds__(kTopkWaves* kWave)
     topk_softmax_kernel(const void* logits, float* topk_w, int32_t* topk_ids, uint32_t tokens,
                         uint32_t experts, uint32_t topk)
@@ -50,36 +33,13 @@ __global__ void __launch_bounds__(kTopkWaves* kWave)
     if(tok >= tokens) return; // uniform per wave
     const size_t row = (size_t)tok * experts;
 
-    // cross-lane steps are DPP reductions (no LDS round trips)
-    float wmax = -INFINITY;
-    for(uint32_t e = lane; e < experts; e += kWave) wmax = fmaxf(wmax, load_logit<F16>(logits, row + e));
-    wmax = wave_max(wmax);
-    float wsum = 0.f;
-    for(uint32_t e = lane; e < experts; e += kWave) wsum += expf(load_logit<F16>(logits, row + e) - wmax);
-    wsum            = wave_sum(wsum);
-    const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
-
-    // a lane owns experts lane, lane+64, ...: `used` marks the chosen ones.
-    // Per pick: each lane's best unused candidate (larger logit, then lower
-    // index), the wave max of those values, then the lowest index among the
-    // lanes holding that max: the same winner as a pairwise reduction.
-    constexpr int kNone = 0x7FFFFFFF;
-    uint64_t      used  = 0;
-    for(uint32_t k = 0; k < topk; ++k) {
-        float bv = -INFINITY;
-        int   bi = kNone;
-        int   j  = 0;
-        for(uint32_t e = lane; e < experts; e += kWave, ++j)
-            if(!((used >> j) & 1u)) better(bv, bi, load_logit<F16>(logits, row + e), (int)e);
-        const float m = wave_max(bv);
-        const int   w = wave_min_i32(bv == m ? bi : kNone);
-        if(w != kNone && (uint32_t)w % kWave == (uint32_t)lane) used |= 1ull << ((uint32_t)w / kWave);
-        if(lane == 0) {
-            const bool ok                    = w != kNone;
-            topk_ids[(size_t)tok * topk + k] = ok ? w : -1;
-            topk_w[(size_t)tok * topk + k]   = ok ? expf(m - wmax) * inv : 0.f;
-        }
-    }
+    route_token([&](uint32_t e) { return load_logit<F16>(logits, row + e); }, experts, topk, lane,
+                [&](uint32_t k, int id, float weight) {
+                    if(lane == 0) {
+                        topk_ids[(size_t)tok * topk + k] = id;
+                        topk_w[(size_t)tok * topk + k]   = weight;
+                    }
+                });
 }
 
 // ---------------------------------------------------------------------------

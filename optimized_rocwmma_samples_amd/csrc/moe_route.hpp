@@ -1,0 +1,68 @@
+// moe_route.hpp -- the routing of one token by one wave, shared by the kernels
+// that route (moe.hip, moe_decode.hip): the same order of operations in each,
+// so the ids and weights are the same bits.
+#pragma once
+
+#include "w8a8_device.hpp"
+
+namespace w8a8 {
+
+// Element i of logits held as fp16 or fp32.
+template <bool F16>
+__device__ __forceinline__ float load_logit(const void* p, size_t i)
+{
+    if constexpr(F16)
+        return half_bits_to_float(static_cast<const uint16_t*>(p)[i]);
+    else
+        return static_cast<const float*>(p)[i];
+}
+
+// (value, index) of the better of two candidates: larger value, then lower index.
+__device__ __forceinline__ void better(float& v, int& i, float ov, int oi)
+{
+    if(ov > v || (ov == v && oi < i)) {
+        v = ov;
+        i = oi;
+    }
+}
+
+// The topk experts of one token, best first: emit(k, id, weight) in every lane
+// for k = 0 .. topk - 1, id = -1 and weight = 0 where only NaN logits are left.
+// Experts are chosen on the logits (softmax is monotonic, so the choice is
+// exact), the lower index winning ties; weight = exp(l - max) * (1 / sum_e
+// exp(l_e - max)).  logit(e): the fp32 value of expert e's logit.  A lane owns
+// experts lane, lane + 64, ...: experts <= 4096 (the bits of `used`).
+template <class Logit, class Emit>
+__device__ __forceinline__ void route_token(Logit logit, uint32_t experts, uint32_t topk, int lane,
+                                            Emit emit)
+{
+    // cross-lane steps are DPP reductions (no LDS round trips)
+    float wmax = -INFINITY;
+    for(uint32_t e = lane; e < experts; e += kWave) wmax = fmaxf(wmax, logit(e));
+    wmax       = wave_max(wmax);
+    float wsum = 0.f;
+    for(uint32_t e = lane; e < experts; e += kWave) wsum += expf(logit(e) - wmax);
+    wsum            = wave_sum(wsum);
+    const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+
+    // `used` marks the chosen ones.  Per pick: each lane's best unused candidate
+    // (larger logit, then lower index), the wave max of those values, then the
+    // lowest index among the lanes holding that max: the same winner as a
+    // pairwise reduction.
+    constexpr int kNone = 0x7FFFFFFF;
+    uint64_t      used  = 0;
+    for(uint32_t k = 0; k < topk; ++k) {
+        float bv = -INFINITY;
+        int   bi = kNone;
+        int   j  = 0;
+        for(uint32_t e = lane; e < experts; e += kWave, ++j)
+            if(!((used >> j) & 1u)) better(bv, bi, logit(e), (int)e);
+        const float m = wave_max(bv);
+        const int   w = wave_min_i32(bv == m ? bi : kNone);
+        if(w != kNone && (uint32_t)w % kWave == (uint32_t)lane) used |= 1ull << ((uint32_t)w / kWave);
+        const bool ok = w != kNone;
+        emit(k, ok ? w : -1, ok ? expf(m - wmax) * inv : 0.f);
+    }
+}
+
+} // namespace w8a8

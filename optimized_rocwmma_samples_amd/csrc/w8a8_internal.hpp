@@ -258,4 +258,59 @@ hipError_t launch_moe_interleave_gate_up(const int8_t* w, const float* sw, uint3
                                          uint32_t inter, uint32_t k, uint32_t ldw, int8_t* wo,
                                          float* swo, hipStream_t stream);
 
+// The expert layer of few tokens (moe_decode.hip).
+struct MoeDecodeArgs {
+    const uint16_t* x;
+    const void*     logits;
+    const float*    s;
+    const int8_t*   wgu;
+    const float*    sgu;
+    const float*    s2; // or null
+    const int8_t*   wd;
+    const float*    sd;
+    uint16_t*       out;
+    uint32_t        tokens, hidden, inter, experts, topk, ldx, ldo;
+    float           qmax;
+    void*           ws;
+};
+size_t     moe_ffn_decode_workspace_bytes(uint32_t tokens, uint32_t topk, uint32_t hidden,
+                                          uint32_t inter);
+hipError_t launch_moe_ffn_decode(const MoeDecodeArgs& a, bool logits_f16, hipStream_t stream);
+
+// ---- Attention (attention.hip, kv4.hip) ---------------------------------------
+struct AttentionArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t*       out;
+    const int32_t*  starts; // [seqs + 1]
+    uint32_t        seqs, tokens, heads, kv_heads, dim;
+    uint32_t        ldq, ldk, ldv, ldo;
+    float           scale;
+};
+hipError_t launch_attention(const AttentionArgs& a, hipStream_t stream);
+
+// Rows in or out of the 4-bit cache.
+struct Kv4Rows {
+    const int32_t* slots;
+    uint32_t       tokens, ldk, ldv;
+};
+hipError_t launch_kv4_store(const w8a8_kv4_cache& c, const Kv4Rows& r, const uint16_t* k,
+                            const uint16_t* v, hipStream_t stream);
+hipError_t launch_kv4_load(const w8a8_kv4_cache& c, const Kv4Rows& r, uint16_t* k, uint16_t* v,
+                           hipStream_t stream);
+
+struct AttentionKv4Args {
+    const uint16_t* q;
+    uint16_t*       out;
+    const int32_t*  table; // [seqs, table_ld]
+    const int32_t*  lens;  // [seqs]
+    uint32_t        seqs, heads, ldq, ldo, table_cols, table_ld;
+    float           scale;
+    void*           ws;
+    size_t          ws_bytes;
+};
+size_t     attention_kv4_workspace_bytes(uint32_t seqs, uint32_t heads, uint32_t kv_heads,
+                                         uint32_t dim, uint32_t max_len);
+hipError_t launch_attention_kv4(const w8a8_kv4_cache& c, const AttentionKv4Args& a,
+                                hipStream_t stream);
+
 } // namespace w8a8

@@ -1,63 +1,357 @@
 // attention.hip -- causal attention of whole prompts for gfx950.
+//
+//   out[t, h] = sum_{j <= t} p[j] v[j],  p = softmax of scale * (q[t, h] . k[j])
+//
+// One pass over the keys with a running maximum m and sum l per query row.  A
+// block owns 128 query rows of one head, 32 per wave, and walks the key tiles of
+// 64 tokens from the diagonal down to the sequence's first.
+//   * Scores are computed transposed, S^T = K Q^T with v_mfma_f32_32x32x16_f16
+//     (srcA = keys, srcB = queries): a lane then holds 16 of 32 keys' scores of
+//     ONE query row (lane % 32), so maximum, exponential, sum and the rescaling
+//     of the result are in-lane but for one exchange between the wave's halves,
+//     and the probabilities, rounded to fp16, already are the srcB operand of
+//     O^T += V^T P^T: the order in which that product takes the keys is free, so
+//     a lane's registers are taken as they lie (key 8 (i / 4) + 4 (lane / 32) +
+//     i % 4 in register i) and V^T is read to match.
+//   * V^T comes out of a row-major tile in LDS with ds_read_b64_tr_b16: 16 lanes
+//     read 4 keys x 16 channels and get 4 keys of one channel each.
+//   * Key and value tiles go from global memory to LDS without registers, one tile
+//     ahead, 16 bytes a lane; the 16-byte chunks of a row are stored XOR-swizzled
+//     (chosen by the global address each lane fetches), so that both kinds of
+//     reads spread over all banks.  Rows past the sequence's end read as zeros.
+//   * The tile on the diagonal comes first and is the only one that masks.
 #include "w8a8_device.hpp"
 #include "w8a8_internal.hpp"
 
 namespace w8a8 {
 namespace {
 
-// One wave per (token, head): lanes over the channels, one key after the other
-// with a running maximum and sum.
-template <int D>
-__global__ void __launch_bounds__(kWave) attention_kernel(AttentionArgs a)
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float    v2f __attribute__((ext_vector_type(2)));
+typedef float    v16f __attribute__((ext_vector_type(16)));
+typedef __fp16   v4fp16 __attribute__((ext_vector_type(4)));
+
+typedef __attribute__((address_space(3))) void   lds_void_t;
+typedef __attribute__((address_space(3))) v4fp16 lds_v4h_t;
+typedef __attribute__((address_space(3))) v8h    lds_v8h_t;
+
+constexpr int kBufferFlags = 0x00020000; // raw buffer, 32-bit data format
+constexpr int kRows        = 128;        // query rows a block
+constexpr int kKeys        = 64;         // keys a tile
+constexpr int kWaves       = kRows / 32;
+constexpr int kThreads     = kWaves * kWave;
+
+// Where a block works: one sequence's rows and a tile of kRows of them.
+struct Span {
+    uint32_t begin, len, tile;
+    bool     live;
+};
+
+// The tile-th tile of kRows query rows over all sequences, by one wave: 64
+// sequences a step, their tile counts summed along the lanes.  Inside a sequence
+// the tiles with the most keys come first.
+__device__ __forceinline__ Span find_tile(const AttentionArgs& a, uint32_t tile, int lane)
 {
-    constexpr int  kC   = D / kWave;
-    const uint32_t head = blockIdx.x % a.heads, t = blockIdx.x / a.heads, lane = threadIdx.x;
-    const uint32_t kvh  = head / (a.heads / a.kv_heads);
-    // the last sequence that starts at or before t
-    uint32_t lo = 0, hi = a.seqs;
-    while(hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if(a.starts[mid] <= (int32_t)t)
-            lo = mid;
-        else
-            hi = mid;
+    uint32_t before = 0;
+    for(uint32_t i0 = 0; i0 < a.seqs; i0 += kWave) {
+        const uint32_t i = i0 + lane;
+        int32_t        b = 0, e = 0;
+        if(i < a.seqs) {
+            b = min(max(a.starts[i], 0), (int32_t)a.tokens);
+            e = min(max(a.starts[i + 1], 0), (int32_t)a.tokens);
+        }
+        const uint32_t n = e > b ? (uint32_t)(e - b + kRows - 1) / kRows : 0;
+        uint32_t       s = n;
+#pragma unroll
+        for(int d = 1; d < kWave; d <<= 1) {
+            const uint32_t o = __shfl_up(s, d, kWave);
+            if(lane >= d) s += o;
+        }
+        const uint64_t past = __ballot(before + s > tile);
+        if(past != 0) {
+            const int      f  = __builtin_ctzll(past);
+            const uint32_t nf = __builtin_amdgcn_readlane(n, f);
+            const uint32_t lo = before + __builtin_amdgcn_readlane(s, f) - nf;
+            const uint32_t bf = __builtin_amdgcn_readlane(b, f);
+            const uint32_t ef = __builtin_amdgcn_readlane(e, f);
+            return {bf, ef - bf, nf - 1 - (tile - lo), tile >= lo && tile - lo < nf};
+        }
+        before += __builtin_amdgcn_readlane(s, kWave - 1);
     }
-    const int32_t begin = max(a.starts[lo], 0);
-    if(begin > (int32_t)t || a.starts[lo + 1] <= (int32_t)t) return;
-    float q[kC], o[kC];
+    return {0, 0, 0, false};
+}
+
+// The 16-byte chunk position of chunk c of row `tok` (an involution in c).
+template <int D>
+__device__ __forceinline__ uint32_t key_chunk(uint32_t tok, uint32_t c)
+{
+    return c ^ (D == 128 ? tok % 16 : tok / 2 % 8);
+}
+
+template <int D>
+__device__ __forceinline__ uint32_t value_chunk(uint32_t tok, uint32_t c)
+{
+    return c ^ (D == 128 ? tok % 4 * 4 : tok / 2 % 2 * 4);
+}
+
+__device__ __forceinline__ v16f mfma(v8h a, v8h b, v16f c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// The value of the other half of the wave (lane ^ 32) and this one's.
+__device__ __forceinline__ v2f both_halves(float v)
+{
+    const uint32_t u = __float_as_uint(v);
+    const auto     r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+
+__device__ __forceinline__ bool nonfinite(uint32_t h16) { return (h16 & 0x7C00u) == 0x7C00u; }
+
+// The fp16 values of a fragment with infinities and NaN as 0.
+__device__ __forceinline__ v8h finite_only(v8h v)
+{
+    v4i u = __builtin_bit_cast(v4i, v);
 #pragma unroll
-    for(int i = 0; i < kC; ++i) {
-        q[i] = half_bits_to_float(a.q[(size_t)t * a.ldq + head * D + lane * kC + i]) * a.scale;
-        o[i] = 0.f;
+    for(int i = 0; i < 4; ++i) {
+        const uint32_t w = (uint32_t)u[i];
+        u[i] = (int)((nonfinite(w) ? 0u : w & 0xFFFFu) | (nonfinite(w >> 16) ? 0u : w & 0xFFFF0000u));
     }
-    float m = -INFINITY, l = 0.f;
-    for(uint32_t j = begin; j <= t; ++j) {
-        float dot = 0.f;
+    return __builtin_bit_cast(v8h, u);
+}
+
+// 16 bytes a lane from a buffer into LDS, lane i to byte `to` + 16 i, with the
+// caller's own waits: a load through the builtin makes the compiler wait for all
+// of them ahead of every transposed read, whichever stage that reads.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm" // m0 is reserved: set and used here alone
+__device__ __forceinline__ void load_lds(v4i rsrc, uint32_t to, uint32_t offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(to), "v"(offset), "s"(rsrc)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+__device__ __forceinline__ v4i buffer(const void* base, uint32_t bytes)
+{
+    const uint64_t at = (uint64_t)base;
+    return v4i{(int)(uint32_t)at, (int)((uint32_t)(at >> 32) & 0xFFFFu), (int)bytes, kBufferFlags};
+}
+
+template <int D>
+__device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* lds)
+{
+    constexpr int kTileBytes = kKeys * D * 2;
+    constexpr int kChunks    = D / 8;                  // 16-byte chunks per row
+    constexpr int kRowsLoad  = kWave / kChunks;        // rows one wave-load fills
+    constexpr int kLoads     = kKeys / kRowsLoad / kWaves; // wave-loads per wave and operand
+    constexpr int kSteps     = D / 16;                 // MFMAs along the channels
+    constexpr int kBlocks    = D / 32;                 // 32-channel blocks of the result
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
+
+    // Blocks go round the 8 XCDs: where the heads divide evenly, an XCD gets
+    // neighbouring heads, whose keys and values then stay in its L2.
+    uint32_t head = blockIdx.x % a.heads;
+    if(a.heads % 8 == 0) head = head % 8 * (a.heads / 8) + head / 8;
+    const Span span = find_tile(a, blockIdx.x / a.heads, lane);
+    if(!span.live) return;
+    const uint32_t kvh   = head / (a.heads / a.kv_heads);
+    const uint32_t row0  = span.tile * kRows;        // the block's first row in the sequence
+    const uint32_t first = row0 + wave * 32;         // the wave's
+    const uint32_t qi    = first + col;              // the lane's
+    const uint32_t rows  = min((uint32_t)kRows, span.len - row0);
+
+    // ---- tiles into LDS -------------------------------------------------------
+    const uint32_t  ldkb = a.ldk * 2, ldvb = a.ldv * 2;
+    const uint16_t* kbase = a.k + (size_t)span.begin * a.ldk + kvh * D;
+    const uint16_t* vbase = a.v + (size_t)span.begin * a.ldv + kvh * D;
+    uint32_t        ko[kLoads], vo[kLoads];
 #pragma unroll
-        for(int i = 0; i < kC; ++i)
-            dot = fmaf(q[i], half_bits_to_float(a.k[(size_t)j * a.ldk + kvh * D + lane * kC + i]), dot);
-        const float s  = wave_sum(dot);
-        const float mn = fmaxf(m, s);
-        const float al = m == mn ? 1.f : __expf(m - mn), p = s == mn ? 1.f : __expf(s - mn);
-        m              = mn;
-        l              = l * al + p;
-#pragma unroll
-        for(int i = 0; i < kC; ++i)
-            o[i] = o[i] * al + p * half_bits_to_float(a.v[(size_t)j * a.ldv + kvh * D + lane * kC + i]);
+    for(int i = 0; i < kLoads; ++i) {
+        const uint32_t tok = (wave * kLoads + i) * kRowsLoad + lane / kChunks;
+        ko[i]              = tok * ldkb + key_chunk<D>(tok, lane % kChunks) * 16;
+        vo[i]              = tok * ldvb + value_chunk<D>(tok, lane % kChunks) * 16;
     }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
+    auto           issue = [&](int stage, uint32_t kt) {
+        const uint32_t n = min((uint32_t)kKeys, span.len - kt * kKeys);
+        const v4i      rk = buffer(kbase + (size_t)kt * kKeys * a.ldk, (n - 1) * ldkb + D * 2);
+        const v4i      rv = buffer(vbase + (size_t)kt * kKeys * a.ldv, (n - 1) * ldvb + D * 2);
+        const uint32_t to = lds0 + stage * 2 * kTileBytes + wave * kLoads * 1024;
 #pragma unroll
-    for(int i = 0; i < kC; ++i)
-        a.out[(size_t)t * a.ldo + head * D + lane * kC + i] = float_to_half_bits(o[i] / l);
+        for(int i = 0; i < kLoads; ++i) load_lds(rk, to + i * 1024, ko[i]);
+#pragma unroll
+        for(int i = 0; i < kLoads; ++i) load_lds(rv, to + kTileBytes + i * 1024, vo[i]);
+    };
+
+    const uint32_t tiles = (row0 + rows + kKeys - 1) / kKeys; // tiles the block's rows see
+    issue(0, tiles - 1);
+
+    // ---- the wave's query rows: lane = row, 8 channels from 16 step + 8 half ----
+    v8h qf[kSteps];
+    {
+        const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(a.q + (size_t)(span.begin + row0) * a.ldq + head * D), 0,
+            (int)((rows - 1) * a.ldq * 2 + D * 2), kBufferFlags);
+#pragma unroll
+        for(int s = 0; s < kSteps; ++s)
+            qf[s] = __builtin_bit_cast(
+                v8h, __builtin_amdgcn_raw_buffer_load_b128(
+                         rq, (wave * 32 + col) * a.ldq * 2 + s * 32 + half * 16, 0, 0));
+    }
+
+    const float c = a.scale * 1.44269504088896341f; // exponents in base 2
+    float       m = -INFINITY, l = 0.f;
+    v16f        o[kBlocks] = {};
+
+    for(uint32_t step = 0; step < tiles; ++step) {
+        const uint32_t kt    = tiles - 1 - step;
+        const uint32_t stage = step % 2;
+        wait_vmcnt<0>();   // this wave's part of the tile is there,
+        wait_lgkmcnt0();   // and its reads of the tile before are done:
+        __syncthreads();   // so are every wave's
+        if(kt > 0) issue(stage ^ 1, kt - 1);
+        if(kt * kKeys > first + 31) continue; // all of the tile is later than the wave's rows
+
+        const uint32_t kl   = lds0 + stage * 2 * kTileBytes, vl = kl + kTileBytes;
+        const bool     diag = (kt + 1) * kKeys > first; // some of it is later than some rows
+        v16f           s[2] = {};
+#pragma unroll
+        for(int sub = 0; sub < 2; ++sub) {
+            const uint32_t tok = sub * 32 + col;
+#pragma unroll
+            for(int st = 0; st < kSteps; ++st)
+                s[sub] = mfma(*(const lds_v8h_t*)(uintptr_t)(
+                                  kl + tok * D * 2 + key_chunk<D>(tok, 2 * st + half) * 16),
+                              qf[st], s[sub]);
+        }
+        if(diag) {
+#pragma unroll
+            for(int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                for(int i = 0; i < 16; ++i) {
+                    const uint32_t j = kt * kKeys + sub * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                    s[sub][i]        = j > qi ? -INFINITY : s[sub][i];
+                }
+        }
+        float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for(int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+        const v2f tops = both_halves(top);
+        const float mn = fmaxf(m, fmaxf(tops[0], tops[1]));
+        if(__ballot(mn > m) != 0) {
+            const float al = __builtin_amdgcn_exp2f((m - mn) * c);
+            m              = mn;
+            l *= al;
+#pragma unroll
+            for(int b = 0; b < kBlocks; ++b) o[b] *= al;
+        }
+        const float mc = m * c;
+        v8h         p[4];
+#pragma unroll
+        for(int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for(int i = 0; i < 16; i += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[sub][i], c, -mc));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[sub][i + 1], c, -mc));
+                l += p0;
+                l += p1;
+                const v2h h = __builtin_convertvector((v2f{p0, p1}), v2h);
+                p[sub * 2 + i / 8][i % 8]     = h[0];
+                p[sub * 2 + i / 8][i % 8 + 1] = h[1];
+            }
+
+        // 4 keys of channel 32 b + col: keys 16 st + 8 part + 4 half ..
+        auto values = [&](int b, int st) {
+            v8h f;
+#pragma unroll
+            for(int part = 0; part < 2; ++part) {
+                const uint32_t tok = 16 * st + 8 * part + 4 * half + lane % 16 / 4;
+                const uint32_t ch  = 32 * b + lane / 16 % 2 * 16 + lane % 4 * 4;
+                const auto     r   = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h_t*)(uintptr_t)(
+                    vl + tok * D * 2 + value_chunk<D>(tok, ch / 8) * 16 + ch % 8 * 2));
+#pragma unroll
+                for(int i = 0; i < 4; ++i) f[part * 4 + i] = (_Float16)r[i];
+            }
+            return f;
+        };
+#pragma unroll
+        for(int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for(int st = 0; st < 4; ++st) o[b] = mfma(values(b, st), p[st], o[b]);
+
+        if(diag) {
+            // A masked probability is 0, but 0 times an infinity or NaN is not: where
+            // the first product of the wave's rows (the diagonal comes first) is not
+            // finite, take it again without such values and add each of them to
+            // exactly the rows that see it.
+            float z = 0.f;
+#pragma unroll
+            for(int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for(int i = 0; i < 16; ++i) z = fmaf(o[b][i], 0.f, z);
+            if(__ballot(z != 0.f) != 0) {
+#pragma unroll
+                for(int b = 0; b < kBlocks; ++b) {
+                    o[b] = v16f{};
+#pragma unroll
+                    for(int st = 0; st < 4; ++st)
+                        o[b] = mfma(finite_only(values(b, st)), p[st], o[b]);
+                }
+                for(uint32_t tok = 0; tok < kKeys; ++tok) {
+                    if(kt * kKeys + tok > qi) break;
+#pragma unroll
+                    for(int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                        for(int i = 0; i < 16; ++i) {
+                            const uint32_t ch = 32 * b + 8 * (i / 4) + 4 * half + i % 4;
+                            const uint32_t v  = *(const __attribute__((address_space(3)))
+                                                     uint16_t*)(uintptr_t)(
+                                vl + tok * D * 2 + value_chunk<D>(tok, ch / 8) * 16 + ch % 8 * 2);
+                            if(nonfinite(v)) o[b][i] += half_bits_to_float(v);
+                        }
+                }
+            }
+        }
+    }
+
+    const v2f   ls  = both_halves(l);
+    const float inv = 1.f / (ls[0] + ls[1]);
+    if(qi >= span.len) return;
+    uint16_t* out = a.out + (size_t)(span.begin + qi) * a.ldo + head * D;
+#pragma unroll
+    for(int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for(int i = 0; i < 16; i += 4) {
+            v2i w;
+            w[0] = (int)float2_to_half2_bits_2step(o[b][i] * inv, o[b][i + 1] * inv);
+            w[1] = (int)float2_to_half2_bits_2step(o[b][i + 2] * inv, o[b][i + 3] * inv);
+            *reinterpret_cast<v2i*>(out + 32 * b + 8 * (i / 4) + 4 * half) = w;
+        }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 2) attention_kernel(AttentionArgs a)
+{
+    __shared__ alignas(16) uint8_t lds[2 * 2 * kKeys * D * 2]; // two stages of keys, values
+    attention_rows<D>(a, lds);
 }
 
 } // namespace
 
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t stream)
 {
+    // no more tiles than full ones of all rows and one partial per sequence
+    const uint32_t blocks = (a.tokens / kRows + a.seqs) * a.heads;
     if(a.dim == 64)
-        attention_kernel<64><<<a.tokens * a.heads, kWave, 0, stream>>>(a);
+        attention_kernel<64><<<blocks, kThreads, 0, stream>>>(a);
     else
-        attention_kernel<128><<<a.tokens * a.heads, kWave, 0, stream>>>(a);
+        attention_kernel<128><<<blocks, kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 

@@ -589,15 +589,17 @@ int w8a8_moe_combine(const void* y, uint32_t ldy, uint32_t rows_y, const float* 
  *   smooth_scale fp32 [experts, hidden]; smooth_scale_down fp32 [experts, inter] or NULL
  *   w_gate_up    int8 [experts, 2 * inter, hidden], sb_gate_up fp32 [experts, 2 * inter]
  *   w_down       int8 [experts, hidden, inter], sb_down fp32 [experts, hidden]
- * tokens <= W8A8_MOE_DECODE_MAX_TOKENS, tokens * hidden <= 131072, experts <=
- * 4096, topk <= 64; hidden, inter multiples of 16 and <= 32768; x, ldx,
- * smooth scales and weights 16-byte aligned (W8A8_ERROR_NOT_SUPPORTED
- * otherwise: the chain takes more tokens).  workspace: 256-byte aligned,
+ * tokens <= W8A8_MOE_DECODE_MAX_TOKENS, tokens * hidden <=
+ * W8A8_MOE_DECODE_MAX_VALUES (16 tokens of 7168), experts <= 4096, topk <= 64;
+ * hidden, inter multiples of 16 and <= 32768; x, ldx, smooth scales and weights
+ * 16-byte aligned (W8A8_ERROR_NOT_SUPPORTED otherwise: the chain takes more
+ * tokens).  workspace: 256-byte aligned,
  * w8a8_moe_ffn_decode_workspace_size bytes; needs no clearing.  Calls that
  * share a workspace must be ordered on one stream.  Results do not depend on
  * the order in which blocks run.
  */
 #define W8A8_MOE_DECODE_MAX_TOKENS 16
+#define W8A8_MOE_DECODE_MAX_VALUES 114688
 size_t w8a8_moe_ffn_decode_workspace_size(uint32_t tokens, uint32_t topk, uint32_t hidden,
                                           uint32_t inter);
 

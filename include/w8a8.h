@@ -590,7 +590,7 @@ int w8a8_moe_combine(const void* y, uint32_t ldy, uint32_t rows_y, const float* 
  *   w_gate_up    int8 [experts, 2 * inter, hidden], sb_gate_up fp32 [experts, 2 * inter]
  *   w_down       int8 [experts, hidden, inter], sb_down fp32 [experts, hidden]
  * tokens <= W8A8_MOE_DECODE_MAX_TOKENS, tokens * hidden <=
- * W8A8_MOE_DECODE_MAX_VALUES (16 tokens of 7168), experts <= 4096, topk <= 64;
+ * W8A8_MOE_DECODE_MAX_VALUES (16 tokens of 7168), experts <= 4096, topk <= 32;
  * hidden, inter multiples of 16 and <= 32768; x, ldx, smooth scales and weights
  * 16-byte aligned (W8A8_ERROR_NOT_SUPPORTED otherwise: the chain takes more
  * tokens).  workspace: 256-byte aligned,

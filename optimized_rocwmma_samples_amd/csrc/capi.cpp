@@ -932,9 +932,9 @@ int w8a8_moe_ffn_decode(const void* x, const void* logits, int logits_f16,
     if(topk > experts)
         return fail(W8A8_ERROR_INVALID_VALUE, "%s: topk=%u > experts=%u", fn, topk, experts);
     if(tokens > W8A8_MOE_DECODE_MAX_TOKENS || (uint64_t)tokens * hidden > W8A8_MOE_DECODE_MAX_VALUES
-       || experts > 4096 || topk > 64)
+       || experts > 4096 || topk > 32)
         return fail(W8A8_ERROR_NOT_SUPPORTED,
-                    "%s: needs tokens <= %u, tokens * hidden <= %u, experts <= 4096, topk <= 64 "
+                    "%s: needs tokens <= %u, tokens * hidden <= %u, experts <= 4096, topk <= 32 "
                     "(tokens=%u hidden=%u experts=%u topk=%u)",
                     fn, W8A8_MOE_DECODE_MAX_TOKENS, W8A8_MOE_DECODE_MAX_VALUES, tokens, hidden, experts, topk);
     if(hidden % 16 != 0 || inter % 16 != 0 || hidden > 32768 || inter > 32768)

@@ -7,10 +7,12 @@
 // L2, while its first weights are in flight.
 //   * v_mfma_i32_16x16x64_i8 with 16 weight rows as srcA (a lane loads 16
 //     contiguous bytes of one row, a wave-load 64 bytes of 16 rows) and up to 16
-//     quantized rows as srcB, read from LDS.  Sums are int32: exact, so the order
-//     of the waves and blocks changes nothing.
-//   * The 8 waves of a block split K; their int32 partials meet in LDS, one
-//     barrier per 16 x 16 tile (the buffer alternates).
+//     quantized rows as srcB, read from LDS.
+//   * A block's steps along K, over all its tiles or experts, are cut into 8 equal
+//     runs, one per wave; a wave adds its int32 sums to LDS where it leaves a tile.
+//     Integer sums are exact, so no order changes anything, and the stream has no
+//     barrier in it (a barrier per tile cost 1.5 us each: 5 tokens of 64 experts of
+//     2048 x 1408 106 us).
 //   * The activations between the two kernels stay fp32 (a few hundred KB).  A row's
 //     absmax comes from per-block maxima that the first kernel leaves beside them.
 #include "moe_route.hpp"
@@ -28,17 +30,15 @@ constexpr int      kRows      = W8A8_MOE_DECODE_MAX_TOKENS; // rows of an expert
 constexpr int      kTile      = 16;                         // weight rows a tile
 constexpr uint32_t kMaxExpert = 4096;
 constexpr int      kWords     = kMaxExpert / 32;
+constexpr uint32_t kMaxTopk   = 32;
 constexpr int      kBufferFlags  = 0x00020000; // raw buffer, 32-bit data format
 constexpr uint32_t kOob          = 0x80000000u;
 constexpr int      kWeightPolicy = 2; // non-temporal: every weight byte is read once
 
 constexpr uint32_t kGateUpBlocks = 512;        // two blocks a CU
-constexpr uint32_t kDownRows     = 96 * 1024;  // bytes of quantized rows a block of down_kernel holds
 constexpr uint32_t kLdsBytes     = 160 * 1024; // of a CU
 
 static_assert(kRows == 16, "the rows are the columns of one 16 x 16 tile");
-static_assert(W8A8_MOE_DECODE_MAX_VALUES + kRows * 80 + 64 * kRows * 4 + 36 * 1024 <= kLdsBytes,
-              "a block of gate_up_kernel holds every token's row");
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -69,83 +69,76 @@ Ws carve(const MoeDecodeArgs& a)
     return w;
 }
 
-__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v)
-{
-#pragma unroll
-    for(int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, kWave);
-    return v;
-}
+// The active experts (those some token is routed to) in ascending order, each with
+// its pairs (token * topk + slot) in ascending order.  In LDS, sized by the pairs.
+struct Lists {
+    int32_t*  ids;    // [pairs] a pair's expert, or -1
+    int32_t*  order;  // [pairs] its place among the active ones
+    int32_t*  expert; // [active]
+    int32_t*  count;  // [active] pairs
+    uint16_t* pair;   // [active][16]
 
-// The set of experts that some token is routed to, as bits in LDS, and its order.
-struct Active {
-    const uint32_t* bits; // [kWords]
-    int             lane;
-
-    __device__ uint32_t count() const
+    __host__ __device__ static constexpr uint32_t up16(uint32_t pairs)
     {
-        return wave_sum_u32(__popc(bits[2 * lane]) + __popc(bits[2 * lane + 1]));
+        return (pairs * 4 + 15) / 16 * 16;
     }
-    // Active experts below e.
-    __device__ uint32_t rank(uint32_t e) const
+    __host__ __device__ static constexpr uint32_t bytes(uint32_t pairs)
     {
-        uint32_t n = 0;
-#pragma unroll
-        for(int i = 0; i < 2; ++i) {
-            const uint32_t w = 2 * lane + i, b = bits[w];
-            n += w < e / 32 ? __popc(b) : w == e / 32 ? __popc(b & ((1u << (e % 32)) - 1)) : 0;
-        }
-        return wave_sum_u32(n);
+        return 4 * up16(pairs) + pairs * kRows * 2;
     }
-    // The i-th active expert, i < count().
-    __device__ uint32_t expert(uint32_t i) const
+    __device__ Lists(uint8_t* lds, uint32_t pairs)
     {
-        const uint32_t w0 = bits[2 * lane], w1 = bits[2 * lane + 1];
-        const uint32_t n = __popc(w0) + __popc(w1);
-        uint32_t       s = n;
-#pragma unroll
-        for(int d = 1; d < kWave; d <<= 1) {
-            const uint32_t o = __shfl_up(s, d, kWave);
-            if(lane >= d) s += o;
+        const uint32_t n = up16(pairs);
+        ids    = reinterpret_cast<int32_t*>(lds);
+        order  = reinterpret_cast<int32_t*>(lds + n);
+        expert = reinterpret_cast<int32_t*>(lds + 2 * n);
+        count  = reinterpret_cast<int32_t*>(lds + 3 * n);
+        pair   = reinterpret_cast<uint16_t*>(lds + 4 * n);
+    }
+    // From the ids in LDS, by all threads, with `bits` [kWords] and `active` zeroed;
+    // barriers before and after.
+    __device__ void build(uint32_t pairs, uint32_t threads, uint32_t* bits, uint32_t* active)
+    {
+        for(uint32_t p = threadIdx.x; p < pairs; p += threads) {
+            count[p] = 0;
+            if(ids[p] >= 0) atomicOr(&bits[ids[p] / 32], 1u << (ids[p] % 32));
         }
-        const int f = __builtin_ctzll(__ballot(s > i));
-        i -= __builtin_amdgcn_readlane(s, f) - __builtin_amdgcn_readlane(n, f);
-        uint32_t w = __builtin_amdgcn_readlane(w0, f), at = 2 * f;
-        if(i >= (uint32_t)__popc(w)) {
-            i -= __popc(w);
-            w = __builtin_amdgcn_readlane(w1, f);
-            ++at;
+        __syncthreads();
+        for(uint32_t p = threadIdx.x; p < pairs; p += threads) {
+            const int32_t e = ids[p];
+            if(e < 0) continue;
+            uint32_t i = __popc(bits[e / 32] & ((1u << (e % 32)) - 1)), at = 0;
+            for(int32_t w = 0; w < e / 32; ++w) i += __popc(bits[w]);
+#pragma unroll 4
+            for(uint32_t o = 0; o < p; ++o) at += ids[o] == e;
+            order[p]  = (int32_t)i;
+            expert[i] = e;
+            if(at < (uint32_t)kRows) pair[i * kRows + at] = (uint16_t)p;
+            if(at == 0) atomicAdd(active, 1u);
+            atomicAdd(&count[i], 1);
         }
-        for(; i > 0; --i) w &= w - 1;
-        return at * 32 + __builtin_ctz(w);
+        __syncthreads();
+    }
+    __device__ uint32_t expert_at(uint32_t i) const
+    {
+        return (uint32_t)__builtin_amdgcn_readfirstlane(expert[i]);
+    }
+    __device__ uint32_t rows(uint32_t i) const
+    {
+        return (uint32_t)__builtin_amdgcn_readfirstlane(min(count[i], kRows));
     }
 };
-
-// The pairs of expert e in ascending order into list[0 .. count), by one wave.
-__device__ __forceinline__ uint32_t pairs_of(const int32_t* ids, uint32_t pairs, int32_t e,
-                                             int lane, int32_t* list)
-{
-    uint32_t n = 0;
-    for(uint32_t p0 = 0; p0 < pairs; p0 += kWave) {
-        const uint32_t p    = p0 + lane;
-        const bool     mine = p < pairs && ids[p] == e;
-        const uint64_t mask = __ballot(mine);
-        const uint32_t at   = n + __popcll(mask & ((1ull << lane) - 1));
-        if(mine && at < (uint32_t)kRows) list[at] = (int32_t)p;
-        n += __popcll(mask);
-    }
-    return min(n, (uint32_t)kRows);
-}
 
 // The columns of all active experts' activations, in tiles of 16, are cut into one
 // contiguous range per block of gate_up_kernel.
 __device__ __forceinline__ uint32_t first_unit(uint32_t block, uint32_t units, uint32_t blocks)
 {
-    return (uint32_t)((uint64_t)block * units / blocks);
+    return block * units / blocks; // units <= 1024 * 2048, blocks <= 512
 }
 
 __device__ __forceinline__ uint32_t block_of(uint32_t unit, uint32_t units, uint32_t blocks)
 {
-    return (uint32_t)((((uint64_t)unit + 1) * blocks - 1) / units);
+    return ((unit + 1) * blocks - 1) / units;
 }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t weight_rows(const int8_t* w, uint32_t k)
@@ -165,29 +158,48 @@ __device__ __forceinline__ v4i mfma(v4i a, v4i b, v4i c)
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-// A wave's share of a row of K: its steps of 64 among `steps`.
-struct Share {
+// A wave's run of `total` batches, and a place in it: batch b of item `item`, `per`
+// batches an item.
+struct Run {
     uint32_t from, to;
-    __device__ Share(uint32_t steps, uint32_t wave)
-        : from(steps * wave / kWaves), to(steps * (wave + 1) / kWaves)
+    __device__ Run(uint32_t total, uint32_t wave)
+        : from(total * wave / kWaves), to(total * (wave + 1) / kWaves)
     {
     }
-    __device__ uint32_t batches(uint32_t per) const { return max(1u, (to - from + per - 1) / per); }
+};
+
+struct Cursor {
+    uint32_t item, b;
+    __device__ Cursor(uint32_t at, uint32_t per) : item(at / per), b(at % per) {}
+    __device__ void advance(uint32_t per)
+    {
+        if(++b == per) {
+            b = 0;
+            ++item;
+        }
+    }
 };
 
 // ---------------------------------------------------------------------------
-// First kernel
+// First kernel: a block owns a range of 16-column tiles of the activations.
 // ---------------------------------------------------------------------------
-constexpr int kGuSteps = 4; // steps a batch: 4 KB of gate rows and 4 KB of up rows a wave
+constexpr int      kGuSteps = 2; // steps a batch: 2 KB of gate rows and 2 KB of up rows a wave
+constexpr int      kGuRing  = 4; // batches in registers, three of them in flight
+constexpr uint32_t kGroup   = 8; // tiles whose sums lie in LDS at a time
 
 struct GateUpLds {
-    v4i      part[2][kWaves][2][kWave];
+    int32_t  acc[kGroup][2][kRows][kTile]; // [tile][gate, up][row][column]
     float    amax[kRows][kWaves];
     float    scale[kRows];
-    float    top[4][kRows];
+    uint32_t top[kRows]; // float bits, >= 0
     uint32_t bits[kWords];
-    int32_t  list[kRows];
+    uint32_t active;
 };
+
+static_assert(W8A8_MOE_DECODE_MAX_VALUES + kRows * 80 + Lists::bytes(kRows * kMaxTopk)
+                      + sizeof(GateUpLds)
+                  <= kLdsBytes,
+              "a block of gate_up_kernel holds every token's row");
 
 template <bool F16>
 __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, GateUpLds& lds,
@@ -196,18 +208,19 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, Ga
     const int      wave  = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int      lane  = threadIdx.x % kWave, col = lane % 16, kg = lane / 16;
     const uint32_t pairs = a.tokens * a.topk, tid = threadIdx.x;
-    int32_t*       ids = reinterpret_cast<int32_t*>(dyn);
-    int8_t*        q   = reinterpret_cast<int8_t*>(dyn + (pairs * 4 + 15) / 16 * 16);
-    const uint32_t rb  = row_bytes(a.hidden);
+    Lists          lists(dyn, pairs);
+    int8_t*        q  = reinterpret_cast<int8_t*>(dyn + Lists::bytes(pairs));
+    const uint32_t rb = row_bytes(a.hidden);
 
     // ---- routing: a wave per token -----------------------------------------------
     if(tid < kWords) lds.bits[tid] = 0;
+    if(tid == 0) lds.active = 0;
     for(uint32_t t = wave; t < a.tokens; t += kWaves)
         route_token(
             [&](uint32_t e) { return load_logit<F16>(a.logits, (size_t)t * a.experts + e); },
             a.experts, a.topk, lane, [&](uint32_t k, int id, float w) {
                 if(lane == 0) {
-                    ids[t * a.topk + k] = id;
+                    lists.ids[t * a.topk + k] = id;
                     if(blockIdx.x == 0) {
                         ws.ids[t * a.topk + k]    = id;
                         ws.weight[t * a.topk + k] = w;
@@ -215,156 +228,178 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, Ga
                 }
             });
     __syncthreads();
-    for(uint32_t p = tid; p < pairs; p += kThreads)
-        if(ids[p] >= 0) atomicOr(&lds.bits[ids[p] / 32], 1u << (ids[p] % 32));
-    __syncthreads();
-    const Active   active{lds.bits, lane};
-    const uint32_t tiles = a.inter / kTile, units = active.count() * tiles;
+    lists.build(pairs, kThreads, lds.bits, &lds.active);
+    const uint32_t tiles = a.inter / kTile, units = lds.active * tiles;
     const uint32_t from  = first_unit(blockIdx.x, units, gridDim.x);
     const uint32_t to    = first_unit(blockIdx.x + 1, units, gridDim.x);
+    const uint32_t steps = (a.hidden + 63) / 64, per = (steps + kGuSteps - 1) / kGuSteps;
 
-    const uint32_t steps = (a.hidden + 63) / 64;
-    const Share    share(steps, wave);
-    const uint32_t batches = share.batches(kGuSteps);
+    uint32_t held = ~0u; // the expert whose rows are in LDS
+    for(uint32_t u0 = from; u0 < to;) { // tiles u0 .. u1 of one expert
+        const uint32_t ai = u0 / tiles, u1 = min(min(to, (ai + 1) * tiles), u0 + kGroup);
+        const uint32_t e = lists.expert_at(ai), rows = lists.rows(ai);
+        const size_t   row0 = (size_t)e * 2 * a.inter + (u0 - ai * tiles) * kTile;
+        const uint16_t* list = lists.pair + ai * kRows;
 
-    for(uint32_t u0 = from; u0 < to;) { // one expert's part of the block's range
-        const uint32_t ai = u0 / tiles, u1 = min(to, (ai + 1) * tiles);
-        const uint32_t e = active.expert(ai);
-        const size_t   rows0 = (size_t)e * 2 * a.inter;
-
-        v4i  ring[2][2][kGuSteps];
-        auto load = [&](int slot, uint32_t at) { // batch `at` of the range, for this wave
-            const uint32_t j0 = (u0 + at / batches - ai * tiles) * kTile;
-            const uint32_t s0 = share.from + at % batches * kGuSteps;
-            const __amdgpu_buffer_rsrc_t rg = weight_rows(a.wgu + (rows0 + j0) * a.hidden, a.hidden);
-            const __amdgpu_buffer_rsrc_t ru
-                = weight_rows(a.wgu + (rows0 + a.inter + j0) * a.hidden, a.hidden);
+        // ---- the first of the expert's rows, ahead of the weights ----------------
+        const float* s     = a.s + (size_t)e * a.hidden;
+        const bool   fresh = held != e;
+        auto         row_x = [&](uint32_t r) {
+            return a.x + (size_t)(list[min(r, rows - 1)] / a.topk) * a.ldx;
+        };
+        v4i h[4] = {};
+        v4f s0 = {}, s1 = {};
+        auto fetch = [&](uint32_t r0, uint32_t k) {
+            if(k < a.hidden) {
+                s0 = *reinterpret_cast<const v4f*>(s + k);
+                s1 = *reinterpret_cast<const v4f*>(s + k + 4);
 #pragma unroll
-            for(int i = 0; i < kGuSteps; ++i) {
-                const uint32_t off
-                    = s0 + i < share.to ? col * a.hidden + (s0 + i) * 64 + kg * 16 : kOob;
-                ring[slot][0][i] = load_weights(rg, off);
-                ring[slot][1][i] = load_weights(ru, off);
+                for(int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const v4i*>(row_x(r0 + i) + k);
+            } else {
+                s0 = s1 = v4f{0, 0, 0, 0};
+#pragma unroll
+                for(int i = 0; i < 4; ++i) h[i] = v4i{0, 0, 0, 0};
             }
         };
-        const uint32_t total = (u1 - u0) * batches;
-        load(0, 0);
+        if(fresh) fetch(0, tid * 8);
 
-        // ---- the expert's rows, quantized into LDS ------------------------------
-        __syncthreads(); // the rows and the list of the expert before are done with
-        const uint32_t rows = pairs_of(ids, pairs, (int32_t)e, lane, lds.list);
-        const float*   s    = a.s + (size_t)e * a.hidden;
-        for(uint32_t r = 0; r < rows; ++r) {
-            const uint16_t* x = a.x + (size_t)(lds.list[r] / a.topk) * a.ldx;
-            float           m = 0.f;
-            for(uint32_t k = tid * 8; k < a.hidden; k += kThreads * 8) {
-                const v4i h  = *reinterpret_cast<const v4i*>(x + k);
-                const v4f s0 = *reinterpret_cast<const v4f*>(s + k);
-                const v4f s1 = *reinterpret_cast<const v4f*>(s + k + 4);
+        // ---- the stream of weights ----------------------------------------------
+        const Run run((u1 - u0) * per, wave);
+        v4i       ring[kGuRing][2][kGuSteps];
+        Cursor    ahead(run.from, per), now = ahead;
+        uint32_t  at   = run.from;
+        auto      load = [&](int slot) {
+            const size_t                 row = row0 + ahead.item * kTile;
+            const __amdgpu_buffer_rsrc_t rg = weight_rows(a.wgu + row * a.hidden, a.hidden);
+            const __amdgpu_buffer_rsrc_t ru
+                = weight_rows(a.wgu + (row + a.inter) * a.hidden, a.hidden);
+#pragma unroll
+            for(int i = 0; i < kGuSteps; ++i) {
+                const uint32_t st  = ahead.b * kGuSteps + i;
+                const uint32_t off = st < steps ? col * a.hidden + st * 64 + kg * 16 : kOob;
+                ring[slot][0][i]   = load_weights(rg, off);
+                ring[slot][1][i]   = load_weights(ru, off);
+            }
+            ahead.advance(per);
+            ++at;
+        };
+#pragma unroll
+        for(int i = 0; i < kGuRing - 1; ++i)
+            if(at < run.to) load(i);
+
+        __syncthreads(); // the sums and rows before are done with
+        for(uint32_t i = tid; i < sizeof(lds.acc) / 16; i += kThreads)
+            reinterpret_cast<v4i*>(lds.acc)[i] = v4i{0, 0, 0, 0};
+        if(tid < (uint32_t)kRows && fresh) lds.top[tid] = 0;
+        // ---- the expert's rows, quantized into LDS: four rows at a time, so that
+        // their loads overlap ------------------------------------------------------
+        if(fresh) {
+            auto product = [&](int i, int c) {
+                const float f = c < 4 ? s0[c] : s1[c - 4];
+                return c % 2 ? mul_h16_f32<true>((uint32_t)h[i][c / 2], f)
+                             : mul_h16_f32<false>((uint32_t)h[i][c / 2], f);
+            };
+            const bool once = rows <= 4 && rb - 16 <= kThreads * 8; // they stay in registers
+            for(uint32_t r0 = 0; r0 < rows; r0 += 4) {
+                float m[4] = {};
+                for(uint32_t k = tid * 8; k < rb - 16; k += kThreads * 8) {
+                    if(r0 > 0 || k != tid * 8) fetch(r0, k);
+#pragma unroll
+                    for(int i = 0; i < 4; ++i)
+#pragma unroll
+                        for(int c = 0; c < 8; ++c) m[i] = fmaxf(m[i], fabsf(product(i, c)));
+                }
 #pragma unroll
                 for(int i = 0; i < 4; ++i) {
-                    const float sa = i < 2 ? s0[2 * i] : s1[2 * i - 4];
-                    const float sb = i < 2 ? s0[2 * i + 1] : s1[2 * i - 3];
-                    m = fmaxf(m, fabsf(mul_h16_f32<false>((uint32_t)h[i], sa)));
-                    m = fmaxf(m, fabsf(mul_h16_f32<true>((uint32_t)h[i], sb)));
+                    m[i] = wave_max(m[i]);
+                    if(lane == 0) lds.amax[r0 + i][wave] = m[i];
                 }
             }
-            m = wave_max(m);
-            if(lane == 0) lds.amax[r][wave] = m;
-        }
-        __syncthreads();
-        for(uint32_t r = 0; r < rows; ++r) {
-            float m = lds.amax[r][0];
+            __syncthreads();
+            for(uint32_t r0 = 0; r0 < rows; r0 += 4) {
+                float inv[4];
 #pragma unroll
-            for(int w = 1; w < kWaves; ++w) m = fmaxf(m, lds.amax[r][w]);
-            const float scale = m / a.qmax;
-            const float inv   = scale > 0.f ? 1.f / scale : 0.f;
-            if(tid == 0) lds.scale[r] = scale;
-            const uint16_t* x = a.x + (size_t)(lds.list[r] / a.topk) * a.ldx;
-            for(uint32_t k = tid * 8; k < rb - 16; k += kThreads * 8) {
-                v2i w = {0, 0};
-                if(k < a.hidden) {
-                    const v4i h  = *reinterpret_cast<const v4i*>(x + k);
-                    const v4f s0 = *reinterpret_cast<const v4f*>(s + k);
-                    const v4f s1 = *reinterpret_cast<const v4f*>(s + k + 4);
-                    float     f[8];
+                for(int i = 0; i < 4; ++i) {
+                    float m = lds.amax[r0 + i][0];
+#pragma unroll
+                    for(int w = 1; w < kWaves; ++w) m = fmaxf(m, lds.amax[r0 + i][w]);
+                    const float scale = m / a.qmax;
+                    inv[i]            = scale > 0.f ? 1.f / scale : 0.f;
+                    if(tid == 0) lds.scale[r0 + i] = scale;
+                }
+                for(uint32_t k = tid * 8; k < rb - 16; k += kThreads * 8) {
+                    if(!once) fetch(r0, k);
 #pragma unroll
                     for(int i = 0; i < 4; ++i) {
-                        const float sa = i < 2 ? s0[2 * i] : s1[2 * i - 4];
-                        const float sb = i < 2 ? s0[2 * i + 1] : s1[2 * i - 3];
-                        f[2 * i] = quant_f(mul_h16_f32<false>((uint32_t)h[i], sa), inv, a.qmax);
-                        f[2 * i + 1] = quant_f(mul_h16_f32<true>((uint32_t)h[i], sb), inv, a.qmax);
+                        float g[8];
+#pragma unroll
+                        for(int c = 0; c < 8; ++c) g[c] = quant_f(product(i, c), inv[i], a.qmax);
+                        const v2i w = {(int)cvt_pack4_i8(g[0], g[1], g[2], g[3]),
+                                       (int)cvt_pack4_i8(g[4], g[5], g[6], g[7])};
+                        if(r0 + i < rows) *reinterpret_cast<v2i*>(q + (r0 + i) * rb + k) = w;
                     }
-                    w[0] = (int)cvt_pack4_i8(f[0], f[1], f[2], f[3]);
-                    w[1] = (int)cvt_pack4_i8(f[4], f[5], f[6], f[7]);
                 }
-                *reinterpret_cast<v2i*>(q + r * rb + k) = w;
             }
+            held = e;
         }
         __syncthreads();
 
         // ---- the products -------------------------------------------------------
         const int8_t* qrow = q + min((uint32_t)col, rows - 1) * rb + kg * 16;
-        // the epilogue's place: waves 0..3, lane = (row lane / 4, column 4 wave + lane % 4)
-        const uint32_t er = lane / 4, ej = 4 * (wave % 4) + lane % 4;
-        const bool     epilogue = wave < 4 && er < rows;
-        const int32_t  epair    = epilogue ? lds.list[er] : 0;
-        const float    escale   = epilogue ? lds.scale[er] : 0.f;
-        float          top = 0.f, sg = 0.f, su = 0.f, s2 = 1.f;
-        v4i            acc[2] = {};
-        auto process = [&](int slot, uint32_t at) {
-            const uint32_t unit = u0 + at / batches, b = at % batches;
-            const uint32_t j = (unit - ai * tiles) * kTile + ej;
-            if(b == 0) {
-                acc[0] = acc[1] = v4i{0, 0, 0, 0};
-                if(epilogue) {
-                    sg = a.sgu[rows0 + j];
-                    su = a.sgu[rows0 + a.inter + j];
-                    if(a.s2) s2 = a.s2[(size_t)e * a.inter + j];
+        v4i           acc[2] = {};
+        for(uint32_t done = run.from; done < run.to;) {
+#pragma unroll
+            for(int slot = 0; slot < kGuRing; ++slot) {
+                if(at < run.to) load((slot + kGuRing - 1) % kGuRing);
+                if(done < run.to) {
+#pragma unroll
+                    for(int i = 0; i < kGuSteps; ++i) {
+                        const uint32_t st = min(now.b * kGuSteps + i, steps - 1);
+                        const v4i      x  = *reinterpret_cast<const v4i*>(qrow + st * 64);
+                        acc[0]            = mfma(ring[slot][0][i], x, acc[0]);
+                        acc[1]            = mfma(ring[slot][1][i], x, acc[1]);
+                    }
+                    ++done;
+                    if(now.b == per - 1 || done == run.to) {
+                        if((uint32_t)col < rows)
+#pragma unroll
+                            for(int w = 0; w < 2; ++w)
+#pragma unroll
+                                for(int i = 0; i < 4; ++i)
+                                    atomicAdd(&lds.acc[now.item][w][col][4 * kg + i], acc[w][i]);
+                        acc[0] = acc[1] = v4i{0, 0, 0, 0};
+                    }
+                    now.advance(per);
                 }
             }
-#pragma unroll
-            for(int i = 0; i < kGuSteps; ++i) {
-                const uint32_t st = min(share.from + b * kGuSteps + i, steps - 1);
-                const v4i      x  = *reinterpret_cast<const v4i*>(qrow + st * 64);
-                acc[0]            = mfma(ring[slot][0][i], x, acc[0]);
-                acc[1]            = mfma(ring[slot][1][i], x, acc[1]);
-            }
-            if(b + 1 < batches) return;
-            v4i(*part)[2][kWave]  = lds.part[unit % 2];
-            part[wave][0][lane] = acc[0];
-            part[wave][1][lane] = acc[1];
-            __syncthreads();
-            if(!epilogue) return;
-            int g = 0, u = 0;
-#pragma unroll
-            for(int w = 0; w < kWaves; ++w) {
-                g += reinterpret_cast<const int*>(part[w][0])[(wave * 16 + er) * 4 + lane % 4];
-                u += reinterpret_cast<const int*>(part[w][1])[(wave * 16 + er) * 4 + lane % 4];
-            }
-            const float h = silu_mul(((float)g * escale) * sg, ((float)u * escale) * su)
-                            * s2;
-            ws.act[(size_t)epair * a.inter + j] = h;
-            top                                 = fmaxf(top, fabsf(h));
-        };
-        for(uint32_t at = 0; at < total; at += 2) {
-            if(at + 1 < total) load(1, at + 1);
-            process(0, at);
-            if(at + 1 < total) {
-                if(at + 2 < total) load(0, at + 2);
-                process(1, at + 1);
-            }
-        }
-        if(epilogue) {
-            top = fmaxf(top, dpp_mov<kDppQuadXor1>(top));
-            top = fmaxf(top, dpp_mov<kDppQuadXor2>(top));
-            if(lane % 4 == 0) lds.top[wave][er] = top;
         }
         __syncthreads();
-        if(tid < rows)
-            ws.top[(size_t)lds.list[tid] * kGateUpBlocks + blockIdx.x] = fmaxf(
-                fmaxf(lds.top[0][tid], lds.top[1][tid]), fmaxf(lds.top[2][tid], lds.top[3][tid]));
+
+        // ---- SiLU(gate) * up: 16 threads a row of a tile ---------------------------
+        for(uint32_t i = tid; i < (u1 - u0) * rows * kTile; i += kThreads) {
+            const uint32_t j = i % kTile, r = i / kTile % rows, u = i / kTile / rows;
+            const uint32_t c = (u0 - ai * tiles + u) * kTile + j;
+            const float    rs = lds.scale[r];
+            const float    g
+                = ((float)lds.acc[u][0][r][j] * rs) * a.sgu[(size_t)e * 2 * a.inter + c];
+            const float v
+                = ((float)lds.acc[u][1][r][j] * rs) * a.sgu[(size_t)e * 2 * a.inter + a.inter + c];
+            float f = silu_mul(g, v);
+            if(a.s2) f *= a.s2[(size_t)e * a.inter + c];
+            ws.act[(size_t)list[r] * a.inter + c] = f;
+            f                                     = fabsf(f);
+            f = fmaxf(f, dpp_mov<kDppQuadXor1>(f));
+            f = fmaxf(f, dpp_mov<kDppQuadXor2>(f));
+            f = fmaxf(f, dpp_mov<kDppRowHalfMirror>(f));
+            f = fmaxf(f, dpp_mov<kDppRowMirror>(f));
+            if(j == 0 && f > 0.f) atomicMax(&lds.top[r], __float_as_uint(f));
+        }
         u0 = u1;
+        if(u0 == to || u0 == (ai + 1) * tiles) { // the expert's last tiles here
+            __syncthreads();
+            if(tid < rows)
+                ws.top[(size_t)list[tid] * kGateUpBlocks + blockIdx.x] = __uint_as_float(lds.top[tid]);
+        }
     }
 }
 
@@ -377,86 +412,54 @@ __global__ void __launch_bounds__(kThreads, 4) gate_up_kernel(MoeDecodeArgs a, W
 }
 
 // ---------------------------------------------------------------------------
-// Second kernel: a block owns 16 output columns of all active experts.
+// Second kernel: a block owns 16 / FOLD output columns of all active experts.
+// FOLD > 1 (at most 16 / FOLD tokens): the tile's 16 weight rows are the columns'
+// FOLD parts along K, and its 16 columns the rows' parts likewise; the blocks on the
+// tile's diagonal are the partial sums, the others are not used.  So a small hidden
+// size still gives a block to every CU, with whole 16-byte loads.
+//
+// ALL: the quantized rows of all pairs lie in LDS.  Otherwise one expert's rows over
+// `chunk` columns, in two buffers: 8 more waves quantize the next while 8 multiply.
 // ---------------------------------------------------------------------------
-constexpr int kDownSteps = 8; // steps a batch: 8 KB a wave
+constexpr int kDownSteps = 4; // steps a batch: 4 KB a wave
+constexpr int kDownRing  = 4; // batches in registers, three of them in flight
 
 struct DownLds {
-    v4i      part[2][kWaves][kWave];
     uint32_t bits[kWords];
-    int32_t  list[2][kWaves][kRows];
+    uint32_t active;
 };
 
-// How the quantized rows lie in LDS: all pairs' whole rows at once (chunk = inter), or
-// one expert's rows over `chunk` columns at a time.
-struct DownPlan {
-    uint32_t chunk;
-    bool     all;
-};
-
-__device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, const DownPlan& plan,
+template <int FOLD, bool ALL>
+__device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint32_t chunk,
                                      uint32_t gu_blocks, DownLds& lds, uint8_t* dyn)
 {
+    constexpr uint32_t kCols = kTile / FOLD, kAll = ALL ? kThreads : 2 * kThreads;
     const int      wave  = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int      lane  = threadIdx.x % kWave, col = lane % 16, kg = lane / 16;
     const uint32_t pairs = a.tokens * a.topk, tid = threadIdx.x;
-    const uint32_t up16  = (pairs * 4 + 15) / 16 * 16;
-    int32_t*       ids   = reinterpret_cast<int32_t*>(dyn);
-    float*         scale = reinterpret_cast<float*>(dyn + up16);
-    float*         y     = reinterpret_cast<float*>(dyn + 2 * up16); // [pairs][16]
-    int8_t*        q     = reinterpret_cast<int8_t*>(dyn + 2 * up16 + pairs * kTile * 4);
-    const uint32_t j0 = blockIdx.x * kTile, rb = row_bytes(plan.chunk);
+    Lists          lists(dyn, pairs);
+    uint8_t*       at0   = dyn + Lists::bytes(pairs);
+    float*         scale = reinterpret_cast<float*>(at0);
+    int32_t*       sums  = reinterpret_cast<int32_t*>(at0 + Lists::up16(pairs)); // [pairs][kCols]
+    int8_t* q = reinterpret_cast<int8_t*>(at0 + Lists::up16(pairs) + pairs * kTile * 4);
+    const uint32_t j0 = blockIdx.x * kCols, rb = row_bytes(chunk);
+    const uint32_t tiles = a.inter / kTile;
 
-    if(tid < kWords) lds.bits[tid] = 0;
-    for(uint32_t p = tid; p < pairs; p += kThreads) ids[p] = ws.ids[p];
+    for(uint32_t i = tid; i < (uint32_t)kWords; i += kAll) lds.bits[i] = 0;
+    if(tid == 0) lds.active = 0;
+    for(uint32_t p = tid; p < pairs; p += kAll) lists.ids[p] = ws.ids[p];
+    for(uint32_t i = tid; i < pairs * kCols; i += kAll) sums[i] = 0;
     __syncthreads();
-    for(uint32_t p = tid; p < pairs; p += kThreads)
-        if(ids[p] >= 0) atomicOr(&lds.bits[ids[p] / 32], 1u << (ids[p] % 32));
-    __syncthreads();
-    const Active   active{lds.bits, lane};
-    const uint32_t n = active.count(), tiles = a.inter / kTile, units = n * tiles;
-    const uint32_t chunks = (a.inter + plan.chunk - 1) / plan.chunk;
-
-    // ---- the stream of weights: (expert, chunk, batch), one batch ahead ------------
-    struct Cursor {
-        uint32_t ai, ci, b, e;
-    };
-    auto steps_of = [&](uint32_t ci) {
-        return (min(plan.chunk, a.inter - ci * plan.chunk) + 63) / 64;
-    };
-    auto advance = [&](Cursor& c) {
-        if(++c.b < Share(steps_of(c.ci), wave).batches(kDownSteps)) return;
-        c.b = 0;
-        if(++c.ci < chunks) return;
-        c.ci = 0;
-        if(++c.ai < n) c.e = active.expert(c.ai);
-    };
-    v4i  ring[2][kDownSteps];
-    auto load = [&](int slot, const Cursor& c) {
-        const Share                  share(steps_of(c.ci), wave);
-        const __amdgpu_buffer_rsrc_t r
-            = weight_rows(a.wd + ((size_t)c.e * a.hidden + j0) * a.inter, a.inter);
-        const uint32_t s0 = share.from + c.b * kDownSteps;
-#pragma unroll
-        for(int i = 0; i < kDownSteps; ++i)
-            ring[slot][i] = load_weights(r, s0 + i < share.to ? col * a.inter + c.ci * plan.chunk
-                                                                    + (s0 + i) * 64 + kg * 16
-                                                              : kOob);
-    };
-    Cursor now{0, 0, 0, n > 0 ? active.expert(0) : 0}, ahead = now;
-    if(n > 0) {
-        load(0, ahead);
-        advance(ahead);
-    }
+    lists.build(pairs, kAll, lds.bits, &lds.active);
+    const uint32_t n = lds.active, units = n * tiles;
 
     // ---- the pairs' scales, from the maxima that the first kernel's blocks left -----
-    for(uint32_t p = wave; p < pairs; p += kWaves) {
+    for(uint32_t p = wave; p < pairs; p += kAll / kWave) {
         float m = 0.f;
-        if(ids[p] >= 0) {
-            const uint32_t ai = active.rank(ids[p]);
-            const uint32_t b0 = block_of(ai * tiles, units, gu_blocks);
-            const uint32_t b1 = block_of(ai * tiles + tiles - 1, units, gu_blocks);
-            for(uint32_t b = b0 + lane; b <= b1; b += kWave)
+        if(lists.ids[p] >= 0) {
+            const uint32_t u  = lists.order[p] * tiles;
+            const uint32_t b1 = block_of(u + tiles - 1, units, gu_blocks);
+            for(uint32_t b = block_of(u, units, gu_blocks) + lane; b <= b1; b += kWave)
                 if(first_unit(b, units, gu_blocks) < first_unit(b + 1, units, gu_blocks))
                     m = fmaxf(m, ws.top[(size_t)p * kGateUpBlocks + b]); // it had work
             m = wave_max(m);
@@ -465,12 +468,12 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, const
     }
     __syncthreads();
 
-    // 16 columns a thread from k0 + 16 i on of one pair's row, to LDS row `row`
-    auto quantize = [&](uint32_t p, uint32_t row, uint32_t k0, uint32_t i) {
-        const float  inv = scale[p] > 0.f ? 1.f / scale[p] : 0.f;
-        const float* h   = ws.act + (size_t)p * a.inter + k0 + 16 * i;
-        v4i          w   = {0, 0, 0, 0};
-        if(k0 + 16 * i < a.inter) {
+    // 16 columns from k on of one pair's activations, to LDS
+    auto quantize = [&](uint32_t p, uint32_t k, int8_t* to) {
+        const float inv = scale[p] > 0.f ? 1.f / scale[p] : 0.f;
+        v4i         w   = {0, 0, 0, 0};
+        if(k < a.inter) {
+            const float* h = ws.act + (size_t)p * a.inter + k;
 #pragma unroll
             for(int c = 0; c < 4; ++c) {
                 const v4f f = *reinterpret_cast<const v4f*>(h + 4 * c);
@@ -478,92 +481,179 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, const
                                          quant_f(f[2], inv, a.qmax), quant_f(f[3], inv, a.qmax));
             }
         }
-        *reinterpret_cast<v4i*>(q + row * rb + 16 * i) = w;
+        *reinterpret_cast<v4i*>(to) = w;
     };
-    const uint32_t per_row = (rb - 16) / 16;
-    if(plan.all) {
-        for(uint32_t i = tid; i < pairs * per_row; i += kThreads)
-            if(ids[i / per_row] >= 0) quantize(i / per_row, i / per_row, 0, i % per_row);
-        __syncthreads();
-    }
+    const uint32_t per_row = (rb - 16) / 16; // 16-column pieces of a row in LDS
+    const uint32_t chunks  = ALL ? 1 : (a.inter + chunk - 1) / chunk;
+    auto           fill    = [&](uint32_t phase, uint32_t from) { // by kThreads threads
+        const uint32_t ai = phase / chunks, k0 = phase % chunks * chunk;
+        const uint32_t rows = lists.rows(ai);
+        int8_t*        to   = q + phase % 2 * a.tokens * rb;
+        for(uint32_t i = from; i < rows * per_row; i += kThreads)
+            quantize(lists.pair[ai * kRows + i / per_row], k0 + i % per_row * 16,
+                     to + i / per_row * rb + i % per_row * 16);
+    };
 
-    v4i           acc  = {};
-    uint32_t      rows = 0;
-    const int8_t* qrow = q;
-    float         sd   = 0.f;
-    // the epilogue's place: waves 0..3, lane = (row lane / 4, column 4 wave + lane % 4)
-    const uint32_t er = lane / 4, ej = 4 * (wave % 4) + lane % 4;
-    auto process = [&](int slot) {
-        if(now.b == 0) {
-            if(now.ci == 0) { // another expert
-                acc  = v4i{0, 0, 0, 0};
-                rows = pairs_of(ids, pairs, (int32_t)now.e, lane, lds.list[now.ai % 2][wave]);
-                sd   = a.sd[(size_t)now.e * a.hidden + j0 + ej];
-            }
-            const int32_t* list = lds.list[now.ai % 2][wave];
-            const uint32_t mine = min((uint32_t)col, rows - 1);
-            if(!plan.all) {
-                __syncthreads(); // the rows before are done with
-                for(uint32_t i = tid; i < rows * per_row; i += kThreads)
-                    quantize(list[i / per_row], i / per_row, now.ci * plan.chunk, i % per_row);
-                __syncthreads();
-            }
-            qrow = q + (plan.all ? list[mine] : mine) * rb + kg * 16;
+    // ---- the stream of weights: items are experts (ALL) or (expert, chunk) -----------
+    const uint32_t most = (ALL ? a.inter : min(chunk, a.inter)) + 63;
+    const uint32_t part = (most / 64 + FOLD - 1) / FOLD; // steps of a part of an item's K
+    const uint32_t per  = (part + kDownSteps - 1) / kDownSteps;
+    const uint32_t items = n * chunks;
+    // one run over all items, or one within every item
+    const Run run(ALL ? items * per : per, wave % kWaves);
+    const bool     streams = ALL || wave < kWaves;
+    const uint32_t mine    = streams ? (ALL ? run.to - run.from : (run.to - run.from) * items) : 0;
+    v4i            ring[kDownRing][kDownSteps];
+    Cursor         ahead(ALL ? run.from : 0, per), now = ahead;
+    if(!ALL) ahead.b = now.b = run.from;
+    auto advance = [&](Cursor& c) {
+        if(ALL)
+            c.advance(per);
+        else if(++c.b == run.to) {
+            c.b = run.from;
+            ++c.item;
         }
-        const uint32_t steps = steps_of(now.ci);
-        const Share    share(steps, wave);
+    };
+    const uint32_t row = col % kCols, fold = col / kCols; // of the weights, and of the tokens
+    uint32_t       loaded = 0;
+    auto           load   = [&](int slot) {
+        const uint32_t               e = lists.expert_at(ahead.item / chunks);
+        const uint32_t               k0 = ahead.item % chunks * chunk;
+        const __amdgpu_buffer_rsrc_t r  = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<int8_t*>(a.wd + ((size_t)e * a.hidden + j0) * a.inter), 0,
+            (int)(kCols * a.inter), kBufferFlags);
 #pragma unroll
         for(int i = 0; i < kDownSteps; ++i) {
-            const uint32_t st = min(share.from + now.b * kDownSteps + i, steps - 1);
-            acc = mfma(ring[slot][i], *reinterpret_cast<const v4i*>(qrow + st * 64), acc);
+            const uint32_t st = ahead.b * kDownSteps + i, k = k0 + (fold * part + st) * 64 + kg * 16;
+            const bool     in = st < part && k < a.inter && (ALL || k < k0 + chunk);
+            ring[slot][i]     = load_weights(r, in ? row * a.inter + k : kOob);
         }
-        const Cursor done = now;
-        advance(now);
-        if(now.ai == done.ai) return;
-        v4i(*part)[kWave] = lds.part[done.ai % 2];
-        part[wave][lane]  = acc;
-        __syncthreads();
-        if(wave >= 4 || er >= rows) return;
-        const int32_t p   = lds.list[done.ai % 2][wave][er];
-        int           sum = 0;
-#pragma unroll
-        for(int w = 0; w < kWaves; ++w)
-            sum += reinterpret_cast<const int*>(part[w])[(wave * 16 + er) * 4 + lane % 4];
-        y[p * kTile + ej] = ((float)sum * scale[p]) * sd;
+        advance(ahead);
+        ++loaded;
     };
-    while(now.ai < n) {
-        if(ahead.ai < n) {
-            load(1, ahead);
-            advance(ahead);
+#pragma unroll
+    for(int i = 0; i < kDownRing - 1; ++i)
+        if(loaded < mine) load(i);
+
+    if constexpr(ALL) {
+        for(uint32_t i = tid; i < pairs * per_row; i += kThreads)
+            if(lists.ids[i / per_row] >= 0)
+                quantize(i / per_row, i % per_row * 16, q + i / per_row * rb + i % per_row * 16);
+    } else if(!streams && n > 0)
+        fill(0, tid - kThreads);
+    __syncthreads();
+
+    if(!streams) {
+        for(uint32_t item = 0; item < items; ++item) {
+            if(item + 1 < items) fill(item + 1, tid - kThreads);
+            __syncthreads();
         }
-        process(0);
-        if(now.ai >= n) break;
-        if(ahead.ai < n) {
-            load(0, ahead);
-            advance(ahead);
+    } else {
+        v4i           acc  = {};
+        uint32_t      done = 0, rows = 0;
+        const int8_t* qrow = q;
+        bool          fresh = true;
+        uint32_t      phase = 0; // items this wave has left behind
+        auto          leave = [&]() { // barriers at the end of an item
+            __syncthreads();
+            ++phase;
+        };
+        auto flush = [&](uint32_t ai) {
+            if(row < rows && (uint32_t)(4 * kg) / kCols == fold) {
+                int32_t* to = sums + lists.pair[ai * kRows + row] * kCols;
+#pragma unroll
+                for(int i = 0; i < 4; ++i) atomicAdd(&to[(4 * kg + i) % kCols], acc[i]);
+            }
+            acc = v4i{0, 0, 0, 0};
+        };
+        while(done < mine) {
+#pragma unroll
+            for(int slot = 0; slot < kDownRing; ++slot) {
+                if(loaded < mine) load((slot + kDownRing - 1) % kDownRing);
+                if(done < mine) {
+                    const uint32_t ai = now.item / chunks;
+                    if(fresh) {
+                        rows                = lists.rows(ai);
+                        const uint32_t r    = min(row, rows - 1);
+                        const uint32_t from = ALL ? lists.pair[ai * kRows + r]
+                                                  : now.item % 2 * a.tokens + r;
+                        qrow                = q + from * rb + kg * 16;
+                        fresh               = false;
+                    }
+#pragma unroll
+                    for(int i = 0; i < kDownSteps; ++i) {
+                        // a step past the part or the row has zero weights: any of them will do
+                        const uint32_t st
+                            = min(fold * part + now.b * kDownSteps + i, (rb - 16) / 64 - 1);
+                        acc = mfma(ring[slot][i], *reinterpret_cast<const v4i*>(qrow + st * 64), acc);
+                    }
+                    ++done;
+                    const uint32_t item = now.item;
+                    advance(now);
+                    if(now.item != item || done == mine) {
+                        fresh = true;
+                        if(ALL || now.item / chunks != ai) flush(ai);
+                        if(!ALL) leave();
+                    }
+                }
+            }
         }
-        process(1);
+        if(!ALL)
+            while(phase < items) leave(); // a wave without a batch of an item
     }
     __syncthreads();
 
     // ---- the weighted sum over a token's slots -------------------------------------
-    for(uint32_t i = tid; i < a.tokens * kTile; i += kThreads) {
-        const uint32_t t = i / kTile, j = i % kTile;
+    for(uint32_t i = tid; i < a.tokens * kCols; i += kAll) {
+        const uint32_t t = i / kCols, j = i % kCols;
         float          out = 0.f;
         for(uint32_t s = 0; s < a.topk; ++s) {
             const uint32_t p = t * a.topk + s;
-            if(ids[p] >= 0) out = fmaf(ws.weight[p], y[p * kTile + j], out);
+            const int32_t  e = lists.ids[p];
+            if(e < 0) continue;
+            const float y = ((float)sums[p * kCols + j] * scale[p]) * a.sd[(size_t)e * a.hidden + j0 + j];
+            out           = fmaf(ws.weight[p], y, out);
         }
         a.out[(size_t)t * a.ldo + j0 + j] = float_to_half_bits(out);
     }
 }
 
-__global__ void __launch_bounds__(kThreads, 4)
-    down_kernel(MoeDecodeArgs a, Ws ws, DownPlan plan, uint32_t gu_blocks)
+template <int FOLD, bool ALL>
+__global__ void __launch_bounds__(ALL ? kThreads : 2 * kThreads, 4)
+    down_kernel(MoeDecodeArgs a, Ws ws, uint32_t chunk, uint32_t gu_blocks)
 {
     extern __shared__ uint8_t dyn[];
     __shared__ DownLds        lds;
-    down(a, ws, plan, gu_blocks, lds, dyn);
+    down<FOLD, ALL>(a, ws, chunk, gu_blocks, lds, dyn);
+}
+
+template <class K>
+void allow_lds(K kernel, uint32_t bytes)
+{
+    if(bytes + 32 * 1024 > 64 * 1024) // with the static part
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+template <int FOLD>
+hipError_t launch_down(const MoeDecodeArgs& a, const Ws& ws, uint32_t gu_blocks, hipStream_t stream)
+{
+    const uint32_t pairs = a.tokens * a.topk, grid = a.hidden / (kTile / FOLD);
+    const uint32_t fixed = Lists::bytes(pairs) + Lists::up16(pairs) + pairs * kTile * 4;
+    const uint32_t room  = kLdsBytes - (uint32_t)sizeof(DownLds) - fixed;
+    // all rows, where two blocks still share a CU or one does with no second to come
+    if((uint64_t)pairs * row_bytes(a.inter) <= std::min<uint32_t>(room, 100 * 1024)) {
+        const uint32_t lds = fixed + pairs * row_bytes(a.inter);
+        allow_lds(down_kernel<FOLD, true>, lds);
+        down_kernel<FOLD, true><<<grid, kThreads, lds, stream>>>(a, ws, a.inter, gu_blocks);
+    } else {
+        const uint32_t chunk
+            = std::min((a.inter + 63) / 64 * 64, (room / (2 * a.tokens) - 16) / 512 * 512);
+        const uint32_t lds = fixed + 2 * a.tokens * row_bytes(chunk);
+        allow_lds(down_kernel<FOLD, false>, lds);
+        down_kernel<FOLD, false><<<grid, 2 * kThreads, lds, stream>>>(a, ws, chunk, gu_blocks);
+    }
+    return hipGetLastError();
 }
 
 } // namespace
@@ -574,41 +664,24 @@ size_t moe_ffn_decode_workspace_bytes(uint32_t tokens, uint32_t topk, uint32_t h
     return up256(n * inter * 4) + up256(n * kGateUpBlocks * 4) + 2 * up256(n * 4);
 }
 
-namespace {
-template <class K>
-void allow_lds(K kernel, uint32_t bytes)
-{
-    if(bytes > 32 * 1024) // beside the static part
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
-} // namespace
-
 hipError_t launch_moe_ffn_decode(const MoeDecodeArgs& a, bool f16, hipStream_t stream)
 {
     const Ws       ws    = carve(a);
-    const uint32_t pairs = a.tokens * a.topk, up16 = (pairs * 4 + 15) / 16 * 16;
-    const uint32_t used   = std::min(pairs, a.experts);
-    const uint32_t blocks = std::min(kGateUpBlocks, used * (a.inter / kTile));
-    const uint32_t gu_lds = up16 + a.tokens * row_bytes(a.hidden);
+    const uint32_t pairs = a.tokens * a.topk;
+    const uint32_t lds   = Lists::bytes(pairs) + a.tokens * row_bytes(a.hidden);
+    // as many blocks as are resident at once
+    const uint32_t resident = lds + sizeof(GateUpLds) <= kLdsBytes / 2 ? kGateUpBlocks : kGateUpBlocks / 2;
+    const uint32_t blocks = std::min(resident, std::min(pairs, a.experts) * (a.inter / kTile));
     const auto     gu     = f16 ? gate_up_kernel<true> : gate_up_kernel<false>;
-    allow_lds(gu, gu_lds);
-    gu<<<blocks, kThreads, gu_lds, stream>>>(a, ws);
-    hipError_t e = hipGetLastError();
+    allow_lds(gu, lds);
+    gu<<<blocks, kThreads, lds, stream>>>(a, ws);
+    const hipError_t e = hipGetLastError();
     if(e != hipSuccess) return e;
-
-    const uint32_t fixed = 2 * up16 + pairs * kTile * 4;
-    const uint32_t rows
-        = std::min<uint32_t>(kDownRows, kLdsBytes - (uint32_t)sizeof(DownLds) - fixed);
-    DownPlan plan{a.inter, true};
-    if((uint64_t)pairs * row_bytes(a.inter) > rows) {
-        plan.all   = false;
-        plan.chunk = std::min(a.inter, (rows / a.tokens - 16) / 512 * 512);
-    }
-    const uint32_t down_lds = fixed + (plan.all ? pairs : a.tokens) * row_bytes(plan.chunk);
-    allow_lds(down_kernel, down_lds);
-    down_kernel<<<a.hidden / kTile, kThreads, down_lds, stream>>>(a, ws, plan, blocks);
-    return hipGetLastError();
+    // a block for every CU, where the tokens leave room in the tile
+    const uint32_t columns = a.hidden / kTile;
+    if(columns < 128 && a.tokens <= 4) return launch_down<4>(a, ws, blocks, stream);
+    if(columns < 256 && a.tokens <= 8) return launch_down<2>(a, ws, blocks, stream);
+    return launch_down<1>(a, ws, blocks, stream);
 }
 
 } // namespace w8a8

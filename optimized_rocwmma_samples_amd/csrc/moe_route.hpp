@@ -31,17 +31,38 @@ __device__ __forceinline__ void better(float& v, int& i, float ov, int oi)
 // Experts are chosen on the logits (softmax is monotonic, so the choice is
 // exact), the lower index winning ties; weight = exp(l - max) * (1 / sum_e
 // exp(l_e - max)).  logit(e): the fp32 value of expert e's logit.  A lane owns
-// experts lane, lane + 64, ...: experts <= 4096 (the bits of `used`).
-template <class Logit, class Emit>
-__device__ __forceinline__ void route_token(Logit logit, uint32_t experts, uint32_t topk, int lane,
-                                            Emit emit)
+// experts lane, lane + 64, ...: experts <= 4096 (the bits of `used`).  HELD > 0:
+// they are read once into that many registers (experts <= 64 * HELD), instead of
+// again for every pick.
+template <int HELD, class Logit, class Emit>
+__device__ __forceinline__ void route_token_held(Logit logit, uint32_t experts, uint32_t topk,
+                                                 int lane, Emit emit)
 {
+    float held[HELD > 0 ? HELD : 1];
+    // each(f): f(j, expert, its logit) over the lane's experts in ascending order
+    auto each = [&](auto f) {
+        if constexpr(HELD > 0) {
+#pragma unroll
+            for(int j = 0; j < HELD; ++j) {
+                const uint32_t e = lane + j * kWave;
+                if(e < experts) f(j, e, held[j]);
+            }
+        } else {
+            int j = 0;
+            for(uint32_t e = lane; e < experts; e += kWave, ++j) f(j, e, logit(e));
+        }
+    };
+    if constexpr(HELD > 0)
+#pragma unroll
+        for(int j = 0; j < HELD; ++j)
+            held[j] = lane + j * kWave < experts ? logit(lane + j * kWave) : 0.f;
+
     // cross-lane steps are DPP reductions (no LDS round trips)
     float wmax = -INFINITY;
-    for(uint32_t e = lane; e < experts; e += kWave) wmax = fmaxf(wmax, logit(e));
+    each([&](int, uint32_t, float v) { wmax = fmaxf(wmax, v); });
     wmax       = wave_max(wmax);
     float wsum = 0.f;
-    for(uint32_t e = lane; e < experts; e += kWave) wsum += expf(logit(e) - wmax);
+    each([&](int, uint32_t, float v) { wsum += expf(v - wmax); });
     wsum            = wave_sum(wsum);
     const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
 
@@ -54,15 +75,27 @@ __device__ __forceinline__ void route_token(Logit logit, uint32_t experts, uint3
     for(uint32_t k = 0; k < topk; ++k) {
         float bv = -INFINITY;
         int   bi = kNone;
-        int   j  = 0;
-        for(uint32_t e = lane; e < experts; e += kWave, ++j)
-            if(!((used >> j) & 1u)) better(bv, bi, logit(e), (int)e);
+        each([&](int j, uint32_t e, float v) {
+            if(!((used >> j) & 1u)) better(bv, bi, v, (int)e);
+        });
         const float m = wave_max(bv);
         const int   w = wave_min_i32(bv == m ? bi : kNone);
         if(w != kNone && (uint32_t)w % kWave == (uint32_t)lane) used |= 1ull << ((uint32_t)w / kWave);
         const bool ok = w != kNone;
         emit(k, ok ? w : -1, ok ? expf(m - wmax) * inv : 0.f);
     }
+}
+
+template <class Logit, class Emit>
+__device__ __forceinline__ void route_token(Logit logit, uint32_t experts, uint32_t topk, int lane,
+                                            Emit emit)
+{
+    if(experts <= kWave)
+        route_token_held<1>(logit, experts, topk, lane, emit);
+    else if(experts <= 4 * kWave)
+        route_token_held<4>(logit, experts, topk, lane, emit);
+    else
+        route_token_held<0>(logit, experts, topk, lane, emit);
 }
 
 } // namespace w8a8

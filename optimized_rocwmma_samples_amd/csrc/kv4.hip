@@ -239,16 +239,35 @@ __device__ __forceinline__ void load_lds(const void* base, uint32_t to, uint32_t
 }
 #pragma clang diagnostic pop
 
-// The 8 codes of a dword as fp16 1 + n / 16, in the order 0 4 1 5 2 6 3 7.
-__device__ __forceinline__ v8h unpack(uint32_t w)
+// The 8 codes of a dword as fp16 1 + n / 16, in the order 0 4 1 5 2 6 3 7: a shift
+// and a v_and_or_b32 a pair.  The constants come in registers, which that
+// instruction needs on gfx950 and the compiler does not arrange by itself.
+struct Unpack {
+    uint32_t mask, one;
+    __device__ Unpack()
+    {
+        asm volatile("v_mov_b32 %0, 0x03c003c0" : "=v"(mask));
+        asm volatile("v_mov_b32 %0, 0x3c003c00" : "=v"(one));
+    }
+    __device__ v8h operator()(uint32_t w) const
+    {
+        v4i u;
+        u[0] = (int)(((w << 6) & mask) | one);
+        u[1] = (int)(((w << 2) & mask) | one);
+        u[2] = (int)(((w >> 2) & mask) | one);
+        u[3] = (int)(((w >> 6) & mask) | one);
+        return __builtin_bit_cast(v8h, u);
+    }
+};
+
+// fp16(p0 * s0) and fp16(p1 * s1), s the low halves of w0 and w1, as a packed pair:
+// each product rounded once, in one instruction.
+__device__ __forceinline__ uint32_t scaled_pair(float p0, uint32_t w0, float p1, uint32_t w1)
 {
-    constexpr uint32_t kMask = 0x03C003C0u, kOne = 0x3C003C00u;
-    v4i                u;
-    u[0] = (int)(((w << 6) & kMask) | kOne);
-    u[1] = (int)(((w << 2) & kMask) | kOne);
-    u[2] = (int)(((w >> 2) & kMask) | kOne);
-    u[3] = (int)(((w >> 6) & kMask) | kOne);
-    return __builtin_bit_cast(v8h, u);
+    uint32_t r;
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(p0), "v"(w0));
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "+v"(r) : "v"(p1), "v"(w1));
+    return r;
 }
 
 __device__ __forceinline__ v4f mfma16(v8h a, v8h b, v4f c)
@@ -357,8 +376,9 @@ __device__ __forceinline__ void attention_kv4_piece(const CacheView& c, const At
     const uint32_t vr = lane / kRowChunks, vp = lane % kRowChunks;
     const uint32_t voff = vr * (D / 2) + (vp ^ (D == 128 ? vr / 4 % 4 : vr / 8 % 2)) * 16;
 
-    float m = -INFINITY, l = 0.f;
-    int   shift = 0; // p s is held times 2^shift
+    const Unpack unpack;
+    float        m = -INFINITY, l = 0.f;
+    int          shift = 0; // p s is held times 2^shift
     v4f   o[kTiles] = {}, total[kNG] = {};
     float osum[kNG] = {};
 
@@ -444,29 +464,26 @@ __device__ __forceinline__ void attention_kv4_piece(const CacheView& c, const At
                     }
                 }
             }
-            uint32_t dead = 0; // the lane's tokens that are not there
-            if(!full) {
+            if(!full) { // tokens that are not there: no score, and no scales (what lies there
+                        // may be NaN)
 #pragma unroll
-                for(int r = 0; r < 16; ++r) {
-                    const uint32_t t = t0 + 16 * (r / 4) + 4 * kg + r % 4;
-                    if(t >= end || !((live >> (r / 4)) & 1u)) {
-                        dead |= 1u << r;
+                for(int r = 0; r < 16; ++r)
+                    if(t0 + 16 * (r / 4) + 4 * kg + r % 4 >= end || !((live >> (r / 4)) & 1u))
                         s[r] = -INFINITY;
-                    }
-                }
+                if(t0 + lane >= end || !((live >> (lane / 16)) & 1u))
+#pragma unroll
+                    for(int g = 0; g < kNG; ++g)
+                        *(lds_u32_t*)(uintptr_t)(at + L::kCodes + L::kScales + (lane * kNG + g) * 4)
+                            = 0;
             }
 
             // ---- the largest scale of the values, and with it the power of two -----
             float big = 0.f;
-            {
-                const uint32_t t = t0 + lane;
-                if(t < end && ((live >> (lane / 16)) & 1u))
 #pragma unroll
-                    for(int g = 0; g < kNG; ++g)
-                        big = fmaxf(big, fabsf(low_half(*(const lds_u32_t*)(uintptr_t)(
-                                             at + L::kCodes + L::kScales + lane * kNG * 4 + g * 4))));
-                big = wave_max(big);
-            }
+            for(int g = 0; g < kNG; ++g)
+                big = fmaxf(big, fabsf(low_half(*(const lds_u32_t*)(uintptr_t)(
+                                     at + L::kCodes + L::kScales + (lane * kNG + g) * 4))));
+            big = wave_max(big);
             float       rescale = 1.f;
             const float now     = ldexpf(big, shift);
             if(big > 0.f && big <= 65504.f && (now < 1.f || now > 64.f)) {
@@ -492,40 +509,49 @@ __device__ __forceinline__ void attention_kv4_piece(const CacheView& c, const At
 #pragma unroll
                 for(int t = 0; t < kTiles; ++t) o[t] *= al * rescale;
             }
-            const float mc = m * c2;
+            const float mc = m == -INFINITY ? 0.f : m * c2; // no token yet: every p is 0
             float       p[16];
 #pragma unroll
             for(int r = 0; r < 16; ++r) {
                 p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -mc));
-                if((dead >> r) & 1u) p[r] = 0.f;
                 l += p[r];
             }
 
             // ---- p times the values' scales, as the operand, group by group --------
             const float pow2 = ldexpf(1.f, shift);
-            v8h         ps[kNG][2];
+            uint32_t    ps[kNG][2][4];
 #pragma unroll
-            for(int i = 0; i < 4; ++i) {
-                v4i sv[kNG];
+            for(int u = 0; u < 2; ++u) { // tiles 2 u and 2 u + 1
+                v4i sv[2][kNG];
 #pragma unroll
-                for(int g = 0; g < kNG; ++g)
-                    sv[g] = *(const lds_v4i_t*)(uintptr_t)(at + L::kCodes + L::kScales
-                                                           + (16 * i + 4 * kg) * kNG * 4 + g * 16);
+                for(int i = 0; i < 2; ++i)
 #pragma unroll
-                for(int j = 0; j < 4; ++j)
+                    for(int g = 0; g < kNG; ++g)
+                        sv[i][g] = *(const lds_v4i_t*)(uintptr_t)(
+                            at + L::kCodes + L::kScales + (32 * u + 16 * i + 4 * kg) * kNG * 4
+                            + g * 16);
+#pragma unroll
+                for(int j = 0; j < 4; ++j) {
+                    const float p0 = p[8 * u + j], p1 = p[8 * u + 4 + j];
+                    const float x0 = p0 * pow2, x1 = p1 * pow2;
 #pragma unroll
                     for(int g = 0; g < kNG; ++g) {
-                        uint32_t w = (uint32_t)sv[(j * kNG + g) / 4][(j * kNG + g) % 4];
-                        if((dead >> (4 * i + j)) & 1u) w = 0; // what lies there may be NaN
-                        osum[g] = fmaf(p[4 * i + j], high_half(w), osum[g]);
-                        ps[g][i / 2][2 * j + i % 2] = (_Float16)(p[4 * i + j] * pow2 * low_half(w));
+                        const uint32_t w0 = (uint32_t)sv[0][(j * kNG + g) / 4][(j * kNG + g) % 4];
+                        const uint32_t w1 = (uint32_t)sv[1][(j * kNG + g) / 4][(j * kNG + g) % 4];
+                        osum[g]     = fmaf(p0, high_half(w0), fmaf(p1, high_half(w1), osum[g]));
+                        ps[g][u][j] = scaled_pair(x0, w0, x1, w1);
                     }
+                }
             }
+            auto operand = [&](int g, int u) {
+                return __builtin_bit_cast(
+                    v8h, v4i{(int)ps[g][u][0], (int)ps[g][u][1], (int)ps[g][u][2], (int)ps[g][u][3]});
+            };
             const v8h ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
             for(int g = 0; g < kNG; ++g)
 #pragma unroll
-                for(int u = 0; u < 2; ++u) total[g] = mfma16(ones, ps[g][u], total[g]);
+                for(int u = 0; u < 2; ++u) total[g] = mfma16(ones, operand(g, u), total[g]);
 
             // ---- values: channel 16 t + col, tokens of source lanes 16 (j / 4) + 4 kg + j % 4
 #pragma unroll
@@ -536,7 +562,7 @@ __device__ __forceinline__ void attention_kv4_piece(const CacheView& c, const At
                     at + tok * (D / 2) + ((t / 2) ^ f) * 16 + t % 2 * 8));
 #pragma unroll
                 for(int u = 0; u < 2; ++u)
-                    o[t] = mfma16(unpack((uint32_t)w[u]), ps[t * 16 / G][u], o[t]);
+                    o[t] = mfma16(unpack((uint32_t)w[u]), operand(t * 16 / G, u), o[t]);
             }
         }
     }
@@ -591,7 +617,7 @@ __device__ __forceinline__ void attention_kv4_piece(const CacheView& c, const At
 }
 
 template <int D, int G>
-__global__ void __launch_bounds__(kAttThreads)
+__global__ void __launch_bounds__(kAttThreads, 2)
     attention_kv4_kernel(CacheView c, AttentionKv4Args a, Pieces pieces, uint32_t pages)
 {
     __shared__ alignas(16) uint8_t lds[KvLds<D, G>::kBytes];
@@ -599,27 +625,50 @@ __global__ void __launch_bounds__(kAttThreads)
     attention_kv4_piece<D, G>(c, a, pieces, pages, lds, page_of);
 }
 
-// Joins the pieces of one (sequence, head), in their order: one thread a channel.
+// Joins the pieces of one (sequence, head): their factors first, then the threads of
+// each channel take every kJoin-th piece, and add up in a fixed order.
+constexpr int kJoinThreads = 512, kJoinPieces = 256; // pieces whose factors lie in LDS at a time
+
 template <int D>
-__global__ void __launch_bounds__(D)
+__global__ void __launch_bounds__(kJoinThreads)
     attention_kv4_join_kernel(CacheView c, AttentionKv4Args a, Pieces pieces)
 {
-    const uint32_t head = blockIdx.x, seq = blockIdx.y, ch = threadIdx.x;
-    const uint32_t most = a.table_cols * c.page_size;
-    const uint32_t len  = (uint32_t)max(0, (int)min((int64_t)a.lens[seq], (int64_t)most));
-    const uint32_t n    = (len + pieces.tokens - 1) / pieces.tokens;
-    const size_t   at   = ((size_t)seq * a.heads + head) * pieces.count;
-    float          m    = -INFINITY;
-    for(uint32_t i = 0; i < n; ++i) m = fmaxf(m, pieces.ml[(at + i) * 2]);
+    constexpr int    kJoin = kJoinThreads / D;
+    __shared__ float factor[kJoinPieces];
+    __shared__ float part[kJoin][D + 1];
+    const uint32_t   head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
+    const uint32_t   ch = tid % D, way = tid / D;
+    const uint32_t   most = a.table_cols * c.page_size;
+    const uint32_t   len  = (uint32_t)max(0, (int)min((int64_t)a.lens[seq], (int64_t)most));
+    const uint32_t   n    = (len + pieces.tokens - 1) / pieces.tokens;
+    const size_t     at   = ((size_t)seq * a.heads + head) * pieces.count;
+    const float*     ml   = pieces.ml + at * 2;
+    float            m    = -INFINITY; // of all pieces, in every wave
+    for(uint32_t i = tid % kWave; i < n; i += kWave) m = fmaxf(m, ml[i * 2]);
+    m         = wave_max(m);
     float sum = 0.f, l = 0.f;
-    for(uint32_t i = 0; i < n; ++i) {
-        const float li = pieces.ml[(at + i) * 2 + 1];
-        const float f  = li != 0.f ? __builtin_amdgcn_exp2f(pieces.ml[(at + i) * 2] - m) : 0.f;
-        if(li != 0.f) {
-            sum = fmaf(f, pieces.o[(at + i) * D + ch], sum);
-            l   = fmaf(f, li, l);
+    for(uint32_t i0 = 0; i0 < n; i0 += kJoinPieces) {
+        const uint32_t here = min(n - i0, (uint32_t)kJoinPieces);
+        __syncthreads();
+        if(tid < here) {
+            const float li = ml[(i0 + tid) * 2 + 1]; // 0: no token seen, its maximum may be -inf
+            factor[tid]    = li != 0.f ? __builtin_amdgcn_exp2f(ml[(i0 + tid) * 2] - m) : 0.f;
+        }
+        __syncthreads();
+#pragma unroll 8
+        for(uint32_t i = way; i < here; i += kJoin) {
+            const float f = factor[i];
+            sum           = fmaf(f, pieces.o[(at + i0 + i) * D + ch], sum);
+            l             = fmaf(f, ml[(i0 + i) * 2 + 1], l);
         }
     }
+    part[way][ch] = sum;
+    if(ch == 0) part[way][D] = l;
+    __syncthreads();
+    if(way != 0) return;
+    for(int w = 1; w < kJoin; ++w) sum += part[w][ch];
+    l = 0.f;
+    for(int w = 0; w < kJoin; ++w) l += part[w][D];
     a.out[(size_t)seq * a.ldo + (size_t)head * D + ch] = float_to_half_bits(l != 0.f ? sum / l : 0.f);
 }
 
@@ -687,7 +736,7 @@ hipError_t launch_attention_kv4(const w8a8_kv4_cache& c, const AttentionKv4Args&
             <<<grid, kAttThreads, 0, stream>>>(view(c), a, pieces, c.pages);
         if(pieces.count > 1)
             attention_kv4_join_kernel<d()>
-                <<<dim3(a.heads, a.seqs), d(), 0, stream>>>(view(c), a, pieces);
+                <<<dim3(a.heads, a.seqs), kJoinThreads, 0, stream>>>(view(c), a, pieces);
     });
     return hipGetLastError();
 }

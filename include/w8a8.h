@@ -705,10 +705,11 @@ int w8a8_kv4_load(void* k, void* v, const int32_t* slots, uint32_t tokens, uint3
  * statistics and sums are fp32, and p * scale of a value is rounded to fp16 as
  * the second product's operand.
  * workspace: 16-byte aligned, w8a8_attention_kv4_workspace_size(seqs, heads,
- * kv_heads, head_dim, table_cols * page_size) bytes, needs no clearing: long
- * contexts are cut into pieces that run side by side, and a second launch joins
- * them in order.  Without one (NULL, or smaller) a sequence's head is one
- * block's work.  Calls that share a workspace must be ordered on one stream.
+ * kv_heads, head_dim, table_cols * page_size) bytes, needs no clearing: the
+ * work of all sequences is cut into equal runs, one a wave, and a second launch
+ * joins what was cut in order.  Without one (NULL, or smaller) all of a key
+ * head's context is one wave's work.  Calls that share a workspace must be
+ * ordered on one stream.
  * 16-byte aligned q, out, ldq and ldo multiples of 8.
  */
 size_t w8a8_attention_kv4_workspace_size(uint32_t seqs, uint32_t heads, uint32_t kv_heads,

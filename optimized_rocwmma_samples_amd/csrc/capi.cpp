@@ -1081,6 +1081,10 @@ int w8a8_attention_kv4(const void* q, const w8a8_kv4_cache* cache, const int32_t
        || (uint64_t)seqs * heads > 0xFFFFFFull)
         return fail(W8A8_ERROR_NOT_SUPPORTED,
                     "%s: needs table_cols * page_size < 2^31 and seqs * heads < 2^24", fn);
+    // the chunks of 64 tokens of all sequences are counted in 31 bits
+    if(((uint64_t)table_cols * cache->page_size / 64 + 1) * seqs * heads > 0x7FFFFFFFull)
+        return fail(W8A8_ERROR_NOT_SUPPORTED,
+                    "%s: needs seqs * heads * (table_cols * page_size / 64 + 1) < 2^31", fn);
     if(!aligned(workspace, 16))
         return fail(W8A8_ERROR_INVALID_VALUE, "%s: workspace must be 16-byte aligned", fn);
     w8a8::AttentionKv4Args a{static_cast<const uint16_t*>(q),

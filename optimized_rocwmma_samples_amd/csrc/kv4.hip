@@ -182,10 +182,14 @@ uint32_t row_blocks(const w8a8_kv4_cache& c, const Kv4Rows& r)
 // ---------------------------------------------------------------------------
 // Attention of single tokens over the cache.
 //
-// A block owns a piece of one sequence's context for the (up to 16) query heads of
-// one key head; its waves take chunks of 64 tokens in turn, each with its own
-// running maximum and sum, and merge at the end.  Both products run on
-// v_mfma_f32_16x16x32_f16 with the query heads as columns:
+// The chunks of 64 tokens of all (sequence, key head) units lie in one line, which is
+// cut into as many equal runs as there are waves; every wave works through its run by
+// itself, its next chunk on the way while it computes.  A unit inside one run is
+// written out; of one cut by runs each wave leaves a partial (its sum of p v, maximum
+// and sum of p), and a second launch joins them in order.  So any mix of lengths
+// keeps the chip evenly busy.  (Blocks that owned a piece of one sequence spent 10 of
+// their 18 us on starting, the first load and merging: 16 x 8192 tokens 42 us.)
+// Both products run on v_mfma_f32_16x16x32_f16 with the query heads as columns:
 //   S^T = K q^T    srcA rows = tokens.  A lane takes 16 (8) bytes of one token's
 //                  codes; dword j is its operand of step j, channels 32 j + 8 kg +
 //                  0..7 (kg = lane / 16), which is the cache's order of keys.
@@ -199,10 +203,17 @@ uint32_t row_blocks(const w8a8_kv4_cache& c, const Kv4Rows& r)
 // per-lane fp32 factors,
 //   q . k    = sum over groups of 16 s (sum_c q_c (x_c - 1.5)) + o (sum_c q_c)
 //   (p v)_c  = 16 (sum_t (p s)_t x_c,t - 1.5 sum_t (p s)_t) + sum_t (p o)_t
-// (the -1.5 makes x the centred code; in S^T it is the accumulator's start, in O^T
+// (the -1.5 makes x the centred code; in O^T with
 // the sum over the tokens of the rounded p s, from a matrix product with ones, so
 // that rounding p s to fp16, the only rounding below fp32, acts on the centred
 // code).  p s is brought to fp16's range by a power of two that follows the scales.
+//
+// With few query heads per key head most of the 16 columns would hold nothing, and
+// the work on scores, which is per column, would be done for nothing.  So C = 4 or 2
+// copies of 4 or 8 heads fill them, copy (class) a for every C-th of the chunk's four
+// 16-token tiles: the tile's product takes a q^T whose other classes are zero, and the
+// products of C tiles add up in one accumulator.  A column is then a partial of its
+// own, with its own maximum, sum and part of the result, merged at the unit's end.
 // ---------------------------------------------------------------------------
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -212,32 +223,11 @@ typedef __attribute__((address_space(3))) v2i      lds_v2i_t;
 typedef __attribute__((address_space(3))) v4i      lds_v4i_t;
 typedef __attribute__((address_space(3))) uint32_t lds_u32_t;
 
-constexpr int kAttWaves   = 4;
-constexpr int kAttThreads = kAttWaves * kWave;
-constexpr int kChunk      = 64;   // tokens a wave takes at a time
-constexpr int kSegment    = 4096; // tokens whose page numbers lie in LDS at a time
-constexpr int kCols       = 16;   // query heads a block takes
-
-// `size` 16 or 4 bytes a lane from base + offset into LDS, lane i to `to` + size * i,
-// with the caller's own wait (the builtin makes the compiler wait for every such
-// load ahead of each transposed read).
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm" // m0 is reserved: set and used here alone
-template <int SIZE>
-__device__ __forceinline__ void load_lds(const void* base, uint32_t to, uint32_t offset)
-{
-    if constexpr(SIZE == 16)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                     :
-                     : "s"(to), "v"(offset), "s"(base)
-                     : "memory", "m0");
-    else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
-                     :
-                     : "s"(to), "v"(offset), "s"(base)
-                     : "memory", "m0");
-}
-#pragma clang diagnostic pop
+constexpr int      kAttWaves   = 4;
+constexpr int      kAttThreads = kAttWaves * kWave;
+constexpr uint32_t kAttBlocks  = 512; // two a CU, all resident: 2 waves a SIMD by registers
+constexpr int      kChunk      = 64;  // tokens a wave takes at a time
+constexpr int      kCols       = 16;  // columns of a product: classes x query heads
 
 // The 8 codes of a dword as fp16 1 + n / 16, in the order 0 4 1 5 2 6 3 7: a shift
 // and a v_and_or_b32 a pair.  The constants come in registers, which that
@@ -260,14 +250,18 @@ struct Unpack {
     }
 };
 
-// fp16(p0 * s0) and fp16(p1 * s1), s the low halves of w0 and w1, as a packed pair:
-// each product rounded once, in one instruction.
-__device__ __forceinline__ uint32_t scaled_pair(float p0, uint32_t w0, float p1, uint32_t w1)
+// fp16(p * s), s the low half of w, into the low half (the high half undefined) or the
+// high half of a register: the product rounded once, in one instruction.
+__device__ __forceinline__ uint32_t scaled_low(float p, uint32_t w)
 {
     uint32_t r;
-    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(p0), "v"(w0));
-    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "+v"(r) : "v"(p1), "v"(w1));
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(p), "v"(w));
     return r;
+}
+
+__device__ __forceinline__ void scaled_high(uint32_t& r, float p, uint32_t w)
+{
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "+v"(r) : "v"(p), "v"(w));
 }
 
 __device__ __forceinline__ v4f mfma16(v8h a, v8h b, v4f c)
@@ -301,392 +295,595 @@ __device__ __forceinline__ float column_sum(float v)
 __device__ __forceinline__ float low_half(uint32_t w) { return half_bits_to_float(w & 0xFFFFu); }
 __device__ __forceinline__ float high_half(uint32_t w) { return half_bits_to_float(w >> 16); }
 
-// Pieces a sequence's context is cut into, and where they leave their results:
-// per (sequence, head) and piece the sum of p v (fp32 [D]), the maximum in powers
-// of two and the sum of p.
-struct Pieces {
-    uint32_t count, tokens;
-    float*   o;
-    float*   ml;
+// How the launch is cut: `waves` runs over all chunks, or (whole) over all units.
+// Partials: slot 2 w + 0 of wave w holds a unit that began before its run, 2 w + 1 one
+// that begins in it and goes on behind it: per head the sum of p v (fp32 [D]), then
+// all slots' (maximum in powers of two, sum of p); then per wave what goes on behind
+// it: (unit + 1, the last wave of it) or (0, 0).
+struct Cut {
+    uint32_t  waves, heads; // heads: query heads of a unit
+    bool      whole;
+    float*    o;
+    float*    ml;
+    uint32_t* next;
 };
+
+__host__ __device__ inline uint32_t chunks_of(uint32_t len)
+{
+    return len == 0 ? 1u : (len + kChunk - 1) / kChunk; // a sequence of no tokens is written too
+}
 
 template <int D, int G>
 struct KvLds {
     static constexpr int kGroups = D / G;
-    static constexpr int kCodes  = kChunk * D / 2;        // bytes of a chunk's value codes
-    static constexpr int kScales = kChunk * kGroups * 4;  // bytes of its (scale, offset) pairs
-    static constexpr int kStage  = kCodes + 2 * kScales;  // value codes, key scales, value scales
-    static constexpr int kRing   = kAttWaves * 2 * kStage;
-    static constexpr int kMerge  = kAttWaves * kCols * (D + 2) * 4;
-    static constexpr int kBytes  = kRing > kMerge ? kRing : kMerge;
+    static constexpr int kCodes  = kChunk * D / 2;       // bytes of a chunk's value codes
+    static constexpr int kScales = kChunk * kGroups * 4; // bytes of its (scale, offset) pairs
+    static constexpr int kWave   = kCodes + 2 * kScales; // value codes, key scales, value scales
 };
 
-template <int D, int G>
-__device__ __forceinline__ void attention_kv4_piece(const CacheView& c, const AttentionKv4Args& a,
-                                                    const Pieces& pieces, uint32_t pages,
-                                                    uint8_t* lds, int32_t* page_of)
+// A chunk on its way: key codes as the product takes them, value codes as they go to
+// LDS, and lane = token the (scale, offset) pairs.
+template <int NG>
+struct Chunk {
+    v4i      k[4], v[4];
+    int32_t  ks[NG], vs[NG];
+    uint32_t ok; // which of its 16-token tiles have a page
+};
+
+// A chunk's place: sequence, unit of it, chunk of the unit (all wave-uniform).
+struct Place {
+    uint32_t seq, unit, chunk, chunks, len;
+};
+
+// N dwords, N = 1, 2 or 4, from global memory or to LDS in one access.
+template <int N>
+__device__ __forceinline__ void load_dwords(int32_t* r, const void* p)
+{
+    if constexpr(N == 4) {
+        const v4i u = *static_cast<const v4i*>(p);
+#pragma unroll
+        for(int i = 0; i < 4; ++i) r[i] = u[i];
+    } else if constexpr(N == 2) {
+        const v2i u = *static_cast<const v2i*>(p);
+        r[0] = u[0];
+        r[1] = u[1];
+    } else
+        r[0] = *static_cast<const int32_t*>(p);
+}
+
+template <int N>
+__device__ __forceinline__ void store_lds(uint32_t to, const int32_t* r)
+{
+    if constexpr(N == 4)
+        *(lds_v4i_t*)(uintptr_t)to = v4i{r[0], r[1], r[2], r[3]};
+    else if constexpr(N == 2)
+        *(lds_v2i_t*)(uintptr_t)to = v2i{r[0], r[1]};
+    else
+        *(lds_u32_t*)(uintptr_t)to = (uint32_t)r[0];
+}
+
+template <int D, int G, int C>
+__device__ __forceinline__ void attention_kv4_run(const CacheView& c, const AttentionKv4Args& a,
+                                                  const Cut& cut, uint32_t pages, uint8_t* lds)
 {
     using L              = KvLds<D, G>;
     constexpr int kSteps = D / 32, kPer = G / 32, kNG = D / G; // MFMA steps: all, per group
     constexpr int kTiles = D / 16;                             // channel tiles of the result
+    constexpr int kHeads = kCols / C;                          // query heads of a unit
+    constexpr int kPasses = 4 / C; // of the chunk's tiles: pass w takes tiles w C .. w C + C - 1
+    constexpr int kRegs   = 4 * kPasses; // scores a lane holds: register 4 w + j is token
+                                         // 16 (w C + class) + 4 kg + j
     const int      wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int      lane = threadIdx.x % kWave, col = lane % 16, kg = lane / 16;
-    const uint32_t per = a.heads / c.kv_heads, qtiles = (per + kCols - 1) / kCols;
-    const uint32_t kvh = blockIdx.x / qtiles, first = blockIdx.x % qtiles * kCols;
-    const uint32_t seq = blockIdx.y, heads = min((uint32_t)kCols, per - first);
-    const uint32_t head0 = kvh * per + first; // the block's first query head
+    const int      cls = col / kHeads;
+    const uint32_t run = blockIdx.x * kAttWaves + wave;
+    if(run >= cut.waves) return;
+    const uint32_t per = a.heads / c.kv_heads, qtiles = (per + kHeads - 1) / kHeads;
+    const uint32_t units = c.kv_heads * qtiles; // of a sequence
     const uint32_t most  = a.table_cols * c.page_size;
-    const uint32_t len   = (uint32_t)max(0, (int)min((int64_t)a.lens[seq], (int64_t)most));
-    const uint32_t begin = blockIdx.z * pieces.tokens;
-    const uint32_t end   = min(len, pieces.count == 1 ? most : begin + pieces.tokens);
-    if(begin >= end && pieces.count > 1) return;
+    auto           length = [&](uint32_t seq) {
+        return (uint32_t)max(0, (int)min((int64_t)a.lens[seq], (int64_t)most));
+    };
 
-    // ---- the queries: column = head, 8 channels a step in the codes' order -------
-    v8h   qf[kSteps];
-    v4f   start[kNG]; // -1.5 times the sum of the group's channels
-    float qsum[kNG];  // the sum / 16
-    {
-        const uint16_t* q = a.q + (size_t)seq * a.ldq + (size_t)(head0 + col) * D;
-        constexpr int   kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+    // ---- the wave's run ------------------------------------------------------------
+    Place    here{0, 0, 0, 1, 0};
+    uint32_t left = 0; // chunks of the run
+    uint32_t q = 0, r = 0;
+    if(cut.whole) {
+        const uint32_t all = a.seqs * units;
+        uint32_t       u   = (uint32_t)((uint64_t)run * all / cut.waves);
+        const uint32_t to  = (uint32_t)((uint64_t)(run + 1) * all / cut.waves);
+        here.seq           = u / units;
+        here.unit          = u % units;
+        for(; u < to; ++u) left += chunks_of(length(u / units));
+    } else {
+        auto scan = [&](uint32_t i0, uint32_t& n, uint32_t& s) { // 64 sequences' chunks
+            const uint32_t i = i0 + lane;
+            n                = i < a.seqs ? chunks_of(length(i)) * units : 0;
+            s                = n;
+#pragma unroll
+            for(int d = 1; d < kWave; d <<= 1) {
+                const uint32_t o = __shfl_up(s, d, kWave);
+                if(lane >= d) s += o;
+            }
+            return (uint32_t)__builtin_amdgcn_readlane(s, kWave - 1);
+        };
+        uint32_t n, s, all = 0;
+        for(uint32_t i = 0; i < a.seqs; i += kWave) all += scan(i, n, s);
+        q                  = all / cut.waves;
+        r                  = all % cut.waves;
+        uint32_t       at  = run * q + min(run, r);
+        left               = q + (run < r ? 1 : 0);
+        if(left != 0)
+            for(uint32_t i = 0; i < a.seqs; i += kWave) {
+                const uint32_t sum = scan(i, n, s);
+                if(at < sum) {
+                    const int f = __builtin_ctzll(__ballot(s > at));
+                    at -= __builtin_amdgcn_readlane(s, f) - __builtin_amdgcn_readlane(n, f);
+                    here.seq = i + f;
+                    break;
+                }
+                at -= sum;
+            }
+        here.chunk = at;
+    }
+    here.len    = left != 0 ? length(here.seq) : 0;
+    here.chunks = chunks_of(here.len);
+    if(!cut.whole) {
+        here.unit  = here.chunk / here.chunks;
+        here.chunk = here.chunk % here.chunks;
+        if(lane == 0) cut.next[2 * run] = 0;
+    }
+    if(left == 0) return;
+    auto advance = [&](Place& p) { // to the next chunk, whichever unit's; not past the run
+        if(++p.chunk != p.chunks) return;
+        p.chunk = 0;
+        if(++p.unit != units) return;
+        p.unit   = 0;
+        p.seq    = min(p.seq + 1, a.seqs - 1);
+        p.len    = length(p.seq);
+        p.chunks = chunks_of(p.len);
+    };
+
+    // ---- chunks on their way ---------------------------------------------------------
+    // a lane's bytes of a 16-token tile: of the keys 16 (8) of token lane % 16, of the
+    // values 16 (8) of token lane / 4, which go to LDS with the 16-byte chunks of a row
+    // swapped so that the transposed reads spread over the banks
+    constexpr int  kBytes = D / 8;
+    const uint32_t at     = (uint32_t)(uintptr_t)lds + wave * L::kWave;
+    const uint32_t koff = lane % 16 * (D / 2) + kg * kBytes, voff = lane * kBytes;
+    auto           row_chunk = [](uint32_t tok, uint32_t x) {
+        return x ^ (D == 128 ? tok / 4 % 4 : tok / 8 % 2);
+    };
+    const uint32_t vto = at + lane / 4 * (D / 2)
+                         + row_chunk(lane / 4, lane % 4 * kBytes / 16) * 16 + lane % 4 * kBytes % 16;
+    auto page_at = [&](const Place& p) { // lane / 16 = tile: its page, or -1
+        const uint32_t t    = p.chunk * kChunk + lane / 16 * 16;
+        int32_t        page = -1;
+        if(t < p.len) {
+            page = a.table[(size_t)p.seq * a.table_ld + (t >> c.page_shift)];
+            if(page < 0 || (uint32_t)page >= pages) page = -1;
+        }
+        return page;
+    };
+    // byte offset of the codes of tile i of a chunk; a tile without a page reads page 0's
+    // rows and is masked
+    auto tile_codes = [&](const Place& p, int32_t page, int i) {
+        const int32_t g = __builtin_amdgcn_readlane(page, 16 * i);
+        return cache_row(c, g >= 0 ? g : 0, p.unit / qtiles,
+                         (p.chunk * kChunk + i * 16) & (c.page_size - 1))
+               * (D / 2);
+    };
+    auto fetch_values = [&](Chunk<kNG>& x, const Place& p, int32_t page) {
+        const uint64_t with = __ballot(page >= 0);
+        x.ok = (uint32_t)(with & 1) | (uint32_t)(with >> 15 & 2) | (uint32_t)(with >> 30 & 4)
+               | (uint32_t)(with >> 45 & 8);
+        const size_t mine = cache_row(c, page >= 0 ? page : 0, p.unit / qtiles, // lane = token
+                                      (p.chunk * kChunk + lane) & (c.page_size - 1));
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+            load_dwords<D / 32>(reinterpret_cast<int32_t*>(&x.v[i]),
+                                c.codes[1] + tile_codes(p, page, i) + voff);
+        load_dwords<kNG>(x.ks, c.scales[0] + mine * kNG);
+        load_dwords<kNG>(x.vs, c.scales[1] + mine * kNG);
+    };
+    auto fetch_keys = [&](Chunk<kNG>& x, const Place& p, int32_t page) {
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+            load_dwords<D / 32>(reinterpret_cast<int32_t*>(&x.k[i]),
+                                c.codes[0] + tile_codes(p, page, i) + koff);
+    };
+
+    // ---- the queries: column = head, 8 channels a step in the codes' order -----------
+    v8h   qf[C][kSteps]; // zero but for the lane's own class
+    float mid[kNG];      // 1.5 times the sum of the group's channels
+    float qsum[kNG];     // the sum / 16
+    auto  queries = [&](const Place& p) {
+        const uint32_t  first = p.unit % qtiles * kHeads, h = first + col % kHeads;
+        const uint16_t* from  = a.q + (size_t)p.seq * a.ldq
+                               + (size_t)(p.unit / qtiles * per + min(h, per - 1)) * D + 8 * kg;
+        constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+        v8h           v[kSteps];
+#pragma unroll
+        for(int j = 0; j < kSteps; ++j) v[j] = *reinterpret_cast<const v8h*>(from + 32 * j);
 #pragma unroll
         for(int g = 0; g < kNG; ++g) {
             float sum = 0.f;
 #pragma unroll
             for(int j = g * kPer; j < (g + 1) * kPer; ++j) {
-                v8h v = {};
-                if((uint32_t)col < heads)
-                    v = *reinterpret_cast<const v8h*>(q + 32 * j + 8 * kg);
+                v8h u;
 #pragma unroll
                 for(int e = 0; e < 8; ++e) {
-                    qf[j][e] = v[kOrder[e]];
-                    sum += (float)v[e];
+                    u[e] = v[j][kOrder[e]];
+                    sum += (float)v[j][e];
                 }
+#pragma unroll
+                for(int x = 0; x < C; ++x) qf[x][j] = cls == x ? u : v8h{};
             }
             sum      = column_sum(sum);
             qsum[g]  = sum * 0.0625f;
-            start[g] = v4f{sum, sum, sum, sum} * -1.5f;
+            mid[g]   = sum * 1.5f;
         }
-    }
-
-    const float    c2    = a.scale * (16.f * 1.44269504088896341f); // scores are held / 16
-    const uint32_t lds0  = (uint32_t)(uintptr_t)lds;
-    const uint32_t ring  = lds0 + wave * 2 * L::kStage;
-    const size_t   row_k = (size_t)(lane % 16) * (D / 2) + kg * (D / 8);
-    constexpr int  kRowChunks = D / 32; // 16-byte chunks of a row of codes
-    const uint32_t vr = lane / kRowChunks, vp = lane % kRowChunks;
-    const uint32_t voff = vr * (D / 2) + (vp ^ (D == 128 ? vr / 4 % 4 : vr / 8 % 2)) * 16;
+    };
 
     const Unpack unpack;
-    float        m = -INFINITY, l = 0.f;
-    int          shift = 0; // p s is held times 2^shift
+    const float  c2 = a.scale * (16.f * 1.44269504088896341f); // scores are held / 16
+    // of the operand of O^T: which halves hold the lane's class in products 0 and 1
+    const uint32_t half = cls % 2 == 0 ? 0xFFFFu : 0xFFFF0000u;
+    const uint32_t half_mask[2]
+        = {C < 4 || cls / 2 == 0 ? half : 0u, C < 4 || cls / 2 == 1 ? half : 0u};
+
+    float m = -INFINITY, l = 0.f;
+    int   shift = 0; // p s is held times 2^shift
     v4f   o[kTiles] = {}, total[kNG] = {};
     float osum[kNG] = {};
+    bool  from_start = here.chunk == 0; // of the unit
 
-    for(uint32_t seg = begin; seg < end; seg += kSegment) {
-        const uint32_t seg_end = min(end, seg + kSegment);
-        __syncthreads();
-        {
-            const uint32_t t = seg + threadIdx.x * 16; // one page number per 16 tokens
-            int32_t        p = -1;
-            if(t < seg_end) {
-                p = a.table[(size_t)seq * a.table_ld + (t >> c.page_shift)];
-                if(p < 0 || (uint32_t)p >= pages) p = -1;
+    Chunk<kNG> x;
+    Place      next = here;
+    {
+        const int32_t page = page_at(here);
+        queries(here);
+        fetch_values(x, here, page);
+        fetch_keys(x, here, page);
+    }
+    int32_t page_next = -1;
+    if(left > 1) {
+        advance(next);
+        page_next = page_at(next);
+    }
+
+    for(; left > 0; --left) {
+        const uint32_t t0   = here.chunk * kChunk;
+        const uint32_t live = x.ok;
+        const bool     full = live == 15u && t0 + kChunk <= here.len;
+        if(!full && (t0 + lane >= here.len || !((live >> (lane / 16)) & 1u)))
+#pragma unroll
+            for(int g = 0; g < kNG; ++g) x.vs[g] = 0; // not there: it may be NaN
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+            store_lds<D / 32>(vto + i * 16 * (D / 2), reinterpret_cast<const int32_t*>(&x.v[i]));
+        store_lds<kNG>(at + L::kCodes + lane * kNG * 4, x.ks);
+        store_lds<kNG>(at + L::kCodes + L::kScales + lane * kNG * 4, x.vs);
+        float big = 0.f; // the largest scale of the values
+#pragma unroll
+        for(int g = 0; g < kNG; ++g) big = fmaxf(big, fabsf(low_half((uint32_t)x.vs[g])));
+        big = wave_max(big);
+        v4i k[4]; // this chunk's: x is the next one's from here on
+#pragma unroll
+        for(int i = 0; i < 4; ++i) k[i] = x.k[i];
+        const Place now = here;
+        if(left > 1) {
+            const int32_t page = page_next;
+            here               = next;
+            if(left > 2) {
+                advance(next);
+                page_next = page_at(next);
             }
-            page_of[threadIdx.x] = p;
+            fetch_values(x, here, page);
+            fetch_keys(x, here, page);
         }
-        __syncthreads();
 
-        v4i      kc[4];  // the key codes of the chunk ahead
-        uint32_t ok = 0; // which of its 16-token tiles have a page
-        auto     issue = [&](uint32_t chunk, uint32_t stage) {
-            ok = 0;
+        // ---- scores -----------------------------------------------------------------
+        float s[kRegs];
 #pragma unroll
-            for(int i = 0; i < 4; ++i) {
-                const uint32_t t = seg + chunk * kChunk + i * 16;
-                const int32_t  p = __builtin_amdgcn_readfirstlane(page_of[chunk * 4 + i]);
-                ok |= (p >= 0 ? 1u : 0u) << i;
-                // a tile without a page reads page 0's rows and is masked
-                const size_t row = cache_row(c, p >= 0 ? p : 0, kvh, t & (c.page_size - 1));
-                const uint8_t* k = c.codes[0] + row * (D / 2) + row_k;
-                if constexpr(D == 128)
-                    kc[i] = *reinterpret_cast<const v4i*>(k);
-                else {
-                    const v2i u = *reinterpret_cast<const v2i*>(k);
-                    kc[i]       = v4i{u[0], u[1], 0, 0};
-                }
-                const uint32_t to = ring + stage * L::kStage;
-                if(lane < 16 * kRowChunks)
-                    load_lds<16>(c.codes[1] + row * (D / 2), to + i * 16 * (D / 2), voff);
-                if(lane < 16 * kNG) {
-                    load_lds<4>(c.scales[0] + row * kNG, to + L::kCodes + i * 64 * kNG, lane * 4);
-                    load_lds<4>(c.scales[1] + row * kNG, to + L::kCodes + L::kScales + i * 64 * kNG,
-                                lane * 4);
-                }
-            }
-        };
-
-        const uint32_t chunks = (seg_end - seg + kChunk - 1) / kChunk;
-        if((uint32_t)wave < chunks) issue(wave, 0);
-        uint32_t stage = 0;
-        for(uint32_t chunk = wave; chunk < chunks; chunk += kAttWaves, stage ^= 1) {
-            wait_vmcnt<0>();  // the chunk is there,
-            wait_lgkmcnt0();  // and the reads of the one before, whose stage is next, are done
-            asm volatile("" ::: "memory");
-            v4i kn[4];
+        for(int w = 0; w < kPasses; ++w) {
+            v4i sk[kNG];
 #pragma unroll
-            for(int i = 0; i < 4; ++i) kn[i] = kc[i];
-            const uint32_t t0   = seg + chunk * kChunk;
-            const uint32_t live = ok;
-            const bool     full = live == 15u && t0 + kChunk <= end;
-            if(chunk + kAttWaves < chunks) issue(chunk + kAttWaves, stage ^ 1);
-            const uint32_t at = ring + stage * L::kStage;
-
-            // ---- scores: register 4 i + j of a lane is token 16 i + 4 kg + j --------
-            float s[16];
+            for(int g = 0; g < kNG; ++g)
+                sk[g] = *(const lds_v4i_t*)(uintptr_t)(
+                    at + L::kCodes + (16 * (w * C + cls) + 4 * kg) * kNG * 4 + g * 16);
 #pragma unroll
-            for(int i = 0; i < 4; ++i) {
-                v4i sk[kNG];
+            for(int g = 0; g < kNG; ++g) {
+                v4f acc = {};
 #pragma unroll
-                for(int g = 0; g < kNG; ++g)
-                    sk[g] = *(const lds_v4i_t*)(uintptr_t)(at + L::kCodes
-                                                           + (16 * i + 4 * kg) * kNG * 4 + g * 16);
-#pragma unroll
-                for(int g = 0; g < kNG; ++g) {
-                    v4f acc = start[g];
+                for(int y = 0; y < C; ++y)
 #pragma unroll
                     for(int j = g * kPer; j < (g + 1) * kPer; ++j)
-                        acc = mfma16(unpack((uint32_t)kn[i][j]), qf[j], acc);
-#pragma unroll
-                    for(int j = 0; j < 4; ++j) {
-                        const uint32_t w = (uint32_t)sk[(j * kNG + g) / 4][(j * kNG + g) % 4];
-                        const float    x = g == 0 ? 0.f : s[4 * i + j];
-                        s[4 * i + j]     = fmaf(low_half(w), acc[j], fmaf(high_half(w), qsum[g], x));
-                    }
-                }
-            }
-            if(!full) { // tokens that are not there: no score, and no scales (what lies there
-                        // may be NaN)
-#pragma unroll
-                for(int r = 0; r < 16; ++r)
-                    if(t0 + 16 * (r / 4) + 4 * kg + r % 4 >= end || !((live >> (r / 4)) & 1u))
-                        s[r] = -INFINITY;
-                if(t0 + lane >= end || !((live >> (lane / 16)) & 1u))
-#pragma unroll
-                    for(int g = 0; g < kNG; ++g)
-                        *(lds_u32_t*)(uintptr_t)(at + L::kCodes + L::kScales + (lane * kNG + g) * 4)
-                            = 0;
-            }
-
-            // ---- the largest scale of the values, and with it the power of two -----
-            float big = 0.f;
-#pragma unroll
-            for(int g = 0; g < kNG; ++g)
-                big = fmaxf(big, fabsf(low_half(*(const lds_u32_t*)(uintptr_t)(
-                                     at + L::kCodes + L::kScales + (lane * kNG + g) * 4))));
-            big = wave_max(big);
-            float       rescale = 1.f;
-            const float now     = ldexpf(big, shift);
-            if(big > 0.f && big <= 65504.f && (now < 1.f || now > 64.f)) {
-                const int next = 4 - __builtin_amdgcn_frexp_expf(big);
-                rescale        = ldexpf(1.f, next - shift);
-                shift          = next;
-            }
-
-            // ---- softmax -------------------------------------------------------
-            float top = s[0];
-#pragma unroll
-            for(int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-            const float mn = fmaxf(m, column_max(top));
-            if(__ballot(mn > m) != 0 || rescale != 1.f) {
-                const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c2);
-                m              = mn;
-                l *= al;
-#pragma unroll
-                for(int g = 0; g < kNG; ++g) {
-                    osum[g] *= al;
-                    total[g] *= al * rescale;
-                }
-#pragma unroll
-                for(int t = 0; t < kTiles; ++t) o[t] *= al * rescale;
-            }
-            const float mc = m == -INFINITY ? 0.f : m * c2; // no token yet: every p is 0
-            float       p[16];
-#pragma unroll
-            for(int r = 0; r < 16; ++r) {
-                p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -mc));
-                l += p[r];
-            }
-
-            // ---- p times the values' scales, as the operand, group by group --------
-            const float pow2 = ldexpf(1.f, shift);
-            uint32_t    ps[kNG][2][4];
-#pragma unroll
-            for(int u = 0; u < 2; ++u) { // tiles 2 u and 2 u + 1
-                v4i sv[2][kNG];
-#pragma unroll
-                for(int i = 0; i < 2; ++i)
-#pragma unroll
-                    for(int g = 0; g < kNG; ++g)
-                        sv[i][g] = *(const lds_v4i_t*)(uintptr_t)(
-                            at + L::kCodes + L::kScales + (32 * u + 16 * i + 4 * kg) * kNG * 4
-                            + g * 16);
+                        acc = mfma16(unpack((uint32_t)k[w * C + y][j]), qf[y][j], acc);
 #pragma unroll
                 for(int j = 0; j < 4; ++j) {
-                    const float p0 = p[8 * u + j], p1 = p[8 * u + 4 + j];
-                    const float x0 = p0 * pow2, x1 = p1 * pow2;
+                    const uint32_t u = (uint32_t)sk[(j * kNG + g) / 4][(j * kNG + g) % 4];
+                    const float    b = g == 0 ? 0.f : s[4 * w + j];
+                    s[4 * w + j]
+                        = fmaf(low_half(u), acc[j] - mid[g], fmaf(high_half(u), qsum[g], b));
+                }
+            }
+        }
+        if(!full) // tokens that are not there
 #pragma unroll
-                    for(int g = 0; g < kNG; ++g) {
-                        const uint32_t w0 = (uint32_t)sv[0][(j * kNG + g) / 4][(j * kNG + g) % 4];
-                        const uint32_t w1 = (uint32_t)sv[1][(j * kNG + g) / 4][(j * kNG + g) % 4];
-                        osum[g]     = fmaf(p0, high_half(w0), fmaf(p1, high_half(w1), osum[g]));
-                        ps[g][u][j] = scaled_pair(x0, w0, x1, w1);
+            for(int i = 0; i < kRegs; ++i) {
+                const uint32_t tile = i / 4 * C + cls;
+                if(t0 + 16 * tile + 4 * kg + i % 4 >= now.len || !((live >> tile) & 1u))
+                    s[i] = -INFINITY;
+            }
+        // ---- the power of two that goes with the largest scale ------------------------
+        float       rescale = 1.f;
+        const float held    = ldexpf(big, shift);
+        if(big > 0.f && big <= 65504.f && (held < 1.f || held > 64.f)) {
+            const int to = 4 - __builtin_amdgcn_frexp_expf(big);
+            rescale      = ldexpf(1.f, to - shift);
+            shift        = to;
+        }
+
+        // ---- softmax ------------------------------------------------------------------
+        float top = s[0];
+#pragma unroll
+        for(int i = 1; i < kRegs; ++i) top = fmaxf(top, s[i]);
+        const float mn = fmaxf(m, column_max(top));
+        if(__ballot(mn > m) != 0 || rescale != 1.f) {
+            const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c2);
+            m              = mn;
+            l *= al;
+#pragma unroll
+            for(int g = 0; g < kNG; ++g) {
+                osum[g] *= al;
+                total[g] *= al * rescale;
+            }
+#pragma unroll
+            for(int t = 0; t < kTiles; ++t) o[t] *= al * rescale;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c2; // no token yet: every p is 0
+        float       p[kRegs];
+#pragma unroll
+        for(int i = 0; i < kRegs; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -mc));
+            l += p[i];
+        }
+
+        // ---- p times the values' scales, as the operand, group by group ----------------
+        // operand register r of product u: token 4 kg + r of tile 2 u in the low and of
+        // tile 2 u + 1 in the high half, zero for tiles of other classes
+        const float pow2 = ldexpf(1.f, shift);
+        uint32_t    ps[kNG][2][4];
+#pragma unroll
+        for(int w = 0; w < kPasses; ++w) {
+            v4i sv[kNG];
+#pragma unroll
+            for(int g = 0; g < kNG; ++g)
+                sv[g] = *(const lds_v4i_t*)(uintptr_t)(
+                    at + L::kCodes + L::kScales + (16 * (w * C + cls) + 4 * kg) * kNG * 4 + g * 16);
+#pragma unroll
+            for(int j = 0; j < 4; ++j) {
+                const float f = p[4 * w + j] * pow2;
+#pragma unroll
+                for(int g = 0; g < kNG; ++g) {
+                    const uint32_t u = (uint32_t)sv[(j * kNG + g) / 4][(j * kNG + g) % 4];
+                    osum[g]          = fmaf(p[4 * w + j], high_half(u), osum[g]);
+                    if constexpr(C == 1) {
+                        if(w % 2 == 0)
+                            ps[g][w / 2][j] = scaled_low(f, u);
+                        else
+                            scaled_high(ps[g][w / 2][j], f, u);
+                    } else {
+                        uint32_t b = scaled_low(f, u);
+                        scaled_high(b, f, u);
+                        if constexpr(C == 2)
+                            ps[g][w][j] = b & half_mask[0];
+                        else
+#pragma unroll
+                            for(int y = 0; y < 2; ++y) ps[g][y][j] = b & half_mask[y];
                     }
                 }
             }
-            auto operand = [&](int g, int u) {
-                return __builtin_bit_cast(
-                    v8h, v4i{(int)ps[g][u][0], (int)ps[g][u][1], (int)ps[g][u][2], (int)ps[g][u][3]});
-            };
-            const v8h ones = {1, 1, 1, 1, 1, 1, 1, 1};
-#pragma unroll
-            for(int g = 0; g < kNG; ++g)
-#pragma unroll
-                for(int u = 0; u < 2; ++u) total[g] = mfma16(ones, operand(g, u), total[g]);
-
-            // ---- values: channel 16 t + col, tokens of source lanes 16 (j / 4) + 4 kg + j % 4
-#pragma unroll
-            for(int t = 0; t < kTiles; ++t) {
-                const uint32_t tok = 16 * (col / 4) + 4 * kg + col % 4;
-                const uint32_t f   = D == 128 ? tok / 4 % 4 : tok / 8 % 2;
-                const v2i      w   = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_v2i_t*)(uintptr_t)(
-                    at + tok * (D / 2) + ((t / 2) ^ f) * 16 + t % 2 * 8));
-#pragma unroll
-                for(int u = 0; u < 2; ++u)
-                    o[t] = mfma16(unpack((uint32_t)w[u]), operand(t * 16 / G, u), o[t]);
-            }
         }
-    }
+        auto operand = [&](int g, int u) {
+            return __builtin_bit_cast(
+                v8h, v4i{(int)ps[g][u][0], (int)ps[g][u][1], (int)ps[g][u][2], (int)ps[g][u][3]});
+        };
+        const v8h ones = {1, 1, 1, 1, 1, 1, 1, 1};
+#pragma unroll
+        for(int g = 0; g < kNG; ++g)
+#pragma unroll
+            for(int u = 0; u < 2; ++u) total[g] = mfma16(ones, operand(g, u), total[g]);
 
-    // ---- merge the waves ---------------------------------------------------------
-    l                = column_sum(l);
-    const float back = ldexpf(16.f, -shift);
+        // ---- values: channel 16 t + col, tokens of source lanes 16 (j / 4) + 4 kg + j % 4
 #pragma unroll
-    for(int g = 0; g < kNG; ++g) osum[g] = column_sum(osum[g]);
-    __syncthreads(); // the ring is done with
-    float* part = reinterpret_cast<float*>(lds);
-    float* ml   = part + kAttWaves * kCols * D;
+        for(int t = 0; t < kTiles; ++t) {
+            const uint32_t tok = 16 * (col / 4) + 4 * kg + col % 4;
+            const v2i      w   = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_v2i_t*)(uintptr_t)(
+                at + tok * (D / 2) + row_chunk(tok, t / 2) * 16 + t % 2 * 8));
 #pragma unroll
-    for(int t = 0; t < kTiles; ++t) {
-        const int g = t * 16 / G;
-        v4f       r;
-#pragma unroll
-        for(int i = 0; i < 4; ++i) r[i] = fmaf(fmaf(total[g][i], -1.5f, o[t][i]), back, osum[g]);
-        *reinterpret_cast<v4f*>(part + (wave * kCols + col) * D + 16 * t + 4 * kg) = r;
-    }
-    if(kg == 0) {
-        ml[(wave * kCols + col) * 2]     = m * c2;
-        ml[(wave * kCols + col) * 2 + 1] = l;
-    }
-    __syncthreads();
-    for(uint32_t i = threadIdx.x; i < heads * D; i += kAttThreads) {
-        const uint32_t h = i / D, ch = i % D;
-        float          mm = -INFINITY;
-#pragma unroll
-        for(int w = 0; w < kAttWaves; ++w) mm = fmaxf(mm, ml[(w * kCols + h) * 2]);
-        float sum = 0.f, ls = 0.f;
-#pragma unroll
-        for(int w = 0; w < kAttWaves; ++w) {
-            const float lw = ml[(w * kCols + h) * 2 + 1];
-            if(lw == 0.f) continue; // no token seen: its maximum may be -inf
-            const float f = __builtin_amdgcn_exp2f(ml[(w * kCols + h) * 2] - mm);
-            sum           = fmaf(f, part[(w * kCols + h) * D + ch], sum);
-            ls            = fmaf(f, lw, ls);
+            for(int u = 0; u < 2; ++u)
+                o[t] = mfma16(unpack((uint32_t)w[u]), operand(t * 16 / G, u), o[t]);
         }
-        if(pieces.count == 1)
-            a.out[(size_t)seq * a.ldo + (size_t)(head0 + h) * D + ch]
-                = float_to_half_bits(ls != 0.f ? sum / ls : 0.f);
-        else {
-            const size_t at         = ((size_t)seq * a.heads + head0 + h) * pieces.count + blockIdx.z;
-            pieces.o[at * D + ch] = sum;
-            if(ch == 0) {
-                pieces.ml[at * 2]     = mm;
-                pieces.ml[at * 2 + 1] = ls;
+
+        // ---- the unit's end, or the run's -----------------------------------------------
+        const bool ends = now.chunk + 1 == now.chunks;
+        if(!ends && left > 1) continue;
+        // classes side by side: a common maximum, then sums over the columns of a head
+        l            = column_sum(l);
+        float common = m;
+        if constexpr(C >= 4) common = fmaxf(common, dpp_mov<kDppRowRor4>(common));
+        if constexpr(C >= 2) common = fmaxf(common, dpp_mov<kDppRowRor8>(common));
+        const float f = l == 0.f ? 0.f : m == common ? 1.f : __builtin_amdgcn_exp2f((m - common) * c2);
+        auto        merged = [&](float v) {
+            v *= f;
+            if constexpr(C >= 4) v += dpp_mov<kDppRowRor4>(v);
+            if constexpr(C >= 2) v += dpp_mov<kDppRowRor8>(v);
+            return v;
+        };
+        l                  = merged(l);
+        const float    back = ldexpf(16.f, -shift);
+        const uint32_t head = now.unit % qtiles * kHeads + col; // of the key head's
+        const bool     mine = cls == 0 && head < per;
+        const bool     done = ends && from_start;
+        const float    inv  = done ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
+        const uint32_t slot = 2 * run + (from_start ? 1 : 0);
+#pragma unroll
+        for(int g = 0; g < kNG; ++g) osum[g] = column_sum(osum[g]);
+#pragma unroll
+        for(int t = 0; t < kTiles; ++t) {
+            const int g = t * 16 / G;
+            v4f       v;
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+                v[i] = merged(fmaf(fmaf(total[g][i], -1.5f, o[t][i]), back, osum[g])) * inv;
+            if(!mine) continue;
+            if(done) {
+                const size_t to = (size_t)now.seq * a.ldo
+                                  + (size_t)(now.unit / qtiles * per + head) * D + 16 * t + 4 * kg;
+                v2i w;
+                w[0] = (int)float2_to_half2_bits_2step(v[0], v[1]);
+                w[1] = (int)float2_to_half2_bits_2step(v[2], v[3]);
+                *reinterpret_cast<v2i*>(a.out + to) = w;
+            } else
+                *reinterpret_cast<v4f*>(cut.o + ((size_t)slot * kHeads + col) * D + 16 * t + 4 * kg)
+                    = v;
+        }
+        if(!done && mine && kg == 0) {
+            cut.ml[((size_t)slot * kHeads + col) * 2]     = common * c2;
+            cut.ml[((size_t)slot * kHeads + col) * 2 + 1] = l;
+        }
+        if(!ends && from_start && lane == 0) { // goes on behind the run: up to which wave
+            const uint32_t end  = run * q + min(run, r) + (q + (run < r ? 1 : 0));
+            const uint32_t last = end + (now.chunks - 1 - now.chunk) - 1; // its last chunk
+            cut.next[2 * run]   = now.seq * units + now.unit + 1;
+            cut.next[2 * run + 1]
+                = last < r * (q + 1) ? last / (q + 1) : r + (last - r * (q + 1)) / q;
+        }
+        if(left > 1) { // the next unit
+            from_start = true;
+            m          = -INFINITY;
+            l          = 0.f;
+#pragma unroll
+            for(int g = 0; g < kNG; ++g) {
+                osum[g]  = 0.f;
+                total[g] = v4f{0, 0, 0, 0};
             }
+#pragma unroll
+            for(int t = 0; t < kTiles; ++t) o[t] = v4f{0, 0, 0, 0};
+            queries(here);
         }
     }
 }
 
-template <int D, int G>
+template <int D, int G, int C>
 __global__ void __launch_bounds__(kAttThreads, 2)
-    attention_kv4_kernel(CacheView c, AttentionKv4Args a, Pieces pieces, uint32_t pages)
+    attention_kv4_kernel(CacheView c, AttentionKv4Args a, Cut cut, uint32_t pages)
 {
-    __shared__ alignas(16) uint8_t lds[KvLds<D, G>::kBytes];
-    __shared__ int32_t             page_of[kSegment / 16];
-    attention_kv4_piece<D, G>(c, a, pieces, pages, lds, page_of);
+    __shared__ alignas(16) uint8_t lds[kAttWaves * KvLds<D, G>::kWave];
+    attention_kv4_run<D, G, C>(c, a, cut, pages, lds);
 }
 
-// Joins the pieces of one (sequence, head): their factors first, then the threads of
-// each channel take every kJoin-th piece, and add up in a fixed order.
-constexpr int kJoinThreads = 512, kJoinPieces = 256; // pieces whose factors lie in LDS at a time
+// Joins the partials of the units that go on behind one of the block's runs: the slot of
+// that wave, then the first slots of the waves after it, in a fixed order.  D / 4
+// threads take 4 channels each of every kWays-th partial of one head.
+constexpr int      kJoinThreads = 1024;
+constexpr uint32_t kJoinRuns    = 4; // runs a block looks after
 
-template <int D>
+template <int D, int HEADS>
 __global__ void __launch_bounds__(kJoinThreads)
-    attention_kv4_join_kernel(CacheView c, AttentionKv4Args a, Pieces pieces)
+    attention_kv4_join_kernel(AttentionKv4Args a, Cut cut, uint32_t kv_heads)
 {
-    constexpr int    kJoin = kJoinThreads / D;
-    __shared__ float factor[kJoinPieces];
-    __shared__ float part[kJoin][D + 1];
-    const uint32_t   head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
-    const uint32_t   ch = tid % D, way = tid / D;
-    const uint32_t   most = a.table_cols * c.page_size;
-    const uint32_t   len  = (uint32_t)max(0, (int)min((int64_t)a.lens[seq], (int64_t)most));
-    const uint32_t   n    = (len + pieces.tokens - 1) / pieces.tokens;
-    const size_t     at   = ((size_t)seq * a.heads + head) * pieces.count;
-    const float*     ml   = pieces.ml + at * 2;
-    float            m    = -INFINITY; // of all pieces, in every wave
-    for(uint32_t i = tid % kWave; i < n; i += kWave) m = fmaxf(m, ml[i * 2]);
-    m         = wave_max(m);
-    float sum = 0.f, l = 0.f;
-    for(uint32_t i0 = 0; i0 < n; i0 += kJoinPieces) {
-        const uint32_t here = min(n - i0, (uint32_t)kJoinPieces);
-        __syncthreads();
-        if(tid < here) {
-            const float li = ml[(i0 + tid) * 2 + 1]; // 0: no token seen, its maximum may be -inf
-            factor[tid]    = li != 0.f ? __builtin_amdgcn_exp2f(ml[(i0 + tid) * 2] - m) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll 8
-        for(uint32_t i = way; i < here; i += kJoin) {
-            const float f = factor[i];
-            sum           = fmaf(f, pieces.o[(at + i0 + i) * D + ch], sum);
-            l             = fmaf(f, ml[(i0 + i) * 2 + 1], l);
-        }
+    constexpr int       kLanes = D / 4, kWays = kJoinThreads / kLanes / HEADS;
+    __shared__ uint32_t next[kJoinRuns][2];
+    __shared__ v4f      part[kWays][HEADS][kLanes];
+    __shared__ float    weight[kWays][HEADS];
+    const uint32_t      tid = threadIdx.x;
+    if(tid < kJoinRuns * 2) {
+        const uint32_t run = blockIdx.x * kJoinRuns + tid / 2;
+        next[tid / 2][tid % 2] = run < cut.waves ? cut.next[2 * run + tid % 2] : 0;
     }
-    part[way][ch] = sum;
-    if(ch == 0) part[way][D] = l;
     __syncthreads();
-    if(way != 0) return;
-    for(int w = 1; w < kJoin; ++w) sum += part[w][ch];
-    l = 0.f;
-    for(int w = 0; w < kJoin; ++w) l += part[w][D];
-    a.out[(size_t)seq * a.ldo + (size_t)head * D + ch] = float_to_half_bits(l != 0.f ? sum / l : 0.f);
+    const uint32_t per = a.heads / kv_heads, qtiles = (per + HEADS - 1) / HEADS;
+    const uint32_t ch = tid % kLanes * 4, col = tid / kLanes % HEADS, way = tid / kLanes / HEADS;
+    for(uint32_t j = 0; j < kJoinRuns; ++j) {
+        const uint32_t id = next[j][0], run = blockIdx.x * kJoinRuns + j;
+        if(id == 0) continue;
+        const uint32_t unit = (id - 1) % (kv_heads * qtiles), seq = (id - 1) / (kv_heads * qtiles);
+        const uint32_t head = unit % qtiles * HEADS + col;
+        const uint32_t n    = next[j][1] - run + 1; // partials
+        auto           at   = [&](uint32_t i) {
+            return (size_t)(2 * (run + i) + (i == 0 ? 1 : 0)) * HEADS + col;
+        };
+        float m = -INFINITY; // of all the head's partials
+        v4f   sum = {};
+        float l   = 0.f;
+        if(head < per) {
+            float mi = -INFINITY;
+            for(uint32_t i0 = 0; i0 < n; i0 += 4 * kLanes)
+#pragma unroll
+                for(int x = 0; x < 4; ++x) {
+                    const uint32_t i = i0 + x * kLanes + tid % kLanes;
+                    if(i < n) mi = fmaxf(mi, cut.ml[at(i) * 2]);
+                }
+#pragma unroll
+            for(int d = kLanes / 2; d > 0; d >>= 1) mi = fmaxf(mi, __shfl_xor(mi, d, kWave));
+            m = mi;
+            for(uint32_t i0 = way; i0 < n; i0 += 8 * kWays) { // 8 partials' loads at a time
+                v4f   v[8];
+                float f[8], li[8];
+#pragma unroll
+                for(int x = 0; x < 8; ++x) {
+                    const size_t from = at(min(i0 + x * kWays, n - 1));
+                    v[x]  = *reinterpret_cast<const v4f*>(cut.o + from * D + ch);
+                    f[x]  = cut.ml[from * 2];
+                    li[x] = cut.ml[from * 2 + 1]; // 0: no token seen, its maximum is -inf
+                }
+#pragma unroll
+                for(int x = 0; x < 8; ++x) {
+                    if(i0 + x * kWays >= n || li[x] == 0.f) continue;
+                    const float e = __builtin_amdgcn_exp2f(f[x] - m);
+#pragma unroll
+                    for(int y = 0; y < 4; ++y) sum[y] = fmaf(e, v[x][y], sum[y]);
+                    l = fmaf(e, li[x], l);
+                }
+            }
+        }
+        __syncthreads(); // the unit before is done with
+        part[way][col][ch / 4] = sum;
+        if(ch == 0) weight[way][col] = l;
+        __syncthreads();
+        if(way != 0 || head >= per) continue;
+        for(int w = 1; w < kWays; ++w) {
+            sum += part[w][col][ch / 4];
+            l += weight[w][col];
+        }
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        v2i         w;
+        w[0] = (int)float2_to_half2_bits_2step(sum[0] * inv, sum[1] * inv);
+        w[1] = (int)float2_to_half2_bits_2step(sum[2] * inv, sum[3] * inv);
+        *reinterpret_cast<v2i*>(a.out + (size_t)seq * a.ldo
+                                + (size_t)(unit / qtiles * per + head) * D + ch)
+            = w;
+    }
 }
 
-// Pieces of equal size, as many as leave every one enough to do and fill the chip
-// when every sequence is as long as its table.
-constexpr uint32_t kPieceLeast = 256, kPieceBlocks = 1024;
+// Query heads a unit takes: all of a key head's where they are few.
+uint32_t unit_heads(uint32_t per) { return per <= 4 ? 4 : per <= 8 ? 8 : 16; }
 
-uint32_t piece_tokens(uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t max_len)
+uint32_t seq_units(uint32_t heads, uint32_t kv_heads)
 {
-    const uint32_t per    = heads / kv_heads;
-    const uint64_t blocks = (uint64_t)seqs * kv_heads * ((per + kCols - 1) / kCols);
-    const uint64_t t      = (blocks * max_len + kPieceBlocks - 1) / kPieceBlocks;
-    return (uint32_t)std::min<uint64_t>((std::max<uint64_t>(t, 1) + kPieceLeast - 1) / kPieceLeast * kPieceLeast, 0x7FFFFF00u);
+    const uint32_t per = heads / kv_heads, b = unit_heads(per);
+    return kv_heads * ((per + b - 1) / b);
 }
 
-uint32_t piece_count(uint32_t tokens, uint32_t max_len)
+// Waves of the launch: no more than chunks at the most.
+uint32_t run_count(uint32_t seqs, uint32_t units, uint32_t max_len)
 {
-    return std::max(1u, (uint32_t)(((uint64_t)max_len + tokens - 1) / tokens));
+    return (uint32_t)std::min<uint64_t>(kAttBlocks * kAttWaves,
+                                        (uint64_t)seqs * units * chunks_of(max_len));
 }
 
 } // namespace
@@ -712,31 +909,42 @@ hipError_t launch_kv4_load(const w8a8_kv4_cache& c, const Kv4Rows& r, uint16_t* 
 size_t attention_kv4_workspace_bytes(uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t dim,
                                      uint32_t max_len)
 {
-    const uint32_t n = piece_count(piece_tokens(seqs, heads, kv_heads, max_len), max_len);
-    return n == 1 ? 0 : (size_t)seqs * heads * n * (dim + 2) * 4;
+    if(chunks_of(max_len) == 1) return 0; // no unit is cut
+    const size_t waves = run_count(seqs, seq_units(heads, kv_heads), max_len);
+    return waves * 2 * unit_heads(heads / kv_heads) * (dim + 2) * 4 + waves * 8;
 }
 
 hipError_t launch_attention_kv4(const w8a8_kv4_cache& c, const AttentionKv4Args& a,
                                 hipStream_t stream)
 {
-    const uint32_t max_len = a.table_cols * c.page_size;
-    Pieces         pieces{1, 0, nullptr, nullptr};
+    const uint32_t max_len = a.table_cols * c.page_size, units = seq_units(a.heads, c.kv_heads);
     const size_t   need
         = attention_kv4_workspace_bytes(a.seqs, a.heads, c.kv_heads, c.head_dim, max_len);
-    if(need != 0 && a.ws_bytes >= need) {
-        pieces.tokens = piece_tokens(a.seqs, a.heads, c.kv_heads, max_len);
-        pieces.count  = piece_count(pieces.tokens, max_len);
-        pieces.o      = static_cast<float*>(a.ws);
-        pieces.ml     = pieces.o + (size_t)a.seqs * a.heads * pieces.count * c.head_dim;
+    Cut cut{};
+    cut.heads = unit_heads(a.heads / c.kv_heads);
+    cut.whole = need == 0 || a.ws_bytes < need;
+    if(cut.whole)
+        cut.waves = std::min(kAttBlocks * kAttWaves, a.seqs * units);
+    else {
+        cut.waves          = run_count(a.seqs, units, max_len);
+        const size_t slots = (size_t)cut.waves * 2 * cut.heads;
+        cut.o              = static_cast<float*>(a.ws);
+        cut.ml             = cut.o + slots * c.head_dim;
+        cut.next           = reinterpret_cast<uint32_t*>(cut.ml + slots * 2);
     }
-    const uint32_t per = a.heads / c.kv_heads;
-    const dim3     grid(c.kv_heads * ((per + kCols - 1) / kCols), a.seqs, pieces.count);
+    const uint32_t blocks = (cut.waves + kAttWaves - 1) / kAttWaves;
     with_widths(c, [&](auto d, auto g) {
-        attention_kv4_kernel<d(), g()>
-            <<<grid, kAttThreads, 0, stream>>>(view(c), a, pieces, c.pages);
-        if(pieces.count > 1)
-            attention_kv4_join_kernel<d()>
-                <<<dim3(a.heads, a.seqs), kJoinThreads, 0, stream>>>(view(c), a, pieces);
+        const auto kernel = cut.heads == 4   ? attention_kv4_kernel<d(), g(), 4>
+                            : cut.heads == 8 ? attention_kv4_kernel<d(), g(), 2>
+                                             : attention_kv4_kernel<d(), g(), 1>;
+        kernel<<<blocks, kAttThreads, 0, stream>>>(view(c), a, cut, c.pages);
+        if(!cut.whole) {
+            const auto join = cut.heads == 4   ? attention_kv4_join_kernel<d(), 4>
+                              : cut.heads == 8 ? attention_kv4_join_kernel<d(), 8>
+                                               : attention_kv4_join_kernel<d(), 16>;
+            join<<<(cut.waves + kJoinRuns - 1) / kJoinRuns, kJoinThreads, 0, stream>>>(a, cut,
+                                                                                   c.kv_heads);
+        }
     });
     return hipGetLastError();
 }

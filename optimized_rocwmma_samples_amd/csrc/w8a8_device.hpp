@@ -16,6 +16,8 @@ constexpr int kWave = 64;
 // DPP controls (GCN/CDNA encoding).
 constexpr int kDppQuadXor1      = 0xB1;  // quad_perm [1,0,3,2]
 constexpr int kDppQuadXor2      = 0x4E;  // quad_perm [2,3,0,1]
+constexpr int kDppRowRor4       = 0x124; // lane i <- lane i + 4 (mod 16) inside each row of 16
+constexpr int kDppRowRor8       = 0x128; // lane i <- lane i + 8 (mod 16)
 constexpr int kDppRowMirror     = 0x140; // lane i <- lane 15-i inside each row of 16
 constexpr int kDppRowHalfMirror = 0x141; // lane i <- lane 7-i inside each half-row of 8
 

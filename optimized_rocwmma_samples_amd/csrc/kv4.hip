@@ -298,14 +298,14 @@ __device__ __forceinline__ float high_half(uint32_t w) { return half_bits_to_flo
 // How the launch is cut: `waves` runs over all chunks, or (whole) over all units.
 // Partials: slot 2 w + 0 of wave w holds a unit that began before its run, 2 w + 1 one
 // that begins in it and goes on behind it: per head the sum of p v (fp32 [D]), then
-// all slots' (maximum in powers of two, sum of p); then per wave what goes on behind
-// it: (unit + 1, the last wave of it) or (0, 0).
+// all slots' (maximum in powers of two, sum of p); then per unit the first wave of a
+// cut one plus 1 (0: not cut) and the last.
 struct Cut {
     uint32_t  waves, heads; // heads: query heads of a unit
     bool      whole;
     float*    o;
     float*    ml;
-    uint32_t* next;
+    uint32_t* unit;
 };
 
 __host__ __device__ inline uint32_t chunks_of(uint32_t len)
@@ -432,7 +432,6 @@ __device__ __forceinline__ void attention_kv4_run(const CacheView& c, const Atte
     if(!cut.whole) {
         here.unit  = here.chunk / here.chunks;
         here.chunk = here.chunk % here.chunks;
-        if(lane == 0) cut.next[2 * run] = 0;
     }
     if(left == 0) return;
     auto advance = [&](Place& p) { // to the next chunk, whichever unit's; not past the run
@@ -755,12 +754,14 @@ __device__ __forceinline__ void attention_kv4_run(const CacheView& c, const Atte
             cut.ml[((size_t)slot * kHeads + col) * 2]     = common * c2;
             cut.ml[((size_t)slot * kHeads + col) * 2 + 1] = l;
         }
-        if(!ends && from_start && lane == 0) { // goes on behind the run: up to which wave
-            const uint32_t end  = run * q + min(run, r) + (q + (run < r ? 1 : 0));
-            const uint32_t last = end + (now.chunks - 1 - now.chunk) - 1; // its last chunk
-            cut.next[2 * run]   = now.seq * units + now.unit + 1;
-            cut.next[2 * run + 1]
-                = last < r * (q + 1) ? last / (q + 1) : r + (last - r * (q + 1)) / q;
+        if(from_start && !cut.whole && lane == 0) {
+            uint32_t* to = cut.unit + 2 * ((size_t)now.seq * units + now.unit);
+            to[0]        = ends ? 0 : run + 1;
+            if(!ends) { // goes on behind the run: up to which wave
+                const uint32_t end  = run * q + min(run, r) + (q + (run < r ? 1 : 0));
+                const uint32_t last = end + (now.chunks - 1 - now.chunk) - 1; // its last chunk
+                to[1] = last < r * (q + 1) ? last / (q + 1) : r + (last - r * (q + 1)) / q;
+            }
         }
         if(left > 1) { // the next unit
             from_start = true;
@@ -786,88 +787,106 @@ __global__ void __launch_bounds__(kAttThreads, 2)
     attention_kv4_run<D, G, C>(c, a, cut, pages, lds);
 }
 
-// Joins the partials of the units that go on behind one of the block's runs: the slot of
-// that wave, then the first slots of the waves after it, in a fixed order.  D / 4
-// threads take 4 channels each of every kWays-th partial of one head.
-constexpr int      kJoinThreads = 1024;
-constexpr uint32_t kJoinRuns    = 4; // runs a block looks after
-
-template <int D, int HEADS>
-__global__ void __launch_bounds__(kJoinThreads)
-    attention_kv4_join_kernel(AttentionKv4Args a, Cut cut, uint32_t kv_heads)
+// Joins the partials of the cut units: the slot of the first wave, then the first slots
+// of the waves after it.  WAVES waves take CH channels of one head of a unit, CH / 4
+// lanes 4 channels each of every kWays-th partial, 8 loads at a time with a running
+// maximum; then the ways are added up, always in the same order.  Few units have many
+// partials each and take all of a block's waves for a part of the channels (1 x 131072
+// tokens, 8 key heads: 256 partials a unit), many units have few and take a wave a head.
+// Blocks are kept few: their start is what a launch of thousands waits for.
+template <int D, int HEADS, int WAVES, int CH>
+__global__ void __launch_bounds__(kAttThreads)
+    attention_kv4_join_kernel(AttentionKv4Args a, Cut cut, uint32_t kv_heads, uint32_t tasks)
 {
-    constexpr int       kLanes = D / 4, kWays = kJoinThreads / kLanes / HEADS;
-    __shared__ uint32_t next[kJoinRuns][2];
-    __shared__ v4f      part[kWays][HEADS][kLanes];
-    __shared__ float    weight[kWays][HEADS];
-    const uint32_t      tid = threadIdx.x;
-    if(tid < kJoinRuns * 2) {
-        const uint32_t run = blockIdx.x * kJoinRuns + tid / 2;
-        next[tid / 2][tid % 2] = run < cut.waves ? cut.next[2 * run + tid % 2] : 0;
-    }
-    __syncthreads();
-    const uint32_t per = a.heads / kv_heads, qtiles = (per + HEADS - 1) / HEADS;
-    const uint32_t ch = tid % kLanes * 4, col = tid / kLanes % HEADS, way = tid / kLanes / HEADS;
-    for(uint32_t j = 0; j < kJoinRuns; ++j) {
-        const uint32_t id = next[j][0], run = blockIdx.x * kJoinRuns + j;
-        if(id == 0) continue;
-        const uint32_t unit = (id - 1) % (kv_heads * qtiles), seq = (id - 1) / (kv_heads * qtiles);
-        const uint32_t head = unit % qtiles * HEADS + col;
-        const uint32_t n    = next[j][1] - run + 1; // partials
-        auto           at   = [&](uint32_t i) {
-            return (size_t)(2 * (run + i) + (i == 0 ? 1 : 0)) * HEADS + col;
+    constexpr uint32_t kLanes = CH / 4, kWays = WAVES * kWave / kLanes, kSlices = D / CH;
+    constexpr uint32_t kGroups = kAttWaves / WAVES;
+    __shared__ v4f   part[WAVES][kLanes];
+    __shared__ float top[WAVES], weight[WAVES];
+    const int        wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t   lane = threadIdx.x % kWave, in = threadIdx.x % (WAVES * kWave);
+    const uint32_t   way = in / kLanes;
+    const uint32_t   per = a.heads / kv_heads, qtiles = (per + HEADS - 1) / HEADS;
+    const uint32_t   units = kv_heads * qtiles; // of a sequence
+    for(uint32_t task = blockIdx.x * kGroups + wave / WAVES; task < tasks;
+        task += gridDim.x * kGroups) {
+        const uint32_t u = task / (HEADS * kSlices), col = task / kSlices % HEADS;
+        const uint32_t ch = task % kSlices * CH + in % kLanes * 4;
+        const uint32_t w0 = __builtin_amdgcn_readfirstlane(cut.unit[2 * (size_t)u]);
+        const uint32_t w1 = __builtin_amdgcn_readfirstlane(cut.unit[2 * (size_t)u + 1]);
+        const uint32_t head = u % units % qtiles * HEADS + col;
+        if(w0 == 0 || head >= per) continue;
+        const uint32_t run = w0 - 1, n = w1 - run + 1; // partials
+        float          m = -INFINITY, l = 0.f;
+        v4f            sum = {};
+        auto take = [&](float mi, float li, v4f v) { // 0: no token seen, its maximum is -inf
+            if(li == 0.f) return;
+            const float now = fmaxf(m, mi);
+            const float al  = m == now ? 1.f : __builtin_amdgcn_exp2f(m - now);
+            const float e   = mi == now ? 1.f : __builtin_amdgcn_exp2f(mi - now);
+            m               = now;
+            l               = fmaf(l, al, e * li);
+#pragma unroll
+            for(int y = 0; y < 4; ++y) sum[y] = fmaf(sum[y], al, e * v[y]);
         };
-        float m = -INFINITY; // of all the head's partials
-        v4f   sum = {};
-        float l   = 0.f;
-        if(head < per) {
-            float mi = -INFINITY;
-            for(uint32_t i0 = 0; i0 < n; i0 += 4 * kLanes)
+        for(uint32_t i0 = way; i0 < n; i0 += 8 * kWays) {
+            v4f v[8];
+            v2f ml[8];
 #pragma unroll
-                for(int x = 0; x < 4; ++x) {
-                    const uint32_t i = i0 + x * kLanes + tid % kLanes;
-                    if(i < n) mi = fmaxf(mi, cut.ml[at(i) * 2]);
-                }
-#pragma unroll
-            for(int d = kLanes / 2; d > 0; d >>= 1) mi = fmaxf(mi, __shfl_xor(mi, d, kWave));
-            m = mi;
-            for(uint32_t i0 = way; i0 < n; i0 += 8 * kWays) { // 8 partials' loads at a time
-                v4f   v[8];
-                float f[8], li[8];
-#pragma unroll
-                for(int x = 0; x < 8; ++x) {
-                    const size_t from = at(min(i0 + x * kWays, n - 1));
-                    v[x]  = *reinterpret_cast<const v4f*>(cut.o + from * D + ch);
-                    f[x]  = cut.ml[from * 2];
-                    li[x] = cut.ml[from * 2 + 1]; // 0: no token seen, its maximum is -inf
-                }
-#pragma unroll
-                for(int x = 0; x < 8; ++x) {
-                    if(i0 + x * kWays >= n || li[x] == 0.f) continue;
-                    const float e = __builtin_amdgcn_exp2f(f[x] - m);
-#pragma unroll
-                    for(int y = 0; y < 4; ++y) sum[y] = fmaf(e, v[x][y], sum[y]);
-                    l = fmaf(e, li[x], l);
-                }
+            for(int x = 0; x < 8; ++x) {
+                const uint32_t i    = min(i0 + x * kWays, n - 1);
+                const size_t   from = (size_t)(2 * (run + i) + (i == 0 ? 1 : 0)) * HEADS + col;
+                v[x]  = *reinterpret_cast<const v4f*>(cut.o + from * D + ch);
+                ml[x] = *reinterpret_cast<const v2f*>(cut.ml + from * 2);
             }
+#pragma unroll
+            for(int x = 0; x < 8; ++x) take(ml[x][0], i0 + x * kWays < n ? ml[x][1] : 0.f, v[x]);
         }
-        __syncthreads(); // the unit before is done with
-        part[way][col][ch / 4] = sum;
-        if(ch == 0) weight[way][col] = l;
-        __syncthreads();
-        if(way != 0 || head >= per) continue;
-        for(int w = 1; w < kWays; ++w) {
-            sum += part[w][col][ch / 4];
-            l += weight[w][col];
+#pragma unroll
+        for(int d = kLanes; d < kWave; d <<= 1) { // the ways of a wave, in pairs
+            const float mo = __shfl_xor(m, d, kWave), lo = __shfl_xor(l, d, kWave);
+            v4f         vo;
+#pragma unroll
+            for(int y = 0; y < 4; ++y) vo[y] = __shfl_xor(sum[y], d, kWave);
+            take(mo, lo, vo);
         }
+        if constexpr(WAVES > 1) { // one task a block: its waves come here together
+            __syncthreads();
+            if(lane < kLanes) part[wave][lane] = sum;
+            if(lane == 0) {
+                top[wave]    = m;
+                weight[wave] = l;
+            }
+            __syncthreads();
+            m   = -INFINITY;
+            l   = 0.f;
+            sum = v4f{0, 0, 0, 0};
+#pragma unroll
+            for(int w = 0; w < WAVES; ++w) take(top[w], weight[w], part[w][in % kLanes]);
+        }
+        if(way != 0) continue;
         const float inv = l != 0.f ? 1.f / l : 0.f;
         v2i         w;
         w[0] = (int)float2_to_half2_bits_2step(sum[0] * inv, sum[1] * inv);
         w[1] = (int)float2_to_half2_bits_2step(sum[2] * inv, sum[3] * inv);
-        *reinterpret_cast<v2i*>(a.out + (size_t)seq * a.ldo
-                                + (size_t)(unit / qtiles * per + head) * D + ch)
+        *reinterpret_cast<v2i*>(a.out + (size_t)(u / units) * a.ldo
+                                + (size_t)(u % units / qtiles * per + head) * D + ch)
             = w;
     }
+}
+
+template <int D, int HEADS>
+void launch_join(const AttentionKv4Args& a, const Cut& cut, uint32_t kv_heads, uint32_t units,
+                 hipStream_t stream)
+{
+    constexpr uint32_t kMostBlocks = 1024;
+    const uint32_t     heads = a.seqs * units * HEADS;
+    if(heads <= 256)
+        attention_kv4_join_kernel<D, HEADS, kAttWaves, 32>
+            <<<heads * (D / 32), kAttThreads, 0, stream>>>(a, cut, kv_heads, heads * (D / 32));
+    else
+        attention_kv4_join_kernel<D, HEADS, 1, D>
+            <<<std::min((heads + kAttWaves - 1) / kAttWaves, kMostBlocks), kAttThreads, 0, stream>>>(
+                a, cut, kv_heads, heads);
 }
 
 // Query heads a unit takes: all of a key head's where they are few.
@@ -911,7 +930,8 @@ size_t attention_kv4_workspace_bytes(uint32_t seqs, uint32_t heads, uint32_t kv_
 {
     if(chunks_of(max_len) == 1) return 0; // no unit is cut
     const size_t waves = run_count(seqs, seq_units(heads, kv_heads), max_len);
-    return waves * 2 * unit_heads(heads / kv_heads) * (dim + 2) * 4 + waves * 8;
+    return waves * 2 * unit_heads(heads / kv_heads) * (dim + 2) * 4
+           + (size_t)seqs * seq_units(heads, kv_heads) * 8;
 }
 
 hipError_t launch_attention_kv4(const w8a8_kv4_cache& c, const AttentionKv4Args& a,
@@ -930,7 +950,7 @@ hipError_t launch_attention_kv4(const w8a8_kv4_cache& c, const AttentionKv4Args&
         const size_t slots = (size_t)cut.waves * 2 * cut.heads;
         cut.o              = static_cast<float*>(a.ws);
         cut.ml             = cut.o + slots * c.head_dim;
-        cut.next           = reinterpret_cast<uint32_t*>(cut.ml + slots * 2);
+        cut.unit           = reinterpret_cast<uint32_t*>(cut.ml + slots * 2);
     }
     const uint32_t blocks = (cut.waves + kAttWaves - 1) / kAttWaves;
     with_widths(c, [&](auto d, auto g) {
@@ -939,11 +959,10 @@ hipError_t launch_attention_kv4(const w8a8_kv4_cache& c, const AttentionKv4Args&
                                              : attention_kv4_kernel<d(), g(), 1>;
         kernel<<<blocks, kAttThreads, 0, stream>>>(view(c), a, cut, c.pages);
         if(!cut.whole) {
-            const auto join = cut.heads == 4   ? attention_kv4_join_kernel<d(), 4>
-                              : cut.heads == 8 ? attention_kv4_join_kernel<d(), 8>
-                                               : attention_kv4_join_kernel<d(), 16>;
-            join<<<(cut.waves + kJoinRuns - 1) / kJoinRuns, kJoinThreads, 0, stream>>>(a, cut,
-                                                                                   c.kv_heads);
+            const auto join = cut.heads == 4   ? launch_join<d(), 4>
+                              : cut.heads == 8 ? launch_join<d(), 8>
+                                               : launch_join<d(), 16>;
+            join(a, cut, c.kv_heads, units, stream);
         }
     });
     return hipGetLastError();

@@ -33,9 +33,13 @@ constexpr int      kWords     = kMaxExpert / 32;
 constexpr uint32_t kMaxTopk   = 32;
 constexpr int      kBufferFlags  = 0x00020000; // raw buffer, 32-bit data format
 constexpr uint32_t kOob          = 0x80000000u;
-constexpr int      kWeightPolicy = 2; // non-temporal: every weight byte is read once
+// Default cache policy, although every byte is read once: a wave-load takes half of each
+// 128-byte line, and non-temporal lines were gone before the other half's load (64
+// experts of 7168 x 2048, 16 tokens, 539 us against 487).
+constexpr int kWeightPolicy = 0;
 
-constexpr uint32_t kGateUpBlocks = 512;        // two blocks a CU
+constexpr uint32_t kCus          = 256;
+constexpr uint32_t kGateUpBlocks = 2 * kCus;
 constexpr uint32_t kLdsBytes     = 160 * 1024; // of a CU
 
 static_assert(kRows == 16, "the rows are the columns of one 16 x 16 tile");
@@ -141,6 +145,14 @@ __device__ __forceinline__ uint32_t block_of(uint32_t unit, uint32_t units, uint
     return ((unit + 1) * blocks - 1) / units;
 }
 
+// Hardware gives blocks to the 8 XCDs in turn; an index such that each XCD has a
+// contiguous range of them.
+__device__ __forceinline__ uint32_t xcd_range(uint32_t block, uint32_t blocks)
+{
+    const uint32_t x = block % 8, r = blocks % 8;
+    return x * (blocks / 8) + min(x, r) + block / 8;
+}
+
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t weight_rows(const int8_t* w, uint32_t k)
 {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(w), 0, (int)(kTile * k),
@@ -184,11 +196,11 @@ struct Cursor {
 // First kernel: a block owns a range of 16-column tiles of the activations.
 // ---------------------------------------------------------------------------
 constexpr int      kGuSteps = 2; // steps a batch: 2 KB of gate rows and 2 KB of up rows a wave
-constexpr int      kGuRing  = 4; // batches in registers, three of them in flight
-constexpr uint32_t kGroup   = 8; // tiles whose sums lie in LDS at a time
+
+// Sums of a tile in LDS: [gate, up][row][column].  As many tiles at a time as `group`.
+typedef int32_t TileSums[2][kRows][kTile];
 
 struct GateUpLds {
-    int32_t  acc[kGroup][2][kRows][kTile]; // [tile][gate, up][row][column]
     float    amax[kRows][kWaves];
     float    scale[kRows];
     uint32_t top[kRows]; // float bits, >= 0
@@ -197,20 +209,22 @@ struct GateUpLds {
 };
 
 static_assert(W8A8_MOE_DECODE_MAX_VALUES + kRows * 80 + Lists::bytes(kRows * kMaxTopk)
-                      + sizeof(GateUpLds)
+                      + sizeof(GateUpLds) + 4 * sizeof(TileSums)
                   <= kLdsBytes,
               "a block of gate_up_kernel holds every token's row");
 
-template <bool F16>
-__device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, GateUpLds& lds,
-                                        uint8_t* dyn)
+// RING: batches in registers, all but one of them in flight.
+template <bool F16, int RING>
+__device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, uint32_t group,
+                                        GateUpLds& lds, uint8_t* dyn)
 {
     const int      wave  = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int      lane  = threadIdx.x % kWave, col = lane % 16, kg = lane / 16;
     const uint32_t pairs = a.tokens * a.topk, tid = threadIdx.x;
     Lists          lists(dyn, pairs);
-    int8_t*        q  = reinterpret_cast<int8_t*>(dyn + Lists::bytes(pairs));
-    const uint32_t rb = row_bytes(a.hidden);
+    TileSums*      sums = reinterpret_cast<TileSums*>(dyn + Lists::bytes(pairs));
+    int8_t*        q    = reinterpret_cast<int8_t*>(sums + group);
+    const uint32_t rb   = row_bytes(a.hidden);
 
     // ---- routing: a wave per token -----------------------------------------------
     if(tid < kWords) lds.bits[tid] = 0;
@@ -230,13 +244,17 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, Ga
     __syncthreads();
     lists.build(pairs, kThreads, lds.bits, &lds.active);
     const uint32_t tiles = a.inter / kTile, units = lds.active * tiles;
-    const uint32_t from  = first_unit(blockIdx.x, units, gridDim.x);
-    const uint32_t to    = first_unit(blockIdx.x + 1, units, gridDim.x);
+    // neighbouring ranges to one XCD: where every other block has a tile more, each XCD
+    // gets as many of both (8 experts of 4096 x 14336, one token: 448 and 448 tiles at
+    // 3.5 a block; round robin gave half the XCDs a third more, 48 us against 38)
+    const uint32_t range = xcd_range(blockIdx.x, gridDim.x);
+    const uint32_t from  = first_unit(range, units, gridDim.x);
+    const uint32_t to    = first_unit(range + 1, units, gridDim.x);
     const uint32_t steps = (a.hidden + 63) / 64, per = (steps + kGuSteps - 1) / kGuSteps;
 
     uint32_t held = ~0u; // the expert whose rows are in LDS
     for(uint32_t u0 = from; u0 < to;) { // tiles u0 .. u1 of one expert
-        const uint32_t ai = u0 / tiles, u1 = min(min(to, (ai + 1) * tiles), u0 + kGroup);
+        const uint32_t ai = u0 / tiles, u1 = min(min(to, (ai + 1) * tiles), u0 + group);
         const uint32_t e = lists.expert_at(ai), rows = lists.rows(ai);
         const size_t   row0 = (size_t)e * 2 * a.inter + (u0 - ai * tiles) * kTile;
         const uint16_t* list = lists.pair + ai * kRows;
@@ -265,7 +283,7 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, Ga
 
         // ---- the stream of weights ----------------------------------------------
         const Run run((u1 - u0) * per, wave);
-        v4i       ring[kGuRing][2][kGuSteps];
+        v4i       ring[RING][2][kGuSteps];
         Cursor    ahead(run.from, per), now = ahead;
         uint32_t  at   = run.from;
         auto      load = [&](int slot) {
@@ -284,12 +302,12 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, Ga
             ++at;
         };
 #pragma unroll
-        for(int i = 0; i < kGuRing - 1; ++i)
+        for(int i = 0; i < RING - 1; ++i)
             if(at < run.to) load(i);
 
         __syncthreads(); // the sums and rows before are done with
-        for(uint32_t i = tid; i < sizeof(lds.acc) / 16; i += kThreads)
-            reinterpret_cast<v4i*>(lds.acc)[i] = v4i{0, 0, 0, 0};
+        for(uint32_t i = tid; i < (u1 - u0) * sizeof(TileSums) / 16; i += kThreads)
+            reinterpret_cast<v4i*>(sums)[i] = v4i{0, 0, 0, 0};
         if(tid < (uint32_t)kRows && fresh) lds.top[tid] = 0;
         // ---- the expert's rows, quantized into LDS: four rows at a time, so that
         // their loads overlap ------------------------------------------------------
@@ -349,8 +367,8 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, Ga
         v4i           acc[2] = {};
         for(uint32_t done = run.from; done < run.to;) {
 #pragma unroll
-            for(int slot = 0; slot < kGuRing; ++slot) {
-                if(at < run.to) load((slot + kGuRing - 1) % kGuRing);
+            for(int slot = 0; slot < RING; ++slot) {
+                if(at < run.to) load((slot + RING - 1) % RING);
                 if(done < run.to) {
 #pragma unroll
                     for(int i = 0; i < kGuSteps; ++i) {
@@ -366,7 +384,7 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, Ga
                             for(int w = 0; w < 2; ++w)
 #pragma unroll
                                 for(int i = 0; i < 4; ++i)
-                                    atomicAdd(&lds.acc[now.item][w][col][4 * kg + i], acc[w][i]);
+                                    atomicAdd(&sums[now.item][w][col][4 * kg + i], acc[w][i]);
                         acc[0] = acc[1] = v4i{0, 0, 0, 0};
                     }
                     now.advance(per);
@@ -381,9 +399,9 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, Ga
             const uint32_t c = (u0 - ai * tiles + u) * kTile + j;
             const float    rs = lds.scale[r];
             const float    g
-                = ((float)lds.acc[u][0][r][j] * rs) * a.sgu[(size_t)e * 2 * a.inter + c];
+                = ((float)sums[u][0][r][j] * rs) * a.sgu[(size_t)e * 2 * a.inter + c];
             const float v
-                = ((float)lds.acc[u][1][r][j] * rs) * a.sgu[(size_t)e * 2 * a.inter + a.inter + c];
+                = ((float)sums[u][1][r][j] * rs) * a.sgu[(size_t)e * 2 * a.inter + a.inter + c];
             float f = silu_mul(g, v);
             if(a.s2) f *= a.s2[(size_t)e * a.inter + c];
             ws.act[(size_t)list[r] * a.inter + c] = f;
@@ -398,17 +416,20 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, Ga
         if(u0 == to || u0 == (ai + 1) * tiles) { // the expert's last tiles here
             __syncthreads();
             if(tid < rows)
-                ws.top[(size_t)list[tid] * kGateUpBlocks + blockIdx.x] = __uint_as_float(lds.top[tid]);
+                ws.top[(size_t)list[tid] * kGateUpBlocks + range] = __uint_as_float(lds.top[tid]);
         }
     }
 }
 
-template <bool F16>
-__global__ void __launch_bounds__(kThreads, 4) gate_up_kernel(MoeDecodeArgs a, Ws ws)
+// BLOCKS a CU.  Batches in flight: 3 where a block is alone on its CU, 2 where there are
+// two; more made it slower (7 and 3 of them: 8 experts of 4096 x 14336, one token, 85
+// us against 80).
+template <bool F16, int BLOCKS>
+__global__ void __launch_bounds__(kThreads, 2 * BLOCKS) gate_up_kernel(MoeDecodeArgs a, Ws ws, uint32_t group)
 {
     extern __shared__ uint8_t dyn[];
     __shared__ GateUpLds      lds;
-    gate_up<F16>(a, ws, lds, dyn);
+    gate_up<F16, BLOCKS == 1 ? 4 : 3>(a, ws, group, lds, dyn);
 }
 
 // ---------------------------------------------------------------------------
@@ -422,14 +443,13 @@ __global__ void __launch_bounds__(kThreads, 4) gate_up_kernel(MoeDecodeArgs a, W
 // `chunk` columns, in two buffers: 8 more waves quantize the next while 8 multiply.
 // ---------------------------------------------------------------------------
 constexpr int kDownSteps = 4; // steps a batch: 4 KB a wave
-constexpr int kDownRing  = 4; // batches in registers, three of them in flight
 
 struct DownLds {
     uint32_t bits[kWords];
     uint32_t active;
 };
 
-template <int FOLD, bool ALL>
+template <int FOLD, bool ALL, int RING>
 __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint32_t chunk,
                                      uint32_t gu_blocks, DownLds& lds, uint8_t* dyn)
 {
@@ -439,9 +459,10 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
     const uint32_t pairs = a.tokens * a.topk, tid = threadIdx.x;
     Lists          lists(dyn, pairs);
     uint8_t*       at0   = dyn + Lists::bytes(pairs);
-    float*         scale = reinterpret_cast<float*>(at0);
-    int32_t*       sums  = reinterpret_cast<int32_t*>(at0 + Lists::up16(pairs)); // [pairs][kCols]
-    int8_t* q = reinterpret_cast<int8_t*>(at0 + Lists::up16(pairs) + pairs * kTile * 4);
+    float*         scale   = reinterpret_cast<float*>(at0);
+    float*         inverse = reinterpret_cast<float*>(at0 + Lists::up16(pairs));
+    int32_t*       sums = reinterpret_cast<int32_t*>(at0 + 2 * Lists::up16(pairs)); // [pairs][kCols]
+    int8_t* q = reinterpret_cast<int8_t*>(at0 + 2 * Lists::up16(pairs) + pairs * kTile * 4);
     const uint32_t j0 = blockIdx.x * kCols, rb = row_bytes(chunk);
     const uint32_t tiles = a.inter / kTile;
 
@@ -464,34 +485,59 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
                     m = fmaxf(m, ws.top[(size_t)p * kGateUpBlocks + b]); // it had work
             m = wave_max(m);
         }
-        if(lane == 0) scale[p] = m / a.qmax;
+        if(lane == 0) {
+            const float r = m / a.qmax;
+            scale[p]      = r;
+            inverse[p]    = r > 0.f ? 1.f / r : 0.f;
+        }
     }
     __syncthreads();
 
-    // 16 columns from k on of one pair's activations, to LDS
-    auto quantize = [&](uint32_t p, uint32_t k, int8_t* to) {
-        const float inv = scale[p] > 0.f ? 1.f / scale[p] : 0.f;
-        v4i         w   = {0, 0, 0, 0};
-        if(k < a.inter) {
-            const float* h = ws.act + (size_t)p * a.inter + k;
+    // 16 columns from k on of one pair's activations, and their quantized form to LDS
+    struct Piece {
+        v4f f[4];
+    };
+    auto fetch = [&](Piece& x, uint32_t p, uint32_t k) {
+        const float* h = ws.act + (size_t)p * a.inter + k;
 #pragma unroll
-            for(int c = 0; c < 4; ++c) {
-                const v4f f = *reinterpret_cast<const v4f*>(h + 4 * c);
-                w[c] = (int)cvt_pack4_i8(quant_f(f[0], inv, a.qmax), quant_f(f[1], inv, a.qmax),
-                                         quant_f(f[2], inv, a.qmax), quant_f(f[3], inv, a.qmax));
-            }
-        }
+        for(int c = 0; c < 4; ++c)
+            x.f[c] = k < a.inter ? *reinterpret_cast<const v4f*>(h + 4 * c) : v4f{0, 0, 0, 0};
+    };
+    auto store = [&](const Piece& x, uint32_t p, int8_t* to) {
+        const float inv = inverse[p];
+        v4i         w;
+#pragma unroll
+        for(int c = 0; c < 4; ++c)
+            w[c] = (int)cvt_pack4_i8(quant_f(x.f[c][0], inv, a.qmax), quant_f(x.f[c][1], inv, a.qmax),
+                                     quant_f(x.f[c][2], inv, a.qmax), quant_f(x.f[c][3], inv, a.qmax));
         *reinterpret_cast<v4i*>(to) = w;
+    };
+    auto quantize = [&](uint32_t p, uint32_t k, int8_t* to) {
+        Piece x;
+        fetch(x, p, k);
+        store(x, p, to);
     };
     const uint32_t per_row = (rb - 16) / 16; // 16-column pieces of a row in LDS
     const uint32_t chunks  = ALL ? 1 : (a.inter + chunk - 1) / chunk;
-    auto           fill    = [&](uint32_t phase, uint32_t from) { // by kThreads threads
-        const uint32_t ai = phase / chunks, k0 = phase % chunks * chunk;
-        const uint32_t rows = lists.rows(ai);
-        int8_t*        to   = q + phase % 2 * a.tokens * rb;
-        for(uint32_t i = from; i < rows * per_row; i += kThreads)
-            quantize(lists.pair[ai * kRows + i / per_row], k0 + i % per_row * 16,
-                     to + i / per_row * rb + i % per_row * 16);
+    // the rows of phase (expert, chunk), by 8 waves of which this is `w`: as many a row as
+    // the rows leave (and no divisions: those by a row's pieces took 2 us a phase)
+    auto fill = [&](uint32_t phase, uint32_t w) {
+        const uint32_t ai = phase / chunks, rows = lists.rows(ai), k0 = phase % chunks * chunk;
+        const uint32_t shift = rows > 4 ? 0 : rows > 2 ? 1 : rows > 1 ? 2 : 3;
+        for(uint32_t r = w >> shift; r < rows; r += kWaves >> shift) {
+            const uint32_t p  = lists.pair[ai * kRows + r];
+            int8_t*        to = q + (phase % 2 * a.tokens + r) * rb;
+            const uint32_t step = kWave << shift;
+            for(uint32_t i0 = (w & ((1u << shift) - 1)) * kWave + lane; i0 < per_row; i0 += 4 * step) {
+                Piece x[4]; // 4 loads overlap
+#pragma unroll
+                for(int j = 0; j < 4; ++j)
+                    if(i0 + j * step < per_row) fetch(x[j], p, k0 + (i0 + j * step) * 16);
+#pragma unroll
+                for(int j = 0; j < 4; ++j)
+                    if(i0 + j * step < per_row) store(x[j], p, to + (i0 + j * step) * 16);
+            }
+        }
     };
 
     // ---- the stream of weights: items are experts (ALL) or (expert, chunk) -----------
@@ -503,7 +549,7 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
     const Run run(ALL ? items * per : per, wave % kWaves);
     const bool     streams = ALL || wave < kWaves;
     const uint32_t mine    = streams ? (ALL ? run.to - run.from : (run.to - run.from) * items) : 0;
-    v4i            ring[kDownRing][kDownSteps];
+    v4i            ring[RING][kDownSteps];
     Cursor         ahead(ALL ? run.from : 0, per), now = ahead;
     if(!ALL) ahead.b = now.b = run.from;
     auto advance = [&](Cursor& c) {
@@ -531,23 +577,42 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
         advance(ahead);
         ++loaded;
     };
+    // a thread's first pieces go out ahead of the weights: behind them they would wait for
+    // all of those
+    constexpr uint32_t kAhead = ALL ? 2 : 0;
+    Piece              first[ALL ? kAhead : 1];
+    const uint32_t     all = pairs * per_row;
+    if constexpr(ALL)
 #pragma unroll
-    for(int i = 0; i < kDownRing - 1; ++i)
+        for(uint32_t x = 0; x < kAhead; ++x)
+            if(tid + x * kThreads < all) {
+                const uint32_t i = tid + x * kThreads;
+                fetch(first[x], i / per_row, i % per_row * 16);
+            }
+#pragma unroll
+    for(int i = 0; i < RING - 1; ++i)
         if(loaded < mine) load(i);
 
     if constexpr(ALL) {
-        for(uint32_t i = tid; i < pairs * per_row; i += kThreads)
-            if(lists.ids[i / per_row] >= 0)
-                quantize(i / per_row, i % per_row * 16, q + i / per_row * rb + i % per_row * 16);
-    } else if(!streams && n > 0)
-        fill(0, tid - kThreads);
+#pragma unroll
+        for(uint32_t x = 0; x < kAhead; ++x)
+            if(tid + x * kThreads < all) {
+                const uint32_t i = tid + x * kThreads;
+                store(first[x], i / per_row, q + i / per_row * rb + i % per_row * 16);
+            }
+        for(uint32_t i = tid + kAhead * kThreads; i < all; i += kThreads)
+            quantize(i / per_row, i % per_row * 16, q + i / per_row * rb + i % per_row * 16);
+    } else if(!streams && n > 0) {
+        fill(0, wave - kWaves);
+    }
     __syncthreads();
 
     if(!streams) {
-        for(uint32_t item = 0; item < items; ++item) {
-            if(item + 1 < items) fill(item + 1, tid - kThreads);
-            __syncthreads();
-        }
+        if constexpr(!ALL)
+            for(uint32_t item = 0; item < items; ++item) {
+                if(item + 1 < items) fill(item + 1, wave - kWaves);
+                __syncthreads();
+            }
     } else {
         v4i           acc  = {};
         uint32_t      done = 0, rows = 0;
@@ -568,8 +633,8 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
         };
         while(done < mine) {
 #pragma unroll
-            for(int slot = 0; slot < kDownRing; ++slot) {
-                if(loaded < mine) load((slot + kDownRing - 1) % kDownRing);
+            for(int slot = 0; slot < RING; ++slot) {
+                if(loaded < mine) load((slot + RING - 1) % RING);
                 if(done < mine) {
                     const uint32_t ai = now.item / chunks;
                     if(fresh) {
@@ -618,13 +683,14 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
     }
 }
 
-template <int FOLD, bool ALL>
-__global__ void __launch_bounds__(ALL ? kThreads : 2 * kThreads, 4)
+// BLOCKS a CU, as in gate_up_kernel (the 16 waves of the chunked form count as two).
+template <int FOLD, bool ALL, int BLOCKS>
+__global__ void __launch_bounds__(ALL ? kThreads : 2 * kThreads, 2 * BLOCKS)
     down_kernel(MoeDecodeArgs a, Ws ws, uint32_t chunk, uint32_t gu_blocks)
 {
     extern __shared__ uint8_t dyn[];
     __shared__ DownLds        lds;
-    down<FOLD, ALL>(a, ws, chunk, gu_blocks, lds, dyn);
+    down<FOLD, ALL, BLOCKS == 1 ? 4 : 3>(a, ws, chunk, gu_blocks, lds, dyn);
 }
 
 template <class K>
@@ -639,19 +705,23 @@ template <int FOLD>
 hipError_t launch_down(const MoeDecodeArgs& a, const Ws& ws, uint32_t gu_blocks, hipStream_t stream)
 {
     const uint32_t pairs = a.tokens * a.topk, grid = a.hidden / (kTile / FOLD);
-    const uint32_t fixed = Lists::bytes(pairs) + Lists::up16(pairs) + pairs * kTile * 4;
+    const uint32_t fixed = Lists::bytes(pairs) + 2 * Lists::up16(pairs) + pairs * kTile * 4;
     const uint32_t room  = kLdsBytes - (uint32_t)sizeof(DownLds) - fixed;
     // all rows, where two blocks still share a CU or one does with no second to come
     if((uint64_t)pairs * row_bytes(a.inter) <= std::min<uint32_t>(room, 100 * 1024)) {
         const uint32_t lds = fixed + pairs * row_bytes(a.inter);
-        allow_lds(down_kernel<FOLD, true>, lds);
-        down_kernel<FOLD, true><<<grid, kThreads, lds, stream>>>(a, ws, a.inter, gu_blocks);
+        const auto     kernel
+            = grid <= kCus ? down_kernel<FOLD, true, 1> : down_kernel<FOLD, true, 2>;
+        allow_lds(kernel, lds);
+        kernel<<<grid, kThreads, lds, stream>>>(a, ws, a.inter, gu_blocks);
     } else {
-        const uint32_t chunk
-            = std::min((a.inter + 63) / 64 * 64, (room / (2 * a.tokens) - 16) / 512 * 512);
+        // as few chunks as fit, all about the same size
+        const uint32_t most   = (room / (2 * a.tokens) - 16) / 64 * 64;
+        const uint32_t chunks = (a.inter + most - 1) / most;
+        const uint32_t chunk  = ((a.inter + chunks - 1) / chunks + 63) / 64 * 64;
         const uint32_t lds = fixed + 2 * a.tokens * row_bytes(chunk);
-        allow_lds(down_kernel<FOLD, false>, lds);
-        down_kernel<FOLD, false><<<grid, 2 * kThreads, lds, stream>>>(a, ws, chunk, gu_blocks);
+        allow_lds(down_kernel<FOLD, false, 2>, lds);
+        down_kernel<FOLD, false, 2><<<grid, 2 * kThreads, lds, stream>>>(a, ws, chunk, gu_blocks);
     }
     return hipGetLastError();
 }
@@ -668,13 +738,19 @@ hipError_t launch_moe_ffn_decode(const MoeDecodeArgs& a, bool f16, hipStream_t s
 {
     const Ws       ws    = carve(a);
     const uint32_t pairs = a.tokens * a.topk;
-    const uint32_t lds   = Lists::bytes(pairs) + a.tokens * row_bytes(a.hidden);
+    // 8 tiles' sums at a time, or 4 where two blocks then share a CU, or where 8 do not fit
+    const uint32_t rest = Lists::bytes(pairs) + a.tokens * row_bytes(a.hidden) + sizeof(GateUpLds);
+    const uint32_t sum  = sizeof(TileSums);
+    const bool     two  = rest + 4 * sum <= kLdsBytes / 2;
+    const uint32_t group = rest + 8 * sum <= (two ? kLdsBytes / 2 : kLdsBytes) ? 8 : 4;
+    const uint32_t lds   = rest - sizeof(GateUpLds) + group * sum;
     // as many blocks as are resident at once
-    const uint32_t resident = lds + sizeof(GateUpLds) <= kLdsBytes / 2 ? kGateUpBlocks : kGateUpBlocks / 2;
-    const uint32_t blocks = std::min(resident, std::min(pairs, a.experts) * (a.inter / kTile));
-    const auto     gu     = f16 ? gate_up_kernel<true> : gate_up_kernel<false>;
+    const uint32_t blocks = std::min(two ? kGateUpBlocks : kCus,
+                                     std::min(pairs, a.experts) * (a.inter / kTile));
+    const auto     gu     = f16 ? (two ? gate_up_kernel<true, 2> : gate_up_kernel<true, 1>)
+                                : (two ? gate_up_kernel<false, 2> : gate_up_kernel<false, 1>);
     allow_lds(gu, lds);
-    gu<<<blocks, kThreads, lds, stream>>>(a, ws);
+    gu<<<blocks, kThreads, lds, stream>>>(a, ws, group);
     const hipError_t e = hipGetLastError();
     if(e != hipSuccess) return e;
     // a block for every CU, where the tokens leave room in the tile

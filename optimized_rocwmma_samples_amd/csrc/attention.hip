@@ -108,6 +108,14 @@ __device__ __forceinline__ v2f both_halves(float v)
     return {__uint_as_float(r[0]), __uint_as_float(r[1])};
 }
 
+// max(a, b, c) without the canonicalizing steps that fmaxf takes on matrix results.
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 __device__ __forceinline__ bool nonfinite(uint32_t h16) { return (h16 & 0x7C00u) == 0x7C00u; }
 
 // The fp16 values of a fragment with infinities and NaN as 0.
@@ -205,6 +213,19 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
                          rq, (wave * 32 + col) * a.ldq * 2 + s * 32 + half * 16, 0, 0));
     }
 
+    // LDS places of the lane's reads, in stage 0: of a key's step and a value's block; all
+    // others are fixed distances away
+    uint32_t kat[kSteps], vat[kBlocks];
+#pragma unroll
+    for(int st = 0; st < kSteps; ++st)
+        kat[st] = lds0 + col * D * 2 + key_chunk<D>(col, 2 * st + half) * 16;
+#pragma unroll
+    for(int b = 0; b < kBlocks; ++b) {
+        const uint32_t tok = 4 * half + lane % 16 / 4;
+        const uint32_t ch  = 32 * b + lane / 16 % 2 * 16 + lane % 4 * 4;
+        vat[b] = lds0 + kTileBytes + tok * D * 2 + value_chunk<D>(tok, ch / 8) * 16 + ch % 8 * 2;
+    }
+
     const float c = a.scale * 1.44269504088896341f; // exponents in base 2
     float       m = -INFINITY, l = 0.f;
     v16f        o[kBlocks] = {};
@@ -218,18 +239,15 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
         if(kt > 0) issue(stage ^ 1, kt - 1);
         if(kt * kKeys > first + 31) continue; // all of the tile is later than the wave's rows
 
-        const uint32_t kl   = lds0 + stage * 2 * kTileBytes, vl = kl + kTileBytes;
+        const uint32_t off  = stage * 2 * kTileBytes;
         const bool     diag = (kt + 1) * kKeys > first; // some of it is later than some rows
         v16f           s[2] = {};
 #pragma unroll
-        for(int sub = 0; sub < 2; ++sub) {
-            const uint32_t tok = sub * 32 + col;
+        for(int st = 0; st < kSteps; ++st)
 #pragma unroll
-            for(int st = 0; st < kSteps; ++st)
-                s[sub] = mfma(*(const lds_v8h_t*)(uintptr_t)(
-                                  kl + tok * D * 2 + key_chunk<D>(tok, 2 * st + half) * 16),
+            for(int sub = 0; sub < 2; ++sub)
+                s[sub] = mfma(*(const lds_v8h_t*)(uintptr_t)(kat[st] + off + sub * 32 * D * 2),
                               qf[st], s[sub]);
-        }
         if(diag) {
 #pragma unroll
             for(int sub = 0; sub < 2; ++sub)
@@ -239,12 +257,16 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
                     s[sub][i]        = j > qi ? -INFINITY : s[sub][i];
                 }
         }
-        float top = fmaxf(s[0][0], s[1][0]);
+        float top = max3(s[0][0], s[1][0], s[0][1]);
 #pragma unroll
-        for(int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
-        const v2f tops = both_halves(top);
-        const float mn = fmaxf(m, fmaxf(tops[0], tops[1]));
-        if(__ballot(mn > m) != 0) {
+        for(int i = 1; i < 15; ++i) top = max3(top, s[1][i], s[0][i + 1]);
+        top             = fmaxf(top, s[1][15]);
+        const v2f   tops = both_halves(top);
+        const float mn   = fmaxf(m, fmaxf(tops[0], tops[1]));
+        // m need not be the maximum itself: the result is rescaled only where some row's
+        // probabilities would pass 2^8 (far inside fp16), which after the first tiles is
+        // never, and not at every new maximum of one of 64 rows
+        if(__ballot((mn - m) * c > 8.f) != 0) {
             const float al = __builtin_amdgcn_exp2f((m - mn) * c);
             m              = mn;
             l *= al;
@@ -252,38 +274,36 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
             for(int b = 0; b < kBlocks; ++b) o[b] *= al;
         }
         const float mc = m * c;
-        v8h         p[4];
-#pragma unroll
-        for(int sub = 0; sub < 2; ++sub)
-#pragma unroll
-            for(int i = 0; i < 16; i += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[sub][i], c, -mc));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[sub][i + 1], c, -mc));
-                l += p0;
-                l += p1;
-                const v2h h = __builtin_convertvector((v2f{p0, p1}), v2h);
-                p[sub * 2 + i / 8][i % 8]     = h[0];
-                p[sub * 2 + i / 8][i % 8 + 1] = h[1];
-            }
 
         // 4 keys of channel 32 b + col: keys 16 st + 8 part + 4 half ..
         auto values = [&](int b, int st) {
             v8h f;
 #pragma unroll
             for(int part = 0; part < 2; ++part) {
-                const uint32_t tok = 16 * st + 8 * part + 4 * half + lane % 16 / 4;
-                const uint32_t ch  = 32 * b + lane / 16 % 2 * 16 + lane % 4 * 4;
-                const auto     r   = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h_t*)(uintptr_t)(
-                    vl + tok * D * 2 + value_chunk<D>(tok, ch / 8) * 16 + ch % 8 * 2));
+                const auto r = __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                    (lds_v4h_t*)(uintptr_t)(vat[b] + off + (16 * st + 8 * part) * D * 2));
 #pragma unroll
                 for(int i = 0; i < 4; ++i) f[part * 4 + i] = (_Float16)r[i];
             }
             return f;
         };
+        v8h p[4];
 #pragma unroll
-        for(int b = 0; b < kBlocks; ++b)
+        for(int st = 0; st < 4; ++st) {
 #pragma unroll
-            for(int st = 0; st < 4; ++st) o[b] = mfma(values(b, st), p[st], o[b]);
+            for(int i = 0; i < 8; i += 2) {
+                const int   sub = st / 2, at = st % 2 * 8 + i;
+                const float p0  = __builtin_amdgcn_exp2f(fmaf(s[sub][at], c, -mc));
+                const float p1  = __builtin_amdgcn_exp2f(fmaf(s[sub][at + 1], c, -mc));
+                l += p0;
+                l += p1;
+                const v2h h  = __builtin_convertvector((v2f{p0, p1}), v2h);
+                p[st][i]     = h[0];
+                p[st][i + 1] = h[1];
+            }
+#pragma unroll
+            for(int b = 0; b < kBlocks; ++b) o[b] = mfma(values(b, st), p[st], o[b]);
+        }
 
         if(diag) {
             // A masked probability is 0, but 0 times an infinity or NaN is not: where
@@ -312,7 +332,8 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
                             const uint32_t ch = 32 * b + 8 * (i / 4) + 4 * half + i % 4;
                             const uint32_t v  = *(const __attribute__((address_space(3)))
                                                      uint16_t*)(uintptr_t)(
-                                vl + tok * D * 2 + value_chunk<D>(tok, ch / 8) * 16 + ch % 8 * 2);
+                                lds0 + off + kTileBytes + tok * D * 2 + value_chunk<D>(tok, ch / 8) * 16
+                                + ch % 8 * 2);
                             if(nonfinite(v)) o[b][i] += half_bits_to_float(v);
                         }
                 }

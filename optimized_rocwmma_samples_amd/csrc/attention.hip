@@ -3,8 +3,8 @@
 //   out[t, h] = sum_{j <= t} p[j] v[j],  p = softmax of scale * (q[t, h] . k[j])
 //
 // One pass over the keys with a running maximum m and sum l per query row.  A
-// block owns 128 query rows of one head, 32 per wave, and walks the key tiles of
-// 64 tokens from the diagonal down to the sequence's first.
+// block owns 128 query rows of one head, 32 per wave, and walks the key tiles from the
+// diagonal down to the sequence's first.
 //   * Scores are computed transposed, S^T = K Q^T with v_mfma_f32_32x32x16_f16
 //     (srcA = keys, srcB = queries): a lane then holds 16 of 32 keys' scores of
 //     ONE query row (lane % 32), so maximum, exponential, sum and the rescaling
@@ -38,9 +38,14 @@ typedef __attribute__((address_space(3))) v8h    lds_v8h_t;
 
 constexpr int kBufferFlags = 0x00020000; // raw buffer, 32-bit data format
 constexpr int kRows        = 128;        // query rows a block
-constexpr int kKeys        = 64;         // keys a tile
 constexpr int kWaves       = kRows / 32;
 constexpr int kThreads     = kWaves * kWave;
+
+// Keys a tile: 8 KB of keys and 8 KB of values either way.  Heads of 128 take 32, whose
+// scores need registers for 3 waves a SIMD (8192 tokens, 32 heads: 622 us; 64 keys
+// and 2 waves 656), heads of 64 take 64 (16 heads: 176 us; 32 keys 193).
+template <int D>
+constexpr int kKeysOf = D == 128 ? 32 : 64;
 
 // Where a block works: one sequence's rows and a tile of kRows of them.
 struct Span {
@@ -108,12 +113,11 @@ __device__ __forceinline__ v2f both_halves(float v)
     return {__uint_as_float(r[0]), __uint_as_float(r[1])};
 }
 
-// max(a, b, c) without the canonicalizing steps that fmaxf takes on matrix results.
+// max(a, b, c), NaN if one is: unlike fmaxf this takes no canonicalizing steps.  (Not in
+// inline asm, which the compiler does not keep apart from the matrix operations before it.)
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
 __device__ __forceinline__ bool nonfinite(uint32_t h16) { return (h16 & 0x7C00u) == 0x7C00u; }
@@ -146,13 +150,16 @@ __device__ __forceinline__ void load_lds(v4i rsrc, uint32_t to, uint32_t offset)
 
 __device__ __forceinline__ v4i buffer(const void* base, uint32_t bytes)
 {
-    const uint64_t at = (uint64_t)base;
-    return v4i{(int)(uint32_t)at, (int)((uint32_t)(at >> 32) & 0xFFFFu), (int)bytes, kBufferFlags};
+    const uint64_t at = (uint64_t)base; // uniform, which the compiler does not always see
+    return v4i{__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
+               __builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xFFFFu)),
+               __builtin_amdgcn_readfirstlane((int)bytes), kBufferFlags};
 }
 
 template <int D>
 __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* lds)
 {
+    constexpr int kKeys      = kKeysOf<D>, kSubs = kKeys / 32;
     constexpr int kTileBytes = kKeys * D * 2;
     constexpr int kChunks    = D / 8;                  // 16-byte chunks per row
     constexpr int kRowsLoad  = kWave / kChunks;        // rows one wave-load fills
@@ -241,31 +248,31 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
 
         const uint32_t off  = stage * 2 * kTileBytes;
         const bool     diag = (kt + 1) * kKeys > first; // some of it is later than some rows
-        v16f           s[2] = {};
+        v16f           s[kSubs] = {};
 #pragma unroll
         for(int st = 0; st < kSteps; ++st)
 #pragma unroll
-            for(int sub = 0; sub < 2; ++sub)
+            for(int sub = 0; sub < kSubs; ++sub)
                 s[sub] = mfma(*(const lds_v8h_t*)(uintptr_t)(kat[st] + off + sub * 32 * D * 2),
                               qf[st], s[sub]);
         if(diag) {
 #pragma unroll
-            for(int sub = 0; sub < 2; ++sub)
+            for(int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
                 for(int i = 0; i < 16; ++i) {
                     const uint32_t j = kt * kKeys + sub * 32 + 8 * (i / 4) + 4 * half + i % 4;
                     s[sub][i]        = j > qi ? -INFINITY : s[sub][i];
                 }
         }
-        float top = max3(s[0][0], s[1][0], s[0][1]);
+        float top = s[kSubs - 1][15];
 #pragma unroll
-        for(int i = 1; i < 15; ++i) top = max3(top, s[1][i], s[0][i + 1]);
-        top             = fmaxf(top, s[1][15]);
+        for(int i = 0; i < 16 * kSubs; i += 2)
+            top = max3(top, s[i / 16][i % 16], s[(i + 1) / 16][(i + 1) % 16]);
         const v2f   tops = both_halves(top);
         const float mn   = fmaxf(m, fmaxf(tops[0], tops[1]));
         // m need not be the maximum itself: the result is rescaled only where some row's
         // probabilities would pass 2^8 (far inside fp16), which after the first tiles is
-        // never, and not at every new maximum of one of 64 rows
+        // never, and not at every new maximum of one of 32 rows
         if(__ballot((mn - m) * c > 8.f) != 0) {
             const float al = __builtin_amdgcn_exp2f((m - mn) * c);
             m              = mn;
@@ -287,9 +294,9 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
             }
             return f;
         };
-        v8h p[4];
+        v8h p[2 * kSubs];
 #pragma unroll
-        for(int st = 0; st < 4; ++st) {
+        for(int st = 0; st < 2 * kSubs; ++st) {
 #pragma unroll
             for(int i = 0; i < 8; i += 2) {
                 const int   sub = st / 2, at = st % 2 * 8 + i;
@@ -320,7 +327,7 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
                 for(int b = 0; b < kBlocks; ++b) {
                     o[b] = v16f{};
 #pragma unroll
-                    for(int st = 0; st < 4; ++st)
+                    for(int st = 0; st < 2 * kSubs; ++st)
                         o[b] = mfma(finite_only(values(b, st)), p[st], o[b]);
                 }
                 for(uint32_t tok = 0; tok < kKeys; ++tok) {
@@ -357,9 +364,9 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 2) attention_kernel(AttentionArgs a)
+__global__ void __launch_bounds__(kThreads, 3) attention_kernel(AttentionArgs a)
 {
-    __shared__ alignas(16) uint8_t lds[2 * 2 * kKeys * D * 2]; // two stages of keys, values
+    __shared__ alignas(16) uint8_t lds[2 * 2 * kKeysOf<D> * D * 2]; // two stages of keys, values
     attention_rows<D>(a, lds);
 }
 

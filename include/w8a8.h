@@ -672,8 +672,9 @@ typedef struct w8a8_kv4_cache {
  *   scale  = half((max - min) / 15),  offset = half(min + 8 * scale)
  *   code   = clamp(rint((x - offset) / scale) + 8, 0, 15), 8 where scale = 0
  * A group of equal values is stored exactly (up to the fp16 it came in); one
- * that holds an infinity or a NaN reads back as NaN.  Two tokens given the same
- * slot leave in it the codes and scales of either, group by group.
+ * that holds an infinity or a NaN reads back as NaN.  The slots inside the cache
+ * are all different: of one that is given twice the row, and no other, is left
+ * with codes and scales of both tokens.
  *   k, v  fp16 [tokens, ldk / ldv] (0 means kv_heads * head_dim), head h in
  *         columns [h * head_dim, ...); 16-byte aligned, strides multiples of 8
  * `cache` is read on the host before the call returns.  tokens = 0 does nothing.

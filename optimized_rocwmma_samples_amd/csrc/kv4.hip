@@ -8,6 +8,9 @@
 namespace w8a8 {
 namespace {
 
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
 constexpr int kRowThreads = 256;
 
 struct CacheView {
@@ -41,116 +44,179 @@ __device__ __forceinline__ uint32_t code_byte(bool keys, uint32_t chunk)
     return keys ? (chunk % 4) * (D / 8) + (chunk / 4) * 4 : chunk * 4;
 }
 
-// Where thread `at` of the store and load kernels works: 8 channels (16 bytes
-// of fp16) of one token's key or value head.  Neighbouring threads take
-// neighbouring chunks, so the fp16 side moves whole lines.
+// How the store and load kernels share out their work: a thread takes 8 channels (16
+// bytes of fp16) of one token and head, of its keys and of its values.  Neighbouring
+// threads take neighbouring channels, so the fp16 side moves whole lines; a block has
+// some whole tokens, and the blocks of one XCD have neighbouring ones, whose rows share
+// lines of the cache (heads, not tokens, lie a page apart there).
+// (Keys and values by threads of their own, each finding its place by two divisions of
+// 64 bits, took 18.9 us to store and 12.8 to load 8192 tokens of 8 heads of 128; this
+// takes 11.3 and 8.7, and with two or four chunks a thread 13.3 and 15.6 to store.)
+struct RowPlan {
+    uint32_t blocks;    // a multiple of 8
+    uint32_t tokens;    // a block's
+    uint32_t per_token; // chunks of a token's keys or values
+    uint32_t inverse;   // ceil(2^32 / per_token) where a block has several tokens, else 0
+};
+
+// The block's first token, `tokens` where it has none: an XCD (block number modulo 8)
+// has a contiguous run.
+__device__ __forceinline__ uint32_t first_token(const RowPlan& p, uint32_t tokens)
+{
+    const uint32_t at = blockIdx.x % 8 * (p.blocks / 8) + blockIdx.x / 8;
+    return (uint32_t)min((uint64_t)at * p.tokens, (uint64_t)tokens);
+}
+
+// Where a block's i-th chunk is.
 template <int D>
 struct RowChunk {
-    uint32_t chunk, head, side;
-    uint64_t token;
-    bool     live;
-    size_t   row;
+    uint32_t chunk, head, token;
+    size_t   row; // in the cache
 
-    __device__ RowChunk(const CacheView& c, const Kv4Rows& r, uint64_t at)
+    __device__ RowChunk(const RowPlan& p, uint32_t token0, uint32_t i)
     {
-        chunk = at % (D / 8);
-        at /= D / 8;
-        head = at % c.kv_heads;
-        at /= c.kv_heads;
-        side  = at % 2;
-        token = at / 2;
-        live  = token < r.tokens;
-        row   = 0;
-        if(live) {
-            const int32_t slot = r.slots[token];
-            live               = slot >= 0 && (uint32_t)slot < c.slots;
-            if(live)
-                row = cache_row(c, (uint32_t)slot >> c.page_shift, head,
-                                (uint32_t)slot & (c.page_size - 1));
-        }
+        // exact: i * (inverse * per_token - 2^32) < 2^32, as a block has few chunks
+        // where inverse is not 0
+        const uint32_t t  = __umulhi(i, p.inverse);
+        const uint32_t at = i - t * p.per_token;
+        chunk             = at % (D / 8);
+        head              = at / (D / 8);
+        token             = token0 + t;
+    }
+
+    // its row; false where the slot lies outside the cache
+    __device__ bool place(const CacheView& c, int32_t slot)
+    {
+        if(slot < 0 || (uint32_t)slot >= c.slots) return false;
+        row = cache_row(c, (uint32_t)slot >> c.page_shift, head, (uint32_t)slot & (c.page_size - 1));
+        return true;
     }
 };
 
 // One step of a reduction over the G / 8 lanes of a group.
-template <int G, class Op>
-__device__ __forceinline__ float group_reduce(float v, Op op)
+template <int G, class T, class Op>
+__device__ __forceinline__ T group_reduce(T v, Op op)
 {
-    v = op(v, dpp_mov<kDppQuadXor1>(v));
-    v = op(v, dpp_mov<kDppQuadXor2>(v));
-    if constexpr(G >= 64) v = op(v, dpp_mov<kDppRowHalfMirror>(v));
-    if constexpr(G >= 128) v = op(v, dpp_mov<kDppRowMirror>(v));
+    const auto step = [&](auto dpp) {
+        v = op(v, __builtin_bit_cast(T, dpp_mov<decltype(dpp)::value>(__builtin_bit_cast(float, v))));
+    };
+    step(std::integral_constant<int, kDppQuadXor1>());
+    step(std::integral_constant<int, kDppQuadXor2>());
+    if constexpr(G >= 64) step(std::integral_constant<int, kDppRowHalfMirror>());
+    if constexpr(G >= 128) step(std::integral_constant<int, kDppRowMirror>());
     return v;
 }
 
-// Quantizes 8 channels a thread; the G / 8 threads of a group share its minimum
-// and maximum by DPP.  Memory bound: 16 bytes read and 4 (+ 4 / 4 of scales)
-// written per thread.
+// a / b rounded once, y = 1 / b rounded once (Markstein's theorem: the product and one
+// correction by the exact remainder), for quotients far from the ends of fp32's range.
+__device__ __forceinline__ float quotient(float a, float b, float y)
+{
+    const float q = a * y;
+    return fmaf(fmaf(-q, b, a), y, q);
+}
+
+// The 8 codes of a thread's channels and its group's (scale, offset).
+template <int G>
+__device__ __forceinline__ v2i quantized(v4i raw)
+{
+    // the group's extremes, two channels a register, NaN if one is
+    const auto x = __builtin_bit_cast(v8h, raw);
+    v2h        low = {x[0], x[1]}, high = low;
+#pragma unroll
+    for(int i = 2; i < 8; i += 2) {
+        const v2h h = {x[i], x[i + 1]};
+        low         = __builtin_elementwise_minimum(low, h);
+        high        = __builtin_elementwise_maximum(high, h);
+    }
+    low  = group_reduce<G>(low, [](v2h a, v2h b) { return __builtin_elementwise_minimum(a, b); });
+    high = group_reduce<G>(high, [](v2h a, v2h b) { return __builtin_elementwise_maximum(a, b); });
+    const float lo = (float)__builtin_elementwise_minimum(low[0], low[1]);
+    const float hi = (float)__builtin_elementwise_maximum(high[0], high[1]);
+
+    uint32_t    s16 = float_to_half_bits(quotient(hi - lo, 15.f, 1.f / 15.f));
+    const float s   = half_bits_to_float(s16);
+    uint32_t    c16 = float_to_half_bits_2step(fmaf(8.f, s, lo));
+    const float mid = half_bits_to_float(c16);
+    const bool  ok  = (hi - lo) * 0.f == 0.f; // no infinity and no NaN
+    if(!ok) s16 = c16 = 0x7E00u;
+    // A code is clamp(rint((x - mid) / s), -8, 7) + 8, and 8 where s is 0 or not finite
+    // (then y = 0).  Adding kRound rounds to an integer, which the sum's low bits
+    // hold; its other bits times the places' weights add up to kRest.
+    const float        y      = s > 0.f && ok ? 1.f / s : 0.f;
+    const float        from   = ok ? mid : 0.f;
+    constexpr float    kRound = 12582912.f + 8.f; // 1.5 2^23: units of 1
+    constexpr uint32_t kRest  = 0x4B400000u * 0x11111111u;
+    uint32_t           codes  = 0u - kRest;
+#pragma unroll
+    for(int i = 0; i < 8; ++i) {
+        const float q = __builtin_amdgcn_fmed3f(quotient((float)x[i] - from, s, y), -8.f, 7.f);
+        codes += __float_as_uint(q + kRound) << (4 * i);
+    }
+    return v2i{(int)(ok ? codes : 0x88888888u), (int)(s16 | (c16 << 16))};
+}
+
+// Quantizes rows.  Bound by memory: 16 bytes read and 4 (and 4 of scales a group)
+// written per 8 channels.
 template <int D, int G>
 __global__ void __launch_bounds__(kRowThreads)
-    kv4_store_kernel(CacheView c, Kv4Rows r, const uint16_t* __restrict__ k,
+    kv4_store_kernel(CacheView c, Kv4Rows r, RowPlan p, const uint16_t* __restrict__ k,
                      const uint16_t* __restrict__ v)
 {
-    const RowChunk<D> t(c, r, (uint64_t)blockIdx.x * kRowThreads + threadIdx.x);
-    // groups are whole within a token, so the lanes of a group are live together
-    float x[8];
-    float low = INFINITY, high = -INFINITY, bad = 0.f;
-    v4i   raw = {};
-    if(t.live)
-        raw = *reinterpret_cast<const v4i*>((t.side ? v + t.token * r.ldv : k + t.token * r.ldk)
-                                            + t.head * D + t.chunk * 8);
+    const uint32_t token0 = first_token(p, r.tokens);
+    const uint32_t count  = min(p.tokens, r.tokens - token0) * p.per_token;
+    for(uint32_t i = threadIdx.x; i < count; i += kRowThreads) {
+        RowChunk<D>    t(p, token0, i);
+        const uint32_t at     = t.head * D + t.chunk * 8;
+        const int32_t  slot   = r.slots[t.token];
+        const v4i      raw[2] = {*reinterpret_cast<const v4i*>(k + (size_t)t.token * r.ldk + at),
+                                 *reinterpret_cast<const v4i*>(v + (size_t)t.token * r.ldv + at)};
+        // groups are whole within a token: their lanes go on together
+        if(!t.place(c, slot)) continue;
 #pragma unroll
-    for(int i = 0; i < 8; ++i) {
-        x[i] = half_bits_to_float((uint32_t)raw[i / 2] >> (16 * (i % 2)));
-        low  = fminf(low, x[i]);
-        high = fmaxf(high, x[i]);
-        bad += x[i] * 0.f; // NaN where x is an infinity or NaN
+        for(int side = 0; side < 2; ++side) {
+            const v2i q = quantized<G>(raw[side]);
+            *reinterpret_cast<int32_t*>(c.codes[side] + t.row * (D / 2)
+                                        + code_byte<D>(side == 0, t.chunk))
+                = q[0];
+            if(t.chunk % (G / 8) == 0)
+                c.scales[side][t.row * (D / G) + t.chunk / (G / 8)] = (uint32_t)q[1];
+        }
     }
-    low  = group_reduce<G>(low, [](float a, float b) { return fminf(a, b); });
-    high = group_reduce<G>(high, [](float a, float b) { return fmaxf(a, b); });
-    bad  = group_reduce<G>(bad, [](float a, float b) { return a + b; });
-    if(!t.live) return;
-    uint32_t     s16 = float_to_half_bits((high - low) / 15.f);
-    const float  s   = half_bits_to_float(s16);
-    uint32_t     c16 = float_to_half_bits_2step(fmaf(8.f, s, low));
-    const float  mid = half_bits_to_float(c16);
-    const bool   ok  = bad == 0.f;
-    if(!ok) s16 = c16 = 0x7E00u;
-    uint32_t codes = 0;
-#pragma unroll
-    for(int i = 0; i < 8; ++i) {
-        const float n = s > 0.f && ok
-                            ? fminf(fmaxf(__builtin_rintf((x[i] - mid) / s) + 8.f, 0.f), 15.f)
-                            : 8.f;
-        codes |= (uint32_t)n << (4 * i);
-    }
-    *reinterpret_cast<uint32_t*>(c.codes[t.side] + t.row * (D / 2)
-                                 + code_byte<D>(t.side == 0, t.chunk))
-        = codes;
-    if(t.chunk % (G / 8) == 0)
-        c.scales[t.side][t.row * (D / G) + t.chunk / (G / 8)] = s16 | (c16 << 16);
 }
 
 template <int D, int G>
 __global__ void __launch_bounds__(kRowThreads)
-    kv4_load_kernel(CacheView c, Kv4Rows r, uint16_t* __restrict__ k, uint16_t* __restrict__ v)
+    kv4_load_kernel(CacheView c, Kv4Rows r, RowPlan p, uint16_t* __restrict__ k,
+                    uint16_t* __restrict__ v)
 {
-    const RowChunk<D> t(c, r, (uint64_t)blockIdx.x * kRowThreads + threadIdx.x);
-    if(!t.live) return;
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(
-        c.codes[t.side] + t.row * (D / 2) + code_byte<D>(t.side == 0, t.chunk));
-    const uint32_t sc  = c.scales[t.side][t.row * (D / G) + t.chunk / (G / 8)];
-    const float    s   = half_bits_to_float(sc & 0xFFFFu);
-    const float    mid = half_bits_to_float(sc >> 16);
-    v4i            out;
+    const uint32_t token0 = first_token(p, r.tokens);
+    const uint32_t count  = min(p.tokens, r.tokens - token0) * p.per_token;
+    for(uint32_t i = threadIdx.x; i < count; i += kRowThreads) {
+        RowChunk<D> t(p, token0, i);
+        if(!t.place(c, r.slots[t.token])) continue;
+        uint32_t codes[2], scales[2];
 #pragma unroll
-    for(int i = 0; i < 4; ++i) {
-        const float a = fmaf(s, (float)((codes >> (8 * i)) & 15u) - 8.f, mid);
-        const float b = fmaf(s, (float)((codes >> (8 * i + 4)) & 15u) - 8.f, mid);
-        out[i]        = (int)float2_to_half2_bits_2step(a, b);
+        for(int side = 0; side < 2; ++side) {
+            codes[side] = *reinterpret_cast<const uint32_t*>(
+                c.codes[side] + t.row * (D / 2) + code_byte<D>(side == 0, t.chunk));
+            scales[side] = c.scales[side][t.row * (D / G) + t.chunk / (G / 8)];
+        }
+#pragma unroll
+        for(int side = 0; side < 2; ++side) {
+            const float s   = half_bits_to_float(scales[side] & 0xFFFFu);
+            const float mid = half_bits_to_float(scales[side] >> 16);
+            v4i         out;
+#pragma unroll
+            for(int j = 0; j < 4; ++j) {
+                const uint32_t w = codes[side] >> (8 * j);
+                const float    a = fmaf(s, (float)(w & 15u) - 8.f, mid);
+                const float    b = fmaf(s, (float)(w >> 4 & 15u) - 8.f, mid);
+                out[j]           = (int)float2_to_half2_bits_2step(a, b);
+            }
+            uint16_t* to = side ? v + (size_t)t.token * r.ldv : k + (size_t)t.token * r.ldk;
+            *reinterpret_cast<v4i*>(to + t.head * D + t.chunk * 8) = out;
+        }
     }
-    *reinterpret_cast<v4i*>((t.side ? v + t.token * r.ldv : k + t.token * r.ldk) + t.head * D
-                            + t.chunk * 8)
-        = out;
 }
 
 // The instantiation for a cache's head width and group.
@@ -173,10 +239,15 @@ void with_widths(const w8a8_kv4_cache& c, F f)
     }
 }
 
-uint32_t row_blocks(const w8a8_kv4_cache& c, const Kv4Rows& r)
+// As many tokens a block as one round of its threads takes, and one where that is less.
+RowPlan row_plan(const w8a8_kv4_cache& c, const Kv4Rows& r)
 {
-    const uint64_t threads = (uint64_t)r.tokens * 2 * c.kv_heads * (c.head_dim / 8);
-    return (uint32_t)((threads + kRowThreads - 1) / kRowThreads);
+    const uint32_t per_token = c.kv_heads * (c.head_dim / 8);
+    const uint32_t tokens    = std::max(1u, kRowThreads / per_token);
+    const uint32_t inverse
+        = tokens > 1 ? (uint32_t)(((1ull << 32) + per_token - 1) / per_token) : 0;
+    const uint32_t blocks = (uint32_t)(((uint64_t)r.tokens + tokens - 1) / tokens);
+    return {(blocks + 7) / 8 * 8, tokens, per_token, inverse};
 }
 
 // ---------------------------------------------------------------------------
@@ -215,8 +286,6 @@ uint32_t row_blocks(const w8a8_kv4_cache& c, const Kv4Rows& r)
 // products of C tiles add up in one accumulator.  A column is then a partial of its
 // own, with its own maximum, sum and part of the result, merged at the unit's end.
 // ---------------------------------------------------------------------------
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float    v2f __attribute__((ext_vector_type(2)));
 
 typedef __attribute__((address_space(3))) v2i      lds_v2i_t;
@@ -911,7 +980,8 @@ hipError_t launch_kv4_store(const w8a8_kv4_cache& c, const Kv4Rows& r, const uin
                             const uint16_t* v, hipStream_t stream)
 {
     with_widths(c, [&](auto d, auto g) {
-        kv4_store_kernel<d(), g()><<<row_blocks(c, r), kRowThreads, 0, stream>>>(view(c), r, k, v);
+        const RowPlan p = row_plan(c, r);
+        kv4_store_kernel<d(), g()><<<p.blocks, kRowThreads, 0, stream>>>(view(c), r, p, k, v);
     });
     return hipGetLastError();
 }
@@ -920,7 +990,8 @@ hipError_t launch_kv4_load(const w8a8_kv4_cache& c, const Kv4Rows& r, uint16_t* 
                            hipStream_t stream)
 {
     with_widths(c, [&](auto d, auto g) {
-        kv4_load_kernel<d(), g()><<<row_blocks(c, r), kRowThreads, 0, stream>>>(view(c), r, k, v);
+        const RowPlan p = row_plan(c, r);
+        kv4_load_kernel<d(), g()><<<p.blocks, kRowThreads, 0, stream>>>(view(c), r, p, k, v);
     });
     return hipGetLastError();
 }

@@ -40,6 +40,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 SOURCES = [
     "capi.cpp",
+    "capi_serving.cpp",
     "smoothquant.hip",
     "gemm_i8.hip",
     "moe.hip",

@@ -1,14 +1,22 @@
 // w8a8_internal.hpp -- launchers shared between the kernel files and the C ABI.
-// Callers (capi.cpp) have validated every argument before these run.
+// Callers (capi.cpp, capi_serving.cpp) have validated every argument before these run.
 #pragma once
 
 #include "../../include/w8a8.h"
 
+#include <cmath>
 #include <hip/hip_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
 
 namespace w8a8 {
+
+// ---- Status of the C entry points (capi.cpp) -----------------------------------
+// Sets the thread's message and returns the code; the status of a HIP call.
+int fail(int code, const char* fmt, ...);
+int hip_status(hipError_t e, const char* what);
+
+inline bool valid_qmax(float q) { return std::isfinite(q) && q > 0.f && q <= 127.f; }
 
 // Describes where quantizer row `i` reads from and writes to.
 struct QuantRows {

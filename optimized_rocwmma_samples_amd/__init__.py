@@ -801,7 +801,8 @@ def attention(q, k, v, seq_starts, scale: float | None = None, out=None):
     slices of one projection's output are fine (any row stride that is a
     multiple of 8; the heads of a token side by side).  seq_starts int32
     [seqs + 1] on the device, ascending: sequence i is rows seq_starts[i] ..
-    seq_starts[i + 1].  scale: 1 / sqrt(head_dim) unless given.  Returns fp16
+    seq_starts[i + 1].  scale: 1 / sqrt(head_dim) unless given.  out may not
+    overlap q, k or v.  Returns fp16
     [tokens, heads, head_dim]; rows of no sequence are left as they were in
     `out` (undefined in a new tensor)."""
     torch = _torch()
@@ -883,7 +884,8 @@ def kv4_store(k, v, slots, cache: KV4Cache) -> None:
     """Quantize the keys and values of some tokens into the cache: k, v fp16
     [tokens, kv_heads, head_dim] (any row stride that is a multiple of 8), token
     t into slot slots[t] = page * page_size + place (int32; a slot outside the
-    cache skips its token; the slots of one call should differ)."""
+    cache skips its token).  The slots of one call inside the cache are all
+    different: a row given twice is left with parts of both tokens."""
     _require_on(cache.device, k=k, v=v, slots=slots)
     n = _kv4_slots(slots)
     ldk = _heads3d("k", k, cache.kv_heads, cache.head_dim)
@@ -932,8 +934,8 @@ def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None
     column stride): the page of each page_size tokens of a sequence; seq_lens
     int32 [seqs]: the tokens to attend to, the new one (stored before) among
     them.  Returns fp16 [seqs, heads, head_dim]; a sequence of no tokens gives
-    zeros.  workspace: 'auto' (allocated here), None (each head of a sequence is
-    one block's work) or a device tensor of attention_kv4_workspace_size bytes."""
+    zeros.  workspace: 'auto' (allocated here), None (all of a key head's
+    context is one wave's work) or a device tensor of attention_kv4_workspace_size bytes."""
     torch = _torch()
     dev = cache.device
     _require_on(dev, q=q, block_table=block_table, seq_lens=seq_lens, out=out)

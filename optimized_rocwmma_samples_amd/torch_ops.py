@@ -12,10 +12,14 @@ them without a graph break.
     pw = w8a8.pack_weights(w)                        # once; the op takes pw.data and pw.n
     c, q, r = torch.ops.w8a8.fused_sq_gemm_packed(x, s, pw.data, pw.n, sb)
     out = torch.ops.w8a8.moe_ffn(x, logits, s, w_gu, sb_gu, w_d, sb_d, 2)
+    out = torch.ops.w8a8.moe_ffn_decode(x, logits, s, w_gu, sb_gu, w_d, sb_d, 2)  # <= 16 tokens
+    out = torch.ops.w8a8.attention(q, k, v, seq_starts)
+    torch.ops.w8a8.kv4_store(k, v, slots, kc, vc, ks, vs)   # a KV4Cache's four tensors
+    out = torch.ops.w8a8.attention_kv4(q, kc, vc, ks, vs, block_table, seq_lens)
 
 The ops are functional (every output is a new tensor), as torch.library
-custom ops must be; the package functions keep the in-place and
-preallocated-output forms.  They run only on device tensors: a CPU tensor
+custom ops must be, but for kv4_store, which writes the cache it is given; the
+package functions keep the in-place and preallocated-output forms.  They run only on device tensors: a CPU tensor
 raises, as everywhere in the package (there is no CPU path).
 
 Reference kernels: smoothquant <- kernel_smoothquant
@@ -34,13 +38,18 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import PackedWeights
+from . import KV4Cache, PackedWeights
 from . import add_rmsnorm_smoothquant as _add_rmsnorm_smoothquant
+from . import attention as _attention
+from . import attention_kv4 as _attention_kv4
 from . import fused_sq_gemm as _fused_sq_gemm
 from . import fused_sq_gemm_packed as _fused_sq_gemm_packed
 from . import gemm as _gemm
 from . import gemm_packed as _gemm_packed
+from . import kv4_load as _kv4_load
+from . import kv4_store as _kv4_store
 from . import moe_ffn as _moe_ffn
+from . import moe_ffn_decode as _moe_ffn_decode
 from . import smoothquant as _smoothquant
 
 Tensor = torch.Tensor
@@ -165,3 +174,72 @@ def moe_ffn(x: Tensor, logits: Tensor, smooth_scale: Tensor, w_gate_up: Tensor,
 def _(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_down, topk,
       smooth_scale_down=None, unit_size=32, gate_up_interleaved=False):
     return torch.empty_like(x, dtype=torch.float16)
+
+
+@torch.library.custom_op("w8a8::moe_ffn_decode", mutates_args=())
+def moe_ffn_decode(x: Tensor, logits: Tensor, smooth_scale: Tensor, w_gate_up: Tensor,
+                   sb_gate_up: Tensor, w_down: Tensor, sb_down: Tensor, topk: int,
+                   smooth_scale_down: Optional[Tensor] = None,
+                   quant_max: float = 127.0) -> Tensor:
+    """The expert FFN of at most 16 tokens x [T, H] (fp16 out [T, H]) in two launches."""
+    return _moe_ffn_decode(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_down, topk,
+                           smooth_scale_down, quant_max)
+
+
+@moe_ffn_decode.register_fake
+def _(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_down, topk,
+      smooth_scale_down=None, quant_max=127.0):
+    return x.new_empty(x.shape, dtype=torch.float16)
+
+
+@torch.library.custom_op("w8a8::attention", mutates_args=())
+def attention(q: Tensor, k: Tensor, v: Tensor, seq_starts: Tensor,
+              scale: Optional[float] = None) -> Tensor:
+    """Causal attention of packed prompts: fp16 [tokens, heads, head_dim]; rows of no
+    sequence are undefined."""
+    return _attention(q, k, v, seq_starts, scale)
+
+
+@attention.register_fake
+def _(q, k, v, seq_starts, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("w8a8::kv4_store",
+                         mutates_args=("k_codes", "v_codes", "k_scales", "v_scales"))
+def kv4_store(k: Tensor, v: Tensor, slots: Tensor, k_codes: Tensor, v_codes: Tensor,
+              k_scales: Tensor, v_scales: Tensor) -> None:
+    """Quantizes k, v [tokens, kv_heads, head_dim] into the slots of a KV4Cache's tensors."""
+    _kv4_store(k, v, slots, KV4Cache(k_codes, v_codes, k_scales, v_scales))
+
+
+@kv4_store.register_fake
+def _(k, v, slots, k_codes, v_codes, k_scales, v_scales):
+    return None
+
+
+@torch.library.custom_op("w8a8::kv4_load", mutates_args=())
+def kv4_load(slots: Tensor, k_codes: Tensor, v_codes: Tensor, k_scales: Tensor,
+             v_scales: Tensor) -> Tuple[Tensor, Tensor]:
+    """(k, v) fp16 [n, kv_heads, head_dim] of the slots; undefined for slots outside."""
+    return _kv4_load(KV4Cache(k_codes, v_codes, k_scales, v_scales), slots)
+
+
+@kv4_load.register_fake
+def _(slots, k_codes, v_codes, k_scales, v_scales):
+    shape = (slots.shape[0], k_codes.shape[1], k_codes.shape[3] * 2)
+    return k_scales.new_empty(shape), k_scales.new_empty(shape)
+
+
+@torch.library.custom_op("w8a8::attention_kv4", mutates_args=())
+def attention_kv4(q: Tensor, k_codes: Tensor, v_codes: Tensor, k_scales: Tensor, v_scales: Tensor,
+                  block_table: Tensor, seq_lens: Tensor, scale: Optional[float] = None) -> Tensor:
+    """Attention of one token per sequence, q [seqs, heads, head_dim], over a KV4Cache's
+    tensors; workspace allocated as the lengths need."""
+    return _attention_kv4(q, KV4Cache(k_codes, v_codes, k_scales, v_scales), block_table, seq_lens,
+                          scale)
+
+
+@attention_kv4.register_fake
+def _(q, k_codes, v_codes, k_scales, v_scales, block_table, seq_lens, scale=None):
+    return q.new_empty(q.shape)

@@ -56,6 +56,8 @@ struct Ws {
     float*   top;    // [pairs, kGateUpBlocks]: max |act| over a block's columns
     int32_t* ids;    // [pairs]
     float*   weight; // [pairs]
+    float*   scale;  // [pairs]: of the quantized activations
+    int8_t*  q;      // [pairs, inter]: those, where the down kernel cannot hold them
 };
 
 Ws carve(const MoeDecodeArgs& a)
@@ -70,6 +72,10 @@ Ws carve(const MoeDecodeArgs& a)
     w.ids = reinterpret_cast<int32_t*>(p);
     p += up256(n * 4);
     w.weight = reinterpret_cast<float*>(p);
+    p += up256(n * 4);
+    w.scale = reinterpret_cast<float*>(p);
+    p += up256(n * 4);
+    w.q = reinterpret_cast<int8_t*>(p);
     return w;
 }
 
@@ -433,27 +439,93 @@ __global__ void __launch_bounds__(kThreads, 2 * BLOCKS) gate_up_kernel(MoeDecode
 }
 
 // ---------------------------------------------------------------------------
-// Second kernel: a block owns 16 / FOLD output columns of all active experts.
-// FOLD > 1 (at most 16 / FOLD tokens): the tile's 16 weight rows are the columns'
-// FOLD parts along K, and its 16 columns the rows' parts likewise; the blocks on the
-// tile's diagonal are the partial sums, the others are not used.  So a small hidden
-// size still gives a block to every CU, with whole 16-byte loads.
-//
-// ALL: the quantized rows of all pairs lie in LDS.  Otherwise one expert's rows over
-// `chunk` columns, in two buffers: 8 more waves quantize the next while 8 multiply.
+// Between them, where the down kernel does not hold the rows itself: the activations in 8
+// bits, once for all of its blocks, 16 columns a thread of one pair's row a block row.
+// (Every block quantizing chunks of the rows into LDS beside its stream: 16 tokens of 8
+// experts of 4096 x 14336 308 us the layer, XX now.)
 // ---------------------------------------------------------------------------
-constexpr int kDownSteps = 4; // steps a batch: 4 KB a wave
+constexpr int kRequantThreads = 256;
 
 struct DownLds {
     uint32_t bits[kWords];
     uint32_t active;
 };
 
-template <int FOLD, bool ALL, int RING>
-__device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint32_t chunk,
-                                     uint32_t gu_blocks, DownLds& lds, uint8_t* dyn)
+// A pair's max |act| by one wave, from the maxima that gate_up_kernel's blocks left.
+__device__ __forceinline__ float row_top(const MoeDecodeArgs& a, const Ws& ws, const Lists& lists,
+                                         uint32_t p, uint32_t active, uint32_t gu_blocks, int lane)
 {
-    constexpr uint32_t kCols = kTile / FOLD, kAll = ALL ? kThreads : 2 * kThreads;
+    if(lists.ids[p] < 0) return 0.f;
+    const uint32_t tiles = a.inter / kTile, units = active * tiles, u = lists.order[p] * tiles;
+    const uint32_t b1 = block_of(u + tiles - 1, units, gu_blocks);
+    float          m  = 0.f;
+    for(uint32_t b = block_of(u, units, gu_blocks) + lane; b <= b1; b += kWave)
+        if(first_unit(b, units, gu_blocks) < first_unit(b + 1, units, gu_blocks))
+            m = fmaxf(m, ws.top[(size_t)p * kGateUpBlocks + b]); // it had work
+    return wave_max(m);
+}
+
+// 16 columns of one pair's activations from k on, and their quantized form.
+struct Piece {
+    v4f f[4];
+};
+
+__device__ __forceinline__ void fetch_piece(Piece& x, const MoeDecodeArgs& a, const Ws& ws,
+                                            uint32_t p, uint32_t k)
+{
+    const float* h = ws.act + (size_t)p * a.inter + k;
+#pragma unroll
+    for(int c = 0; c < 4; ++c)
+        x.f[c] = k < a.inter ? *reinterpret_cast<const v4f*>(h + 4 * c) : v4f{0, 0, 0, 0};
+}
+
+__device__ __forceinline__ void store_piece(const Piece& x, float inv, float qmax, int8_t* to)
+{
+    v4i w;
+#pragma unroll
+    for(int c = 0; c < 4; ++c)
+        w[c] = (int)cvt_pack4_i8(quant_f(x.f[c][0], inv, qmax), quant_f(x.f[c][1], inv, qmax),
+                                 quant_f(x.f[c][2], inv, qmax), quant_f(x.f[c][3], inv, qmax));
+    *reinterpret_cast<v4i*>(to) = w;
+}
+
+__global__ void __launch_bounds__(kRequantThreads)
+    requant_kernel(MoeDecodeArgs a, Ws ws, uint32_t gu_blocks)
+{
+    extern __shared__ uint8_t dyn[];
+    __shared__ DownLds        lds;
+    const uint32_t tid = threadIdx.x, pairs = a.tokens * a.topk, p = blockIdx.y;
+    const uint32_t k = (blockIdx.x * kRequantThreads + tid) * 16;
+    Lists          lists(dyn, pairs);
+    Piece          x;
+    fetch_piece(x, a, ws, p, k);
+    for(uint32_t i = tid; i < (uint32_t)kWords; i += kRequantThreads) lds.bits[i] = 0;
+    if(tid == 0) lds.active = 0;
+    for(uint32_t i = tid; i < pairs; i += kRequantThreads) lists.ids[i] = ws.ids[i];
+    __syncthreads();
+    lists.build(pairs, kRequantThreads, lds.bits, &lds.active);
+    const float r = row_top(a, ws, lists, p, lds.active, gu_blocks, tid % kWave) / a.qmax;
+    if(k < a.inter) store_piece(x, r > 0.f ? 1.f / r : 0.f, a.qmax, ws.q + (size_t)p * a.inter + k);
+    if(blockIdx.x == 0 && tid == 0) ws.scale[p] = r;
+}
+
+// ---------------------------------------------------------------------------
+// Second kernel: a block owns 16 / FOLD output columns of all active experts.
+// FOLD > 1 (at most 16 / FOLD tokens): the tile's 16 weight rows are the columns'
+// FOLD parts along K, and its 16 columns the rows' parts likewise; the blocks on the
+// tile's diagonal are the partial sums, the others are not used.  So a small hidden
+// size still gives a block to every CU, with whole 16-byte loads.
+//
+// HOLD: the block quantizes the rows of all pairs into LDS itself.  Otherwise it reads
+// them as operands from requant_kernel's, out of L2, beside its weights: that is as
+// many loads again, but no barrier and nothing that every block does anew.
+// ---------------------------------------------------------------------------
+template <int FOLD, bool HOLD, int RING>
+__device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint32_t gu_blocks,
+                                     DownLds& lds, uint8_t* dyn)
+{
+    constexpr uint32_t kCols  = kTile / FOLD;
+    constexpr int      kSteps = HOLD ? 4 : 2; // steps a batch: 4 KB a wave, or 2 and 2
     const int      wave  = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int      lane  = threadIdx.x % kWave, col = lane % 16, kg = lane / 16;
     const uint32_t pairs = a.tokens * a.topk, tid = threadIdx.x;
@@ -463,213 +535,142 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
     float*         inverse = reinterpret_cast<float*>(at0 + Lists::up16(pairs));
     int32_t*       sums = reinterpret_cast<int32_t*>(at0 + 2 * Lists::up16(pairs)); // [pairs][kCols]
     int8_t* q = reinterpret_cast<int8_t*>(at0 + 2 * Lists::up16(pairs) + pairs * kTile * 4);
-    const uint32_t j0 = blockIdx.x * kCols, rb = row_bytes(chunk);
-    const uint32_t tiles = a.inter / kTile;
+    const uint32_t j0 = blockIdx.x * kCols, rb = row_bytes(a.inter);
 
-    for(uint32_t i = tid; i < (uint32_t)kWords; i += kAll) lds.bits[i] = 0;
+    for(uint32_t i = tid; i < (uint32_t)kWords; i += kThreads) lds.bits[i] = 0;
     if(tid == 0) lds.active = 0;
-    for(uint32_t p = tid; p < pairs; p += kAll) lists.ids[p] = ws.ids[p];
-    for(uint32_t i = tid; i < pairs * kCols; i += kAll) sums[i] = 0;
-    __syncthreads();
-    lists.build(pairs, kAll, lds.bits, &lds.active);
-    const uint32_t n = lds.active, units = n * tiles;
-
-    // ---- the pairs' scales, from the maxima that the first kernel's blocks left -----
-    for(uint32_t p = wave; p < pairs; p += kAll / kWave) {
-        float m = 0.f;
-        if(lists.ids[p] >= 0) {
-            const uint32_t u  = lists.order[p] * tiles;
-            const uint32_t b1 = block_of(u + tiles - 1, units, gu_blocks);
-            for(uint32_t b = block_of(u, units, gu_blocks) + lane; b <= b1; b += kWave)
-                if(first_unit(b, units, gu_blocks) < first_unit(b + 1, units, gu_blocks))
-                    m = fmaxf(m, ws.top[(size_t)p * kGateUpBlocks + b]); // it had work
-            m = wave_max(m);
-        }
-        if(lane == 0) {
-            const float r = m / a.qmax;
-            scale[p]      = r;
-            inverse[p]    = r > 0.f ? 1.f / r : 0.f;
-        }
+    for(uint32_t p = tid; p < pairs; p += kThreads) {
+        lists.ids[p] = ws.ids[p];
+        if constexpr(!HOLD) scale[p] = ws.scale[p];
     }
+    for(uint32_t i = tid; i < pairs * kCols; i += kThreads) sums[i] = 0;
     __syncthreads();
+    lists.build(pairs, kThreads, lds.bits, &lds.active);
+    const uint32_t n = lds.active;
 
-    // 16 columns from k on of one pair's activations, and their quantized form to LDS
-    struct Piece {
-        v4f f[4];
-    };
-    auto fetch = [&](Piece& x, uint32_t p, uint32_t k) {
-        const float* h = ws.act + (size_t)p * a.inter + k;
-#pragma unroll
-        for(int c = 0; c < 4; ++c)
-            x.f[c] = k < a.inter ? *reinterpret_cast<const v4f*>(h + 4 * c) : v4f{0, 0, 0, 0};
-    };
-    auto store = [&](const Piece& x, uint32_t p, int8_t* to) {
-        const float inv = inverse[p];
-        v4i         w;
-#pragma unroll
-        for(int c = 0; c < 4; ++c)
-            w[c] = (int)cvt_pack4_i8(quant_f(x.f[c][0], inv, a.qmax), quant_f(x.f[c][1], inv, a.qmax),
-                                     quant_f(x.f[c][2], inv, a.qmax), quant_f(x.f[c][3], inv, a.qmax));
-        *reinterpret_cast<v4i*>(to) = w;
-    };
-    auto quantize = [&](uint32_t p, uint32_t k, int8_t* to) {
-        Piece x;
-        fetch(x, p, k);
-        store(x, p, to);
-    };
-    const uint32_t per_row = (rb - 16) / 16; // 16-column pieces of a row in LDS
-    const uint32_t chunks  = ALL ? 1 : (a.inter + chunk - 1) / chunk;
-    // the rows of phase (expert, chunk), by 8 waves of which this is `w`: as many a row as
-    // the rows leave (and no divisions: those by a row's pieces took 2 us a phase)
-    auto fill = [&](uint32_t phase, uint32_t w) {
-        const uint32_t ai = phase / chunks, rows = lists.rows(ai), k0 = phase % chunks * chunk;
-        const uint32_t shift = rows > 4 ? 0 : rows > 2 ? 1 : rows > 1 ? 2 : 3;
-        for(uint32_t r = w >> shift; r < rows; r += kWaves >> shift) {
-            const uint32_t p  = lists.pair[ai * kRows + r];
-            int8_t*        to = q + (phase % 2 * a.tokens + r) * rb;
-            const uint32_t step = kWave << shift;
-            for(uint32_t i0 = (w & ((1u << shift) - 1)) * kWave + lane; i0 < per_row; i0 += 4 * step) {
-                Piece x[4]; // 4 loads overlap
-#pragma unroll
-                for(int j = 0; j < 4; ++j)
-                    if(i0 + j * step < per_row) fetch(x[j], p, k0 + (i0 + j * step) * 16);
-#pragma unroll
-                for(int j = 0; j < 4; ++j)
-                    if(i0 + j * step < per_row) store(x[j], p, to + (i0 + j * step) * 16);
+    if constexpr(HOLD) {
+        for(uint32_t p = wave; p < pairs; p += kWaves) {
+            const float r = row_top(a, ws, lists, p, n, gu_blocks, lane) / a.qmax;
+            if(lane == 0) {
+                scale[p]   = r;
+                inverse[p] = r > 0.f ? 1.f / r : 0.f;
             }
         }
-    };
+        __syncthreads();
+    }
 
-    // ---- the stream of weights: items are experts (ALL) or (expert, chunk) -----------
-    const uint32_t most = (ALL ? a.inter : min(chunk, a.inter)) + 63;
-    const uint32_t part = (most / 64 + FOLD - 1) / FOLD; // steps of a part of an item's K
-    const uint32_t per  = (part + kDownSteps - 1) / kDownSteps;
-    const uint32_t items = n * chunks;
-    // one run over all items, or one within every item
-    const Run run(ALL ? items * per : per, wave % kWaves);
-    const bool     streams = ALL || wave < kWaves;
-    const uint32_t mine    = streams ? (ALL ? run.to - run.from : (run.to - run.from) * items) : 0;
-    v4i            ring[RING][kDownSteps];
-    Cursor         ahead(ALL ? run.from : 0, per), now = ahead;
-    if(!ALL) ahead.b = now.b = run.from;
-    auto advance = [&](Cursor& c) {
-        if(ALL)
-            c.advance(per);
-        else if(++c.b == run.to) {
-            c.b = run.from;
-            ++c.item;
-        }
-    };
+    // ---- the stream of weights, all experts in one run a wave ------------------------
+    const uint32_t part = ((a.inter + 63) / 64 + FOLD - 1) / FOLD; // steps of a part of K
+    const uint32_t per  = (part + kSteps - 1) / kSteps;
+    const Run      run(n * per, wave);
+    const uint32_t mine = run.to - run.from;
+    v4i            ring[RING][kSteps], rows8[HOLD ? 1 : RING][kSteps];
+    Cursor         ahead(run.from, per), now = ahead;
     const uint32_t row = col % kCols, fold = col / kCols; // of the weights, and of the tokens
-    uint32_t       loaded = 0;
-    auto           load   = [&](int slot) {
-        const uint32_t               e = lists.expert_at(ahead.item / chunks);
-        const uint32_t               k0 = ahead.item % chunks * chunk;
-        const __amdgpu_buffer_rsrc_t r  = __builtin_amdgcn_make_buffer_rsrc(
+    uint32_t       loaded = 0, item = ~0u, from8 = 0;
+    const __amdgpu_buffer_rsrc_t r8 = __builtin_amdgcn_make_buffer_rsrc(
+        ws.q, 0, (int)(pairs * a.inter), kBufferFlags);
+    auto load = [&](int slot) {
+        const uint32_t               e = lists.expert_at(ahead.item);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<int8_t*>(a.wd + ((size_t)e * a.hidden + j0) * a.inter), 0,
             (int)(kCols * a.inter), kBufferFlags);
+        if constexpr(!HOLD)
+            if(ahead.item != item) { // lanes past the expert's rows take its last one
+                item  = ahead.item;
+                from8 = lists.pair[item * kRows + min(row, lists.rows(item) - 1)] * a.inter;
+            }
 #pragma unroll
-        for(int i = 0; i < kDownSteps; ++i) {
-            const uint32_t st = ahead.b * kDownSteps + i, k = k0 + (fold * part + st) * 64 + kg * 16;
-            const bool     in = st < part && k < a.inter && (ALL || k < k0 + chunk);
+        for(int i = 0; i < kSteps; ++i) {
+            const uint32_t st = ahead.b * kSteps + i, k = (fold * part + st) * 64 + kg * 16;
+            const bool     in = st < part && k < a.inter;
             ring[slot][i]     = load_weights(r, in ? row * a.inter + k : kOob);
+            if constexpr(!HOLD)
+                rows8[slot][i] = __builtin_bit_cast(
+                    v4i, __builtin_amdgcn_raw_buffer_load_b128(r8, in ? from8 + k : kOob, 0, 0));
         }
-        advance(ahead);
+        ahead.advance(per);
         ++loaded;
     };
     // a thread's first pieces go out ahead of the weights: behind them they would wait for
     // all of those
-    constexpr uint32_t kAhead = ALL ? 2 : 0;
-    Piece              first[ALL ? kAhead : 1];
-    const uint32_t     all = pairs * per_row;
-    if constexpr(ALL)
+    constexpr uint32_t kAhead = HOLD ? 2 : 0;
+    const uint32_t     per_row = (rb - 16) / 16, all = HOLD ? pairs * per_row : 0;
+    Piece              first[HOLD ? kAhead : 1];
+    if constexpr(HOLD)
 #pragma unroll
         for(uint32_t x = 0; x < kAhead; ++x)
             if(tid + x * kThreads < all) {
                 const uint32_t i = tid + x * kThreads;
-                fetch(first[x], i / per_row, i % per_row * 16);
+                fetch_piece(first[x], a, ws, i / per_row, i % per_row * 16);
             }
 #pragma unroll
     for(int i = 0; i < RING - 1; ++i)
         if(loaded < mine) load(i);
 
-    if constexpr(ALL) {
+    if constexpr(HOLD) {
+        auto put = [&](const Piece& x, uint32_t i) {
+            store_piece(x, inverse[i / per_row], a.qmax, q + i / per_row * rb + i % per_row * 16);
+        };
 #pragma unroll
         for(uint32_t x = 0; x < kAhead; ++x)
-            if(tid + x * kThreads < all) {
-                const uint32_t i = tid + x * kThreads;
-                store(first[x], i / per_row, q + i / per_row * rb + i % per_row * 16);
-            }
-        for(uint32_t i = tid + kAhead * kThreads; i < all; i += kThreads)
-            quantize(i / per_row, i % per_row * 16, q + i / per_row * rb + i % per_row * 16);
-    } else if(!streams && n > 0) {
-        fill(0, wave - kWaves);
+            if(tid + x * kThreads < all) put(first[x], tid + x * kThreads);
+        for(uint32_t i = tid + kAhead * kThreads; i < all; i += kThreads) {
+            Piece x;
+            fetch_piece(x, a, ws, i / per_row, i % per_row * 16);
+            put(x, i);
+        }
+        __syncthreads();
     }
-    __syncthreads();
 
-    if(!streams) {
-        if constexpr(!ALL)
-            for(uint32_t item = 0; item < items; ++item) {
-                if(item + 1 < items) fill(item + 1, wave - kWaves);
-                __syncthreads();
-            }
-    } else {
-        v4i           acc  = {};
-        uint32_t      done = 0, rows = 0;
-        const int8_t* qrow = q;
-        bool          fresh = true;
-        uint32_t      phase = 0; // items this wave has left behind
-        auto          leave = [&]() { // barriers at the end of an item
-            __syncthreads();
-            ++phase;
-        };
-        auto flush = [&](uint32_t ai) {
-            if(row < rows && (uint32_t)(4 * kg) / kCols == fold) {
-                int32_t* to = sums + lists.pair[ai * kRows + row] * kCols;
+    v4i           acc  = {};
+    uint32_t      done = 0, rows = 0;
+    const int8_t* qrow = q;
+    bool          fresh = true;
+    auto          flush = [&](uint32_t ai) {
+        if(row < rows && (uint32_t)(4 * kg) / kCols == fold) {
+            int32_t* to = sums + lists.pair[ai * kRows + row] * kCols;
 #pragma unroll
-                for(int i = 0; i < 4; ++i) atomicAdd(&to[(4 * kg + i) % kCols], acc[i]);
-            }
-            acc = v4i{0, 0, 0, 0};
-        };
-        while(done < mine) {
+            for(int i = 0; i < 4; ++i) atomicAdd(&to[(4 * kg + i) % kCols], acc[i]);
+        }
+        acc = v4i{0, 0, 0, 0};
+    };
+    while(done < mine) {
 #pragma unroll
-            for(int slot = 0; slot < RING; ++slot) {
-                if(loaded < mine) load((slot + RING - 1) % RING);
-                if(done < mine) {
-                    const uint32_t ai = now.item / chunks;
-                    if(fresh) {
-                        rows                = lists.rows(ai);
-                        const uint32_t r    = min(row, rows - 1);
-                        const uint32_t from = ALL ? lists.pair[ai * kRows + r]
-                                                  : now.item % 2 * a.tokens + r;
-                        qrow                = q + from * rb + kg * 16;
-                        fresh               = false;
-                    }
+        for(int slot = 0; slot < RING; ++slot) {
+            if(loaded < mine) load((slot + RING - 1) % RING);
+            if(done < mine) {
+                const uint32_t ai = now.item;
+                if(fresh) {
+                    rows  = lists.rows(ai);
+                    if constexpr(HOLD)
+                        qrow = q + lists.pair[ai * kRows + min(row, rows - 1)] * rb + kg * 16;
+                    fresh = false;
+                }
 #pragma unroll
-                    for(int i = 0; i < kDownSteps; ++i) {
-                        // a step past the part or the row has zero weights: any of them will do
+                for(int i = 0; i < kSteps; ++i) {
+                    if constexpr(HOLD) {
+                        // a step past the part or the row has zero weights: any will do
                         const uint32_t st
-                            = min(fold * part + now.b * kDownSteps + i, (rb - 16) / 64 - 1);
+                            = min(fold * part + now.b * kSteps + i, (rb - 16) / 64 - 1);
                         acc = mfma(ring[slot][i], *reinterpret_cast<const v4i*>(qrow + st * 64), acc);
+                    } else {
+                        acc = mfma(ring[slot][i], rows8[slot][i], acc);
                     }
-                    ++done;
-                    const uint32_t item = now.item;
-                    advance(now);
-                    if(now.item != item || done == mine) {
-                        fresh = true;
-                        if(ALL || now.item / chunks != ai) flush(ai);
-                        if(!ALL) leave();
-                    }
+                }
+                ++done;
+                now.advance(per);
+                if(now.item != ai || done == mine) {
+                    fresh = true;
+                    flush(ai);
                 }
             }
         }
-        if(!ALL)
-            while(phase < items) leave(); // a wave without a batch of an item
     }
     __syncthreads();
 
     // ---- the weighted sum over a token's slots -------------------------------------
-    for(uint32_t i = tid; i < a.tokens * kCols; i += kAll) {
+    for(uint32_t i = tid; i < a.tokens * kCols; i += kThreads) {
         const uint32_t t = i / kCols, j = i % kCols;
         float          out = 0.f;
         for(uint32_t s = 0; s < a.topk; ++s) {
@@ -683,14 +684,14 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
     }
 }
 
-// BLOCKS a CU, as in gate_up_kernel (the 16 waves of the chunked form count as two).
-template <int FOLD, bool ALL, int BLOCKS>
-__global__ void __launch_bounds__(ALL ? kThreads : 2 * kThreads, 2 * BLOCKS)
-    down_kernel(MoeDecodeArgs a, Ws ws, uint32_t chunk, uint32_t gu_blocks)
+// BLOCKS a CU, as in gate_up_kernel.
+template <int FOLD, bool HOLD, int BLOCKS>
+__global__ void __launch_bounds__(kThreads, 2 * BLOCKS)
+    down_kernel(MoeDecodeArgs a, Ws ws, uint32_t gu_blocks)
 {
     extern __shared__ uint8_t dyn[];
     __shared__ DownLds        lds;
-    down<FOLD, ALL, BLOCKS == 1 ? 4 : 3>(a, ws, chunk, gu_blocks, lds, dyn);
+    down<FOLD, HOLD, BLOCKS == 1 ? 4 : 3>(a, ws, gu_blocks, lds, dyn);
 }
 
 template <class K>
@@ -707,22 +708,19 @@ hipError_t launch_down(const MoeDecodeArgs& a, const Ws& ws, uint32_t gu_blocks,
     const uint32_t pairs = a.tokens * a.topk, grid = a.hidden / (kTile / FOLD);
     const uint32_t fixed = Lists::bytes(pairs) + 2 * Lists::up16(pairs) + pairs * kTile * 4;
     const uint32_t room  = kLdsBytes - (uint32_t)sizeof(DownLds) - fixed;
+    const bool     one   = grid <= kCus;
     // all rows, where two blocks still share a CU or one does with no second to come
-    if((uint64_t)pairs * row_bytes(a.inter) <= std::min<uint32_t>(room, 100 * 1024)) {
-        const uint32_t lds = fixed + pairs * row_bytes(a.inter);
-        const auto     kernel
-            = grid <= kCus ? down_kernel<FOLD, true, 1> : down_kernel<FOLD, true, 2>;
-        allow_lds(kernel, lds);
-        kernel<<<grid, kThreads, lds, stream>>>(a, ws, a.inter, gu_blocks);
-    } else {
-        // as few chunks as fit, all about the same size
-        const uint32_t most   = (room / (2 * a.tokens) - 16) / 64 * 64;
-        const uint32_t chunks = (a.inter + most - 1) / most;
-        const uint32_t chunk  = ((a.inter + chunks - 1) / chunks + 63) / 64 * 64;
-        const uint32_t lds = fixed + 2 * a.tokens * row_bytes(chunk);
-        allow_lds(down_kernel<FOLD, false, 2>, lds);
-        down_kernel<FOLD, false, 2><<<grid, 2 * kThreads, lds, stream>>>(a, ws, chunk, gu_blocks);
+    const bool hold = (uint64_t)pairs * row_bytes(a.inter) <= std::min<uint32_t>(room, 100 * 1024);
+    const uint32_t lds    = fixed + (hold ? pairs * row_bytes(a.inter) : 0);
+    const auto     kernel = hold ? (one ? down_kernel<FOLD, true, 1> : down_kernel<FOLD, true, 2>)
+                                 : (one ? down_kernel<FOLD, false, 1> : down_kernel<FOLD, false, 2>);
+    if(!hold) {
+        constexpr uint32_t kColumns = kRequantThreads * 16;
+        requant_kernel<<<dim3((a.inter + kColumns - 1) / kColumns, pairs), kRequantThreads,
+                         Lists::bytes(pairs), stream>>>(a, ws, gu_blocks);
     }
+    allow_lds(kernel, lds);
+    kernel<<<grid, kThreads, lds, stream>>>(a, ws, gu_blocks);
     return hipGetLastError();
 }
 
@@ -731,7 +729,8 @@ hipError_t launch_down(const MoeDecodeArgs& a, const Ws& ws, uint32_t gu_blocks,
 size_t moe_ffn_decode_workspace_bytes(uint32_t tokens, uint32_t topk, uint32_t hidden, uint32_t inter)
 {
     const size_t n = (size_t)tokens * topk;
-    return up256(n * inter * 4) + up256(n * kGateUpBlocks * 4) + 2 * up256(n * 4);
+    return up256(n * inter * 4) + up256(n * kGateUpBlocks * 4) + 3 * up256(n * 4)
+           + up256(n * inter);
 }
 
 hipError_t launch_moe_ffn_decode(const MoeDecodeArgs& a, bool f16, hipStream_t stream)

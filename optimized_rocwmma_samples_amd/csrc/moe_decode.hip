@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 2 * BLOCKS) gate_up_kernel(MoeDecode
 // Between them, where the down kernel does not hold the rows itself: the activations in 8
 // bits, once for all of its blocks, 16 columns a thread of one pair's row a block row.
 // (Every block quantizing chunks of the rows into LDS beside its stream: 16 tokens of 8
-// experts of 4096 x 14336 308 us the layer, XX now.)
+// experts of 4096 x 14336 308 us the layer, 253 now.)
 // ---------------------------------------------------------------------------
 constexpr int kRequantThreads = 256;
 
@@ -520,12 +520,11 @@ __global__ void __launch_bounds__(kRequantThreads)
 // them as operands from requant_kernel's, out of L2, beside its weights: that is as
 // many loads again, but no barrier and nothing that every block does anew.
 // ---------------------------------------------------------------------------
-template <int FOLD, bool HOLD, int RING>
+template <int FOLD, bool HOLD, int RING, int kSteps>
 __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint32_t gu_blocks,
                                      DownLds& lds, uint8_t* dyn)
 {
-    constexpr uint32_t kCols  = kTile / FOLD;
-    constexpr int      kSteps = HOLD ? 4 : 2; // steps a batch: 4 KB a wave, or 2 and 2
+    constexpr uint32_t kCols = kTile / FOLD;
     const int      wave  = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int      lane  = threadIdx.x % kWave, col = lane % 16, kg = lane / 16;
     const uint32_t pairs = a.tokens * a.topk, tid = threadIdx.x;
@@ -684,14 +683,17 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
     }
 }
 
-// BLOCKS a CU, as in gate_up_kernel.
+// BLOCKS a CU, as in gate_up_kernel.  A batch is 4 steps, 4 KB a wave, or 2 where two
+// blocks a CU leave no registers for 4 of weights and rows (16 tokens of 64 experts of
+// 7168 x 2048, top 6, 394 us against 408; one block, 8 experts of 4096 x 14336: 4 steps
+// 253 us, 2 steps 274).
 template <int FOLD, bool HOLD, int BLOCKS>
 __global__ void __launch_bounds__(kThreads, 2 * BLOCKS)
     down_kernel(MoeDecodeArgs a, Ws ws, uint32_t gu_blocks)
 {
     extern __shared__ uint8_t dyn[];
     __shared__ DownLds        lds;
-    down<FOLD, HOLD, BLOCKS == 1 ? 4 : 3>(a, ws, gu_blocks, lds, dyn);
+    down<FOLD, HOLD, BLOCKS == 1 ? 4 : 3, HOLD || BLOCKS == 1 ? 4 : 2>(a, ws, gu_blocks, lds, dyn);
 }
 
 template <class K>

@@ -570,7 +570,7 @@ int w8a8_moe_combine(const void* y, uint32_t ldy, uint32_t rows_y, const float* 
                      void* out, uint32_t ldo, hipStream_t stream);
 
 /*
- * The whole expert layer for the few tokens of a decode step, in two launches:
+ * The whole expert layer for the few tokens of a decode step, in three launches:
  * routing, the MoE quantizer, the gate_up GEMM, SiLU(gate) * up, the
  * requantization, the down GEMM and the weighted combine of the chain above
  * (w8a8_topk_softmax ... w8a8_moe_combine), without its sort and without an

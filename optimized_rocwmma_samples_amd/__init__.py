@@ -19,7 +19,7 @@ The functions mirror the reference kernels this path replaces:
                    <- the expert FFN chain (rocwmma_fused_moe.cpp:96-211), gate*up form
 and beside them, without a counterpart there, what a decoder layer needs next to
 its linear layers:
-  moe_ffn_decode   the expert FFN of a few tokens in two launches
+  moe_ffn_decode   the expert FFN of a few tokens in three launches
   attention        causal attention of packed prompts
   KV4Cache, kv4_store, kv4_load, attention_kv4
                    a paged 4-bit cache of keys and values, and the attention of
@@ -731,7 +731,7 @@ def moe_ffn_decode_workspace_size(tokens: int, topk: int, hidden: int, inter: in
 
 def moe_ffn_decode(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_down, topk: int,
                    smooth_scale_down=None, quant_max: float = 127.0, out=None, workspace="auto"):
-    """The expert FFN of moe_ffn for at most 16 tokens, in two launches.
+    """The expert FFN of moe_ffn for at most 16 tokens, in three launches.
 
     x fp16 [T, H] (any row stride that is a multiple of 8), logits fp32 or fp16
     [T, E], smooth_scale fp32 [E, H], w_gate_up int8 [E, 2*I, H] with sb_gate_up

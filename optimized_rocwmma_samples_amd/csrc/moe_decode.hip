@@ -1,20 +1,24 @@
 // moe_decode.hip -- the expert layer of the few tokens of a decode step for
-// gfx950, in two launches (the chain of moe.hip takes nine):
+// gfx950, in three launches (the chain of moe.hip takes nine):
 //   gate_up_kernel  routing, the MoE quantizer, the gate_up products, SiLU(gate) * up
-//   down_kernel     requantization, the down products, the weighted combine
-// Both are streams of the active experts' weights, each byte read once; what the
-// chain spreads over launches every block does again for itself, on a few KB from
-// L2, while its first weights are in flight.
+//   requant_kernel  the activations in 8 bits
+//   down_kernel     the down products, the weighted combine
+// The first and the last are streams of the active experts' weights, each byte read once
+// (8 experts of 4096 x 14336: one token 75 us, 4.7 TB/s; 16 tokens 256 us, 5.5 TB/s).
+// Routing and quantization, which the chain has launches for, every block of the first
+// does again for itself, on a few KB from L2.  What is left above the bytes is that
+// start, a chain of short dependent steps (about 11 us of the first kernel), and the
+// second launch (3 us).
 //   * v_mfma_i32_16x16x64_i8 with 16 weight rows as srcA (a lane loads 16
 //     contiguous bytes of one row, a wave-load 64 bytes of 16 rows) and up to 16
-//     quantized rows as srcB, read from LDS.
+//     quantized rows as srcB, read from LDS or L2.
 //   * A block's steps along K, over all its tiles or experts, are cut into 8 equal
 //     runs, one per wave; a wave adds its int32 sums to LDS where it leaves a tile.
 //     Integer sums are exact, so no order changes anything, and the stream has no
 //     barrier in it (a barrier per tile cost 1.5 us each: 5 tokens of 64 experts of
-//     2048 x 1408 106 us).
-//   * The activations between the two kernels stay fp32 (a few hundred KB).  A row's
-//     absmax comes from per-block maxima that the first kernel leaves beside them.
+//     2048 x 1408 106 us, 51 now).
+//   * The activations between the kernels stay fp32 until they are quantized (a few
+//     hundred KB).  A row's absmax comes from per-block maxima beside them.
 #include "moe_route.hpp"
 #include "w8a8_device.hpp"
 #include "w8a8_internal.hpp"
@@ -53,37 +57,18 @@ __host__ __device__ constexpr uint32_t row_bytes(uint32_t n) { return (n + 63) /
 // Workspace between the kernels.
 struct Ws {
     float*   act;    // [pairs, inter]
-    float*   top;    // [pairs, kGateUpBlocks]: max |act| over a block's columns
-    int32_t* ids;    // [pairs]
+    float*   top;    // [kGateUpBlocks, pairs]: max |act| over a block's columns
+    uint8_t* lists;  // as in LDS
+    int32_t* active; // experts in them
     float*   weight; // [pairs]
     float*   scale;  // [pairs]: of the quantized activations
-    int8_t*  q;      // [pairs, inter]: those, where the down kernel cannot hold them
+    int8_t*  q;      // [pairs, inter]: those
 };
-
-Ws carve(const MoeDecodeArgs& a)
-{
-    uint8_t*     p = static_cast<uint8_t*>(a.ws);
-    const size_t n = (size_t)a.tokens * a.topk;
-    Ws           w;
-    w.act = reinterpret_cast<float*>(p);
-    p += up256(n * a.inter * 4);
-    w.top = reinterpret_cast<float*>(p);
-    p += up256(n * kGateUpBlocks * 4);
-    w.ids = reinterpret_cast<int32_t*>(p);
-    p += up256(n * 4);
-    w.weight = reinterpret_cast<float*>(p);
-    p += up256(n * 4);
-    w.scale = reinterpret_cast<float*>(p);
-    p += up256(n * 4);
-    w.q = reinterpret_cast<int8_t*>(p);
-    return w;
-}
 
 // The active experts (those some token is routed to) in ascending order, each with
 // its pairs (token * topk + slot) in ascending order.  In LDS, sized by the pairs.
 struct Lists {
     int32_t*  ids;    // [pairs] a pair's expert, or -1
-    int32_t*  order;  // [pairs] its place among the active ones
     int32_t*  expert; // [active]
     int32_t*  count;  // [active] pairs
     uint16_t* pair;   // [active][16]
@@ -94,34 +79,32 @@ struct Lists {
     }
     __host__ __device__ static constexpr uint32_t bytes(uint32_t pairs)
     {
-        return 4 * up16(pairs) + pairs * kRows * 2;
+        return 3 * up16(pairs) + (pairs * kRows * 2 + 15) / 16 * 16;
     }
     __device__ Lists(uint8_t* lds, uint32_t pairs)
     {
         const uint32_t n = up16(pairs);
         ids    = reinterpret_cast<int32_t*>(lds);
-        order  = reinterpret_cast<int32_t*>(lds + n);
-        expert = reinterpret_cast<int32_t*>(lds + 2 * n);
-        count  = reinterpret_cast<int32_t*>(lds + 3 * n);
-        pair   = reinterpret_cast<uint16_t*>(lds + 4 * n);
+        expert = reinterpret_cast<int32_t*>(lds + n);
+        count  = reinterpret_cast<int32_t*>(lds + 2 * n);
+        pair   = reinterpret_cast<uint16_t*>(lds + 3 * n);
     }
     // From the ids in LDS, by all threads, with `bits` [kWords] and `active` zeroed;
     // barriers before and after.
-    __device__ void build(uint32_t pairs, uint32_t threads, uint32_t* bits, uint32_t* active)
+    __device__ void build(uint32_t pairs, uint32_t* bits, uint32_t* active)
     {
-        for(uint32_t p = threadIdx.x; p < pairs; p += threads) {
+        for(uint32_t p = threadIdx.x; p < pairs; p += kThreads) {
             count[p] = 0;
             if(ids[p] >= 0) atomicOr(&bits[ids[p] / 32], 1u << (ids[p] % 32));
         }
         __syncthreads();
-        for(uint32_t p = threadIdx.x; p < pairs; p += threads) {
+        for(uint32_t p = threadIdx.x; p < pairs; p += kThreads) {
             const int32_t e = ids[p];
             if(e < 0) continue;
             uint32_t i = __popc(bits[e / 32] & ((1u << (e % 32)) - 1)), at = 0;
             for(int32_t w = 0; w < e / 32; ++w) i += __popc(bits[w]);
 #pragma unroll 4
             for(uint32_t o = 0; o < p; ++o) at += ids[o] == e;
-            order[p]  = (int32_t)i;
             expert[i] = e;
             if(at < (uint32_t)kRows) pair[i * kRows + at] = (uint16_t)p;
             if(at == 0) atomicAdd(active, 1u);
@@ -139,16 +122,31 @@ struct Lists {
     }
 };
 
+Ws carve(const MoeDecodeArgs& a)
+{
+    uint8_t*       p = static_cast<uint8_t*>(a.ws);
+    const uint32_t n = a.tokens * a.topk;
+    auto           take = [&](size_t bytes) {
+        uint8_t* at = p;
+        p += up256(bytes);
+        return at;
+    };
+    Ws w;
+    w.act    = reinterpret_cast<float*>(take((size_t)n * a.inter * 4));
+    w.top    = reinterpret_cast<float*>(take((size_t)n * kGateUpBlocks * 4));
+    w.lists  = take(Lists::bytes(n));
+    w.active = reinterpret_cast<int32_t*>(take(4));
+    w.weight = reinterpret_cast<float*>(take(n * 4));
+    w.scale  = reinterpret_cast<float*>(take(n * 4));
+    w.q      = reinterpret_cast<int8_t*>(take((size_t)n * a.inter));
+    return w;
+}
+
 // The columns of all active experts' activations, in tiles of 16, are cut into one
 // contiguous range per block of gate_up_kernel.
 __device__ __forceinline__ uint32_t first_unit(uint32_t block, uint32_t units, uint32_t blocks)
 {
     return block * units / blocks; // units <= 1024 * 2048, blocks <= 512
-}
-
-__device__ __forceinline__ uint32_t block_of(uint32_t unit, uint32_t units, uint32_t blocks)
-{
-    return ((unit + 1) * blocks - 1) / units;
 }
 
 // Hardware gives blocks to the 8 XCDs in turn; an index such that each XCD has a
@@ -209,13 +207,12 @@ typedef int32_t TileSums[2][kRows][kTile];
 struct GateUpLds {
     float    amax[kRows][kWaves];
     float    scale[kRows];
-    uint32_t top[kRows]; // float bits, >= 0
     uint32_t bits[kWords];
     uint32_t active;
 };
 
 static_assert(W8A8_MOE_DECODE_MAX_VALUES + kRows * 80 + Lists::bytes(kRows * kMaxTopk)
-                      + sizeof(GateUpLds) + 4 * sizeof(TileSums)
+                      + Lists::up16(kRows * kMaxTopk) + sizeof(GateUpLds) + 4 * sizeof(TileSums)
                   <= kLdsBytes,
               "a block of gate_up_kernel holds every token's row");
 
@@ -228,27 +225,31 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, ui
     const int      lane  = threadIdx.x % kWave, col = lane % 16, kg = lane / 16;
     const uint32_t pairs = a.tokens * a.topk, tid = threadIdx.x;
     Lists          lists(dyn, pairs);
-    TileSums*      sums = reinterpret_cast<TileSums*>(dyn + Lists::bytes(pairs));
+    uint32_t*      top  = reinterpret_cast<uint32_t*>(dyn + Lists::bytes(pairs)); // [pairs]
+    TileSums*      sums = reinterpret_cast<TileSums*>(dyn + Lists::bytes(pairs) + Lists::up16(pairs));
     int8_t*        q    = reinterpret_cast<int8_t*>(sums + group);
     const uint32_t rb   = row_bytes(a.hidden);
 
     // ---- routing: a wave per token -----------------------------------------------
     if(tid < kWords) lds.bits[tid] = 0;
     if(tid == 0) lds.active = 0;
+    for(uint32_t p = tid; p < pairs; p += kThreads) top[p] = 0; // float bits, >= 0
     for(uint32_t t = wave; t < a.tokens; t += kWaves)
         route_token(
             [&](uint32_t e) { return load_logit<F16>(a.logits, (size_t)t * a.experts + e); },
             a.experts, a.topk, lane, [&](uint32_t k, int id, float w) {
                 if(lane == 0) {
                     lists.ids[t * a.topk + k] = id;
-                    if(blockIdx.x == 0) {
-                        ws.ids[t * a.topk + k]    = id;
-                        ws.weight[t * a.topk + k] = w;
-                    }
+                    if(blockIdx.x == 0) ws.weight[t * a.topk + k] = w;
                 }
             });
     __syncthreads();
-    lists.build(pairs, kThreads, lds.bits, &lds.active);
+    lists.build(pairs, lds.bits, &lds.active);
+    if(blockIdx.x == 0) { // for the down kernel
+        for(uint32_t i = tid; i < Lists::bytes(pairs) / 16; i += kThreads)
+            reinterpret_cast<v4i*>(ws.lists)[i] = reinterpret_cast<const v4i*>(dyn)[i];
+        if(tid == 0) *ws.active = (int32_t)lds.active;
+    }
     const uint32_t tiles = a.inter / kTile, units = lds.active * tiles;
     // neighbouring ranges to one XCD: where every other block has a tile more, each XCD
     // gets as many of both (8 experts of 4096 x 14336, one token: 448 and 448 tiles at
@@ -314,7 +315,6 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, ui
         __syncthreads(); // the sums and rows before are done with
         for(uint32_t i = tid; i < (u1 - u0) * sizeof(TileSums) / 16; i += kThreads)
             reinterpret_cast<v4i*>(sums)[i] = v4i{0, 0, 0, 0};
-        if(tid < (uint32_t)kRows && fresh) lds.top[tid] = 0;
         // ---- the expert's rows, quantized into LDS: four rows at a time, so that
         // their loads overlap ------------------------------------------------------
         if(fresh) {
@@ -416,15 +416,13 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, ui
             f = fmaxf(f, dpp_mov<kDppQuadXor2>(f));
             f = fmaxf(f, dpp_mov<kDppRowHalfMirror>(f));
             f = fmaxf(f, dpp_mov<kDppRowMirror>(f));
-            if(j == 0 && f > 0.f) atomicMax(&lds.top[r], __float_as_uint(f));
+            if(j == 0 && f > 0.f) atomicMax(&top[list[r]], __float_as_uint(f));
         }
         u0 = u1;
-        if(u0 == to || u0 == (ai + 1) * tiles) { // the expert's last tiles here
-            __syncthreads();
-            if(tid < rows)
-                ws.top[(size_t)list[tid] * kGateUpBlocks + range] = __uint_as_float(lds.top[tid]);
-        }
     }
+    __syncthreads();
+    for(uint32_t p = tid; p < pairs; p += kThreads)
+        ws.top[(size_t)range * pairs + p] = __uint_as_float(top[p]);
 }
 
 // BLOCKS a CU.  Batches in flight: 3 where a block is alone on its CU, 2 where there are
@@ -439,229 +437,119 @@ __global__ void __launch_bounds__(kThreads, 2 * BLOCKS) gate_up_kernel(MoeDecode
 }
 
 // ---------------------------------------------------------------------------
-// Between them, where the down kernel does not hold the rows itself: the activations in 8
-// bits, once for all of its blocks, 16 columns a thread of one pair's row a block row.
-// (Every block quantizing chunks of the rows into LDS beside its stream: 16 tokens of 8
-// experts of 4096 x 14336 308 us the layer, 253 now.)
+// Second kernel: the activations in 8 bits, once for all blocks of the third, 16 columns
+// a thread of one pair's row a block row.  (Every block of the third kernel quantizing
+// the rows for itself, into LDS: one token of 8 experts of 4096 x 14336 78 us the layer,
+// 75 now; 16 tokens, whose rows did not fit, 308 and 256.)
 // ---------------------------------------------------------------------------
 constexpr int kRequantThreads = 256;
-
-struct DownLds {
-    uint32_t bits[kWords];
-    uint32_t active;
-};
-
-// A pair's max |act| by one wave, from the maxima that gate_up_kernel's blocks left.
-__device__ __forceinline__ float row_top(const MoeDecodeArgs& a, const Ws& ws, const Lists& lists,
-                                         uint32_t p, uint32_t active, uint32_t gu_blocks, int lane)
-{
-    if(lists.ids[p] < 0) return 0.f;
-    const uint32_t tiles = a.inter / kTile, units = active * tiles, u = lists.order[p] * tiles;
-    const uint32_t b1 = block_of(u + tiles - 1, units, gu_blocks);
-    float          m  = 0.f;
-    for(uint32_t b = block_of(u, units, gu_blocks) + lane; b <= b1; b += kWave)
-        if(first_unit(b, units, gu_blocks) < first_unit(b + 1, units, gu_blocks))
-            m = fmaxf(m, ws.top[(size_t)p * kGateUpBlocks + b]); // it had work
-    return wave_max(m);
-}
-
-// 16 columns of one pair's activations from k on, and their quantized form.
-struct Piece {
-    v4f f[4];
-};
-
-__device__ __forceinline__ void fetch_piece(Piece& x, const MoeDecodeArgs& a, const Ws& ws,
-                                            uint32_t p, uint32_t k)
-{
-    const float* h = ws.act + (size_t)p * a.inter + k;
-#pragma unroll
-    for(int c = 0; c < 4; ++c)
-        x.f[c] = k < a.inter ? *reinterpret_cast<const v4f*>(h + 4 * c) : v4f{0, 0, 0, 0};
-}
-
-__device__ __forceinline__ void store_piece(const Piece& x, float inv, float qmax, int8_t* to)
-{
-    v4i w;
-#pragma unroll
-    for(int c = 0; c < 4; ++c)
-        w[c] = (int)cvt_pack4_i8(quant_f(x.f[c][0], inv, qmax), quant_f(x.f[c][1], inv, qmax),
-                                 quant_f(x.f[c][2], inv, qmax), quant_f(x.f[c][3], inv, qmax));
-    *reinterpret_cast<v4i*>(to) = w;
-}
 
 __global__ void __launch_bounds__(kRequantThreads)
     requant_kernel(MoeDecodeArgs a, Ws ws, uint32_t gu_blocks)
 {
-    extern __shared__ uint8_t dyn[];
-    __shared__ DownLds        lds;
-    const uint32_t tid = threadIdx.x, pairs = a.tokens * a.topk, p = blockIdx.y;
-    const uint32_t k = (blockIdx.x * kRequantThreads + tid) * 16;
-    Lists          lists(dyn, pairs);
-    Piece          x;
-    fetch_piece(x, a, ws, p, k);
-    for(uint32_t i = tid; i < (uint32_t)kWords; i += kRequantThreads) lds.bits[i] = 0;
-    if(tid == 0) lds.active = 0;
-    for(uint32_t i = tid; i < pairs; i += kRequantThreads) lists.ids[i] = ws.ids[i];
+    __shared__ float tops[kRequantThreads / kWave];
+    const uint32_t   tid = threadIdx.x, pairs = a.tokens * a.topk, p = blockIdx.y;
+    const uint32_t   k = (blockIdx.x * kRequantThreads + tid) * 16;
+    const float*     h = ws.act + (size_t)p * a.inter + k;
+    v4f              f[4] = {};
+#pragma unroll
+    for(int c = 0; c < 4; ++c)
+        if(k < a.inter) f[c] = *reinterpret_cast<const v4f*>(h + 4 * c);
+    float m = 0.f; // of a row of no expert too, whose activations are whatever was there
+    for(uint32_t b = tid; b < gu_blocks; b += kRequantThreads)
+        m = fmaxf(m, ws.top[(size_t)b * pairs + p]);
+    m = wave_max(m);
+    if(tid % kWave == 0) tops[tid / kWave] = m;
     __syncthreads();
-    lists.build(pairs, kRequantThreads, lds.bits, &lds.active);
-    const float r = row_top(a, ws, lists, p, lds.active, gu_blocks, tid % kWave) / a.qmax;
-    if(k < a.inter) store_piece(x, r > 0.f ? 1.f / r : 0.f, a.qmax, ws.q + (size_t)p * a.inter + k);
+    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float r = m / a.qmax, inv = r > 0.f ? 1.f / r : 0.f;
+    v4i         w;
+#pragma unroll
+    for(int c = 0; c < 4; ++c)
+        w[c] = (int)cvt_pack4_i8(quant_f(f[c][0], inv, a.qmax), quant_f(f[c][1], inv, a.qmax),
+                                 quant_f(f[c][2], inv, a.qmax), quant_f(f[c][3], inv, a.qmax));
+    if(k < a.inter) *reinterpret_cast<v4i*>(ws.q + (size_t)p * a.inter + k) = w;
     if(blockIdx.x == 0 && tid == 0) ws.scale[p] = r;
 }
 
 // ---------------------------------------------------------------------------
-// Second kernel: a block owns 16 / FOLD output columns of all active experts.
+// Third kernel: a block owns 16 / FOLD output columns of all active experts.
 // FOLD > 1 (at most 16 / FOLD tokens): the tile's 16 weight rows are the columns'
 // FOLD parts along K, and its 16 columns the rows' parts likewise; the blocks on the
 // tile's diagonal are the partial sums, the others are not used.  So a small hidden
 // size still gives a block to every CU, with whole 16-byte loads.
-//
-// HOLD: the block quantizes the rows of all pairs into LDS itself.  Otherwise it reads
-// them as operands from requant_kernel's, out of L2, beside its weights: that is as
-// many loads again, but no barrier and nothing that every block does anew.
+// The quantized rows come as operands straight from L2, beside the weights: that is as
+// many loads again, but no LDS, no barrier and nothing that every block does anew.
 // ---------------------------------------------------------------------------
-template <int FOLD, bool HOLD, int RING, int kSteps>
-__device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint32_t gu_blocks,
-                                     DownLds& lds, uint8_t* dyn)
+template <int FOLD, int RING, int kSteps>
+__device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint8_t* dyn)
 {
     constexpr uint32_t kCols = kTile / FOLD;
     const int      wave  = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int      lane  = threadIdx.x % kWave, col = lane % 16, kg = lane / 16;
     const uint32_t pairs = a.tokens * a.topk, tid = threadIdx.x;
     Lists          lists(dyn, pairs);
-    uint8_t*       at0   = dyn + Lists::bytes(pairs);
-    float*         scale   = reinterpret_cast<float*>(at0);
-    float*         inverse = reinterpret_cast<float*>(at0 + Lists::up16(pairs));
-    int32_t*       sums = reinterpret_cast<int32_t*>(at0 + 2 * Lists::up16(pairs)); // [pairs][kCols]
-    int8_t* q = reinterpret_cast<int8_t*>(at0 + 2 * Lists::up16(pairs) + pairs * kTile * 4);
-    const uint32_t j0 = blockIdx.x * kCols, rb = row_bytes(a.inter);
+    int32_t*       sums = reinterpret_cast<int32_t*>(dyn + Lists::bytes(pairs)); // [pairs][kCols]
+    const uint32_t j0   = blockIdx.x * kCols;
 
-    for(uint32_t i = tid; i < (uint32_t)kWords; i += kThreads) lds.bits[i] = 0;
-    if(tid == 0) lds.active = 0;
-    for(uint32_t p = tid; p < pairs; p += kThreads) {
-        lists.ids[p] = ws.ids[p];
-        if constexpr(!HOLD) scale[p] = ws.scale[p];
-    }
+    const uint32_t n = (uint32_t)__builtin_amdgcn_readfirstlane(*ws.active);
+    for(uint32_t i = tid; i < Lists::bytes(pairs) / 16; i += kThreads)
+        reinterpret_cast<v4i*>(dyn)[i] = reinterpret_cast<const v4i*>(ws.lists)[i];
     for(uint32_t i = tid; i < pairs * kCols; i += kThreads) sums[i] = 0;
     __syncthreads();
-    lists.build(pairs, kThreads, lds.bits, &lds.active);
-    const uint32_t n = lds.active;
-
-    if constexpr(HOLD) {
-        for(uint32_t p = wave; p < pairs; p += kWaves) {
-            const float r = row_top(a, ws, lists, p, n, gu_blocks, lane) / a.qmax;
-            if(lane == 0) {
-                scale[p]   = r;
-                inverse[p] = r > 0.f ? 1.f / r : 0.f;
-            }
-        }
-        __syncthreads();
-    }
 
     // ---- the stream of weights, all experts in one run a wave ------------------------
     const uint32_t part = ((a.inter + 63) / 64 + FOLD - 1) / FOLD; // steps of a part of K
     const uint32_t per  = (part + kSteps - 1) / kSteps;
     const Run      run(n * per, wave);
     const uint32_t mine = run.to - run.from;
-    v4i            ring[RING][kSteps], rows8[HOLD ? 1 : RING][kSteps];
+    v4i            weights[RING][kSteps], rows[RING][kSteps];
     Cursor         ahead(run.from, per), now = ahead;
     const uint32_t row = col % kCols, fold = col / kCols; // of the weights, and of the tokens
-    uint32_t       loaded = 0, item = ~0u, from8 = 0;
-    const __amdgpu_buffer_rsrc_t r8 = __builtin_amdgcn_make_buffer_rsrc(
+    uint32_t       loaded = 0, item = ~0u, from = 0;
+    const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
         ws.q, 0, (int)(pairs * a.inter), kBufferFlags);
     auto load = [&](int slot) {
         const uint32_t               e = lists.expert_at(ahead.item);
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<int8_t*>(a.wd + ((size_t)e * a.hidden + j0) * a.inter), 0,
             (int)(kCols * a.inter), kBufferFlags);
-        if constexpr(!HOLD)
-            if(ahead.item != item) { // lanes past the expert's rows take its last one
-                item  = ahead.item;
-                from8 = lists.pair[item * kRows + min(row, lists.rows(item) - 1)] * a.inter;
-            }
+        if(ahead.item != item) { // lanes past the expert's rows take its last one
+            item = ahead.item;
+            from = lists.pair[item * kRows + min(row, lists.rows(item) - 1)] * a.inter;
+        }
 #pragma unroll
         for(int i = 0; i < kSteps; ++i) {
             const uint32_t st = ahead.b * kSteps + i, k = (fold * part + st) * 64 + kg * 16;
             const bool     in = st < part && k < a.inter;
-            ring[slot][i]     = load_weights(r, in ? row * a.inter + k : kOob);
-            if constexpr(!HOLD)
-                rows8[slot][i] = __builtin_bit_cast(
-                    v4i, __builtin_amdgcn_raw_buffer_load_b128(r8, in ? from8 + k : kOob, 0, 0));
+            weights[slot][i]  = load_weights(rw, in ? row * a.inter + k : kOob);
+            rows[slot][i]     = load_weights(rq, in ? from + k : kOob);
         }
         ahead.advance(per);
         ++loaded;
     };
-    // a thread's first pieces go out ahead of the weights: behind them they would wait for
-    // all of those
-    constexpr uint32_t kAhead = HOLD ? 2 : 0;
-    const uint32_t     per_row = (rb - 16) / 16, all = HOLD ? pairs * per_row : 0;
-    Piece              first[HOLD ? kAhead : 1];
-    if constexpr(HOLD)
-#pragma unroll
-        for(uint32_t x = 0; x < kAhead; ++x)
-            if(tid + x * kThreads < all) {
-                const uint32_t i = tid + x * kThreads;
-                fetch_piece(first[x], a, ws, i / per_row, i % per_row * 16);
-            }
 #pragma unroll
     for(int i = 0; i < RING - 1; ++i)
         if(loaded < mine) load(i);
 
-    if constexpr(HOLD) {
-        auto put = [&](const Piece& x, uint32_t i) {
-            store_piece(x, inverse[i / per_row], a.qmax, q + i / per_row * rb + i % per_row * 16);
-        };
-#pragma unroll
-        for(uint32_t x = 0; x < kAhead; ++x)
-            if(tid + x * kThreads < all) put(first[x], tid + x * kThreads);
-        for(uint32_t i = tid + kAhead * kThreads; i < all; i += kThreads) {
-            Piece x;
-            fetch_piece(x, a, ws, i / per_row, i % per_row * 16);
-            put(x, i);
-        }
-        __syncthreads();
-    }
-
-    v4i           acc  = {};
-    uint32_t      done = 0, rows = 0;
-    const int8_t* qrow = q;
-    bool          fresh = true;
-    auto          flush = [&](uint32_t ai) {
-        if(row < rows && (uint32_t)(4 * kg) / kCols == fold) {
-            int32_t* to = sums + lists.pair[ai * kRows + row] * kCols;
-#pragma unroll
-            for(int i = 0; i < 4; ++i) atomicAdd(&to[(4 * kg + i) % kCols], acc[i]);
-        }
-        acc = v4i{0, 0, 0, 0};
-    };
-    while(done < mine) {
+    v4i acc = {};
+    for(uint32_t done = 0; done < mine;) {
 #pragma unroll
         for(int slot = 0; slot < RING; ++slot) {
             if(loaded < mine) load((slot + RING - 1) % RING);
             if(done < mine) {
-                const uint32_t ai = now.item;
-                if(fresh) {
-                    rows  = lists.rows(ai);
-                    if constexpr(HOLD)
-                        qrow = q + lists.pair[ai * kRows + min(row, rows - 1)] * rb + kg * 16;
-                    fresh = false;
-                }
 #pragma unroll
-                for(int i = 0; i < kSteps; ++i) {
-                    if constexpr(HOLD) {
-                        // a step past the part or the row has zero weights: any will do
-                        const uint32_t st
-                            = min(fold * part + now.b * kSteps + i, (rb - 16) / 64 - 1);
-                        acc = mfma(ring[slot][i], *reinterpret_cast<const v4i*>(qrow + st * 64), acc);
-                    } else {
-                        acc = mfma(ring[slot][i], rows8[slot][i], acc);
-                    }
-                }
+                for(int i = 0; i < kSteps; ++i) acc = mfma(weights[slot][i], rows[slot][i], acc);
                 ++done;
+                const uint32_t ai = now.item;
                 now.advance(per);
                 if(now.item != ai || done == mine) {
-                    fresh = true;
-                    flush(ai);
+                    if(row < lists.rows(ai) && (uint32_t)(4 * kg) / kCols == fold) {
+                        int32_t* to = sums + lists.pair[ai * kRows + row] * kCols;
+#pragma unroll
+                        for(int i = 0; i < 4; ++i) atomicAdd(&to[(4 * kg + i) % kCols], acc[i]);
+                    }
+                    acc = v4i{0, 0, 0, 0};
                 }
             }
         }
@@ -676,8 +564,9 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
             const uint32_t p = t * a.topk + s;
             const int32_t  e = lists.ids[p];
             if(e < 0) continue;
-            const float y = ((float)sums[p * kCols + j] * scale[p]) * a.sd[(size_t)e * a.hidden + j0 + j];
-            out           = fmaf(ws.weight[p], y, out);
+            const float y
+                = ((float)sums[p * kCols + j] * ws.scale[p]) * a.sd[(size_t)e * a.hidden + j0 + j];
+            out = fmaf(ws.weight[p], y, out);
         }
         a.out[(size_t)t * a.ldo + j0 + j] = float_to_half_bits(out);
     }
@@ -687,13 +576,11 @@ __device__ __forceinline__ void down(const MoeDecodeArgs& a, const Ws& ws, uint3
 // blocks a CU leave no registers for 4 of weights and rows (16 tokens of 64 experts of
 // 7168 x 2048, top 6, 394 us against 408; one block, 8 experts of 4096 x 14336: 4 steps
 // 253 us, 2 steps 274).
-template <int FOLD, bool HOLD, int BLOCKS>
-__global__ void __launch_bounds__(kThreads, 2 * BLOCKS)
-    down_kernel(MoeDecodeArgs a, Ws ws, uint32_t gu_blocks)
+template <int FOLD, int BLOCKS>
+__global__ void __launch_bounds__(kThreads, 2 * BLOCKS) down_kernel(MoeDecodeArgs a, Ws ws)
 {
     extern __shared__ uint8_t dyn[];
-    __shared__ DownLds        lds;
-    down<FOLD, HOLD, BLOCKS == 1 ? 4 : 3, HOLD || BLOCKS == 1 ? 4 : 2>(a, ws, gu_blocks, lds, dyn);
+    down<FOLD, BLOCKS == 1 ? 4 : 3, BLOCKS == 1 ? 4 : 2>(a, ws, dyn);
 }
 
 template <class K>
@@ -705,24 +592,13 @@ void allow_lds(K kernel, uint32_t bytes)
 }
 
 template <int FOLD>
-hipError_t launch_down(const MoeDecodeArgs& a, const Ws& ws, uint32_t gu_blocks, hipStream_t stream)
+hipError_t launch_down(const MoeDecodeArgs& a, const Ws& ws, hipStream_t stream)
 {
     const uint32_t pairs = a.tokens * a.topk, grid = a.hidden / (kTile / FOLD);
-    const uint32_t fixed = Lists::bytes(pairs) + 2 * Lists::up16(pairs) + pairs * kTile * 4;
-    const uint32_t room  = kLdsBytes - (uint32_t)sizeof(DownLds) - fixed;
-    const bool     one   = grid <= kCus;
-    // all rows, where two blocks still share a CU or one does with no second to come
-    const bool hold = (uint64_t)pairs * row_bytes(a.inter) <= std::min<uint32_t>(room, 100 * 1024);
-    const uint32_t lds    = fixed + (hold ? pairs * row_bytes(a.inter) : 0);
-    const auto     kernel = hold ? (one ? down_kernel<FOLD, true, 1> : down_kernel<FOLD, true, 2>)
-                                 : (one ? down_kernel<FOLD, false, 1> : down_kernel<FOLD, false, 2>);
-    if(!hold) {
-        constexpr uint32_t kColumns = kRequantThreads * 16;
-        requant_kernel<<<dim3((a.inter + kColumns - 1) / kColumns, pairs), kRequantThreads,
-                         Lists::bytes(pairs), stream>>>(a, ws, gu_blocks);
-    }
+    const uint32_t lds    = Lists::bytes(pairs) + pairs * kTile * 4;
+    const auto     kernel = grid <= kCus ? down_kernel<FOLD, 1> : down_kernel<FOLD, 2>;
     allow_lds(kernel, lds);
-    kernel<<<grid, kThreads, lds, stream>>>(a, ws, gu_blocks);
+    kernel<<<grid, kThreads, lds, stream>>>(a, ws);
     return hipGetLastError();
 }
 
@@ -731,8 +607,8 @@ hipError_t launch_down(const MoeDecodeArgs& a, const Ws& ws, uint32_t gu_blocks,
 size_t moe_ffn_decode_workspace_bytes(uint32_t tokens, uint32_t topk, uint32_t hidden, uint32_t inter)
 {
     const size_t n = (size_t)tokens * topk;
-    return up256(n * inter * 4) + up256(n * kGateUpBlocks * 4) + 3 * up256(n * 4)
-           + up256(n * inter);
+    return up256(n * inter * 4) + up256(n * kGateUpBlocks * 4)
+           + up256(Lists::bytes((uint32_t)n)) + 256 + 2 * up256(n * 4) + up256(n * inter);
 }
 
 hipError_t launch_moe_ffn_decode(const MoeDecodeArgs& a, bool f16, hipStream_t stream)
@@ -740,7 +616,7 @@ hipError_t launch_moe_ffn_decode(const MoeDecodeArgs& a, bool f16, hipStream_t s
     const Ws       ws    = carve(a);
     const uint32_t pairs = a.tokens * a.topk;
     // 8 tiles' sums at a time, or 4 where two blocks then share a CU, or where 8 do not fit
-    const uint32_t rest = Lists::bytes(pairs) + a.tokens * row_bytes(a.hidden) + sizeof(GateUpLds);
+    const uint32_t rest = Lists::bytes(pairs) + Lists::up16(pairs) + a.tokens * row_bytes(a.hidden) + sizeof(GateUpLds);
     const uint32_t sum  = sizeof(TileSums);
     const bool     two  = rest + 4 * sum <= kLdsBytes / 2;
     const uint32_t group = rest + 8 * sum <= (two ? kLdsBytes / 2 : kLdsBytes) ? 8 : 4;
@@ -752,13 +628,16 @@ hipError_t launch_moe_ffn_decode(const MoeDecodeArgs& a, bool f16, hipStream_t s
                                 : (two ? gate_up_kernel<false, 2> : gate_up_kernel<false, 1>);
     allow_lds(gu, lds);
     gu<<<blocks, kThreads, lds, stream>>>(a, ws, group);
+    constexpr uint32_t kColumns = kRequantThreads * 16;
+    requant_kernel<<<dim3((a.inter + kColumns - 1) / kColumns, pairs), kRequantThreads, 0, stream>>>(
+        a, ws, blocks);
     const hipError_t e = hipGetLastError();
     if(e != hipSuccess) return e;
     // a block for every CU, where the tokens leave room in the tile
     const uint32_t columns = a.hidden / kTile;
-    if(columns < 128 && a.tokens <= 4) return launch_down<4>(a, ws, blocks, stream);
-    if(columns < 256 && a.tokens <= 8) return launch_down<2>(a, ws, blocks, stream);
-    return launch_down<1>(a, ws, blocks, stream);
+    if(columns < 128 && a.tokens <= 4) return launch_down<4>(a, ws, stream);
+    if(columns < 256 && a.tokens <= 8) return launch_down<2>(a, ws, stream);
+    return launch_down<1>(a, ws, stream);
 }
 
 } // namespace w8a8

@@ -181,7 +181,7 @@ def moe_ffn_decode(x: Tensor, logits: Tensor, smooth_scale: Tensor, w_gate_up: T
                    sb_gate_up: Tensor, w_down: Tensor, sb_down: Tensor, topk: int,
                    smooth_scale_down: Optional[Tensor] = None,
                    quant_max: float = 127.0) -> Tensor:
-    """The expert FFN of at most 16 tokens x [T, H] (fp16 out [T, H]) in two launches."""
+    """The expert FFN of at most 16 tokens x [T, H] (fp16 out [T, H]) in three launches."""
     return _moe_ffn_decode(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_down, topk,
                            smooth_scale_down, quant_max)
 

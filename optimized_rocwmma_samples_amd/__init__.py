@@ -28,6 +28,7 @@ its linear layers:
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 
 from . import _lib
@@ -397,7 +398,8 @@ def _workspace(workspace, size_fn, device):
         size = size_fn()
         if size == 0:
             return None, 0
-        workspace = _torch().empty(size, dtype=_torch().uint8, device=device)
+        torch = _torch()
+        return torch.empty(size, dtype=torch.uint8, device=device), size
     if workspace is None:
         return None, 0
     _require_cuda(workspace)
@@ -781,17 +783,28 @@ def moe_ffn_decode(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_do
 
 def _heads3d(name, t, heads=None, dim=None) -> int:
     """Checks fp16 [tokens, heads, dim] whose heads lie side by side; its row stride."""
-    torch = _torch()
-    if t.dim() != 3 or t.dtype != torch.float16:
+    shape = t.shape
+    if len(shape) != 3 or t.dtype != _torch_module.float16:
         raise ValueError(f"{name} must be a 3-D fp16 tensor [tokens, heads, head_dim]")
-    if (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
-        raise ValueError(f"{name} must have {heads} heads of {dim} channels, "
-                         f"got {tuple(t.shape)}")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    n, h, d = shape
+    if (heads is not None and h != heads) or (dim is not None and d != dim):
+        raise ValueError(f"{name} must have {heads} heads of {dim} channels, got {tuple(shape)}")
+    row, head, channel = t.stride()
+    if channel != 1 or (h > 1 and head != d):
         raise ValueError(f"{name}: the heads of a token must lie side by side "
-                         f"(strides {tuple(t.stride())})")
+                         f"(strides {(row, head, channel)})")
     # a single row may carry any stride
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return row if n > 1 else h * d
+
+
+def _heads_out(out, q, tokens: int, heads: int, dim: int):
+    # the result and its row stride: a new tensor where none is given
+    if out is None:
+        return q.new_empty((tokens, heads, dim)), heads * dim
+    ldo = _heads3d("out", out, heads, dim)
+    if out.shape[0] != tokens:
+        raise ValueError(f"out must have {tokens} rows")
+    return out, ldo
 
 
 def attention(q, k, v, seq_starts, scale: float | None = None, out=None):
@@ -812,19 +825,15 @@ def attention(q, k, v, seq_starts, scale: float | None = None, out=None):
     ldq = _heads3d("q", q)
     tokens, heads, dim = q.shape
     ldk, ldv = _heads3d("k", k, None, dim), _heads3d("v", v, None, dim)
-    kv_heads = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != tokens:
+    shape = k.shape
+    if shape != v.shape or shape[0] != tokens:
         raise ValueError("k and v must have q's tokens and head_dim, and one number of heads")
     if seq_starts.dtype != torch.int32 or seq_starts.dim() != 1 or not seq_starts.is_contiguous() \
             or seq_starts.numel() < 1:
         raise ValueError("seq_starts must be a contiguous int32 tensor [seqs + 1]")
-    if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=torch.float16, device=dev)
-    ldo = _heads3d("out", out, heads, dim)
-    if out.shape[0] != tokens:
-        raise ValueError(f"out must have {tokens} rows")
+    out, ldo = _heads_out(out, q, tokens, heads, dim)
     _call_on(dev, "w8a8_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-             seq_starts.data_ptr(), seq_starts.numel() - 1, tokens, heads, kv_heads, dim, ldq, ldk,
+             seq_starts.data_ptr(), seq_starts.numel() - 1, tokens, heads, shape[1], dim, ldq, ldk,
              ldv, ldo, dim ** -0.5 if scale is None else float(scale), _stream(dev))
     return out
 
@@ -900,19 +909,19 @@ def kv4_load(cache: KV4Cache, slots, out=None):
     """Read slots of the cache back: (k, v) fp16 [n, kv_heads, head_dim].  Rows
     of slots outside the cache are left as they were in `out`, a (k, v) pair
     (undefined in new tensors)."""
-    torch = _torch()
     _require_on(cache.device, slots=slots)
     n = _kv4_slots(slots)
     if out is None:
         shape = (n, cache.kv_heads, cache.head_dim)
-        out = (torch.empty(shape, dtype=torch.float16, device=cache.device),
-               torch.empty(shape, dtype=torch.float16, device=cache.device))
-    k, v = out
-    _require_on(cache.device, k=k, v=v)
-    ldk = _heads3d("k", k, cache.kv_heads, cache.head_dim)
-    ldv = _heads3d("v", v, cache.kv_heads, cache.head_dim)
-    if k.shape[0] != n or v.shape[0] != n:
-        raise ValueError(f"k and v must have {n} rows, one per slot")
+        k, v = cache.k_scales.new_empty(shape), cache.k_scales.new_empty(shape)
+        ldk = ldv = cache.kv_heads * cache.head_dim
+    else:
+        k, v = out
+        _require_on(cache.device, k=k, v=v)
+        ldk = _heads3d("k", k, cache.kv_heads, cache.head_dim)
+        ldv = _heads3d("v", v, cache.kv_heads, cache.head_dim)
+        if k.shape[0] != n or v.shape[0] != n:
+            raise ValueError(f"k and v must have {n} rows, one per slot")
     _call_on(cache.device, "w8a8_kv4_load", k.data_ptr(), v.data_ptr(), slots.data_ptr(), n, ldk,
              ldv, cache._ref, _stream(cache.device))
     return k, v
@@ -924,6 +933,10 @@ def attention_kv4_workspace_size(seqs: int, heads: int, kv_heads: int, head_dim:
     table's columns times the page size."""
     return int(library().w8a8_attention_kv4_workspace_size(seqs, heads, kv_heads, head_dim,
                                                            max_len))
+
+
+# a step after step of decoding asks for the same size
+_kv4_workspace_size = functools.lru_cache(maxsize=64)(attention_kv4_workspace_size)
 
 
 def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None = None, out=None,
@@ -949,14 +962,10 @@ def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None
         raise ValueError("seq_lens must be a contiguous int32 tensor [seqs]")
     cols = block_table.shape[1]
     table_ld = block_table.stride(0) if seqs > 1 else cols
-    if out is None:
-        out = torch.empty((seqs, heads, dim), dtype=torch.float16, device=dev)
-    ldo = _heads3d("out", out, heads, dim)
-    if out.shape[0] != seqs:
-        raise ValueError(f"out must have {seqs} rows")
+    out, ldo = _heads_out(out, q, seqs, heads, dim)
     ws, ws_bytes = _workspace(
-        workspace, lambda: attention_kv4_workspace_size(seqs, heads, cache.kv_heads, dim,
-                                                        cols * cache.page_size), dev)
+        workspace, lambda: _kv4_workspace_size(seqs, heads, cache.kv_heads, dim,
+                                               cols * cache.page_size), dev)
     _call_on(dev, "w8a8_attention_kv4", q.data_ptr(), cache._ref, block_table.data_ptr(), cols,
              table_ld, seq_lens.data_ptr(), out.data_ptr(), seqs, heads, ldq, ldo,
              dim ** -0.5 if scale is None else float(scale), _ptr(ws), ws_bytes, _stream(dev))

@@ -228,18 +228,13 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
                          rq, (wave * 32 + col) * a.ldq * 2 + s * 32 + half * 16, 0, 0));
     }
 
-    // LDS places of the lane's reads, in stage 0: of a key's step and a value's block; all
-    // others are fixed distances away
-    uint32_t kat[kSteps], vat[kBlocks];
-#pragma unroll
-    for(int st = 0; st < kSteps; ++st)
-        kat[st] = lds0 + col * D * 2 + key_chunk<D>(col, 2 * st + half) * 16;
-#pragma unroll
-    for(int b = 0; b < kBlocks; ++b) {
-        const uint32_t tok = 4 * half + lane % 16 / 4;
-        const uint32_t ch  = 32 * b + lane / 16 % 2 * 16 + lane % 4 * 4;
-        vat[b] = lds0 + kTileBytes + tok * D * 2 + value_chunk<D>(tok, ch / 8) * 16 + ch % 8 * 2;
-    }
+    // LDS places of the lane's reads, in stage 0: of a key's first step and a value's first
+    // block.  Rows are D * 2 bytes and LDS starts on such a border, so the swizzle of a
+    // later step or block is one XOR away; all else are fixed distances.
+    const uint32_t kat = lds0 + col * D * 2 + key_chunk<D>(col, half) * 16;
+    const uint32_t tok0 = 4 * half + lane % 16 / 4, ch0 = lane / 16 % 2 * 16 + lane % 4 * 4;
+    const uint32_t vat
+        = lds0 + kTileBytes + tok0 * D * 2 + value_chunk<D>(tok0, ch0 / 8) * 16 + ch0 % 8 * 2;
 
     const float c = a.scale * 1.44269504088896341f; // exponents in base 2
     float       m = -INFINITY, l = 0.f;
@@ -261,7 +256,7 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
         for(int st = 0; st < kSteps; ++st)
 #pragma unroll
             for(int sub = 0; sub < kSubs; ++sub)
-                s[sub] = mfma(*(const lds_v8h_t*)(uintptr_t)(kat[st] + off + sub * 32 * D * 2),
+                s[sub] = mfma(*(const lds_v8h_t*)(uintptr_t)(((kat + off) ^ (st * 32)) + sub * 32 * D * 2),
                               qf[st], s[sub]);
         if(diag) {
 #pragma unroll
@@ -296,7 +291,7 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
 #pragma unroll
             for(int part = 0; part < 2; ++part) {
                 const auto r = __builtin_amdgcn_ds_read_tr16_b64_v4f16(
-                    (lds_v4h_t*)(uintptr_t)(vat[b] + off + (16 * st + 8 * part) * D * 2));
+                    (lds_v4h_t*)(uintptr_t)(((vat + off) ^ (b * 64)) + (16 * st + 8 * part) * D * 2));
 #pragma unroll
                 for(int i = 0; i < 4; ++i) f[part * 4 + i] = (_Float16)r[i];
             }
@@ -374,7 +369,7 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 3) attention_kernel(AttentionArgs a)
 {
-    __shared__ alignas(16) uint8_t lds[2 * 2 * kKeysOf<D> * D * 2]; // two stages of keys, values
+    __shared__ alignas(256) uint8_t lds[2 * 2 * kKeysOf<D> * D * 2]; // two stages of keys, values
     attention_rows<D>(a, lds);
 }
 

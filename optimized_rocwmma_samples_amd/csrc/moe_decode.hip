@@ -455,10 +455,12 @@ __global__ void __launch_bounds__(kRequantThreads)
 #pragma unroll
     for(int c = 0; c < 4; ++c)
         if(k < a.inter) f[c] = *reinterpret_cast<const v4f*>(h + 4 * c);
-    float m = 0.f; // of a row of no expert too, whose activations are whatever was there
-    for(uint32_t b = tid; b < gu_blocks; b += kRequantThreads)
-        m = fmaxf(m, ws.top[(size_t)b * pairs + p]);
-    m = wave_max(m);
+    // (0 for a row of no expert, whose activations are whatever was there)
+    static_assert(kGateUpBlocks <= 2 * kRequantThreads, "two maxima a thread");
+    const uint32_t b = tid + kRequantThreads;
+    const float    m0 = tid < gu_blocks ? ws.top[tid * pairs + p] : 0.f;
+    const float    m1 = b < gu_blocks ? ws.top[b * pairs + p] : 0.f;
+    float          m  = wave_max(fmaxf(m0, m1));
     if(tid % kWave == 0) tops[tid / kWave] = m;
     __syncthreads();
     m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));

@@ -751,6 +751,7 @@ def moe_ffn_decode(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_do
                 smooth_scale_down=smooth_scale_down, out=out)
     _rows2d("x", x)
     t, h = x.shape
+    ldx = _row_stride("x", t, x.stride(0), h)
     if w_down.dim() != 3:
         raise ValueError("w_down must be [E, H, I]")
     e, _, i = w_down.shape
@@ -770,15 +771,34 @@ def moe_ffn_decode(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_do
         _rows2d("out", out, h)
         if out.shape[0] != t:
             raise ValueError(f"out must have {t} rows")
+    ldo = _row_stride("out", t, out.stride(0), h)
     if workspace is None:
         raise ValueError("moe_ffn_decode needs a workspace")
+    _workspace_on(workspace, dev)
     ws, ws_bytes = _workspace(workspace, lambda: moe_ffn_decode_workspace_size(t, topk, h, i), dev)
     _call_on(dev, "w8a8_moe_ffn_decode", x.data_ptr(), logits.data_ptr(),
              1 if logits.dtype == torch.float16 else 0, smooth_scale.data_ptr(),
              w_gate_up.data_ptr(), sb_gate_up.data_ptr(), _ptr(smooth_scale_down),
              w_down.data_ptr(), sb_down.data_ptr(), out.data_ptr(), t, h, i, e, topk,
-             float(quant_max), x.stride(0), out.stride(0), _ptr(ws), ws_bytes, _stream(dev))
+             float(quant_max), ldx, ldo, _ptr(ws), ws_bytes, _stream(dev))
     return out
+
+
+def _row_stride(name, rows: int, stride: int, columns: int) -> int:
+    # a single row may carry any stride; rows that overlap (an expanded tensor's) are
+    # refused, a stride of 0 above all, which the library takes for whole rows
+    if rows <= 1:
+        return columns
+    if stride < columns:
+        raise ValueError(f"{name}: rows of {columns} values overlap (row stride {stride})")
+    return stride
+
+
+def _workspace_on(workspace, device) -> None:
+    if hasattr(workspace, "device"):
+        _require_on(device, workspace=workspace)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
 
 
 def _heads3d(name, t, heads=None, dim=None) -> int:
@@ -793,8 +813,7 @@ def _heads3d(name, t, heads=None, dim=None) -> int:
     if channel != 1 or (h > 1 and head != d):
         raise ValueError(f"{name}: the heads of a token must lie side by side "
                          f"(strides {(row, head, channel)})")
-    # a single row may carry any stride
-    return row if n > 1 else h * d
+    return _row_stride(name, n, row, h * d)
 
 
 def _heads_out(out, q, tokens: int, heads: int, dim: int):
@@ -963,6 +982,7 @@ def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None
     cols = block_table.shape[1]
     table_ld = block_table.stride(0) if seqs > 1 else cols
     out, ldo = _heads_out(out, q, seqs, heads, dim)
+    _workspace_on(workspace, dev)
     ws, ws_bytes = _workspace(
         workspace, lambda: _kv4_workspace_size(seqs, heads, cache.kv_heads, dim,
                                                cols * cache.page_size), dev)

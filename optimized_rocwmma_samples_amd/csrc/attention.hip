@@ -237,7 +237,7 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
         = lds0 + kTileBytes + tok0 * D * 2 + value_chunk<D>(tok0, ch0 / 8) * 16 + ch0 % 8 * 2;
 
     const float c = a.scale * 1.44269504088896341f; // exponents in base 2
-    float       m = -INFINITY, l = 0.f;
+    float       m = -INFINITY, l = 0.f, mc = 0.f; // mc = m c, 0 while no score is finite
     v16f        o[kBlocks] = {};
 
     for(uint32_t step = 0; step < tiles; ++step) {
@@ -277,13 +277,14 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
         // probabilities would pass 2^8 (far inside fp16), which after the first tiles is
         // never, and not at every new maximum of one of 32 rows
         if(__ballot((mn - m) * c > 8.f) != 0) {
-            const float al = __builtin_amdgcn_exp2f((m - mn) * c);
-            m              = mn;
+            const float next = mn == -INFINITY ? 0.f : mn * c;
+            const float al   = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - next);
+            m                = mn;
+            mc               = next;
             l *= al;
 #pragma unroll
             for(int b = 0; b < kBlocks; ++b) o[b] *= al;
         }
-        const float mc = m * c;
 
         // 4 keys of channel 32 b + col: keys 16 st + 8 part + 4 half ..
         auto values = [&](int b, int st) {

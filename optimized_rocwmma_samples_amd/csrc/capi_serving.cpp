@@ -67,8 +67,8 @@ int check_kv4_rows(const char* fn, const w8a8_kv4_cache* c, const void* k, const
     if(ldk == 0) ldk = (uint32_t)row;
     if(ldv == 0) ldv = (uint32_t)row;
     if(ldk < row || ldv < row)
-        return fail(W8A8_ERROR_INVALID_VALUE, "%s: ldk=%u / ldv=%u smaller than kv_heads * head_dim",
-                    fn, ldk, ldv);
+        return fail(W8A8_ERROR_INVALID_VALUE,
+                    "%s: ldk=%u / ldv=%u smaller than kv_heads * head_dim", fn, ldk, ldv);
     if(!aligned(k, 16) || !aligned(v, 16) || ldk % 8 || ldv % 8)
         return fail(W8A8_ERROR_NOT_SUPPORTED,
                     "%s: needs 16-byte aligned k, v and row strides of multiples of 8", fn);
@@ -111,7 +111,8 @@ int w8a8_moe_ffn_decode(const void* x, const void* logits, int logits_f16,
         return fail(W8A8_ERROR_NOT_SUPPORTED,
                     "%s: needs tokens <= %u, tokens * hidden <= %u, experts <= 4096, topk <= 32 "
                     "(tokens=%u hidden=%u experts=%u topk=%u)",
-                    fn, W8A8_MOE_DECODE_MAX_TOKENS, W8A8_MOE_DECODE_MAX_VALUES, tokens, hidden, experts, topk);
+                    fn, W8A8_MOE_DECODE_MAX_TOKENS, W8A8_MOE_DECODE_MAX_VALUES, tokens, hidden,
+                    experts, topk);
     if(hidden % 16 != 0 || inter % 16 != 0 || hidden > 32768 || inter > 32768)
         return fail(W8A8_ERROR_NOT_SUPPORTED,
                     "%s: needs hidden and inter multiples of 16, at most 32768 (hidden=%u "

@@ -88,7 +88,8 @@ struct RowChunk {
     __device__ bool place(const CacheView& c, int32_t slot)
     {
         if(slot < 0 || (uint32_t)slot >= c.slots) return false;
-        row = cache_row(c, (uint32_t)slot >> c.page_shift, head, (uint32_t)slot & (c.page_size - 1));
+        const uint32_t at = (uint32_t)slot;
+        row = cache_row(c, at >> c.page_shift, head, at & (c.page_size - 1));
         return true;
     }
 };
@@ -98,7 +99,8 @@ template <int G, class T, class Op>
 __device__ __forceinline__ T group_reduce(T v, Op op)
 {
     const auto step = [&](auto dpp) {
-        v = op(v, __builtin_bit_cast(T, dpp_mov<decltype(dpp)::value>(__builtin_bit_cast(float, v))));
+        const float o = dpp_mov<decltype(dpp)::value>(__builtin_bit_cast(float, v));
+        v             = op(v, __builtin_bit_cast(T, o));
     };
     step(std::integral_constant<int, kDppQuadXor1>());
     step(std::integral_constant<int, kDppQuadXor2>());
@@ -258,8 +260,11 @@ RowPlan row_plan(const w8a8_kv4_cache& c, const Kv4Rows& r)
 // itself, its next chunk on the way while it computes.  A unit inside one run is
 // written out; of one cut by runs each wave leaves a partial (its sum of p v, maximum
 // and sum of p), and a second launch joins them in order.  So any mix of lengths
-// keeps the chip evenly busy.  (Blocks that owned a piece of one sequence spent 10 of
-// their 18 us on starting, the first load and merging: 16 x 8192 tokens 42 us.)
+// keeps the chip evenly busy.  Bound by the stream of codes: about 6 TB/s once it runs, less
+// 5.5 us of start (lengths, page numbers, then codes) and the join's 5 (131072 tokens,
+// 32 / 8 heads of 128, 168 MB, 41 us; 48 sequences of 249 MB in all 64).  (Blocks that
+// owned a piece of one sequence spent 10 of their 18 us on starting, the first load and
+// merging: 16 x 8192 tokens 42 us.)
 // Both products run on v_mfma_f32_16x16x32_f16 with the query heads as columns:
 //   S^T = K q^T    srcA rows = tokens.  A lane takes 16 (8) bytes of one token's
 //                  codes; dword j is its operand of step j, channels 32 j + 8 kg +

@@ -226,7 +226,8 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, ui
     const uint32_t pairs = a.tokens * a.topk, tid = threadIdx.x;
     Lists          lists(dyn, pairs);
     uint32_t*      top  = reinterpret_cast<uint32_t*>(dyn + Lists::bytes(pairs)); // [pairs]
-    TileSums*      sums = reinterpret_cast<TileSums*>(dyn + Lists::bytes(pairs) + Lists::up16(pairs));
+    TileSums*      sums
+        = reinterpret_cast<TileSums*>(dyn + Lists::bytes(pairs) + Lists::up16(pairs));
     int8_t*        q    = reinterpret_cast<int8_t*>(sums + group);
     const uint32_t rb   = row_bytes(a.hidden);
 
@@ -429,7 +430,8 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, ui
 // two; more made it slower (7 and 3 of them: 8 experts of 4096 x 14336, one token, 85
 // us against 80).
 template <bool F16, int BLOCKS>
-__global__ void __launch_bounds__(kThreads, 2 * BLOCKS) gate_up_kernel(MoeDecodeArgs a, Ws ws, uint32_t group)
+__global__ void __launch_bounds__(kThreads, 2 * BLOCKS)
+    gate_up_kernel(MoeDecodeArgs a, Ws ws, uint32_t group)
 {
     extern __shared__ uint8_t dyn[];
     __shared__ GateUpLds      lds;
@@ -606,7 +608,8 @@ hipError_t launch_down(const MoeDecodeArgs& a, const Ws& ws, hipStream_t stream)
 
 } // namespace
 
-size_t moe_ffn_decode_workspace_bytes(uint32_t tokens, uint32_t topk, uint32_t hidden, uint32_t inter)
+size_t moe_ffn_decode_workspace_bytes(uint32_t tokens, uint32_t topk, uint32_t hidden,
+                                      uint32_t inter)
 {
     const size_t n = (size_t)tokens * topk;
     return up256(n * inter * 4) + up256(n * kGateUpBlocks * 4)
@@ -618,7 +621,8 @@ hipError_t launch_moe_ffn_decode(const MoeDecodeArgs& a, bool f16, hipStream_t s
     const Ws       ws    = carve(a);
     const uint32_t pairs = a.tokens * a.topk;
     // 8 tiles' sums at a time, or 4 where two blocks then share a CU, or where 8 do not fit
-    const uint32_t rest = Lists::bytes(pairs) + Lists::up16(pairs) + a.tokens * row_bytes(a.hidden) + sizeof(GateUpLds);
+    const uint32_t rest = Lists::bytes(pairs) + Lists::up16(pairs)
+                          + a.tokens * row_bytes(a.hidden) + sizeof(GateUpLds);
     const uint32_t sum  = sizeof(TileSums);
     const bool     two  = rest + 4 * sum <= kLdsBytes / 2;
     const uint32_t group = rest + 8 * sum <= (two ? kLdsBytes / 2 : kLdsBytes) ? 8 : 4;
@@ -631,8 +635,8 @@ hipError_t launch_moe_ffn_decode(const MoeDecodeArgs& a, bool f16, hipStream_t s
     allow_lds(gu, lds);
     gu<<<blocks, kThreads, lds, stream>>>(a, ws, group);
     constexpr uint32_t kColumns = kRequantThreads * 16;
-    requant_kernel<<<dim3((a.inter + kColumns - 1) / kColumns, pairs), kRequantThreads, 0, stream>>>(
-        a, ws, blocks);
+    const dim3         grid((a.inter + kColumns - 1) / kColumns, pairs);
+    requant_kernel<<<grid, kRequantThreads, 0, stream>>>(a, ws, blocks);
     const hipError_t e = hipGetLastError();
     if(e != hipSuccess) return e;
     // a block for every CU, where the tokens leave room in the tile

@@ -24,8 +24,8 @@
 // cycles of products a wave and about as many of exponentials (a quarter of the rate),
 // sums, maxima and roundings, which 3 waves a SIMD overlap in part.  8192 tokens, 32
 // query and 8 key heads of 128: 565 to 650 us by the card's clock, 975 to 850
-// TFLOP/s; 16 heads of 64: 172 us, 800.  A block alone on its CU takes 0.76 us a
-// tile, which is what a single prompt of 1000 tokens waits for (31 us).
+// TFLOP/s; 16 heads of 64: 172 us, 800.  A block alone on its CU takes 1.2 us for 64 keys,
+// which is what a prompt of 1024 tokens waits for (26 us).
 #include "w8a8_device.hpp"
 #include "w8a8_internal.hpp"
 
@@ -48,11 +48,10 @@ constexpr int kWaves       = kRows / 32;
 constexpr int kThreads     = kWaves * kWave;
 constexpr uint32_t kCus    = 256;
 
-// Keys a tile: 8 KB of keys and 8 KB of values either way.  Heads of 128 take 32, whose
-// scores need registers for 3 waves a SIMD (8192 tokens, 32 heads: 622 us; 64 keys
-// and 2 waves 656), heads of 64 take 64 (16 heads: 176 us; 32 keys 193).
-template <int D>
-constexpr int kKeysOf = D == 128 ? 32 : 64;
+// Blocks a CU.  Keys a tile are 4096 / D, whose scores leave registers for 3 waves a SIMD
+// and more, or twice as many, two independent chains a wave, for 2.
+template <int D, int KEYS>
+constexpr int kBlocksOf = D * KEYS == 4096 ? 3 : 2;
 
 // Where a block works: one sequence's rows and a tile of kRows of them.
 struct Span {
@@ -215,10 +214,10 @@ __device__ __forceinline__ v4i buffer(const void* base, uint32_t bytes)
                __builtin_amdgcn_readfirstlane((int)bytes), kBufferFlags};
 }
 
-template <int D>
+template <int D, int kKeys>
 __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* lds)
 {
-    constexpr int kKeys      = kKeysOf<D>, kSubs = kKeys / 32;
+    constexpr int kSubs      = kKeys / 32;
     constexpr int kTileBytes = kKeys * D * 2;
     constexpr int kChunks    = D / 8;                  // 16-byte chunks per row
     constexpr int kRowsLoad  = kWave / kChunks;        // rows one wave-load fills
@@ -427,11 +426,11 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
         }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, 3) attention_kernel(AttentionArgs a)
+template <int D, int KEYS>
+__global__ void __launch_bounds__(kThreads, (kBlocksOf<D, KEYS>)) attention_kernel(AttentionArgs a)
 {
-    __shared__ alignas(256) uint8_t lds[2 * 2 * kKeysOf<D> * D * 2]; // two stages of keys, values
-    attention_rows<D>(a, lds);
+    __shared__ alignas(256) uint8_t lds[2 * 2 * KEYS * D * 2]; // two stages of keys, values
+    attention_rows<D, KEYS>(a, lds);
 }
 
 } // namespace
@@ -440,10 +439,21 @@ hipError_t launch_attention(const AttentionArgs& a, hipStream_t stream)
 {
     // no more tiles than full ones of all rows and one partial per sequence
     const uint32_t blocks = (a.tokens / kRows + a.seqs) * a.heads;
-    if(a.dim == 64)
-        attention_kernel<64><<<blocks, kThreads, 0, stream>>>(a);
-    else
-        attention_kernel<128><<<blocks, kThreads, 0, stream>>>(a);
+    // With few blocks a CU the time is a block's own, tile after tile, and the larger tiles
+    // take less of it per key; with many the smaller ones' third wave fills the gaps.
+    // us at tiles of 4096 / D and 8192 / D keys:
+    //   heads of 128, one sequence: 2048 tokens, 8 heads 55.1, 45.5; 32 heads (544 blocks)
+    //   61.1, 53.7; 4096 tokens, 32 heads (1056) 156, 161; 8192 tokens 616, 656
+    //   several, any of which may be the long one: 1 to 2047 tokens, 32 heads (1184) 75.5,
+    //   68.7; 8 x 512 (1280) 39.6, 39.7; 4 x 2048 (2176) 163, 168
+    //   heads of 64: 4096 tokens, 16 heads (528) 59.9, 55.2; 8 x 512 (640) 13.2, 12.8; 4 x
+    //   2048 (1088) 49.8, 55.3; 61 tokens, whose keys are one smaller tile, 4.7, 5.5
+    const uint32_t most = a.dim == 128 && a.seqs > 1 ? 5 * kCus : 3 * kCus;
+    const bool     few  = blocks <= most && (a.dim == 128 || a.tokens / a.seqs > 128);
+    const auto     kernel
+        = a.dim == 64 ? (few ? attention_kernel<64, 128> : attention_kernel<64, 64>)
+                      : (few ? attention_kernel<128, 64> : attention_kernel<128, 32>);
+    kernel<<<blocks, kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 

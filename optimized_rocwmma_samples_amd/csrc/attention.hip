@@ -38,7 +38,6 @@ typedef float    v2f __attribute__((ext_vector_type(2)));
 typedef float    v16f __attribute__((ext_vector_type(16)));
 typedef __fp16   v4fp16 __attribute__((ext_vector_type(4)));
 
-typedef __attribute__((address_space(3))) void   lds_void_t;
 typedef __attribute__((address_space(3))) v4fp16 lds_v4h_t;
 typedef __attribute__((address_space(3))) v8h    lds_v8h_t;
 

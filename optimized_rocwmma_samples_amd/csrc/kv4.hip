@@ -324,18 +324,13 @@ struct Unpack {
     }
 };
 
-// fp16(p * s), s the low half of w, into the low half (the high half undefined) or the
-// high half of a register: the product rounded once, in one instruction.
-__device__ __forceinline__ uint32_t scaled_low(float p, uint32_t w)
+// fp16(p * s), s the low half of w: one v_fma_mixlo_f16 or v_fma_mixhi_f16, which round the
+// product once.  Not in inline asm: the results are operands of matrix instructions, which
+// may read them two wait states later at the earliest, and the compiler keeps that distance
+// only from instructions that it sees.
+__device__ __forceinline__ _Float16 scaled(float p, uint32_t w)
 {
-    uint32_t r;
-    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(p), "v"(w));
-    return r;
-}
-
-__device__ __forceinline__ void scaled_high(uint32_t& r, float p, uint32_t w)
-{
-    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "+v"(r) : "v"(p), "v"(w));
+    return (_Float16)(p * (float)__builtin_bit_cast(_Float16, (uint16_t)w));
 }
 
 __device__ __forceinline__ v4f mfma16(v8h a, v8h b, v4f c)
@@ -728,7 +723,7 @@ __device__ __forceinline__ void attention_kv4_run(const CacheView& c, const Atte
         // operand register r of product u: token 4 kg + r of tile 2 u in the low and of
         // tile 2 u + 1 in the high half, zero for tiles of other classes
         const float pow2 = ldexpf(1.f, shift);
-        uint32_t    ps[kNG][2][4];
+        v2h         ps[kNG][2][4];
 #pragma unroll
         for(int w = 0; w < kPasses; ++w) {
             v4i sv[kNG];
@@ -743,26 +738,26 @@ __device__ __forceinline__ void attention_kv4_run(const CacheView& c, const Atte
                 for(int g = 0; g < kNG; ++g) {
                     const uint32_t u = (uint32_t)sv[(j * kNG + g) / 4][(j * kNG + g) % 4];
                     osum[g]          = fmaf(p[4 * w + j], high_half(u), osum[g]);
-                    if constexpr(C == 1) {
-                        if(w % 2 == 0)
-                            ps[g][w / 2][j] = scaled_low(f, u);
-                        else
-                            scaled_high(ps[g][w / 2][j], f, u);
-                    } else {
-                        uint32_t b = scaled_low(f, u);
-                        scaled_high(b, f, u);
+                    const _Float16 h = scaled(f, u);
+                    if constexpr(C == 1)
+                        ps[g][w / 2][j][w % 2] = h;
+                    else {
+                        const uint32_t b = __builtin_bit_cast(uint32_t, (v2h{h, h}));
                         if constexpr(C == 2)
-                            ps[g][w][j] = b & half_mask[0];
+                            ps[g][w][j] = __builtin_bit_cast(v2h, b & half_mask[0]);
                         else
 #pragma unroll
-                            for(int y = 0; y < 2; ++y) ps[g][y][j] = b & half_mask[y];
+                            for(int y = 0; y < 2; ++y)
+                                ps[g][y][j] = __builtin_bit_cast(v2h, b & half_mask[y]);
                     }
                 }
             }
         }
         auto operand = [&](int g, int u) {
-            return __builtin_bit_cast(
-                v8h, v4i{(int)ps[g][u][0], (int)ps[g][u][1], (int)ps[g][u][2], (int)ps[g][u][3]});
+            v8h f;
+#pragma unroll
+            for(int i = 0; i < 8; ++i) f[i] = ps[g][u][i / 2][i % 2];
+            return f;
         };
         const v8h ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll

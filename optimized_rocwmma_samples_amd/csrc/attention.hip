@@ -191,17 +191,22 @@ __device__ __forceinline__ v8h finite_only(v8h v)
     return __builtin_bit_cast(v8h, u);
 }
 
-// 16 bytes a lane from a buffer into LDS, lane i to byte `to` + 16 i, with the
-// caller's own waits: a load through the builtin makes the compiler wait for all
-// of them ahead of every transposed read, whichever stage that reads.
+// Twice 16 bytes a lane from a buffer into LDS, lane i to bytes `to` + 16 i and, from its
+// second offset, 1024 further, with the caller's own waits: a load through the builtin makes
+// the compiler wait for all of them ahead of every transposed read, whichever stage that
+// reads.  The compiler does not see what asm reads, so the block itself keeps the five wait
+// states between a vector instruction that writes a scalar register, such as the
+// readfirstlane of a descriptor, and a memory instruction that reads it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm" // m0 is reserved: set and used here alone
-__device__ __forceinline__ void load_lds(v4i rsrc, uint32_t to, uint32_t offset)
+__device__ __forceinline__ void load_lds(v4i rsrc, uint32_t to, uint32_t offset0,
+                                         uint32_t offset1)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+                 "s_add_u32 m0, %0, 1024\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
                  :
-                 : "s"(to), "v"(offset), "s"(rsrc)
-                 : "memory", "m0");
+                 : "s"(to), "v"(offset0), "v"(offset1), "s"(rsrc)
+                 : "memory", "m0", "scc");
 }
 #pragma clang diagnostic pop
 
@@ -223,6 +228,7 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
     constexpr int kLoads     = kKeys / kRowsLoad / kWaves; // wave-loads per wave and operand
     constexpr int kSteps     = D / 16;                 // MFMAs along the channels
     constexpr int kBlocks    = D / 32;                 // 32-channel blocks of the result
+    static_assert(kLoads % 2 == 0, "wave-loads go in pairs");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
 
@@ -263,9 +269,10 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
         const v4i      rv = buffer(vbase + (size_t)kt * kKeys * a.ldv, (n - 1) * ldvb + D * 2);
         const uint32_t to = lds0 + stage * 2 * kTileBytes + wave * kLoads * 1024;
 #pragma unroll
-        for(int i = 0; i < kLoads; ++i) load_lds(rk, to + i * 1024, ko[i]);
+        for(int i = 0; i < kLoads; i += 2) load_lds(rk, to + i * 1024, ko[i], ko[i + 1]);
 #pragma unroll
-        for(int i = 0; i < kLoads; ++i) load_lds(rv, to + kTileBytes + i * 1024, vo[i]);
+        for(int i = 0; i < kLoads; i += 2)
+            load_lds(rv, to + kTileBytes + i * 1024, vo[i], vo[i + 1]);
     };
 
     const uint32_t tiles = (row0 + rows + kKeys - 1) / kKeys; // tiles the block's rows see

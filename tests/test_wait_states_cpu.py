@@ -91,3 +91,20 @@ def test_scalar_registers_of_memory_instructions(kernels):
                 if o.startswith("v_") and registers(a[0], "s") & reads:
                     late.append((name, o, a, at, op, args))
     assert not late, late
+
+
+def test_loads_in_asm_keep_it_themselves(kernels):
+    # the loads into LDS of prompt attention: nothing but the asm block's own instructions
+    # lies in those five wait states, whatever stands in front of the block
+    found = 0
+    for name, code in kernels.items():
+        if "16attention_kernel" not in name:
+            continue
+        for i, (op, args, _) in enumerate(code):
+            if not (op.startswith("buffer_load") and args[-1] == "lds"):
+                continue
+            found += 1
+            for o, a, at in before(code[max(0, i - 5):i], 5):
+                own = o == "s_nop" or a[0] == "m0" or (o.startswith("buffer_load") and a[-1] == "lds")
+                assert own, (name, o, a, at)
+    assert found >= 16

@@ -332,3 +332,49 @@ def test_prompt_then_token(w8a8, gpu):
     wo = torch.randint(-127, 128, (hidden, hidden), generator=g, dtype=torch.int8).to(gpu)
     y, _, _ = w8a8.fused_sq_gemm(got.flatten(1), s, wo, sw[:hidden].contiguous())
     assert torch.isfinite(y).all()
+
+
+def _check_decode(w8a8, gpu, c, table, lens, heads, seed, spread=2.0):
+    """Attention over the cache with and without a workspace against the formula."""
+    import torch
+    R = _ref()
+    q = R.randn((len(lens), heads, c.head_dim), seed, gpu, spread)
+    n = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    out, bound = R.attention_kv4(q, c, table, lens, c.head_dim ** -0.5)
+    for ws in ("auto", None):
+        got = w8a8.attention_kv4(q, c, table, n, workspace=ws)
+        R.assert_within(got, out, bound, f"workspace {ws}")
+
+
+@pytest.mark.parametrize("dim,group", WIDTHS)
+@pytest.mark.parametrize("page,lens", [(16, [15, 16, 17, 0, 63, 64]), (64, [1, 127, 128, 129]),
+                                       (128, [700, 3])])
+@pytest.mark.parametrize("heads,kv_heads", [(8, 1), (5, 1), (16, 2), (18, 3), (32, 2), (36, 1)])
+def test_decode_heads_of_a_key_head(w8a8, gpu, dim, group, page, lens, heads, kv_heads):
+    # 5, 6 and 8 query heads a key head take half of a product's columns twice; 16 all of
+    # them; 36 three units, the last of four heads
+    cols = -(-max(lens) // page)
+    c = _filled(w8a8, gpu, cols + 3, kv_heads, dim, page, group, dim + page + heads)
+    table = _table(cols + 3, cols, len(lens), heads, gpu)
+    _check_decode(w8a8, gpu, c, table, lens, heads, heads + 1)
+
+
+@pytest.mark.parametrize("dim,group,heads,kv_heads", [(128, 32, 64, 8), (128, 64, 40, 8),
+                                                      (128, 128, 8, 1), (64, 32, 12, 2)])
+def test_decode_long_contexts_of_5_to_8_heads(w8a8, gpu, dim, group, heads, kv_heads):
+    lens = [4999, 1, 8192, 0, 3333, 64]
+    c = _filled(w8a8, gpu, 140, kv_heads, dim, 64, group, 78)
+    _check_decode(w8a8, gpu, c, _table(140, 128, len(lens), 6, gpu), lens, heads, 7)
+
+
+@pytest.mark.parametrize("seqs,heads,kv_heads,dim,group", [(130, 8, 1, 128, 32),
+                                                           (130, 6, 2, 64, 64),
+                                                           (300, 32, 8, 128, 64),
+                                                           (300, 64, 8, 64, 32)])
+def test_decode_many_sequences(w8a8, gpu, seqs, heads, kv_heads, dim, group):
+    # more sequences than lanes; more units than waves, and more heads to join than blocks
+    rng = np.random.default_rng(seqs + heads)
+    lens = [int(v) for v in rng.integers(0, 250, seqs)]
+    lens[:3] = [256, 0, 1]
+    c = _filled(w8a8, gpu, 40, kv_heads, dim, 32, group, seqs)
+    _check_decode(w8a8, gpu, c, _table(40, 8, seqs, seqs, gpu), lens, heads, 9)

@@ -212,3 +212,104 @@ def test_full_size(w8a8, gpu, tokens, e, topk, h, i):
     layer = Layer(e, h, i, tokens, gpu)
     x, logits = layer.x(tokens), layer.logits(tokens)
     _check(layer.run(w8a8, x, logits, topk), layer.reference(x, logits, topk))
+
+
+class Steps:
+    """The layer's result with its whole numbers settled.  The first quantizer's steps are
+    single fp32 operations, taken here one by one on the CPU, so its codes and scales are
+    the kernel's, and so are the gate and up values (exact integer sums, two products).
+    From there on, what may differ from the 64-bit values below:
+      * an activation by 2^-20: 1 ulp of the exponential and one of its correction, one of
+        the sum, one of the quotient, two products make 8 * 2^-24, taken twice
+      * the second quantizer's quotient by 2 * 2^-20 and three roundings, at most NEAR of a
+        step: within that of a half the code may be either neighbour, one step of its
+        column of the weights
+      * a product with its scales and weight by 2^-17: the weight's sum over 4096 experts
+        is 72 roundings, all others less than 16
+      * the result by one rounding to fp16"""
+
+    NEAR = 127 * 2.0 ** -18
+
+    def __init__(self, layer):
+        self.layer = layer
+
+    @staticmethod
+    def _codes(p, qmax):
+        import torch
+        qmax = torch.tensor(qmax)
+        r = p.abs().max() / qmax
+        inv = 1.0 / r if float(r) > 0 else torch.tensor(0.0)
+        return torch.clamp(torch.round(p * inv), -qmax, qmax), r
+
+    def expert(self, row, e, qmax):
+        """(y, bound) fp64 [hidden] of one token's row through one expert."""
+        import torch
+        m = self.layer
+        cpu = lambda t: t[e].cpu()  # noqa: E731
+        q, r = self._codes(row.cpu().float() * cpu(m.s), qmax)
+        sums = (m.wgu[e].double() @ q.double().to(m.gpu)).cpu()
+        gu = (sums.float() * r * cpu(m.sgu)).double()  # in fp32, step by step
+        g, u = gu[: m.i], gu[m.i:]
+        a = g * torch.sigmoid(g) * u
+        if m.s2 is not None:
+            a = a * cpu(m.s2).double()
+        r2 = a.abs().max() / qmax
+        if float(r2) == 0.0:
+            return torch.zeros(m.h, dtype=torch.float64), torch.zeros(m.h, dtype=torch.float64)
+        z = a / r2
+        q2 = torch.clamp(torch.round(z), -qmax, qmax)
+        near = ((z - torch.floor(z) - 0.5).abs() < self.NEAR).double()
+        wd, scale = m.wd[e].double(), (r2 * cpu(m.sd).double())
+        y = (wd @ q2.to(m.gpu)).cpu() * scale
+        dy = (wd.abs() @ near.to(m.gpu)).cpu() * scale
+        return y, dy + 2.0 ** -17 * (y.abs() + dy)
+
+    def layer_result(self, x, logits, topk, qmax=127.0):
+        import torch
+        lg = logits.cpu().double()
+        p = torch.softmax(lg, 1)
+        out = torch.zeros((x.shape[0], self.layer.h), dtype=torch.float64)
+        bound = torch.zeros_like(out)
+        for t in range(x.shape[0]):
+            row = lg[t].tolist()
+            for e in sorted(range(self.layer.e), key=lambda e: (-row[e], e))[:topk]:
+                y, dy = self.expert(x[t], e, qmax)
+                out[t] += p[t, e] * y
+                bound[t] += p[t, e] * dy
+        return out, bound + 2.0 ** -11 * (out.abs() + bound) + 2.0 ** -25
+
+
+def _check_steps(layer, got, x, logits, topk, qmax=127.0):
+    out, bound = Steps(layer).layer_result(x, logits, topk, qmax)
+    rms = float(out.square().mean().sqrt())
+    assert float(bound.median()) < 0.02 * rms and float(bound.max()) < 0.2 * rms, \
+        "the bound says nothing"
+    over = (got.cpu().double() - out).abs() - bound
+    assert float(over.max()) <= 0, (int((over > 0).sum()), float(over.max()), rms)
+
+
+@pytest.mark.parametrize("e,topk,h,i,tokens", [
+    (8, 2, 256, 352, 1), (8, 2, 256, 352, 5), (64, 6, 512, 96, 16), (100, 8, 1040, 272, 1),
+    (100, 8, 1040, 272, 7), (16, 1, 128, 4096, 16), (8, 2, 4096, 64, 3), (12, 3, 2048, 80, 8),
+    (2, 2, 32768, 16, 3), (2, 1, 16, 32768, 16), (64, 6, 2048, 1408, 5), (6, 2, 1024, 144, 4)])
+def test_layer_step_by_step(w8a8, gpu, e, topk, h, i, tokens):
+    layer = Layer(e, h, i, 3 * e + tokens, gpu)
+    x, logits = layer.x(tokens), layer.logits(tokens)
+    _check_steps(layer, layer.run(w8a8, x, logits, topk), x, logits, topk)
+
+
+@pytest.mark.parametrize("tokens,e,topk,h,i", [(1, 8, 2, 4096, 14336), (2, 8, 2, 4096, 14336),
+                                               (16, 8, 2, 4096, 14336), (16, 16, 6, 7168, 2048),
+                                               (3, 16, 6, 7168, 2048)])
+def test_full_size_step_by_step(w8a8, gpu, tokens, e, topk, h, i):
+    layer = Layer(e, h, i, tokens, gpu)
+    x, logits = layer.x(tokens), layer.logits(tokens)
+    _check_steps(layer, layer.run(w8a8, x, logits, topk), x, logits, topk)
+
+
+@pytest.mark.parametrize("qmax", [127.0, 100.0, 7.0])
+def test_fp16_logits_without_down_scale_step_by_step(w8a8, gpu, qmax):
+    import torch
+    layer = Layer(16, 384, 160, 25, gpu, down=False)
+    x, logits = layer.x(7), layer.logits(7, torch.float16)
+    _check_steps(layer, layer.run(w8a8, x, logits, 4, quant_max=qmax), x, logits, 4, qmax)

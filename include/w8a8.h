@@ -671,8 +671,9 @@ typedef struct w8a8_kv4_cache {
  * the cache skips its token).  Per group of channels, fp32 arithmetic:
  *   scale  = half((max - min) / 15),  offset = half(min + 8 * scale)
  *   code   = clamp(rint((x - offset) / scale) + 8, 0, 15), 8 where scale = 0
- * A group of equal values is stored exactly (up to the fp16 it came in); one
- * that holds an infinity or a NaN reads back as NaN.  The slots inside the cache
+ * A group of equal values is stored exactly (up to the fp16 it came in), any
+ * finite one reads back finite; one that holds an infinity or a NaN reads back as
+ * NaN.  The slots inside the cache
  * are all different: of one that is given twice the row, and no other, is left
  * with codes and scales of both tokens.
  *   k, v  fp16 [tokens, ldk / ldv] (0 means kv_heads * head_dim), head h in
@@ -684,8 +685,8 @@ int w8a8_kv4_store(const void* k, const void* v, const int32_t* slots, uint32_t 
 
 /*
  * Reads rows of the cache back: k, v fp16 [tokens, ldk / ldv] of the slots
- * given, half(fma(scale, code - 8, offset)).  Rows of slots outside the cache
- * are left as they were.
+ * given, half(fma(scale, code - 8, offset)), and 65504 with its sign where that
+ * passes the range of fp16.  Rows of slots outside the cache are left as they were.
  */
 int w8a8_kv4_load(void* k, void* v, const int32_t* slots, uint32_t tokens, uint32_t ldk,
                   uint32_t ldv, const w8a8_kv4_cache* cache, hipStream_t stream);
@@ -704,7 +705,7 @@ int w8a8_kv4_load(void* k, void* v, const int32_t* slots, uint32_t tokens, uint3
  *   zeros.
  * Codes enter the matrix products as they are, exactly; scores, softmax
  * statistics and sums are fp32, and p * scale of a value is rounded to fp16 as
- * the second product's operand.
+ * the second product's operand.  Results past the range of fp16 are its ends.
  * workspace: 16-byte aligned, w8a8_attention_kv4_workspace_size(seqs, heads,
  * kv_heads, head_dim, table_cols * page_size) bytes, needs no clearing: the
  * work of all sequences is cut into equal runs, one a wave, and a second launch

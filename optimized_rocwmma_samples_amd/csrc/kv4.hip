@@ -117,6 +117,17 @@ __device__ __forceinline__ float quotient(float a, float b, float y)
     return fmaf(fmaf(-q, b, a), y, q);
 }
 
+// Two fp32 results as packed fp16, those past its range as its ends: the last code of a
+// group that reaches 65504 may stand for a little more, its step being rounded (0 .. 65504
+// has steps of 4368 and ends at 65520, which would be an infinity).  NaN stays NaN.
+__device__ __forceinline__ uint32_t finite_halves(float a, float b)
+{
+    const v2h most = {(_Float16)65504.f, (_Float16)65504.f};
+    const v2h h    = __builtin_bit_cast(v2h, float2_to_half2_bits_2step(a, b));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_minimum(
+                                            __builtin_elementwise_maximum(h, -most), most));
+}
+
 // The 8 codes of a thread's channels and its group's (scale, offset).
 template <int G>
 __device__ __forceinline__ v2i quantized(v4i raw)
@@ -213,7 +224,7 @@ __global__ void __launch_bounds__(kRowThreads)
                 const uint32_t w = codes[side] >> (8 * j);
                 const float    a = fmaf(s, (float)(w & 15u) - 8.f, mid);
                 const float    b = fmaf(s, (float)(w >> 4 & 15u) - 8.f, mid);
-                out[j]           = (int)float2_to_half2_bits_2step(a, b);
+                out[j]           = (int)finite_halves(a, b);
             }
             uint16_t* to = side ? v + (size_t)t.token * r.ldv : k + (size_t)t.token * r.ldk;
             *reinterpret_cast<v4i*>(to + t.head * D + t.chunk * 8) = out;
@@ -812,8 +823,8 @@ __device__ __forceinline__ void attention_kv4_run(const CacheView& c, const Atte
                 const size_t to = (size_t)now.seq * a.ldo
                                   + (size_t)(now.unit / qtiles * per + head) * D + 16 * t + 4 * kg;
                 v2i w;
-                w[0] = (int)float2_to_half2_bits_2step(v[0], v[1]);
-                w[1] = (int)float2_to_half2_bits_2step(v[2], v[3]);
+                w[0] = (int)finite_halves(v[0], v[1]);
+                w[1] = (int)finite_halves(v[2], v[3]);
                 *reinterpret_cast<v2i*>(a.out + to) = w;
             } else
                 *reinterpret_cast<v4f*>(cut.o + ((size_t)slot * kHeads + col) * D + 16 * t + 4 * kg)
@@ -935,8 +946,8 @@ __global__ void __launch_bounds__(kAttThreads)
         if(way != 0) continue;
         const float inv = l != 0.f ? 1.f / l : 0.f;
         v2i         w;
-        w[0] = (int)float2_to_half2_bits_2step(sum[0] * inv, sum[1] * inv);
-        w[1] = (int)float2_to_half2_bits_2step(sum[2] * inv, sum[3] * inv);
+        w[0] = (int)finite_halves(sum[0] * inv, sum[1] * inv);
+        w[1] = (int)finite_halves(sum[2] * inv, sum[3] * inv);
         *reinterpret_cast<v2i*>(a.out + (size_t)(u / units) * a.ldo
                                 + (size_t)(u % units / qtiles * per + head) * D + ch)
             = w;

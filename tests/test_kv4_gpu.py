@@ -378,3 +378,47 @@ def test_decode_many_sequences(w8a8, gpu, seqs, heads, kv_heads, dim, group):
     lens[:3] = [256, 0, 1]
     c = _filled(w8a8, gpu, 40, kv_heads, dim, 32, group, seqs)
     _check_decode(w8a8, gpu, c, _table(40, 8, seqs, seqs, gpu), lens, heads, 9)
+
+
+def test_ends_of_fp16_read_back_finite(w8a8, gpu):
+    # groups that reach 65504: the step and the offset are rounded to fp16, so the last code
+    # may stand for more, and a finite group reads back finite all the same
+    import torch
+    R = _ref()
+    c = _zeros(w8a8, gpu, 2, 2, 128, 16, 32)
+    g = torch.Generator().manual_seed(1)
+    x = torch.rand((6, 2, 128), generator=g)
+    low = torch.tensor([0.0, -65504.0, -65504.0, 60000.0, -65504.0, 32768.0])[:, None, None]
+    high = torch.tensor([65504.0, 65504.0, -34772.0, 65504.0, 0.0, 65504.0])[:, None, None]
+    x = low + (high - low) * x
+    x[..., 0::32], x[..., 1::32] = low.expand(6, 2, 4), high.expand(6, 2, 4)
+    x = x.to(torch.float16).to(gpu)
+    assert torch.isfinite(x).all()
+    slots = torch.arange(6, dtype=torch.int32, device=gpu) + 5
+    w8a8.kv4_store(x, x.flip(2).contiguous(), slots, c)
+    k, v = w8a8.kv4_load(c, slots)
+    whole = R.cache_values(c, True)[0][0, :, 5:11].transpose(0, 1)
+    assert (whole.abs() >= 65520).any()  # what the codes stand for: past fp16
+    for got, want in ((k, x), (v, x.flip(2))):
+        assert torch.isfinite(got).all()
+        # half a step of 8736 at the most, and the roundings of step and offset
+        assert ((got.double() - want.double()).abs() <= 4368 + 15 * 8 + 16).all()
+    # and attended to: a context of one such token is its values
+    table = torch.zeros((1, 1), dtype=torch.int32, device=gpu)
+    q = R.randn((1, 4, 128), 6, gpu)
+    for t in range(6):
+        d = w8a8.KV4Cache.empty(1, 2, 128, 16, 32, gpu)
+        w8a8.kv4_store(x[t:t + 1] * 0, x[t:t + 1], torch.zeros(1, dtype=torch.int32, device=gpu), d)
+        _, want = w8a8.kv4_load(d, torch.zeros(1, dtype=torch.int32, device=gpu))
+        got = w8a8.attention_kv4(q, d, table, torch.ones(1, dtype=torch.int32, device=gpu))
+        assert torch.isfinite(got).all()
+        err = (got[0].view(2, 2, 128).double() - want[0, :, None].double()).abs()
+        # p is 1: the scale of the centred code is rounded once as fp16, the result once
+        assert (err <= 2.0 ** -11 * 8 * 8736 + 2.0 ** -11 * 65504).all()
+    # cut by runs, whose parts a second launch joins: 256 such tokens
+    d = w8a8.KV4Cache.empty(16, 1, 128, 16, 32, gpu)
+    many = x[:1, :1].expand(256, 1, 128).contiguous()
+    w8a8.kv4_store(many * 0, many, torch.arange(256, dtype=torch.int32, device=gpu), d)
+    got = w8a8.attention_kv4(q[:, :2], d, torch.arange(16, dtype=torch.int32, device=gpu)[None],
+                             torch.tensor([256], dtype=torch.int32, device=gpu))
+    assert torch.isfinite(got).all() and float(got.max()) >= 65504 - 2.0 ** -11 * 8 * 8736

@@ -791,6 +791,8 @@ def _row_stride(name, rows: int, stride: int, columns: int) -> int:
         return columns
     if stride < columns:
         raise ValueError(f"{name}: rows of {columns} values overlap (row stride {stride})")
+    if stride > 0xFFFFFFFF:  # the library takes it in 32 bits
+        raise ValueError(f"{name}: row stride {stride} is past 32 bits")
     return stride
 
 
@@ -980,7 +982,7 @@ def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None
             or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be a contiguous int32 tensor [seqs]")
     cols = block_table.shape[1]
-    table_ld = block_table.stride(0) if seqs > 1 else cols
+    table_ld = _row_stride("block_table", seqs, block_table.stride(0), cols)
     out, ldo = _heads_out(out, q, seqs, heads, dim)
     _workspace_on(workspace, dev)
     ws, ws_bytes = _workspace(

@@ -54,3 +54,15 @@ def test_workspaces():
         W._workspace_on(torch.zeros(8)[::2], torch.device("cpu"))
     with pytest.raises(ValueError, match="device tensors"):
         W._workspace_on(torch.zeros(8), torch.device("meta"))
+
+
+def test_row_strides_past_32_bits():
+    # the library takes strides in 32 bits: 2^32 + 256 must not become 256
+    far = 2 ** 32 + 256
+    t = torch.empty_strided((2, 4, 64), (far, 64, 1), dtype=torch.float16, device="meta")
+    with pytest.raises(ValueError, match="row stride"):
+        W._heads3d("k", t)
+    with pytest.raises(ValueError, match="row stride"):
+        W._row_stride("block_table", 2, 2 ** 32 + 16, 16)
+    assert W._row_stride("x", 2, 2 ** 32 - 8, 256) == 2 ** 32 - 8
+    assert W._row_stride("x", 1, far, 256) == 256  # one row: never read

@@ -803,7 +803,7 @@ def _workspace_on(workspace, device) -> None:
             raise ValueError("workspace must be contiguous")
 
 
-def _heads3d(name, t, heads=None, dim=None) -> int:
+def _heads3d(name, t, heads=None, dim=None, rows=None) -> int:
     """Checks fp16 [tokens, heads, dim] whose heads lie side by side; its row stride."""
     shape = t.shape
     if len(shape) != 3 or t.dtype != _torch_module.float16:
@@ -811,6 +811,8 @@ def _heads3d(name, t, heads=None, dim=None) -> int:
     n, h, d = shape
     if (heads is not None and h != heads) or (dim is not None and d != dim):
         raise ValueError(f"{name} must have {heads} heads of {dim} channels, got {tuple(shape)}")
+    if rows is not None and n != rows:
+        raise ValueError(f"{name} must have {rows} rows, got {n}")
     row, head, channel = t.stride()
     if channel != 1 or (h > 1 and head != d):
         raise ValueError(f"{name}: the heads of a token must lie side by side "
@@ -822,10 +824,7 @@ def _heads_out(out, q, tokens: int, heads: int, dim: int):
     # the result and its row stride: a new tensor where none is given
     if out is None:
         return q.new_empty((tokens, heads, dim)), heads * dim
-    ldo = _heads3d("out", out, heads, dim)
-    if out.shape[0] != tokens:
-        raise ValueError(f"out must have {tokens} rows")
-    return out, ldo
+    return out, _heads3d("out", out, heads, dim, tokens)
 
 
 def attention(q, k, v, seq_starts, scale: float | None = None, out=None):
@@ -863,7 +862,9 @@ class KV4Cache:
     """A paged cache of keys and values in 4 bits (w8a8_kv4_cache), over four
     tensors: k_codes, v_codes uint8 [pages, kv_heads, page_size, head_dim / 2]
     and k_scales, v_scales fp16 [pages, kv_heads, page_size, head_dim / group, 2].
-    KV4Cache.empty allocates them; the cache keeps them alive."""
+    KV4Cache.empty allocates them; the cache keeps them alive.  It is made for these
+    tensors: they are not to be given other memory (`.data = ...`, `set_`, a `resize_`
+    that moves them), which the calls refuse."""
 
     def __init__(self, k_codes, v_codes, k_scales, v_scales):
         torch = _torch()
@@ -880,16 +881,28 @@ class KV4Cache:
             _require(name, t, torch.float16, (pages, kv_heads, page_size, groups, 2))
         if 2 * half % groups != 0:
             raise ValueError("the groups must divide the channels of a head")
-        self.k_codes, self.v_codes, self.k_scales, self.v_scales = (k_codes, v_codes, k_scales,
-                                                                    v_scales)
+        self._k_codes, self._v_codes, self._k_scales, self._v_scales = (k_codes, v_codes, k_scales,
+                                                                        v_scales)
         self.pages, self.kv_heads, self.page_size, self.head_dim = (pages, kv_heads, page_size,
                                                                     2 * half)
         self.group = 2 * half // groups
         self.device = k_codes.device
-        self._desc = _lib.Kv4Cache(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(),
-                                   v_scales.data_ptr(), pages, page_size, kv_heads, 2 * half,
-                                   self.group)
+        self._where = (k_codes.data_ptr, v_codes.data_ptr, k_scales.data_ptr, v_scales.data_ptr)
+        self._at = tuple(where() for where in self._where)
+        self._desc = _lib.Kv4Cache(*self._at, pages, page_size, kv_heads, 2 * half, self.group)
         self._ref = ctypes.byref(self._desc)
+
+    k_codes = property(lambda self: self._k_codes)
+    v_codes = property(lambda self: self._v_codes)
+    k_scales = property(lambda self: self._k_scales)
+    v_scales = property(lambda self: self._v_scales)
+
+    def _descriptor(self):
+        # the descriptor made once, as long as the tensors lie where they did then
+        k, v, ks, vs = self._where
+        if (k(), v(), ks(), vs()) != self._at:
+            raise ValueError("a tensor of the cache was given other memory: make a new KV4Cache")
+        return self._ref
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, group: int = 32,
@@ -918,12 +931,10 @@ def kv4_store(k, v, slots, cache: KV4Cache) -> None:
     different: a row given twice is left with parts of both tokens."""
     _require_on(cache.device, k=k, v=v, slots=slots)
     n = _kv4_slots(slots)
-    ldk = _heads3d("k", k, cache.kv_heads, cache.head_dim)
-    ldv = _heads3d("v", v, cache.kv_heads, cache.head_dim)
-    if k.shape[0] != n or v.shape[0] != n:
-        raise ValueError(f"k and v must have {n} tokens, one per slot")
+    ldk = _heads3d("k", k, cache.kv_heads, cache.head_dim, n)
+    ldv = _heads3d("v", v, cache.kv_heads, cache.head_dim, n)
     _call_on(cache.device, "w8a8_kv4_store", k.data_ptr(), v.data_ptr(), slots.data_ptr(), n, ldk,
-             ldv, cache._ref, _stream(cache.device))
+             ldv, cache._descriptor(), _stream(cache.device))
 
 
 def kv4_load(cache: KV4Cache, slots, out=None):
@@ -934,17 +945,16 @@ def kv4_load(cache: KV4Cache, slots, out=None):
     n = _kv4_slots(slots)
     if out is None:
         shape = (n, cache.kv_heads, cache.head_dim)
-        k, v = cache.k_scales.new_empty(shape), cache.k_scales.new_empty(shape)
+        new = cache._k_scales.new_empty
+        k, v = new(shape), new(shape)
         ldk = ldv = cache.kv_heads * cache.head_dim
     else:
         k, v = out
         _require_on(cache.device, k=k, v=v)
-        ldk = _heads3d("k", k, cache.kv_heads, cache.head_dim)
-        ldv = _heads3d("v", v, cache.kv_heads, cache.head_dim)
-        if k.shape[0] != n or v.shape[0] != n:
-            raise ValueError(f"k and v must have {n} rows, one per slot")
+        ldk = _heads3d("k", k, cache.kv_heads, cache.head_dim, n)
+        ldv = _heads3d("v", v, cache.kv_heads, cache.head_dim, n)
     _call_on(cache.device, "w8a8_kv4_load", k.data_ptr(), v.data_ptr(), slots.data_ptr(), n, ldk,
-             ldv, cache._ref, _stream(cache.device))
+             ldv, cache._descriptor(), _stream(cache.device))
     return k, v
 
 
@@ -975,20 +985,20 @@ def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None
     _require_on(dev, q=q, block_table=block_table, seq_lens=seq_lens, out=out)
     ldq = _heads3d("q", q, None, cache.head_dim)
     seqs, heads, dim = q.shape
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != seqs \
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    table = block_table.shape
+    cols = table[1] if len(table) == 2 else 0
+    if block_table.dtype != torch.int32 or table != (seqs, cols) \
+            or (cols > 1 and block_table.stride(1) != 1):
         raise ValueError("block_table must be int32 [seqs, columns] with unit column stride")
-    if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (seqs,) \
-            or not seq_lens.is_contiguous():
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (seqs,) or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be a contiguous int32 tensor [seqs]")
-    cols = block_table.shape[1]
     table_ld = _row_stride("block_table", seqs, block_table.stride(0), cols)
     out, ldo = _heads_out(out, q, seqs, heads, dim)
     _workspace_on(workspace, dev)
     ws, ws_bytes = _workspace(
         workspace, lambda: _kv4_workspace_size(seqs, heads, cache.kv_heads, dim,
                                                cols * cache.page_size), dev)
-    _call_on(dev, "w8a8_attention_kv4", q.data_ptr(), cache._ref, block_table.data_ptr(), cols,
+    _call_on(dev, "w8a8_attention_kv4", q.data_ptr(), cache._descriptor(), block_table.data_ptr(), cols,
              table_ld, seq_lens.data_ptr(), out.data_ptr(), seqs, heads, ldq, ldo,
              dim ** -0.5 if scale is None else float(scale), _ptr(ws), ws_bytes, _stream(dev))
     return out

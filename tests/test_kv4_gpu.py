@@ -422,3 +422,28 @@ def test_ends_of_fp16_read_back_finite(w8a8, gpu):
     got = w8a8.attention_kv4(q[:, :2], d, torch.arange(16, dtype=torch.int32, device=gpu)[None],
                              torch.tensor([256], dtype=torch.int32, device=gpu))
     assert torch.isfinite(got).all() and float(got.max()) >= 65504 - 2.0 ** -11 * 8 * 8736
+
+
+def test_cache_whose_tensors_move_is_refused(w8a8, gpu):
+    # the handle knows where its tensors lay: calls must not write where they no longer are
+    import torch
+    c = _filled(w8a8, gpu, 3, 2, 64, 16, 32, 5)
+    with pytest.raises(AttributeError):
+        c.k_codes = torch.zeros_like(c.k_codes)
+    kv = _ref().randn((2, 2, 64), 1, gpu)
+    slots = torch.tensor([3, 40], dtype=torch.int32, device=gpu)
+    table = torch.tensor([[0, 1], [2, 0]], dtype=torch.int32, device=gpu)
+    q, n = _ref().randn((2, 4, 64), 2, gpu), torch.tensor([20, 9], dtype=torch.int32, device=gpu)
+    want = w8a8.attention_kv4(q, c, table, n)
+    for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
+        t = getattr(c, name)
+        keep = t.data
+        t.data = t.clone()
+        for call in (lambda: w8a8.kv4_store(kv, kv, slots, c), lambda: w8a8.kv4_load(c, slots),
+                     lambda: w8a8.attention_kv4(q, c, table, n)):
+            with pytest.raises(ValueError, match="KV4Cache"):
+                call()
+        assert torch.equal(w8a8.attention_kv4(
+            q, w8a8.KV4Cache(c.k_codes, c.v_codes, c.k_scales, c.v_scales), table, n), want)
+        t.data = keep
+    assert torch.equal(w8a8.attention_kv4(q, c, table, n), want)

@@ -909,6 +909,8 @@ class KV4Cache:
               device="cuda"):
         """A cache of newly allocated pages (contents undefined)."""
         torch = _torch()
+        if group <= 0 or head_dim % group != 0:
+            raise ValueError(f"group must divide head_dim (group={group} head_dim={head_dim})")
         codes = (pages, kv_heads, page_size, head_dim // 2)
         scales = (pages, kv_heads, page_size, head_dim // group, 2)
         return cls(torch.empty(codes, dtype=torch.uint8, device=device),

@@ -66,3 +66,10 @@ def test_row_strides_past_32_bits():
         W._row_stride("block_table", 2, 2 ** 32 + 16, 16)
     assert W._row_stride("x", 2, 2 ** 32 - 8, 256) == 2 ** 32 - 8
     assert W._row_stride("x", 1, far, 256) == 256  # one row: never read
+
+
+@pytest.mark.parametrize("dim,group", [(128, 48), (128, 100), (64, 128), (64, 0), (96, 64)])
+def test_cache_groups_that_do_not_divide_the_head(dim, group):
+    # 128 channels in groups of 48 are not two groups of 64
+    with pytest.raises(ValueError, match="group"):
+        W.KV4Cache.empty(2, 2, dim, 16, group, device="meta")

@@ -431,6 +431,8 @@ int w8a8_grouped_gemm(const w8a8_group_desc* groups, uint32_t num_groups, int ou
  *           the reference's input type, :42)
  *   topk_weights fp32 [tokens, topk] = softmax probability of each choice
  *   topk_ids     int32 [tokens, topk], best first; ties go to the lower id.
+ * NaN logits are never chosen (id -1 where only such are left), and a token that
+ * has one gets weights of 0, since the sum below the line is NaN.
  * experts <= 4096, topk <= experts (the reference caps at 64 experts, :172).
  */
 int w8a8_topk_softmax(const void* logits, int logits_f16, float* topk_weights,
@@ -576,18 +578,23 @@ int w8a8_moe_combine(const void* y, uint32_t ldy, uint32_t rows_y, const float* 
  * (w8a8_topk_softmax ... w8a8_moe_combine), without its sort and without an
  * fp16 rounding between the steps.  Per token t and slot s, with e = the
  * token's s-th expert and its softmax weight as w8a8_topk_softmax gives them
- * (a slot without an expert contributes nothing), all in fp32:
+ * (a slot without an expert contributes nothing, a token with a NaN logit gives
+ * zeros), all in fp32:
  *   q, r   = quantizer of float(x[t]) * smooth_scale[e]
  *   g, u   = (float(q . w_gate_up[e]^T) * r) * sb_gate_up[e]   (rows [0, inter), [inter, 2 inter))
  *   a      = (g / (1 + exp(-g))) * u [* smooth_scale_down[e]]
  *   q2, r2 = quantizer of a
  *   y      = (float(q2 . w_down[e]^T) * r2) * sb_down[e]
  *   out[t] = half(sum over slots s (ascending) of fma(weight[t, s], y, acc))
+ * The quantizer is w8a8_smoothquant's, at NaN too: a NaN value counts for nothing in its
+ * row's maximum and becomes -quant_max, so a NaN in x does not make a token's row NaN.
  *   x            fp16 [tokens, ldx] (ldx = 0 means hidden), out fp16 [tokens, ldo]
  *                (ldo = 0 means hidden); out may not overlap x
  *   logits       fp32 or (logits_f16 = 1) fp16 [tokens, experts]
  *   smooth_scale fp32 [experts, hidden]; smooth_scale_down fp32 [experts, inter] or NULL
- *   w_gate_up    int8 [experts, 2 * inter, hidden], sb_gate_up fp32 [experts, 2 * inter]
+ *   w_gate_up    int8 [experts, 2 * inter, hidden], sb_gate_up fp32 [experts, 2 * inter]:
+ *                all gate rows, then all up rows, not the interleaved blocks of
+ *                w8a8_moe_interleave_gate_up, which have the same shape
  *   w_down       int8 [experts, hidden, inter], sb_down fp32 [experts, hidden]
  * tokens <= W8A8_MOE_DECODE_MAX_TOKENS, tokens * hidden <=
  * W8A8_MOE_DECODE_MAX_VALUES (16 tokens of 7168), experts <= 4096, topk <= 32;

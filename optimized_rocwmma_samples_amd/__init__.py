@@ -736,11 +736,13 @@ def moe_ffn_decode(x, logits, smooth_scale, w_gate_up, sb_gate_up, w_down, sb_do
     """The expert FFN of moe_ffn for at most 16 tokens, in three launches.
 
     x fp16 [T, H] (any row stride that is a multiple of 8), logits fp32 or fp16
-    [T, E], smooth_scale fp32 [E, H], w_gate_up int8 [E, 2*I, H] with sb_gate_up
+    [T, E], smooth_scale fp32 [E, H], w_gate_up int8 [E, 2*I, H] (gate rows, then up
+    rows: not moe_interleave_gate_up's blocks, which look the same) with sb_gate_up
     fp32 [E, 2*I], w_down int8 [E, H, I] with sb_down fp32 [E, H],
     smooth_scale_down fp32 [E, I] or None.  Returns out fp16 [T, H].  The
     intermediate values stay fp32 (moe_ffn rounds the GEMM outputs to fp16), so
-    the result is moe_ffn's up to those roundings.
+    the result is moe_ffn's up to those roundings.  A NaN in x becomes -quant_max in the
+    quantizer, as everywhere in the package; a token with a NaN logit gives zeros.
     workspace: 'auto' (allocated here) or a device tensor of
     moe_ffn_decode_workspace_size bytes."""
     torch = _torch()

@@ -27,7 +27,8 @@ __device__ __forceinline__ void better(float& v, int& i, float ov, int oi)
 }
 
 // The topk experts of one token, best first: emit(k, id, weight) in every lane
-// for k = 0 .. topk - 1, id = -1 and weight = 0 where only NaN logits are left.
+// for k = 0 .. topk - 1, id = -1 and weight = 0 where only NaN logits are left; one NaN
+// makes the sum NaN and with it every weight 0.
 // Experts are chosen on the logits (softmax is monotonic, so the choice is
 // exact), the lower index winning ties; weight = exp(l - max) * (1 / sum_e
 // exp(l_e - max)).  logit(e): the fp32 value of expert e's logit.  A lane owns

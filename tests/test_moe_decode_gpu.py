@@ -237,9 +237,10 @@ class Steps:
     def _codes(p, qmax):
         import torch
         qmax = torch.tensor(qmax)
-        r = p.abs().max() / qmax
+        r = p.abs().nan_to_num(nan=0.0, posinf=torch.inf).max() / qmax
         inv = 1.0 / r if float(r) > 0 else torch.tensor(0.0)
-        return torch.clamp(torch.round(p * inv), -qmax, qmax), r
+        q = torch.clamp(torch.round(p * inv), -qmax, qmax)
+        return torch.where(torch.isnan(q), -qmax, q), r  # NaN as the package's quantizer has it
 
     def expert(self, row, e, qmax):
         """(y, bound) fp64 [hidden] of one token's row through one expert."""
@@ -313,3 +314,27 @@ def test_fp16_logits_without_down_scale_step_by_step(w8a8, gpu, qmax):
     layer = Layer(16, 384, 160, 25, gpu, down=False)
     x, logits = layer.x(7), layer.logits(7, torch.float16)
     _check_steps(layer, layer.run(w8a8, x, logits, 4, quant_max=qmax), x, logits, 4, qmax)
+
+
+def test_nan_values_and_logits(w8a8, gpu):
+    # a NaN value is the quantizer's -quant_max, in its own token only; a NaN logit makes a
+    # token's weights 0, in topk_softmax and here
+    import torch
+    layer = Layer(8, 256, 352, 31, gpu)
+    x, logits = layer.x(5), layer.logits(5)
+    want = layer.run(w8a8, x, logits, 2)
+    x[1, 9] = x[1, 200] = float("nan")
+    _check_steps(layer, layer.run(w8a8, x, logits, 2), x, logits, 2)
+    logits[3, 5] = float("nan")
+    got = layer.run(w8a8, x, logits, 2)
+    assert (got[3] == 0).all()
+    assert torch.equal(got[[0, 2, 4]], want[[0, 2, 4]])
+    w, ids = w8a8.topk_softmax(logits, 2)
+    assert (w[3] == 0).all() and (ids[3] != 5).all() and (ids[3] >= 0).all()
+    chain, _ = w8a8.moe_ffn(x, logits, layer.s, layer.wgu, layer.sgu, layer.wd, layer.sd, 2,
+                            layer.s2)
+    assert torch.isfinite(chain).all() and (chain[3] == 0).all()
+    # the one expert that is left of two has no weight either
+    logits = layer.logits(5)
+    logits[4, 1:] = float("nan")
+    assert (layer.run(w8a8, x, logits, 2)[4] == 0).all()

@@ -638,7 +638,8 @@ int w8a8_moe_ffn_decode(const void* x, const void* logits, int logits_f16,
  *       [seq_starts[i], seq_starts[i + 1]), any length including 0.  Rows
  *       before the first and behind the last sequence are left as they were;
  *       values outside [0, tokens] count as the nearer end.
- * What a token may not see does not reach it, infinities and NaN included.
+ * What a token may not see does not reach it, infinities and NaN included.  A mean
+ * of finite values is finite: results past the range of fp16 are its ends.
  * kv_heads divides heads; head_dim 64 or 128; scale > 0; pointers 16-byte
  * aligned, row strides multiples of 8 (W8A8_ERROR_NOT_SUPPORTED otherwise).
  * tokens = 0 or seqs = 0 does nothing.

@@ -191,6 +191,19 @@ __device__ __forceinline__ v8h finite_only(v8h v)
     return __builtin_bit_cast(v8h, u);
 }
 
+// From here on the wave's conversions to fp16 give +-65504 where a finite value passes the
+// range (the mode register's FP16_OVFL; infinities and NaN stay what they are).  Matrix
+// instructions lose NaN operands in this mode, so it begins behind those whose results `o`
+// are; the converted values have to depend on the returned v.
+template <int N>
+__device__ __forceinline__ float finite_halves_from_here(float v, v16f (&o)[N])
+{
+#pragma unroll
+    for(int i = 0; i < N; ++i) asm volatile("" : "+v"(o[i]));
+    asm volatile("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 23, 1), 1" : "+v"(v));
+    return v;
+}
+
 // Twice 16 bytes a lane from a buffer into LDS, lane i to bytes `to` + 16 i and, from its
 // second offset, 1024 further, with the caller's own waits: a load through the builtin makes
 // the compiler wait for all of them ahead of every transposed read, whichever stage that
@@ -418,7 +431,9 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
     }
 
     const v2f   ls  = both_halves(l);
-    const float inv = 1.f / (ls[0] + ls[1]);
+    // The rounded probabilities may add up to a little more than l (2^-11 of it at the most),
+    // which must not carry a mean of values of 65504 past fp16.
+    const float inv = finite_halves_from_here(1.f / (ls[0] + ls[1]), o);
     if(qi >= span.len) return;
     uint16_t* out = a.out + (size_t)(span.begin + qi) * a.ldo + head * D;
 #pragma unroll

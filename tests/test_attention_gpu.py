@@ -176,3 +176,27 @@ def test_graph_replays_and_other_streams(w8a8, gpu):
         q.copy_(_inputs(333, 8, 2, 128, 50 + i, gpu)[0])
         starts[1] = 100 + i
         want = w8a8.attention(q, k, v, starts)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,lens", [(2, [700, 33]), (64, [1100])])
+def test_values_at_the_ends_of_fp16(w8a8, gpu, dim, heads, lens):
+    # a result is a mean of the values: those of 65504 cannot make an infinity, whatever the
+    # rounded probabilities add up to
+    import torch
+    R = _ref()
+    n = sum(lens)
+    q, k, v = _inputs(n, heads, 1, dim, 41, gpu)
+    v[..., 0::4], v[..., 1::4] = 65504.0, -65504.0
+    starts, spans = _starts(lens, gpu)
+    got = w8a8.attention(q, k, v, starts)
+    out, bound, _ = R.attention(q, k, v, spans, dim ** -0.5)
+    assert float(out.max()) > 65503.9 and float(out.min()) < -65503.9
+    R.assert_within(got, out, bound)
+    # an infinite value is seen as one
+    v[20, 0, 2] = math.inf
+    got = w8a8.attention(q, k, v, starts)
+    assert (got[20:lens[0], :, 2] == math.inf).all()
+    v[20, 0, 6] = math.nan
+    got = w8a8.attention(q, k, v, starts)
+    assert torch.isnan(got[20:lens[0], :, 6]).all() and torch.isfinite(got[..., 0]).all()

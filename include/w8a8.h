@@ -713,7 +713,9 @@ int w8a8_kv4_load(void* k, void* v, const int32_t* slots, uint32_t tokens, uint3
  *   zeros.
  * Codes enter the matrix products as they are, exactly; scores, softmax
  * statistics and sums are fp32, and p * scale of a value is rounded to fp16 as
- * the second product's operand.  Results past the range of fp16 are its ends.
+ * the second product's operand, in units of the largest scale of the 64 tokens and
+ * the key head it is taken with: the codes of groups whose scale is below about
+ * 2^-10 of that lose bits.  Results past the range of fp16 are its ends.
  * workspace: 16-byte aligned, w8a8_attention_kv4_workspace_size(seqs, heads,
  * kv_heads, head_dim, table_cols * page_size) bytes, needs no clearing: the
  * work of all sequences is cut into equal runs, one a wave, and a second launch

@@ -20,12 +20,15 @@
 //     (chosen by the global address each lane fetches), so that both kinds of
 //     reads spread over all banks.  Rows past the sequence's end read as zeros.
 //   * The tile on the diagonal comes first and is the only one that masks.
-// Bound by the matrix and the vector unit together: a tile of 32 keys of 128 channels is 512
-// cycles of products a wave and about as many of exponentials (a quarter of the rate),
-// sums, maxima and roundings, which 3 waves a SIMD overlap in part.  8192 tokens, 32
-// query and 8 key heads of 128: 565 to 650 us by the card's clock, 975 to 850
-// TFLOP/s; 16 heads of 64: 172 us, 800.  A block alone on its CU takes 1.2 us for 64 keys,
-// which is what a prompt of 1024 tokens waits for (26 us).
+// A tile of 32 keys of 128 channels is 512 cycles of products a wave and about as many of
+// exponentials (a quarter of the rate), sums, maxima and roundings, which 3 waves a SIMD
+// overlap in part.  8192 tokens, 32 query and 8 key heads of 128: 545 to 590 us by the
+// card's clock, 1010 to 930 TFLOP/s, the matrix unit busy in 54 % of the cycles, vector
+// instructions in 52 %, waves waiting for 31 % of their time; 16 heads of 64: 161 to 172 us.
+// Bound, where blocks are few, by the chain of a block's own steps: the score product's key
+// fragments come from LDS into one register quad (two for two chains), so that each product
+// waits for its own read.  A block alone on its CU takes 1.2 us for 64 keys, whose products
+// are half of that, which is what a prompt of 1024 tokens waits for (26 us).
 #include "w8a8_device.hpp"
 #include "w8a8_internal.hpp"
 
@@ -114,7 +117,8 @@ __device__ __forceinline__ Span find_tile_of_few(const AttentionArgs& a, uint32_
 
 // Any number of sequences: the tile-th tile of kRows query rows, 64 sequences a step,
 // their tile counts summed along the lanes.  Inside a sequence the tiles with the most
-// keys come first.
+// keys come first; the sequences keep their order, so a long one at the end starts last
+// (64 tokens and a prompt of 4096, 16 heads of 64: 63 us, 60 with the prompt first).
 __device__ __forceinline__ Span find_tile(const AttentionArgs& a, uint32_t tile, int lane)
 {
     if(a.seqs <= kWave) return find_tile_of_few(a, tile, lane);
@@ -247,9 +251,10 @@ __device__ __forceinline__ void attention_rows(const AttentionArgs& a, uint8_t* 
 
     // Blocks go round the 8 XCDs: where the heads divide evenly, an XCD gets
     // neighbouring heads, whose keys and values then stay in its L2.
-    // Heads of 64, 4 blocks a CU: every other full round of one block a CU is turned around
-    // (inside each XCD), so that tiles of many and of few keys share a CU and not like
-    // with like (8 x 512 tokens, 16 heads, 17.2 -> 15.4 us, 8192 tokens 181 -> 170).
+    // Heads of 64: every other full round of one block a CU is turned around (inside each
+    // XCD), so that tiles of many and of few keys share a CU and not like with like (key
+    // tiles of 128, 2 blocks a CU: 8 x 512 tokens, 16 heads, 13.8 -> 13.0 us, 4096 tokens
+    // 57 -> 55.5; key tiles of 64, 4 blocks: 8192 tokens 181 -> 170).
     // With heads of 128, 3 blocks a CU, it takes 2 % more.
     uint32_t block = blockIdx.x;
     if(D == 64 && block / kCus % 2 == 1 && (block / kCus + 1) * kCus <= gridDim.x)
@@ -469,6 +474,8 @@ hipError_t launch_attention(const AttentionArgs& a, hipStream_t stream)
     //   68.7; 8 x 512 (1280) 39.6, 39.7; 4 x 2048 (2176) 163, 168
     //   heads of 64: 4096 tokens, 16 heads (528) 59.9, 55.2; 8 x 512 (640) 13.2, 12.8; 4 x
     //   2048 (1088) 49.8, 55.3; 61 tokens, whose keys are one smaller tile, 4.7, 5.5
+    // (The sequences' lengths are on the device: the mean stands for them, and a long
+    // prompt beside many of a token takes the smaller tiles; 4096 and 63 of one: 61.)
     const uint32_t most = a.dim == 128 && a.seqs > 1 ? 5 * kCus : 3 * kCus;
     const bool     few  = blocks <= most && (a.dim == 128 || a.tokens / a.seqs > 128);
     const auto     kernel

@@ -271,11 +271,13 @@ RowPlan row_plan(const w8a8_kv4_cache& c, const Kv4Rows& r)
 // itself, its next chunk on the way while it computes.  A unit inside one run is
 // written out; of one cut by runs each wave leaves a partial (its sum of p v, maximum
 // and sum of p), and a second launch joins them in order.  So any mix of lengths
-// keeps the chip evenly busy.  Bound by the stream of codes: about 6 TB/s once it runs, less
-// 5.5 us of start (lengths, page numbers, then codes) and the join's 5 (131072 tokens,
-// 32 / 8 heads of 128, 168 MB, 41 us; 48 sequences of 249 MB in all 64).  (Blocks that
-// owned a piece of one sequence spent 10 of their 18 us on starting, the first load and
-// merging: 16 x 8192 tokens 42 us.)
+// keeps the chip evenly busy.  131072 tokens, 32 / 8 heads of 128, 168 MB: 39 us and 5 of
+// the join, 4.3 TB/s, 5.0 behind the 5.5 us of start (lengths, page numbers, then codes);
+// 48 sequences of 249 MB in all 62 and 5, 4.0 TB/s.  Bound by a wave's chain from chunk to
+// chunk and its 690 vector instructions: the page number of the chunk after next is waited
+// for where it is loaded, ahead of the next chunk's loads, and the queue is empty again at
+// the loop's end.  (Blocks that owned a piece of one sequence spent 10 of their 18 us on
+// starting, the first load and merging: 16 x 8192 tokens 42 us.)
 // Both products run on v_mfma_f32_16x16x32_f16 with the query heads as columns:
 //   S^T = K q^T    srcA rows = tokens.  A lane takes 16 (8) bytes of one token's
 //                  codes; dword j is its operand of step j, channels 32 j + 8 kg +
@@ -293,7 +295,12 @@ RowPlan row_plan(const w8a8_kv4_cache& c, const Kv4Rows& r)
 // (the -1.5 makes x the centred code; in O^T with
 // the sum over the tokens of the rounded p s, from a matrix product with ones, so
 // that rounding p s to fp16, the only rounding below fp32, acts on the centred
-// code).  p s is brought to fp16's range by a power of two that follows the scales.
+// code).  p s is brought to fp16's range by a power of two that follows the scales: one a
+// chunk and key head, taken from its largest scale s, which then lies between 1 and 64.  A
+// p s below 2^-14 has fewer than fp16's 11 bits and one below 2^-25 none, so the centred
+// codes of a group whose scales are a small part of the largest lose precision (their
+// offsets, in fp32, do not).  A power for each group would take its own maximum, rescaling
+// and product a group in a loop that is bound by such instructions.
 //
 // With few query heads per key head most of the 16 columns would hold nothing, and
 // the work on scores, which is per column, would be done for nothing.  So C = 4 or 2

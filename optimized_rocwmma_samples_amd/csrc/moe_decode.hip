@@ -7,8 +7,10 @@
 // (8 experts of 4096 x 14336: one token 75 us, 4.7 TB/s; 16 tokens 256 us, 5.5 TB/s).
 // Routing and quantization, which the chain has launches for, every block of the first
 // does again for itself, on a few KB from L2.  What is left above the bytes is that
-// start, a chain of short dependent steps (about 11 us of the first kernel), and the
-// second launch (3 us).
+// start, a chain of short dependent steps, the second launch (4.7 us), and weight loads
+// that are not ahead: they are issued under conditions (the run's end), and where the
+// paths meet the compiler waits for all of them, so that every batch ends on an empty
+// queue and other waves alone fill the time.
 //   * v_mfma_i32_16x16x64_i8 with 16 weight rows as srcA (a lane loads 16
 //     contiguous bytes of one row, a wave-load 64 bytes of 16 rows) and up to 16
 //     quantized rows as srcB, read from LDS or L2.
@@ -146,7 +148,7 @@ Ws carve(const MoeDecodeArgs& a)
 // contiguous range per block of gate_up_kernel.
 __device__ __forceinline__ uint32_t first_unit(uint32_t block, uint32_t units, uint32_t blocks)
 {
-    return block * units / blocks; // units <= 1024 * 2048, blocks <= 512
+    return block * units / blocks; // units <= 512 * 2048, blocks <= 512
 }
 
 // Hardware gives blocks to the 8 XCDs in turn; an index such that each XCD has a
@@ -216,7 +218,7 @@ static_assert(W8A8_MOE_DECODE_MAX_VALUES + kRows * 80 + Lists::bytes(kRows * kMa
                   <= kLdsBytes,
               "a block of gate_up_kernel holds every token's row");
 
-// RING: batches in registers, all but one of them in flight.
+// RING: batches in registers, loaded up to RING - 1 ahead (see above for the waits).
 template <bool F16, int RING>
 __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, uint32_t group,
                                         GateUpLds& lds, uint8_t* dyn)
@@ -426,9 +428,9 @@ __device__ __forceinline__ void gate_up(const MoeDecodeArgs& a, const Ws& ws, ui
         ws.top[(size_t)range * pairs + p] = __uint_as_float(top[p]);
 }
 
-// BLOCKS a CU.  Batches in flight: 3 where a block is alone on its CU, 2 where there are
-// two; more made it slower (7 and 3 of them: 8 experts of 4096 x 14336, one token, 85
-// us against 80).
+// BLOCKS a CU.  Batches ahead: 3 where a block is alone on its CU, 2 where there are
+// two; 7 and 3 of them made it slower (8 experts of 4096 x 14336, one token, 85 us against
+// 80), as they have to where each batch waits for all of them.
 template <bool F16, int BLOCKS>
 __global__ void __launch_bounds__(kThreads, 2 * BLOCKS)
     gate_up_kernel(MoeDecodeArgs a, Ws ws, uint32_t group)

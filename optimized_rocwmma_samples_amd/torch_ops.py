@@ -235,7 +235,7 @@ def _(slots, k_codes, v_codes, k_scales, v_scales):
 def attention_kv4(q: Tensor, k_codes: Tensor, v_codes: Tensor, k_scales: Tensor, v_scales: Tensor,
                   block_table: Tensor, seq_lens: Tensor, scale: Optional[float] = None) -> Tensor:
     """Attention of one token per sequence, q [seqs, heads, head_dim], over a KV4Cache's
-    tensors; workspace allocated as the lengths need."""
+    tensors; workspace allocated for the table's columns."""
     return _attention_kv4(q, KV4Cache(k_codes, v_codes, k_scales, v_scales), block_table, seq_lens,
                           scale)
 

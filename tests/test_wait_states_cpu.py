@@ -105,6 +105,6 @@ def test_loads_in_asm_keep_it_themselves(kernels):
                 continue
             found += 1
             for o, a, at in before(code[max(0, i - 5):i], 5):
-                own = o == "s_nop" or a[0] == "m0" or (o.startswith("buffer_load") and a[-1] == "lds")
+                own = o == "s_nop" or a[0] == "m0" or a[-1] == "lds"
                 assert own, (name, o, a, at)
     assert found >= 16

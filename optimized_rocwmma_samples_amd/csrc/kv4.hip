@@ -299,7 +299,8 @@ RowPlan row_plan(const w8a8_kv4_cache& c, const Kv4Rows& r)
 // chunk and key head, taken from its largest scale s, which then lies between 1 and 64.  A
 // p s below 2^-14 has fewer than fp16's 11 bits and one below 2^-25 none, so the centred
 // codes of a group whose scales are a small part of the largest lose precision (their
-// offsets, in fp32, do not).  A power for each group would take its own maximum, rescaling
+// offsets, in fp32, do not).  The two held sums cancel 1.5 of each code in fp32: some 2^-20
+// of the largest scale is left where a result is far smaller than that.  A power for each group would take its own maximum, rescaling
 // and product a group in a loop that is bound by such instructions.
 //
 // With few query heads per key head most of the 16 columns would hold nothing, and

@@ -1002,7 +1002,8 @@ def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None
     ws, ws_bytes = _workspace(
         workspace, lambda: _kv4_workspace_size(seqs, heads, cache.kv_heads, dim,
                                                cols * cache.page_size), dev)
-    _call_on(dev, "w8a8_attention_kv4", q.data_ptr(), cache._descriptor(), block_table.data_ptr(), cols,
-             table_ld, seq_lens.data_ptr(), out.data_ptr(), seqs, heads, ldq, ldo,
+    _call_on(dev, "w8a8_attention_kv4", q.data_ptr(), cache._descriptor(),
+             block_table.data_ptr(), cols, table_ld, seq_lens.data_ptr(), out.data_ptr(), seqs,
+             heads, ldq, ldo,
              dim ** -0.5 if scale is None else float(scale), _ptr(ws), ws_bytes, _stream(dev))
     return out

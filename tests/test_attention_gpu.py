@@ -200,3 +200,23 @@ def test_values_at_the_ends_of_fp16(w8a8, gpu, dim, heads, lens):
     v[20, 0, 6] = math.nan
     got = w8a8.attention(q, k, v, starts)
     assert torch.isnan(got[20:lens[0], :, 6]).all() and torch.isfinite(got[..., 0]).all()
+
+
+def test_long_offsets(w8a8, gpu):
+    # rows that lie past 2^31 values and 2^32 bytes from the tensors' starts
+    import torch
+    R = _ref()
+    tokens, width, n = 40000, 65536, 300
+    qkv = torch.empty((tokens, width), dtype=torch.float16, device=gpu)
+    assert (tokens - n) * width > 2 ** 31
+    q, k, v, out = (qkv[:, at:at + h * 64].unflatten(1, (h, 64))
+                    for at, h in ((0, 4), (1024, 2), (2048, 2), (3200, 4)))
+    small = [R.randn((n, t.shape[1], 64), s, gpu) for s, t in ((1, q), (2, k), (3, v))]
+    for t, x in zip((q, k, v), small):
+        t[-n:] = x
+    out[-n - 1] = 7.0
+    starts = torch.tensor([tokens - n, tokens - 77, tokens], dtype=torch.int32, device=gpu)
+    w8a8.attention(q, k, v, starts, out=out)
+    ref, bound, _ = R.attention(*small, [(0, n - 77), (n - 77, n)], 0.125)
+    R.assert_within(out[-n:], ref, bound)
+    assert (out[-n - 1] == 7).all()

@@ -732,6 +732,152 @@ int w8a8_attention_kv4(const void* q, const w8a8_kv4_cache* cache, const int32_t
                        uint32_t seqs, uint32_t heads, uint32_t ldq, uint32_t ldo, float scale,
                        void* workspace, size_t ws_bytes, hipStream_t stream);
 
+/*
+ * The paged cache in service.  A server keeps, on the device, each sequence's
+ * length and row of the block table, and a stack of free pages: free_pages
+ * int32 [free_capacity], of which the first free_count[0] are free, the next
+ * one to be used last.  page_size is a power of two in 16..1024; lengths count
+ * as the nearer end of [0, table_cols * page_size].
+ *
+ * w8a8_kv4_extend finds places for new_tokens[i] tokens (negative: 0) behind the
+ * seq_lens[i] tokens that sequence i has:
+ *   seq_starts int32 [seqs + 1]: the sequences' new tokens one after the other,
+ *              at most `tokens`; the rows of q, k and v of the step
+ *   slots      int32 [tokens]: of each new token, for w8a8_kv4_store; -1 in rows
+ *              behind the last sequence
+ *   block_table: the columns of the pages that a sequence needs in addition are
+ *              written, all others left as they were
+ *   lens_out int32 [seqs]: seq_lens + new_tokens; count_out int32 [1]: the free
+ *              pages that are left
+ * Pages are taken from the stack's top, by sequence, then by column.  A sequence
+ * gets all of its places or none: none where its rows would pass `tokens`, its
+ * tokens the table's columns, or where the pages that are left behind the
+ * sequences before it do not suffice (one that finds too few leaves none to those
+ * behind it that need any).  Then its slots are -1 and its length stays.
+ * lens_out may be seq_lens and count_out free_count; other arguments may not
+ * overlap.
+ */
+int w8a8_kv4_extend(const int32_t* new_tokens, const int32_t* seq_lens, uint32_t seqs,
+                    int32_t* block_table, uint32_t table_cols, uint32_t table_ld,
+                    const int32_t* free_pages, uint32_t free_capacity, const int32_t* free_count,
+                    uint32_t page_size, int32_t* slots, uint32_t tokens, int32_t* seq_starts,
+                    int32_t* lens_out, int32_t* count_out, hipStream_t stream);
+
+/*
+ * Takes tokens back: sequence i is left with lens_out[i] = the smaller of keep[i]
+ * (negative: 0) and seq_lens[i] tokens, and the pages that it no longer needs go
+ * back on the stack, in the reverse of the order in which w8a8_kv4_extend takes
+ * them (so that trimming what was just handed out restores the stack); pages past
+ * free_capacity are dropped.  The block table is left as it was.  lens_out may be
+ * seq_lens and count_out free_count; other arguments may not overlap.
+ */
+int w8a8_kv4_trim(const int32_t* keep, const int32_t* seq_lens, uint32_t seqs,
+                  const int32_t* block_table, uint32_t table_cols, uint32_t table_ld,
+                  int32_t* free_pages, uint32_t free_capacity, const int32_t* free_count,
+                  uint32_t page_size, int32_t* lens_out, int32_t* count_out, hipStream_t stream);
+
+/*
+ * Attention of the last tokens of each sequence over the cache, in which their
+ * keys and values are already stored: a prompt in chunks, tokens behind a cached
+ * prefix, speculated tokens to be verified, or a mixed batch of them.
+ *   q   fp16 [tokens, ldq], out fp16 [tokens, ldo], heads as in w8a8_attention;
+ *       seq_starts int32 [seqs + 1], ascending: sequence i's new tokens are rows
+ *       [seq_starts[i], seq_starts[i + 1]), and its last of seq_lens[i] in all
+ *   block_table, seq_lens as in w8a8_attention_kv4
+ * Row j of a sequence's n rows sees its tokens up to position seq_lens[i] - n + j,
+ * its own; a row that sees none gives zeros.  Tokens of a page number outside
+ * [0, pages) are left out, rows of no sequence left as they were.  What a row may
+ * not see does not reach it, NaN included; a group whose scale or offset is an
+ * infinity counts as NaN.
+ * Keys and values enter the matrix products as fp16 (half of what w8a8_kv4_load
+ * gives, rounded once), probabilities as well; scores, softmax statistics and sums
+ * are fp32.  Results past the range of fp16 are its ends.
+ * max_new: no sequence has more new tokens than this (0: not known); more of them are
+ * computed all the same, more slowly.
+ * workspace: 256-byte aligned, w8a8_attention_kv4_chunks_workspace_size bytes (for
+ * the same cache, seqs, tokens, heads, table_cols and max_new), needs no clearing;
+ * calls that share one must be ordered on one stream.
+ * 16-byte aligned q, out, ldq and ldo multiples of 8.
+ */
+size_t w8a8_attention_kv4_chunks_workspace_size(const w8a8_kv4_cache* cache, uint32_t seqs,
+                                                uint32_t tokens, uint32_t heads,
+                                                uint32_t table_cols, uint32_t max_new);
+
+int w8a8_attention_kv4_chunks(const void* q, const w8a8_kv4_cache* cache,
+                              const int32_t* block_table, uint32_t table_cols, uint32_t table_ld,
+                              const int32_t* seq_lens, const int32_t* seq_starts, void* out,
+                              uint32_t seqs, uint32_t tokens, uint32_t heads, uint32_t max_new,
+                              uint32_t ldq, uint32_t ldo, float scale, void* workspace,
+                              size_t ws_bytes, hipStream_t stream);
+
+/*
+ * Page keys: for each page and key head the mean of its tokens' keys in 8 bits,
+ *   codes int8 [pages, kv_heads, head_dim], scales fp32 [pages, kv_heads]
+ * where a code n stands for n * scale and the scale is the least power of two with
+ * which all codes lie in -127..127 (0 where all means are 0, NaN where one is not
+ * finite).  Both 16-byte aligned.
+ */
+typedef struct w8a8_kv4_page_keys {
+    int8_t*  codes;
+    float*   scales;
+    uint32_t pages, kv_heads, head_dim;
+} w8a8_kv4_page_keys;
+
+/*
+ * Computes the page keys of the pages in which the last seq_starts[i + 1] -
+ * seq_starts[i] of the seq_lens[i] tokens of each sequence lie, from the cache:
+ * of a page the mean of all its tokens, those before them included.  Sums and
+ * quotients are in 64 bits and exact but for the quotient's rounding.  `tokens` is
+ * the rows of the step, as in w8a8_attention_kv4_chunks; seq_starts ascends.
+ */
+int w8a8_kv4_summarize(const w8a8_kv4_cache* cache, const w8a8_kv4_page_keys* keys,
+                       const int32_t* block_table, uint32_t table_cols, uint32_t table_ld,
+                       const int32_t* seq_lens, const int32_t* seq_starts, uint32_t seqs,
+                       uint32_t tokens, hipStream_t stream);
+
+/*
+ * Values of page keys: out fp32 [count, kv_heads, head_dim] of the pages given
+ * (rows of pages outside [0, keys->pages) are left as they were); 16-byte aligned.
+ */
+int w8a8_kv4_page_keys_load(const w8a8_kv4_page_keys* keys, const int32_t* pages, uint32_t count,
+                            float* out, hipStream_t stream);
+
+/*
+ * Chooses the pages that one new token per sequence attends to, for each key head:
+ * its last page and the keep - 1 others of the largest score, the lower column first
+ * among equals; all of them where there are no more than `keep`.  The score of a page
+ * is its scale times the whole-number product of its codes with those of the query:
+ * the sum of q over the key head's query heads (64 bits) in 8 bits with a power of two,
+ * as in page keys.  Page keys of NaN and pages outside [0, keys->pages) come last; the
+ * codes of a query that is not finite are zeros.
+ *   q fp16 [seqs, ldq], heads as in w8a8_attention; block_table, seq_lens as in
+ *     w8a8_attention_kv4
+ *   chosen int32 [seqs, kv_heads, keep]: pages in the order of their columns, -1
+ *     behind the last; lens_out int32 [seqs]: the tokens in them, the same for all
+ *     key heads.  Both for w8a8_attention_kv4_selected; neither may overlap an input.
+ * workspace: w8a8_kv4_select_workspace_size bytes (0 where table_cols <= keep), 16-byte
+ * aligned, needs no clearing; calls that share one must be ordered on one stream.
+ */
+size_t w8a8_kv4_select_workspace_size(uint32_t seqs, uint32_t kv_heads, uint32_t table_cols,
+                                      uint32_t keep);
+
+int w8a8_kv4_select(const void* q, const w8a8_kv4_page_keys* keys, const int32_t* block_table,
+                    uint32_t table_cols, uint32_t table_ld, const int32_t* seq_lens,
+                    uint32_t page_size, int32_t* chosen, uint32_t keep, int32_t* lens_out,
+                    uint32_t seqs, uint32_t heads, uint32_t ldq, void* workspace, size_t ws_bytes,
+                    hipStream_t stream);
+
+/*
+ * w8a8_attention_kv4 with a block table for each key head: block_tables int32 [seqs,
+ * kv_heads, table_cols].  The length of a sequence counts the tokens of the pages in its
+ * tables.  Workspace as for w8a8_attention_kv4.
+ */
+int w8a8_attention_kv4_selected(const void* q, const w8a8_kv4_cache* cache,
+                                const int32_t* block_tables, uint32_t table_cols,
+                                const int32_t* seq_lens, void* out, uint32_t seqs, uint32_t heads,
+                                uint32_t ldq, uint32_t ldo, float scale, void* workspace,
+                                size_t ws_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,6 +24,12 @@ its linear layers:
   KV4Cache, kv4_store, kv4_load, attention_kv4
                    a paged 4-bit cache of keys and values, and the attention of
                    single tokens over it
+  kv4_extend, kv4_trim
+                   that cache's pages handed out and taken back on the device
+  attention_kv4_chunks
+                   attention of several new tokens per sequence over the cache
+  KV4PageKeys, kv4_summarize, kv4_page_keys, kv4_select
+                   a key for each page, and the pages that suit a query
 """
 from __future__ import annotations
 
@@ -55,7 +61,9 @@ __all__ = [
     "moe_combine", "moe_ffn", "add_rmsnorm_smoothquant", "rmsnorm", "add_rmsnorm",
     "quantize_weights", "moe_ffn_decode", "moe_ffn_decode_workspace_size",
     "attention", "KV4Cache", "kv4_store", "kv4_load", "attention_kv4",
-    "attention_kv4_workspace_size",
+    "attention_kv4_workspace_size", "kv4_extend", "kv4_trim", "attention_kv4_chunks",
+    "attention_kv4_chunks_workspace_size", "KV4PageKeys", "kv4_summarize", "kv4_page_keys",
+    "kv4_select", "kv4_select_workspace_size",
 ]
 
 
@@ -962,6 +970,21 @@ def kv4_load(cache: KV4Cache, slots, out=None):
     return k, v
 
 
+def _kv4_ints(name, t, count: int) -> None:
+    if t.dtype != _torch_module.int32 or t.shape != (count,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor [{count}]")
+
+
+def _kv4_table(block_table, seqs: int):
+    # columns and row stride of a block table
+    table = block_table.shape
+    cols = table[1] if len(table) == 2 else 0
+    if block_table.dtype != _torch_module.int32 or table != (seqs, cols) \
+            or (cols > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be int32 [seqs, columns] with unit column stride")
+    return cols, _row_stride("block_table", seqs, block_table.stride(0), cols)
+
+
 def attention_kv4_workspace_size(seqs: int, heads: int, kv_heads: int, head_dim: int,
                                  max_len: int) -> int:
     """Bytes of workspace attention_kv4 can use (0: none); max_len is the block
@@ -979,7 +1002,8 @@ def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None
     """Attention of one new token per sequence over the cache.
 
     q fp16 [seqs, heads, head_dim]; block_table int32 [seqs, columns] (unit
-    column stride): the page of each page_size tokens of a sequence; seq_lens
+    column stride): the page of each page_size tokens of a sequence, or contiguous
+    [seqs, kv_heads, columns], a table for each key head (kv4_select); seq_lens
     int32 [seqs]: the tokens to attend to, the new one (stored before) among
     them.  Returns fp16 [seqs, heads, head_dim]; a sequence of no tokens gives
     zeros.  workspace: 'auto' (allocated here), None (all of a key head's
@@ -989,21 +1013,266 @@ def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None
     _require_on(dev, q=q, block_table=block_table, seq_lens=seq_lens, out=out)
     ldq = _heads3d("q", q, None, cache.head_dim)
     seqs, heads, dim = q.shape
-    table = block_table.shape
-    cols = table[1] if len(table) == 2 else 0
-    if block_table.dtype != torch.int32 or table != (seqs, cols) \
-            or (cols > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be int32 [seqs, columns] with unit column stride")
-    if seq_lens.dtype != torch.int32 or seq_lens.shape != (seqs,) or not seq_lens.is_contiguous():
-        raise ValueError("seq_lens must be a contiguous int32 tensor [seqs]")
-    table_ld = _row_stride("block_table", seqs, block_table.stride(0), cols)
+    by_head = block_table.dim() == 3
+    if by_head:
+        cols = block_table.shape[2]
+        _require("block_table", block_table, torch.int32, (seqs, cache.kv_heads, cols))
+        tables = (cols,)
+    else:
+        cols, table_ld = _kv4_table(block_table, seqs)
+        tables = (cols, table_ld)
+    _kv4_ints("seq_lens", seq_lens, seqs)
     out, ldo = _heads_out(out, q, seqs, heads, dim)
     _workspace_on(workspace, dev)
     ws, ws_bytes = _workspace(
         workspace, lambda: _kv4_workspace_size(seqs, heads, cache.kv_heads, dim,
                                                cols * cache.page_size), dev)
-    _call_on(dev, "w8a8_attention_kv4", q.data_ptr(), cache._descriptor(),
-             block_table.data_ptr(), cols, table_ld, seq_lens.data_ptr(), out.data_ptr(), seqs,
-             heads, ldq, ldo,
+    _call_on(dev, "w8a8_attention_kv4_selected" if by_head else "w8a8_attention_kv4",
+             q.data_ptr(), cache._descriptor(), block_table.data_ptr(), *tables,
+             seq_lens.data_ptr(), out.data_ptr(), seqs, heads, ldq, ldo,
              dim ** -0.5 if scale is None else float(scale), _ptr(ws), ws_bytes, _stream(dev))
     return out
+
+
+def kv4_extend(new_tokens, seq_lens, block_table, free_pages, free_count, page_size: int,
+               tokens: int, out=None):
+    """Places in the cache for the tokens to come: new_tokens int32 [seqs] behind the
+    seq_lens int32 [seqs] tokens that each sequence has.
+
+    block_table int32 [seqs, columns]: the columns of the pages that a sequence needs in
+    addition are written.  free_pages int32 [n] is a stack of which the first free_count
+    (int32 [1], on the device) are free; pages are taken from its top, by sequence and
+    column.  tokens: the rows of the step.  Returns (slots [tokens] for kv4_store, starts
+    [seqs + 1] of the sequences' rows, lengths [seqs], free pages left [1]), all int32.
+    A sequence gets all of its places or none (slots of -1, its length stays): none where
+    its rows would pass `tokens`, its tokens the table's columns, or where the pages that
+    the sequences before it leave are too few.  out: these four; the lengths and the
+    count may be seq_lens and free_count themselves."""
+    torch = _torch()
+    _require_cuda(block_table)
+    dev = block_table.device
+    _require_on(dev, new_tokens=new_tokens, seq_lens=seq_lens, free_pages=free_pages,
+                free_count=free_count)
+    seqs = block_table.shape[0]
+    cols, table_ld = _kv4_table(block_table, seqs)
+    _kv4_ints("new_tokens", new_tokens, seqs)
+    _kv4_ints("seq_lens", seq_lens, seqs)
+    _kv4_ints("free_pages", free_pages, free_pages.numel())
+    _kv4_ints("free_count", free_count, 1)
+    if tokens < 0:
+        raise ValueError("tokens must not be negative")
+    if out is None:
+        new = seq_lens.new_empty
+        slots, starts, lens, count = new(tokens), new(seqs + 1), new(seqs), new(1)
+    else:
+        slots, starts, lens, count = out
+        _require_on(dev, slots=slots, starts=starts, lens=lens, count=count)
+        _kv4_ints("slots", slots, tokens)
+        _kv4_ints("starts", starts, seqs + 1)
+        _kv4_ints("lens", lens, seqs)
+        _kv4_ints("count", count, 1)
+    _call_on(dev, "w8a8_kv4_extend", new_tokens.data_ptr(), seq_lens.data_ptr(), seqs,
+             block_table.data_ptr(), cols, table_ld, free_pages.data_ptr(), free_pages.numel(),
+             free_count.data_ptr(), page_size, slots.data_ptr(), tokens, starts.data_ptr(),
+             lens.data_ptr(), count.data_ptr(), _stream(dev))
+    return slots, starts, lens, count
+
+
+def kv4_trim(keep, seq_lens, block_table, free_pages, free_count, page_size: int, out=None):
+    """Takes tokens back: sequence i is left with min(keep[i], seq_lens[i]) tokens (0: it is
+    done), and the pages that it no longer needs go back on the stack of kv4_extend, in the
+    reverse of the order in which that takes them.  Returns (lengths [seqs], free pages
+    [1]), int32; out: these two, which may be seq_lens and free_count themselves."""
+    torch = _torch()
+    _require_cuda(block_table)
+    dev = block_table.device
+    _require_on(dev, keep=keep, seq_lens=seq_lens, free_pages=free_pages, free_count=free_count)
+    seqs = block_table.shape[0]
+    cols, table_ld = _kv4_table(block_table, seqs)
+    _kv4_ints("keep", keep, seqs)
+    _kv4_ints("seq_lens", seq_lens, seqs)
+    _kv4_ints("free_pages", free_pages, free_pages.numel())
+    _kv4_ints("free_count", free_count, 1)
+    if out is None:
+        lens, count = torch.empty_like(seq_lens), torch.empty_like(free_count)
+    else:
+        lens, count = out
+        _require_on(dev, lens=lens, count=count)
+        _kv4_ints("lens", lens, seqs)
+        _kv4_ints("count", count, 1)
+    _call_on(dev, "w8a8_kv4_trim", keep.data_ptr(), seq_lens.data_ptr(), seqs,
+             block_table.data_ptr(), cols, table_ld, free_pages.data_ptr(), free_pages.numel(),
+             free_count.data_ptr(), page_size, lens.data_ptr(), count.data_ptr(), _stream(dev))
+    return lens, count
+
+
+@functools.lru_cache(maxsize=256)
+def _kv4_chunks_workspace_size(pages, page_size, kv_heads, head_dim, group, seqs, tokens, heads,
+                               columns, max_new) -> int:
+    # the descriptor's pointers are not followed
+    desc = _lib.Kv4Cache(16, 16, 16, 16, pages, page_size, kv_heads, head_dim, group)
+    return int(library().w8a8_attention_kv4_chunks_workspace_size(
+        ctypes.byref(desc), seqs, tokens, heads, columns, max_new))
+
+
+def attention_kv4_chunks_workspace_size(cache: KV4Cache, seqs: int, tokens: int, heads: int,
+                                        columns: int, max_new: int | None = None) -> int:
+    """Bytes of workspace attention_kv4_chunks needs (0: none); columns of the block table."""
+    return _kv4_chunks_workspace_size(cache.pages, cache.page_size, cache.kv_heads, cache.head_dim,
+                                      cache.group, seqs, tokens, heads, columns, max_new or 0)
+
+
+def attention_kv4_chunks(q, cache: KV4Cache, block_table, seq_lens, starts,
+                         scale: float | None = None, out=None, workspace="auto",
+                         max_new: int | None = None):
+    """Attention of each sequence's last tokens over the cache: prompts in chunks or behind a
+    cached prefix, speculated tokens, mixed batches.
+
+    q fp16 [tokens, heads, head_dim]: rows starts[i] .. starts[i + 1] (int32 [seqs + 1],
+    ascending) are the last tokens of sequence i, whose keys and values kv4_store has
+    already stored; seq_lens int32 [seqs] counts them.  Each row sees the tokens of its
+    sequence up to its own.  block_table as in attention_kv4.  Returns fp16 [tokens,
+    heads, head_dim]; rows of no sequence are left as they were in `out` (undefined in a
+    new tensor).  max_new: the most new tokens a sequence has, where it is known.
+    workspace: 'auto' (allocated here) or a device tensor of
+    attention_kv4_chunks_workspace_size bytes, for the same max_new."""
+    torch = _torch()
+    dev = cache.device
+    _require_on(dev, q=q, block_table=block_table, seq_lens=seq_lens, starts=starts, out=out)
+    ldq = _heads3d("q", q, None, cache.head_dim)
+    tokens, heads, dim = q.shape
+    seqs = seq_lens.numel()
+    cols, table_ld = _kv4_table(block_table, seqs)
+    _kv4_ints("seq_lens", seq_lens, seqs)
+    _kv4_ints("starts", starts, seqs + 1)
+    max_new = 0 if max_new is None else max_new
+    if max_new < 0:
+        raise ValueError("max_new must not be negative")
+    out, ldo = _heads_out(out, q, tokens, heads, dim)
+    _workspace_on(workspace, dev)
+    ws, ws_bytes = _workspace(
+        workspace, lambda: _kv4_chunks_workspace_size(
+            cache.pages, cache.page_size, cache.kv_heads, dim, cache.group, seqs, tokens, heads,
+            cols, max_new), dev)
+    _call_on(dev, "w8a8_attention_kv4_chunks", q.data_ptr(), cache._descriptor(),
+             block_table.data_ptr(), cols, table_ld, seq_lens.data_ptr(), starts.data_ptr(),
+             out.data_ptr(), seqs, tokens, heads, max_new, ldq, ldo,
+             dim ** -0.5 if scale is None else float(scale), _ptr(ws), ws_bytes, _stream(dev))
+    return out
+
+
+class KV4PageKeys:
+    """A key for each page of a KV4Cache (w8a8_kv4_page_keys): codes int8 [pages, kv_heads,
+    head_dim], the mean of the page's keys in units of scales fp32 [pages, kv_heads], powers
+    of two.  KV4PageKeys.empty allocates them for a cache.  They are not to be given other
+    memory, which the calls refuse."""
+
+    def __init__(self, codes, scales):
+        torch = _torch()
+        _require_cuda(codes)
+        _require_on(codes.device, scales=scales)
+        if codes.dim() != 3:
+            raise ValueError("codes must be [pages, kv_heads, head_dim]")
+        _require("codes", codes, torch.int8, codes.shape)
+        _require("scales", scales, torch.float32, codes.shape[:2])
+        self._codes, self._scales = codes, scales
+        self.pages, self.kv_heads, self.head_dim = codes.shape
+        self.device = codes.device
+        self._where = (codes.data_ptr, scales.data_ptr)
+        self._at = tuple(where() for where in self._where)
+        self._desc = _lib.Kv4PageKeys(*self._at, *codes.shape)
+        self._ref = ctypes.byref(self._desc)
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+
+    def _descriptor(self):
+        if tuple(where() for where in self._where) != self._at:
+            raise ValueError("a tensor of the page keys was given other memory: make new "
+                             "KV4PageKeys")
+        return self._ref
+
+    @classmethod
+    def empty(cls, cache: KV4Cache):
+        """Page keys of a cache's pages (contents undefined until kv4_summarize)."""
+        torch = _torch()
+        shape = (cache.pages, cache.kv_heads, cache.head_dim)
+        return cls(torch.empty(shape, dtype=torch.int8, device=cache.device),
+                   torch.empty(shape[:2], dtype=torch.float32, device=cache.device))
+
+
+def kv4_summarize(cache: KV4Cache, keys: KV4PageKeys, block_table, seq_lens, starts,
+                  tokens: int) -> None:
+    """Computes the page keys of the pages that the last tokens of each sequence lie in, after
+    kv4_store: seq_lens int32 [seqs], of which the last starts[i + 1] - starts[i] are new
+    (starts int32 [seqs + 1], ascending; `tokens` rows in all)."""
+    _torch()
+    dev = cache.device
+    _require_on(dev, block_table=block_table, seq_lens=seq_lens, starts=starts, codes=keys._codes)
+    seqs = seq_lens.numel()
+    cols, table_ld = _kv4_table(block_table, seqs)
+    _kv4_ints("seq_lens", seq_lens, seqs)
+    _kv4_ints("starts", starts, seqs + 1)
+    if tokens < 0:
+        raise ValueError("tokens must not be negative")
+    _call_on(dev, "w8a8_kv4_summarize", cache._descriptor(), keys._descriptor(),
+             block_table.data_ptr(), cols, table_ld, seq_lens.data_ptr(), starts.data_ptr(), seqs,
+             tokens, _stream(dev))
+
+
+def kv4_page_keys(keys: KV4PageKeys, pages, out=None):
+    """Values of page keys: fp32 [n, kv_heads, head_dim] of pages int32 [n].  Rows of pages
+    outside are left as they were in `out` (undefined in a new tensor)."""
+    torch = _torch()
+    _require_on(keys.device, pages=pages, out=out)
+    n = pages.numel()
+    _kv4_ints("pages", pages, n)
+    shape = (n, keys.kv_heads, keys.head_dim)
+    if out is None:
+        out = keys._scales.new_empty(shape)
+    else:
+        _require("out", out, torch.float32, shape)
+    _call_on(keys.device, "w8a8_kv4_page_keys_load", keys._descriptor(), pages.data_ptr(), n,
+             out.data_ptr(), _stream(keys.device))
+    return out
+
+
+def kv4_select_workspace_size(seqs: int, kv_heads: int, columns: int, keep: int) -> int:
+    """Bytes of workspace kv4_select needs (0: none)."""
+    return int(library().w8a8_kv4_select_workspace_size(seqs, kv_heads, columns, keep))
+
+
+def kv4_select(q, keys: KV4PageKeys, block_table, seq_lens, keep: int, page_size: int, out=None,
+               workspace="auto"):
+    """The pages that one new token per sequence attends to, for each key head: the last
+    one and the keep - 1 others whose page keys have the largest product with the sum of the
+    head's queries (the lower column first among equals).
+
+    q fp16 [seqs, heads, head_dim], block_table and seq_lens as in attention_kv4.  Returns
+    (pages int32 [seqs, kv_heads, keep], by column and -1 behind the last, tokens in them
+    int32 [seqs]), which attention_kv4 takes as its block_table and seq_lens; out: these
+    two.  workspace: 'auto' or a device tensor of kv4_select_workspace_size bytes."""
+    torch = _torch()
+    dev = keys.device
+    _require_on(dev, q=q, block_table=block_table, seq_lens=seq_lens)
+    ldq = _heads3d("q", q, None, keys.head_dim)
+    seqs, heads, _ = q.shape
+    cols, table_ld = _kv4_table(block_table, seqs)
+    _kv4_ints("seq_lens", seq_lens, seqs)
+    if keep <= 0:
+        raise ValueError("keep must be > 0")
+    shape = (seqs, keys.kv_heads, keep)
+    if out is None:
+        chosen, lens = seq_lens.new_empty(shape), seq_lens.new_empty(seqs)
+    else:
+        chosen, lens = out
+        _require_on(dev, pages=chosen, lens=lens)
+        _require("pages", chosen, torch.int32, shape)
+        _kv4_ints("lens", lens, seqs)
+    _workspace_on(workspace, dev)
+    ws, ws_bytes = _workspace(
+        workspace, lambda: kv4_select_workspace_size(seqs, keys.kv_heads, cols, keep), dev)
+    _call_on(dev, "w8a8_kv4_select", q.data_ptr(), keys._descriptor(), block_table.data_ptr(),
+             cols, table_ld, seq_lens.data_ptr(), page_size, chosen.data_ptr(), keep,
+             lens.data_ptr(), seqs, heads, ldq, _ptr(ws), ws_bytes, _stream(dev))
+    return chosen, lens

@@ -65,6 +65,13 @@ class Kv4Cache(ctypes.Structure):
                 ("group", ctypes.c_uint32)]
 
 
+class Kv4PageKeys(ctypes.Structure):
+    """w8a8_kv4_page_keys (include/w8a8.h)."""
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("pages", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32)]
+
+
 # name -> (restype, argtypes); mirrors include/w8a8.h
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "w8a8_version": (ctypes.c_char_p, []),
@@ -129,6 +136,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "w8a8_attention_kv4_workspace_size": (_size, [_u32, _u32, _u32, _u32, _u32]),
     "w8a8_attention_kv4": (_i32, [_ptr, ctypes.POINTER(Kv4Cache), _ptr, _u32, _u32, _ptr, _ptr,
                                   _u32, _u32, _u32, _u32, _f32, _ptr, _size, _ptr]),
+    "w8a8_kv4_extend": (_i32, [_ptr, _ptr, _u32, _ptr, _u32, _u32, _ptr, _u32, _ptr, _u32, _ptr,
+                               _u32, _ptr, _ptr, _ptr, _ptr]),
+    "w8a8_kv4_trim": (_i32, [_ptr, _ptr, _u32, _ptr, _u32, _u32, _ptr, _u32, _ptr, _u32, _ptr,
+                             _ptr, _ptr]),
+    "w8a8_attention_kv4_chunks_workspace_size": (_size, [ctypes.POINTER(Kv4Cache), _u32, _u32,
+                                                         _u32, _u32, _u32]),
+    "w8a8_attention_kv4_chunks": (_i32, [_ptr, ctypes.POINTER(Kv4Cache), _ptr, _u32, _u32, _ptr,
+                                         _ptr, _ptr, _u32, _u32, _u32, _u32, _u32, _u32, _f32,
+                                         _ptr, _size, _ptr]),
+    "w8a8_kv4_summarize": (_i32, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4PageKeys), _ptr,
+                                  _u32, _u32, _ptr, _ptr, _u32, _u32, _ptr]),
+    "w8a8_kv4_page_keys_load": (_i32, [ctypes.POINTER(Kv4PageKeys), _ptr, _u32, _ptr, _ptr]),
+    "w8a8_kv4_select_workspace_size": (_size, [_u32, _u32, _u32, _u32]),
+    "w8a8_kv4_select": (_i32, [_ptr, ctypes.POINTER(Kv4PageKeys), _ptr, _u32, _u32, _ptr, _u32,
+                               _ptr, _u32, _ptr, _u32, _u32, _u32, _ptr, _size, _ptr]),
+    "w8a8_attention_kv4_selected": (_i32, [_ptr, ctypes.POINTER(Kv4Cache), _ptr, _u32, _ptr, _ptr,
+                                           _u32, _u32, _u32, _u32, _f32, _ptr, _size, _ptr]),
 }
 
 

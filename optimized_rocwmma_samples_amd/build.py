@@ -41,6 +41,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 SOURCES = [
     "capi.cpp",
     "capi_serving.cpp",
+    "capi_paged.cpp",
     "smoothquant.hip",
     "gemm_i8.hip",
     "moe.hip",
@@ -48,6 +49,8 @@ SOURCES = [
     "weights.hip",
     "attention.hip",
     "kv4.hip",
+    "kv4_pages.hip",
+    "kv4_chunks.hip",
     "moe_decode.hip",
 ]
 

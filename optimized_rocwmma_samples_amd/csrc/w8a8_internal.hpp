@@ -315,10 +315,83 @@ struct AttentionKv4Args {
     float           scale;
     void*           ws;
     size_t          ws_bytes;
+    uint32_t        table_head = 0; // from a key head's table to the next one's, 0: all have one
 };
 size_t     attention_kv4_workspace_bytes(uint32_t seqs, uint32_t heads, uint32_t kv_heads,
                                          uint32_t dim, uint32_t max_len);
 hipError_t launch_attention_kv4(const w8a8_kv4_cache& c, const AttentionKv4Args& a,
                                 hipStream_t stream);
+
+// ---- The 4-bit cache's pages (kv4_pages.hip) ------------------------------------
+struct Kv4ExtendArgs {
+    const int32_t *fresh, *lens; // [seqs]
+    int32_t*       table;        // [seqs, table_ld]
+    const int32_t *free, *count; // [capacity], [1]
+    int32_t *      slots, *starts, *lens_out, *count_out;
+    uint32_t       seqs, tokens, table_cols, table_ld, capacity, page_shift;
+};
+struct Kv4TrimArgs {
+    const int32_t *keep, *lens, *table;
+    int32_t*       free;
+    const int32_t* count;
+    int32_t *      lens_out, *count_out;
+    uint32_t       seqs, table_cols, table_ld, capacity, page_shift;
+};
+// Tokens to place, or pages to take back, that one block handles in one launch.
+constexpr uint32_t kOneBlockItems = 8192;
+hipError_t launch_kv4_extend(const Kv4ExtendArgs& a, hipStream_t stream);
+hipError_t launch_kv4_trim(const Kv4TrimArgs& a, hipStream_t stream);
+
+struct Kv4SummarizeArgs {
+    const int32_t *table, *lens, *starts;
+    int8_t*        codes;  // [pages, kv_heads, head_dim]
+    float*         scales; // [pages, kv_heads]
+    uint32_t       seqs, tokens, table_cols, table_ld;
+};
+// Pages that `tokens` new tokens of `seqs` sequences lie in, at the most.
+inline uint64_t kv4_touched_pages(uint32_t tokens, uint32_t seqs, uint32_t page_size)
+{
+    return (uint64_t)tokens / page_size + 2ull * (tokens < seqs ? tokens : seqs);
+}
+hipError_t launch_kv4_summarize(const w8a8_kv4_cache& c, const Kv4SummarizeArgs& a,
+                                hipStream_t stream);
+
+struct Kv4PageKeysArgs {
+    const int8_t*  codes;
+    const float*   scales;
+    const int32_t* list; // [count]
+    float*         out;  // [count, kv_heads, head_dim]
+    uint32_t       count, pages, kv_heads, head_dim;
+};
+hipError_t launch_kv4_page_keys(const Kv4PageKeysArgs& a, hipStream_t stream);
+
+struct Kv4SelectArgs {
+    const uint16_t* q;
+    const int8_t*   codes;
+    const float*    scales;
+    const int32_t * table, *lens;
+    int32_t *       chosen, *lens_out; // [seqs, kv_heads, keep], [seqs]
+    uint32_t        seqs, heads, kv_heads, head_dim, ldq, table_cols, table_ld, keep, page_shift;
+    uint32_t        pages;
+    void*           ws;
+};
+size_t     kv4_select_workspace_bytes(uint32_t seqs, uint32_t kv_heads, uint32_t cols,
+                                      uint32_t keep);
+hipError_t launch_kv4_select(const Kv4SelectArgs& a, hipStream_t stream);
+
+// ---- Attention of chunks over the 4-bit cache (kv4_chunks.hip) --------------------
+struct ChunkArgs {
+    const uint16_t* q;
+    uint16_t*       out;
+    const int32_t * table, *lens, *starts; // [seqs, table_ld], [seqs], [seqs + 1]
+    uint32_t        seqs, tokens, heads, ldq, ldo, table_cols, table_ld, max_new;
+    float           scale;
+    void*           ws;
+};
+size_t     attention_kv4_chunks_workspace_bytes(const w8a8_kv4_cache& c, uint32_t seqs,
+                                                uint32_t tokens, uint32_t heads,
+                                                uint32_t table_cols, uint32_t max_new);
+hipError_t launch_attention_kv4_chunks(const w8a8_kv4_cache& c, const ChunkArgs& a,
+                                       hipStream_t stream);
 
 } // namespace w8a8

@@ -51,6 +51,7 @@ SOURCES = [
     "kv4.hip",
     "kv4_pages.hip",
     "kv4_chunks.hip",
+    "kv4_unpacked.hip",
     "moe_decode.hip",
 ]
 

@@ -21,7 +21,7 @@
 // (n - 8), rounded once: half of what kv4_load gives, since a group that reaches the ends of
 // fp16 may pass them by half a step (the halves go into the scale of the scores and of the
 // result).
-#include "kv4_device.hpp"
+#include "kv4_chunks.hpp"
 
 #include <algorithm>
 
@@ -43,39 +43,9 @@ constexpr int      kStep    = kWaves * kKeys;  // keys of a step
 constexpr int      kRows    = 32;              // rows of a unit
 constexpr uint32_t kBlocks  = 512;             // two a CU
 
-// What the join needs of a unit that goes on behind the run it begins in.
-struct Piece {
-    uint32_t last;  // run that has its last step, plus 1; 0: no such unit
-    uint32_t token; // first row of q of its sequence
-    uint32_t row0, rows; // its rows row0 .. of the sequence's `rows`
-    uint32_t head;       // first query head
-    uint32_t unused[3];
-};
-
-// Partials: slot 2 r of run r holds a unit that began before it, 2 r + 1 one that begins in it
-// and goes on: fp32 [rows, head_dim] in the codes' order, then (maximum, sum) of each row.
-struct Runs {
-    uint32_t count;
-    float*   o;
-    float*   ml;
-    Piece*   cut;
-};
-
 __host__ __device__ inline uint32_t steps_of(uint32_t len)
 {
     return len == 0 ? 1u : (len + kStep - 1) / kStep; // a sequence of no tokens is written too
-}
-
-// One sequence of the call.
-struct Chunk {
-    uint32_t begin, fresh, len; // first row of q, new tokens, tokens in all
-};
-
-__device__ __forceinline__ Chunk chunk_of(const ChunkArgs& a, uint32_t i, uint32_t most)
-{
-    const int32_t b = min(max(a.starts[i], 0), (int32_t)a.tokens);
-    const int32_t e = min(max(a.starts[i + 1], 0), (int32_t)a.tokens);
-    return {(uint32_t)b, (uint32_t)max(e - b, 0), (uint32_t)max(min(a.lens[i], (int32_t)most), 0)};
 }
 
 __device__ __forceinline__ v16f mfma(v8h a, v8h b, v16f c)
@@ -156,7 +126,8 @@ struct Place {
 
 template <int D, int G>
 __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& a, const Runs& runs,
-                                           uint32_t pages, uint8_t* lds, float* lds_ml)
+                                           const uint8_t* others, uint32_t pages,
+                                           uint8_t* lds, float* lds_ml)
 {
     using R = Raw<D, G>;
     constexpr int  kSteps = D / 16, kBlk = D / 32; // products along the channels; result blocks
@@ -165,6 +136,11 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
     const int      lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
     const uint32_t run = blockIdx.x;
     const uint32_t per = a.heads / c.kv_heads, most = a.table_cols << c.page_shift;
+    auto           chunk_at = [&](uint32_t i) { // without rows where they go another way
+        Chunk x = chunk_of(a, i, most);
+        if(others != nullptr && others[i] != 0) x.fresh = 0;
+        return x;
+    };
     auto           tiles_of = [&](const Chunk& s) { return (s.fresh * per + kRows - 1) / kRows; };
 
     // ---- the block's run ---------------------------------------------------------------
@@ -173,7 +149,7 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
         const uint32_t i = i0 + lane;
         n                = 0;
         if(i < a.seqs) {
-            const Chunk x = chunk_of(a, i, most);
+            const Chunk x = chunk_at(i);
             n             = tiles_of(x) * c.kv_heads * steps_of(x.len);
         }
         s = n;
@@ -208,7 +184,7 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
         at -= sum;
     }
     auto enter = [&](Place& p) { // the sequence p.seq
-        p.c     = chunk_of(a, p.seq, most);
+        p.c     = chunk_at(p.seq);
         p.steps = steps_of(p.c.len);
         p.tiles = tiles_of(p.c);
     };
@@ -491,12 +467,13 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
 
 template <int D, int G>
 __global__ void __launch_bounds__(kThreads, 2)
-    attention_kv4_chunks_kernel(CacheView c, ChunkArgs a, Runs runs, uint32_t pages)
+    attention_kv4_chunks_kernel(CacheView c, ChunkArgs a, Runs runs, const uint8_t* others,
+                                uint32_t pages)
 {
     // the waves' values, or two waves' results
     __shared__ alignas(256) uint8_t lds[kWaves * kKeys * D * 2];
     __shared__ float                ml[kWaves * 32 * 2];
-    chunks_run<D, G>(c, a, runs, pages, lds, ml);
+    chunks_run<D, G>(c, a, runs, others, pages, lds, ml);
 }
 
 // Joins the partials of the cut units: the second slot of the run a unit begins in, then the
@@ -567,33 +544,61 @@ uint32_t run_count(uint32_t seqs, uint32_t tokens, uint32_t heads, uint32_t kv_h
     return (uint32_t)std::min<uint64_t>(kBlocks, tiles * kv_heads * steps_of(max_len));
 }
 
+// Where everything lies in the workspace: the partials of this file's kernel, then what the
+// other one uses.
+struct Layout {
+    uint32_t       runs;
+    size_t         ml, cut, other, bytes;
+    UnpackedLayout u;
+};
+
+Layout layout(const w8a8_kv4_cache& c, uint32_t seqs, uint32_t tokens, uint32_t heads,
+              uint32_t table_cols, uint32_t max_new)
+{
+    Layout         w{};
+    const uint32_t max_len = table_cols * c.page_size;
+    w.runs                 = run_count(seqs, tokens, heads, c.kv_heads, max_len);
+    if(steps_of(max_len) > 1) { // else no unit is cut
+        const size_t slots = (size_t)w.runs * 2 * kRows;
+        w.ml               = slots * c.head_dim * 4;
+        w.cut              = w.ml + slots * 8;
+        w.other            = (w.cut + w.runs * sizeof(Piece) + 255) / 256 * 256;
+    }
+    w.u     = unpacked_layout(c, seqs, tokens, heads, table_cols, max_new);
+    w.bytes = w.other + w.u.bytes;
+    return w;
+}
+
 } // namespace
 
 size_t attention_kv4_chunks_workspace_bytes(const w8a8_kv4_cache& c, uint32_t seqs,
                                             uint32_t tokens, uint32_t heads, uint32_t table_cols,
-                                            uint32_t)
+                                            uint32_t max_new)
 {
-    const uint32_t max_len = table_cols * c.page_size;
-    if(steps_of(max_len) == 1 || seqs == 0 || tokens == 0) return 0; // no unit is cut
-    const size_t runs = run_count(seqs, tokens, heads, c.kv_heads, max_len);
-    return runs * (2 * kRows * (c.head_dim + 2) * 4 + sizeof(Piece));
+    if(seqs == 0 || tokens == 0) return 0;
+    return layout(c, seqs, tokens, heads, table_cols, max_new == 0 ? tokens : max_new).bytes;
 }
 
 hipError_t launch_attention_kv4_chunks(const w8a8_kv4_cache& c, const ChunkArgs& a,
                                        hipStream_t stream)
 {
-    const uint32_t max_len = a.table_cols * c.page_size;
-    Runs           runs{};
-    runs.count = run_count(a.seqs, a.tokens, a.heads, c.kv_heads, max_len);
-    if(steps_of(max_len) > 1) {
-        const size_t slots = (size_t)runs.count * 2 * kRows;
-        runs.o             = static_cast<float*>(a.ws);
-        runs.ml            = runs.o + slots * c.head_dim;
-        runs.cut           = reinterpret_cast<Piece*>(runs.ml + slots * 2);
+    const Layout w  = layout(c, a.seqs, a.tokens, a.heads, a.table_cols, a.max_new);
+    auto*        ws = static_cast<uint8_t*>(a.ws);
+    Runs         runs{};
+    runs.count = w.runs;
+    if(w.cut != 0) {
+        runs.o   = reinterpret_cast<float*>(ws);
+        runs.ml  = reinterpret_cast<float*>(ws + w.ml);
+        runs.cut = reinterpret_cast<Piece*>(ws + w.cut);
+    }
+    const uint8_t* others = nullptr;
+    if(w.u.bytes != 0) {
+        launch_unpacked(c, a, w.u, ws + w.other, stream);
+        others = ws + w.other + w.u.flags;
     }
     with_widths(c, [&](auto d, auto g) {
         attention_kv4_chunks_kernel<d(), g()>
-            <<<runs.count, kThreads, 0, stream>>>(view(c), a, runs, c.pages);
+            <<<runs.count, kThreads, 0, stream>>>(view(c), a, runs, others, c.pages);
         if(runs.cut)
             attention_kv4_chunks_join_kernel<d()>
                 <<<std::min(runs.count * kRows / kWaves, 1024u), kThreads, 0, stream>>>(

@@ -1,0 +1,76 @@
+// kv4_chunks.hpp -- what the two kernels of attention of chunks over the 4-bit cache share: the
+// sequences of a call, which of them go which way, and the pieces that runs cut units into.
+#pragma once
+
+#include "kv4_device.hpp"
+
+namespace w8a8 {
+namespace {
+
+// A sequence with more rows (new tokens x query heads a key head) than this has its keys
+// and values unpacked to fp16 first, once, and then takes the prompts' kernel over them;
+// the others unpack the codes they use where they use them, which costs each 32 rows
+// twice what the products take.
+constexpr uint32_t kFewRows = 256;
+
+// One sequence of the call.
+struct Chunk {
+    uint32_t begin, fresh, len; // first row of q, new tokens, tokens in all
+};
+
+__device__ __forceinline__ Chunk chunk_of(const ChunkArgs& a, uint32_t i, uint32_t most)
+{
+    const int32_t b = min(max(a.starts[i], 0), (int32_t)a.tokens);
+    const int32_t e = min(max(a.starts[i + 1], 0), (int32_t)a.tokens);
+    return {(uint32_t)b, (uint32_t)max(e - b, 0), (uint32_t)max(min(a.lens[i], (int32_t)most), 0)};
+}
+
+// A sequence that is unpacked: its tokens are rows base + pad .. of the unpacked keys and
+// values (`need` rows in all, whole key tiles), so that its first new token begins a tile.
+struct Long {
+    uint32_t seq, base, need, pad;
+    Chunk    c;
+    uint32_t unused;
+};
+
+// Which sequences are unpacked; in the workspace.
+struct LongList {
+    uint32_t  most;  // the list's room
+    uint32_t  rows;  // room for unpacked tokens
+    uint32_t* total; // [0] sequences in the list, [1] their rows
+    Long*     list;
+    uint8_t*  flags; // [seqs] 1: in the list
+};
+
+// What the join needs of a unit that goes on behind the run it begins in.
+struct Piece {
+    uint32_t last;  // run that has its last step, plus 1; 0: no such unit
+    uint32_t token; // first row of q of its sequence
+    uint32_t row0, rows; // its rows row0 .. of the sequence's `rows`
+    uint32_t head;       // first query head
+    uint32_t unused[3];
+};
+
+// Partials: slot 2 r of run r holds a unit that began before it, 2 r + 1 one that begins in it
+// and goes on: fp32 [rows, head_dim], then (maximum, sum) of each row.
+struct Runs {
+    uint32_t count;
+    float*   o;
+    float*   ml;
+    Piece*   cut;
+};
+
+} // namespace
+
+// The kernels over unpacked keys and values (kv4_unpacked.hip).
+struct UnpackedLayout {
+    uint32_t runs, members, heads, tiles; // members = heads x tiles blocks share a run's keys
+    uint32_t room, rows;                  // of the list, of unpacked tokens; 0: none
+    size_t   o, ml, cut, total, list, flags, missing, k, v, bytes; // offsets
+};
+UnpackedLayout unpacked_layout(const w8a8_kv4_cache& c, uint32_t seqs, uint32_t tokens,
+                               uint32_t heads, uint32_t table_cols, uint32_t max_new);
+void launch_unpacked(const w8a8_kv4_cache& c, const ChunkArgs& a, const UnpackedLayout& u,
+                     uint8_t* ws, hipStream_t stream);
+
+} // namespace w8a8

@@ -376,7 +376,9 @@ __device__ __forceinline__ void store_lds(uint32_t to, const int32_t* r)
         *(lds_u32_t*)(uintptr_t)to = (uint32_t)r[0];
 }
 
-template <int D, int G, int C>
+// TABLES: each key head has a block table of its own (a variant, since the address of a page
+// number is on every chunk's way: 1 to 2 % of a long context's time).
+template <int D, int G, int C, bool TABLES>
 __device__ __forceinline__ void attention_kv4_run(const CacheView& c, const AttentionKv4Args& a,
                                                   const Cut& cut, uint32_t pages, uint8_t* lds)
 {
@@ -474,8 +476,9 @@ __device__ __forceinline__ void attention_kv4_run(const CacheView& c, const Atte
         const uint32_t t    = p.chunk * kChunk + lane / 16 * 16;
         int32_t        page = -1;
         if(t < p.len) {
-            page = a.table[(size_t)p.seq * a.table_ld + (size_t)(p.unit / qtiles) * a.table_head
-                           + (t >> c.page_shift)];
+            const size_t row = (size_t)p.seq * a.table_ld
+                               + (TABLES ? (size_t)(p.unit / qtiles) * a.table_head : 0);
+            page             = a.table[row + (t >> c.page_shift)];
             if(page < 0 || (uint32_t)page >= pages) page = -1;
         }
         return page;
@@ -794,12 +797,12 @@ __device__ __forceinline__ void attention_kv4_run(const CacheView& c, const Atte
     }
 }
 
-template <int D, int G, int C>
+template <int D, int G, int C, bool TABLES>
 __global__ void __launch_bounds__(kAttThreads, 2)
     attention_kv4_kernel(CacheView c, AttentionKv4Args a, Cut cut, uint32_t pages)
 {
     __shared__ alignas(16) uint8_t lds[kAttWaves * KvLds<D, G>::kWave];
-    attention_kv4_run<D, G, C>(c, a, cut, pages, lds);
+    attention_kv4_run<D, G, C, TABLES>(c, a, cut, pages, lds);
 }
 
 // Joins the partials of the cut units: the slot of the first wave, then the first slots
@@ -971,9 +974,12 @@ hipError_t launch_attention_kv4(const w8a8_kv4_cache& c, const AttentionKv4Args&
     }
     const uint32_t blocks = (cut.waves + kAttWaves - 1) / kAttWaves;
     with_widths(c, [&](auto d, auto g) {
-        const auto kernel = cut.heads == 4   ? attention_kv4_kernel<d(), g(), 4>
-                            : cut.heads == 8 ? attention_kv4_kernel<d(), g(), 2>
-                                             : attention_kv4_kernel<d(), g(), 1>;
+        const auto pick = [&](auto t) {
+            return cut.heads == 4   ? attention_kv4_kernel<d(), g(), 4, t()>
+                   : cut.heads == 8 ? attention_kv4_kernel<d(), g(), 2, t()>
+                                    : attention_kv4_kernel<d(), g(), 1, t()>;
+        };
+        const auto kernel = a.table_head != 0 ? pick(std::true_type()) : pick(std::false_type());
         kernel<<<blocks, kAttThreads, 0, stream>>>(view(c), a, cut, c.pages);
         if(!cut.whole) {
             const auto join = cut.heads == 4   ? launch_join<d(), 4>

@@ -40,7 +40,6 @@ constexpr int      kWaves   = 4;
 constexpr int      kThreads = kWaves * kWave;
 constexpr int      kKeys    = 32;              // a wave's a step
 constexpr int      kStep    = kWaves * kKeys;  // keys of a step
-constexpr int      kRows    = 32;              // rows of a unit
 constexpr uint32_t kBlocks  = 512;             // two a CU
 
 __host__ __device__ inline uint32_t steps_of(uint32_t len)
@@ -124,7 +123,7 @@ struct Place {
     Chunk    c;
 };
 
-template <int D, int G>
+template <int D, int G, int T>
 __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& a, const Runs& runs,
                                            const uint8_t* others, uint32_t pages,
                                            uint8_t* lds, float* lds_ml)
@@ -132,13 +131,18 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
     using R = Raw<D, G>;
     constexpr int  kSteps = D / 16, kBlk = D / 32; // products along the channels; result blocks
     constexpr int  kTile = kKeys * D * 2;          // bytes of a wave's values
+    constexpr uint32_t kRows = 32 * T;             // rows of a unit
     const int      wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int      lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
     const uint32_t run = blockIdx.x;
     const uint32_t per = a.heads / c.kv_heads, most = a.table_cols << c.page_shift;
+    // LDS: the waves' values (at a unit's end two waves' results), then the queries
+    const uint32_t lds0 = (uint32_t)(uintptr_t)lds, tile = lds0 + wave * kTile;
+    const uint32_t qat = lds0 + kWaves * kTile + lane * 16;
     auto           chunk_at = [&](uint32_t i) { // without rows where they go another way
         Chunk x = chunk_of(a, i, most);
         if(others != nullptr && others[i] != 0) x.fresh = 0;
+        if((x.fresh * per > 32) != (T > 1)) x.fresh = 0;
         return x;
     };
     auto           tiles_of = [&](const Chunk& s) { return (s.fresh * per + kRows - 1) / kRows; };
@@ -226,35 +230,53 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
         load_dwords<R::kValuePairs>(x.vs, c.scales[1] + row * (D / G) + half * (D / 2) / G);
     };
 
-    // ---- the queries: lane = row, 8 channels a product in the codes' order --------------
-    v8h      qf[kSteps];
-    uint32_t sees = 0, least = 0; // keys the lane's row sees, and the unit's first row
-    auto     queries = [&](const Place& p) {
+    // ---- the queries, in LDS as the products take them: [32 rows][product][lane] ---------
+    uint32_t   sees[T] = {}, least = 0; // keys the lane's rows see, and the unit's first row
+    const auto queries = [&](const Place& p) {
         const uint32_t row0 = p.unit % p.tiles * kRows, rows = p.c.fresh * per;
-        const uint32_t row = min(row0 + col, rows - 1), tok = row / per;
-        const uint16_t* from = a.q + (size_t)(p.c.begin + tok) * a.ldq
-                               + (size_t)(p.unit / p.tiles * per + row % per) * D + 8 * half;
+        auto           seen = [&](uint32_t row) {
+            return (uint32_t)max((int32_t)(p.c.len + row / per + 1 - p.c.fresh), 0);
+        };
         constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+        least                   = seen(row0);
 #pragma unroll
-        for(int st = 0; st < kSteps; ++st) {
-            const v8h v = *reinterpret_cast<const v8h*>(from + 16 * st);
+        for(int t = 0; t < T; ++t) {
+            const uint32_t row = min(row0 + 32 * t + col, rows - 1);
+            sees[t]            = seen(row);
+            const uint16_t* from = a.q + (size_t)(p.c.begin + row / per) * a.ldq
+                                   + (size_t)(p.unit / p.tiles * per + row % per) * D + 8 * half;
 #pragma unroll
-            for(int e = 0; e < 8; ++e) qf[st][e] = v[kOrder[e]];
+            for(int st = wave; st < kSteps; st += kWaves) {
+                const v8h v = *reinterpret_cast<const v8h*>(from + 16 * st);
+                v8h       u;
+#pragma unroll
+                for(int e = 0; e < 8; ++e) u[e] = v[kOrder[e]];
+                *(lds_v4i_t*)(uintptr_t)(qat + (t * kSteps + st) * kWave * 16)
+                    = __builtin_bit_cast(v4i, u);
+            }
         }
-        auto seen = [&](uint32_t t) { return (uint32_t)max((int32_t)(p.c.len + t + 1 - p.c.fresh), 0); };
-        sees  = seen(tok);
-        least = seen(row0 / per);
     };
 
     const Unpack unpack;
     const float  c2 = a.scale * (2.f * 1.44269504088896341f); // base 2, of halved keys
-    const uint32_t lds0 = (uint32_t)(uintptr_t)lds, tile = lds0 + wave * kTile;
     const uint32_t tok0 = 4 * half + lane % 16 / 4, ch0 = lane / 16 % 2 * 16 + lane % 4 * 4;
     const uint32_t vat  = tile + tok0 * D * 2 + value_chunk<D>(tok0, ch0 / 8) * 16 + ch0 % 8 * 2;
 
-    float m = -INFINITY, l = 0.f, mc = 0.f; // mc = m c2, 0 while no score is finite
-    v16f  o[kBlk] = {};
-    bool  from_start = here.step == 0; // of the unit
+    // of each 32 rows: maximum, mc = m c2 (0 while no score is finite), sum, result
+    float m[T], l[T], mc[T];
+    v16f  o[T][kBlk];
+    auto  begin_unit = [&] {
+#pragma unroll
+        for(int t = 0; t < T; ++t) {
+            m[t]  = -INFINITY;
+            mc[t] = 0.f;
+            l[t]  = 0.f;
+#pragma unroll
+            for(int b = 0; b < kBlk; ++b) o[t][b] = v16f{};
+        }
+    };
+    begin_unit();
+    bool from_start = here.step == 0; // of the unit
 
     R     x;
     Place next = here;
@@ -268,6 +290,89 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
         advance(next);
         page_next = page_at(next);
     }
+    __syncthreads(); // the queries are there
+
+    // The waves' results of 32 rows joined and written, at the unit's end or the run's.
+    auto finish = [&](const int t, const Place& now, bool ends) {
+        const v2f ls = both_halves(l[t]);
+        const float lw = ls[0] + ls[1];
+        if(half == 0) {
+            lds_ml[(wave * 32 + col) * 2]     = m[t];
+            lds_ml[(wave * 32 + col) * 2 + 1] = lw;
+        }
+        __syncthreads();
+        float common = -INFINITY, sum = 0.f;
+#pragma unroll
+        for(int w = 0; w < kWaves; ++w) common = fmaxf(common, lds_ml[(w * 32 + col) * 2]);
+        auto weight = [&](float mw) {
+            return mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - common) * c2);
+        };
+#pragma unroll
+        for(int w = 0; w < kWaves; ++w)
+            sum = fmaf(weight(lds_ml[(w * 32 + col) * 2]), lds_ml[(w * 32 + col) * 2 + 1], sum);
+        const float mine = weight(m[t]);
+#pragma unroll
+        for(int b = 0; b < kBlk; ++b) o[t][b] *= mine;
+        // the waves' results added up: 2 and 3 to 0 and 1, then 1 to 0
+#pragma unroll
+        for(int d = 2; d > 0; d /= 2) {
+            const uint32_t buf = lds0 + (wave % d) * (kBlk * 16 * kWave * 4) + lane * 16;
+            if(wave >= d && wave < 2 * d)
+#pragma unroll
+                for(int b = 0; b < kBlk; ++b)
+#pragma unroll
+                    for(int i = 0; i < 16; i += 4)
+                        *(lds_v4f_t*)(uintptr_t)(buf + (b * 4 + i / 4) * kWave * 16)
+                            = v4f{o[t][b][i], o[t][b][i + 1], o[t][b][i + 2], o[t][b][i + 3]};
+            __syncthreads();
+            if(wave < d)
+#pragma unroll
+                for(int b = 0; b < kBlk; ++b)
+#pragma unroll
+                    for(int i = 0; i < 16; i += 4) {
+                        const v4f u
+                            = *(lds_v4f_t*)(uintptr_t)(buf + (b * 4 + i / 4) * kWave * 16);
+#pragma unroll
+                        for(int e = 0; e < 4; ++e) o[t][b][i + e] += u[e];
+                    }
+            __syncthreads();
+        }
+        if(wave != 0) return;
+        const uint32_t row0 = now.unit % now.tiles * kRows + 32 * t, rows = now.c.fresh * per;
+        const uint32_t row = row0 + col, head0 = now.unit / now.tiles * per;
+        if(ends && from_start) {
+            const float inv = sum != 0.f ? 2.f / sum : 0.f;
+            uint16_t*   out = a.out + (size_t)(now.c.begin + row / per) * a.ldo
+                            + (size_t)(head0 + row % per) * D + 4 * half;
+#pragma unroll
+            for(int b = 0; b < kBlk; ++b)
+#pragma unroll
+                for(int i = 0; i < 16; i += 4) {
+                    // this half has channels 0 1, 4 5 (2 3, 6 7) of a chunk of 8
+                    const auto w = __builtin_amdgcn_permlane32_swap(
+                        finite_halves(o[t][b][i] * inv, o[t][b][i + 2] * inv),
+                        finite_halves(o[t][b][i + 1] * inv, o[t][b][i + 3] * inv), false, false);
+                    if(row < rows)
+                        *reinterpret_cast<v2i*>(out + 32 * b + 8 * (i / 4))
+                            = v2i{(int)w[0], (int)w[1]};
+                }
+        } else if(row < rows) {
+            const size_t slot = (size_t)(2 * run + (from_start ? 1 : 0)) * kRows + 32 * t + col;
+#pragma unroll
+            for(int b = 0; b < kBlk; ++b)
+#pragma unroll
+                for(int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<v4f*>(runs.o + slot * D + 32 * b + 2 * i + 4 * half)
+                        = v4f{o[t][b][i], o[t][b][i + 1], o[t][b][i + 2], o[t][b][i + 3]};
+            if(half == 0) *reinterpret_cast<v2f*>(runs.ml + slot * 2) = v2f{common * c2, sum};
+        }
+        if(t == 0 && !ends && from_start && lane == 0) { // goes on behind the run: up to which
+            const uint32_t last = end - 1 + (now.steps - 1 - now.step); // its last step
+            runs.cut[run]       = {(last < r * (q + 1) ? last / (q + 1)
+                                                       : r + (last - r * (q + 1)) / q) + 1,
+                             now.c.begin, row0, rows, head0, {}};
+        }
+    };
 
     for(; left > 0; --left) {
         const Place    now  = here;
@@ -296,11 +401,17 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
                 = __builtin_bit_cast(v4i, v);
         }
         // ---- scores -----------------------------------------------------------------------
-        v16f sc = {};
+        v16f sc[T] = {};
 #pragma unroll
-        for(int st = 0; st < kSteps; ++st)
-            sc = mfma(unpack((uint32_t)x.k[st % 2][st / 2], halved(x.ks[st / 2 * 32 / G])), qf[st],
-                      sc);
+        for(int st = 0; st < kSteps; ++st) {
+            const v8h k = unpack((uint32_t)x.k[st % 2][st / 2], halved(x.ks[st / 2 * 32 / G]));
+#pragma unroll
+            for(int t = 0; t < T; ++t)
+                sc[t] = mfma(k,
+                             __builtin_bit_cast(v8h, *(lds_v4i_t*)(uintptr_t)(
+                                                         qat + (t * kSteps + st) * kWave * 16)),
+                             sc[t]);
+        }
         if(left > 1) { // the next step's loads, over the rest of this one
             const int32_t page = page_next;
             here               = next;
@@ -314,37 +425,44 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
 #pragma unroll
             for(int i = 0; i < 16; ++i) {
                 const uint32_t j = 8 * (i / 4) + 4 * half + i % 4;
-                if(key0 + j >= sees || !((live >> j) & 1u)) sc[i] = -INFINITY;
+#pragma unroll
+                for(int t = 0; t < T; ++t)
+                    if(key0 + j >= sees[t] || !((live >> j) & 1u)) sc[t][i] = -INFINITY;
             }
-        float top = sc[15];
 #pragma unroll
-        for(int i = 0; i < 16; i += 2) top = max3(top, sc[i], sc[i + 1]);
-        const v2f   tops = both_halves(top);
-        const float mn   = fmaxf(m, fmaxf(tops[0], tops[1]));
-        // m need not be the maximum itself: rescaled only where probabilities would pass 2^8
-        if(__ballot((mn - m) * c2 > 8.f) != 0) {
-            const float to = mn == -INFINITY ? 0.f : mn * c2;
-            const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - to);
-            m              = mn;
-            mc             = to;
-            l *= al;
+        for(int t = 0; t < T; ++t) {
+            float top = sc[t][15];
 #pragma unroll
-            for(int b = 0; b < kBlk; ++b) o[b] *= al;
+            for(int i = 0; i < 16; i += 2) top = max3(top, sc[t][i], sc[t][i + 1]);
+            const v2f   tops = both_halves(top);
+            const float mn   = fmaxf(m[t], fmaxf(tops[0], tops[1]));
+            // m need not be the maximum itself: rescaled only where probabilities would pass 2^8
+            if(__ballot((mn - m[t]) * c2 > 8.f) != 0) {
+                const float to = mn == -INFINITY ? 0.f : mn * c2;
+                const float al = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc[t] - to);
+                m[t]           = mn;
+                mc[t]          = to;
+                l[t] *= al;
+#pragma unroll
+                for(int b = 0; b < kBlk; ++b) o[t][b] *= al;
+            }
         }
         // ---- O^T += V^T P^T ----------------------------------------------------------------
 #pragma unroll
         for(int st = 0; st < 2; ++st) {
-            v8h p;
+            v8h p[T];
 #pragma unroll
-            for(int i = 0; i < 8; i += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[st * 8 + i], c2, -mc));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[st * 8 + i + 1], c2, -mc));
-                l += p0;
-                l += p1;
-                const v2h h = __builtin_convertvector((v2f{p0, p1}), v2h);
-                p[i]        = h[0];
-                p[i + 1]    = h[1];
-            }
+            for(int t = 0; t < T; ++t)
+#pragma unroll
+                for(int i = 0; i < 8; i += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[t][st * 8 + i], c2, -mc[t]));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[t][st * 8 + i + 1], c2, -mc[t]));
+                    l[t] += p0;
+                    l[t] += p1;
+                    const v2h h = __builtin_convertvector((v2f{p0, p1}), v2h);
+                    p[t][i]     = h[0];
+                    p[t][i + 1] = h[1];
+                }
 #pragma unroll
             for(int b = 0; b < kBlk; ++b) {
                 v8h f; // 4 keys of channel 32 b + col (in the codes' order), and 4 more
@@ -355,7 +473,8 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
 #pragma unroll
                     for(int i = 0; i < 4; ++i) f[part * 4 + i] = (_Float16)t[i];
                 }
-                o[b] = mfma(f, p, o[b]);
+#pragma unroll
+                for(int t = 0; t < T; ++t) o[t][b] = mfma(f, p[t], o[t][b]);
             }
         }
         if(!full) { // NaN values, to exactly the rows that see them
@@ -363,192 +482,137 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
             for(int g = 0; g < R::kValuePairs; ++g)
                 for(uint64_t left_bad = bad[g]; left_bad != 0; left_bad &= left_bad - 1) {
                     const int f = __builtin_ctzll(left_bad), grp = f / 32 * (D / 2) / G + g;
-                    if(key0 + f % 32 < sees)
 #pragma unroll
-                        for(int b = 0; b < kBlk; ++b)
-                            if(b * 32 / G == grp) o[b] += NAN;
+                    for(int t = 0; t < T; ++t)
+                        if(key0 + f % 32 < sees[t])
+#pragma unroll
+                            for(int b = 0; b < kBlk; ++b)
+                                if(b * 32 / G == grp) o[t][b] += NAN;
                 }
         }
 
-        // ---- the unit's end, or the run's --------------------------------------------------
         const bool ends = now.step + 1 == now.steps;
         if(!ends && left > 1) continue;
-        const v2f ls = both_halves(l);
-        l            = ls[0] + ls[1];
-        if(half == 0) {
-            lds_ml[(wave * 32 + col) * 2]     = m;
-            lds_ml[(wave * 32 + col) * 2 + 1] = l;
-        }
-        __syncthreads();
-        float common = -INFINITY, sum = 0.f;
 #pragma unroll
-        for(int w = 0; w < kWaves; ++w) common = fmaxf(common, lds_ml[(w * 32 + col) * 2]);
-        auto weight = [&](float mw) {
-            return mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - common) * c2);
-        };
-#pragma unroll
-        for(int w = 0; w < kWaves; ++w)
-            sum = fmaf(weight(lds_ml[(w * 32 + col) * 2]), lds_ml[(w * 32 + col) * 2 + 1], sum);
-        const float mine = weight(m);
-#pragma unroll
-        for(int b = 0; b < kBlk; ++b) o[b] *= mine;
-        // the waves' results added up: 2 and 3 to 0 and 1, then 1 to 0
-#pragma unroll
-        for(int d = 2; d > 0; d /= 2) {
-            const uint32_t buf = lds0 + (wave % d) * (kBlk * 16 * kWave * 4) + lane * 16;
-            if(wave >= d && wave < 2 * d)
-#pragma unroll
-                for(int b = 0; b < kBlk; ++b)
-#pragma unroll
-                    for(int i = 0; i < 16; i += 4)
-                        *(lds_v4f_t*)(uintptr_t)(buf + (b * 4 + i / 4) * kWave * 16)
-                            = v4f{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]};
-            __syncthreads();
-            if(wave < d)
-#pragma unroll
-                for(int b = 0; b < kBlk; ++b)
-#pragma unroll
-                    for(int i = 0; i < 16; i += 4) {
-                        const v4f u
-                            = *(lds_v4f_t*)(uintptr_t)(buf + (b * 4 + i / 4) * kWave * 16);
-#pragma unroll
-                        for(int e = 0; e < 4; ++e) o[b][i + e] += u[e];
-                    }
-            __syncthreads();
-        }
-        if(wave == 0) {
-            const uint32_t row0 = now.unit % now.tiles * kRows, rows = now.c.fresh * per;
-            const uint32_t row = row0 + col, head0 = now.unit / now.tiles * per;
-            if(ends && from_start) {
-                const float inv = sum != 0.f ? 2.f / sum : 0.f;
-                uint16_t*   out = a.out + (size_t)(now.c.begin + row / per) * a.ldo
-                                + (size_t)(head0 + row % per) * D + 4 * half;
-#pragma unroll
-                for(int b = 0; b < kBlk; ++b)
-#pragma unroll
-                    for(int i = 0; i < 16; i += 4) {
-                        // this half has channels 0 1, 4 5 (2 3, 6 7) of a chunk of 8
-                        const auto w = __builtin_amdgcn_permlane32_swap(
-                            finite_halves(o[b][i] * inv, o[b][i + 2] * inv),
-                            finite_halves(o[b][i + 1] * inv, o[b][i + 3] * inv), false, false);
-                        if(row < rows)
-                            *reinterpret_cast<v2i*>(out + 32 * b + 8 * (i / 4))
-                                = v2i{(int)w[0], (int)w[1]};
-                    }
-            } else if(row < rows) {
-                const size_t slot = (size_t)(2 * run + (from_start ? 1 : 0)) * kRows + col;
-#pragma unroll
-                for(int b = 0; b < kBlk; ++b)
-#pragma unroll
-                    for(int i = 0; i < 16; i += 4)
-                        *reinterpret_cast<v4f*>(runs.o + slot * D + 32 * b + 2 * i + 4 * half)
-                            = v4f{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]};
-                if(half == 0)
-                    *reinterpret_cast<v2f*>(runs.ml + slot * 2) = v2f{common * c2, sum};
-            }
-            if(!ends && from_start && lane == 0) { // goes on behind the run: up to which one
-                const uint32_t last = end - 1 + (now.steps - 1 - now.step); // its last step
-                runs.cut[run] = {(last < r * (q + 1) ? last / (q + 1)
-                                                     : r + (last - r * (q + 1)) / q) + 1,
-                                 now.c.begin, row0, rows, head0, {}};
-            }
-        }
+        for(int t = 0; t < T; ++t) finish(t, now, ends);
         if(left > 1) { // the next unit
             from_start = true;
-            m          = -INFINITY;
-            mc         = 0.f;
-            l          = 0.f;
-#pragma unroll
-            for(int b = 0; b < kBlk; ++b) o[b] = v16f{};
+            begin_unit();
             queries(here);
+            __syncthreads();
         }
     }
 }
 
-template <int D, int G>
+// Sequences of up to 32 rows a key head, then (MORE: there may be any) those of more, two
+// times 32 rows a unit, which unpacks its codes once for both.
+template <int D, int G, bool MORE>
 __global__ void __launch_bounds__(kThreads, 2)
-    attention_kv4_chunks_kernel(CacheView c, ChunkArgs a, Runs runs, const uint8_t* others,
-                                uint32_t pages)
+    attention_kv4_chunks_kernel(CacheView c, ChunkArgs a, Runs few, Runs more,
+                                const uint8_t* others, uint32_t pages)
 {
-    // the waves' values, or two waves' results
-    __shared__ alignas(256) uint8_t lds[kWaves * kKeys * D * 2];
+    __shared__ alignas(256) uint8_t lds[kWaves * kKeys * D * 2 + (MORE ? 64 : 32) * D * 2];
     __shared__ float                ml[kWaves * 32 * 2];
-    chunks_run<D, G>(c, a, runs, others, pages, lds, ml);
+    if(blockIdx.x < few.count) chunks_run<D, G, 1>(c, a, few, others, pages, lds, ml);
+    if constexpr(MORE) {
+        __syncthreads();
+        if(blockIdx.x < more.count) chunks_run<D, G, 2>(c, a, more, others, pages, lds, ml);
+    }
 }
 
 // Joins the partials of the cut units: the second slot of the run a unit begins in, then the
-// first ones of the runs after it.  A wave takes a row; its lanes are 8 channels each of every
-// kWays-th partial, then the ways are added up, in the same order always.
+// first ones of the runs after it.  A wave has 4 rows, lanes being 8 channels each.  Few
+// partials are taken by all four rows' lanes at once, each its own; of many a row at a time,
+// its lanes each every fourth, then the four are added up, in the same order always.
 template <int D>
 __global__ void __launch_bounds__(kThreads)
-    attention_kv4_chunks_join_kernel(ChunkArgs a, Runs runs, uint32_t per)
+    attention_kv4_chunks_join_kernel(ChunkArgs a, Runs few, Runs more, uint32_t per)
 {
-    constexpr uint32_t kLanes = D / 8, kWays = kWave / kLanes;
+    constexpr uint32_t kLanes = D / 8, kWays = kWave / kLanes, kMany = 16;
     const uint32_t     lane = threadIdx.x % kWave, ch = lane % kLanes, way = lane / kLanes;
-    for(uint32_t task = blockIdx.x * kWaves + threadIdx.x / kWave; task < runs.count * kRows;
+    const uint32_t     first = few.count * (32 / kWays), all = first + more.count * (64 / kWays);
+    for(uint32_t task = blockIdx.x * kWaves + threadIdx.x / kWave; task < all;
         task += gridDim.x * kWaves) {
-        const uint32_t run = __builtin_amdgcn_readfirstlane(task / kRows);
-        const uint32_t in  = task % kRows;
-        const Piece    u   = runs.cut[run];
-        const uint32_t row = u.row0 + in;
-        if(u.last == 0 || row >= u.rows) continue;
+        const bool     is_few = task < first;
+        const Runs&    runs   = is_few ? few : more;
+        const uint32_t rows = is_few ? 32 : 64, of = is_few ? task : task - first;
+        const uint32_t run  = __builtin_amdgcn_readfirstlane(of / (rows / kWays));
+        const uint32_t in0  = of % (rows / kWays) * kWays;
+        const Piece    u    = runs.cut[run];
+        if(u.last == 0 || u.row0 + in0 >= u.rows) continue;
         const uint32_t n = u.last - run; // partials
-        float          m = -INFINITY, l = 0.f, sum[8] = {};
+        float          m, l, sum[8];
+        auto           clear = [&] {
+            m = -INFINITY;
+            l = 0.f;
+#pragma unroll
+            for(int y = 0; y < 8; ++y) sum[y] = 0.f;
+        };
         auto take = [&](float mi, float li, const float* v) { // -inf: no key seen
-            if(mi == -INFINITY) {
-                l += li; // 0, or NaN
-                return;
-            }
             const float now = fmaxf(m, mi);
             const float al  = m == now ? 1.f : __builtin_amdgcn_exp2f(m - now);
-            const float e   = mi == now ? 1.f : __builtin_amdgcn_exp2f(mi - now);
+            const float e   = mi == -INFINITY ? 0.f : mi == now ? 1.f : __builtin_amdgcn_exp2f(mi - now);
             m               = now;
-            l               = fmaf(l, al, e * li);
+            l               = fmaf(l, al, mi == -INFINITY ? li : e * li); // 0, or NaN
+            if(e != 0.f)
 #pragma unroll
-            for(int y = 0; y < 8; ++y) sum[y] = fmaf(sum[y], al, e * v[y]);
+                for(int y = 0; y < 8; ++y) sum[y] = fmaf(sum[y], al, e * v[y]);
         };
-        for(uint32_t i = way; i < n; i += kWays) {
-            const size_t slot = (size_t)(2 * (run + i) + (i == 0 ? 1 : 0)) * kRows + in;
+        auto add = [&](uint32_t i, uint32_t in) {
+            const size_t slot = (size_t)(2 * (run + i) + (i == 0 ? 1 : 0)) * rows + in;
             const v2f    ml   = *reinterpret_cast<const v2f*>(runs.ml + slot * 2);
             const v4f*   v    = reinterpret_cast<const v4f*>(runs.o + slot * D + ch * 8);
             const v4f    v0 = v[0], v1 = v[1];
-            const float  all[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-            take(ml[0], ml[1], all);
+            const float  both[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+            take(ml[0], ml[1], both);
+        };
+        auto write = [&](uint32_t in) {
+            const uint32_t row = u.row0 + in;
+            const float    inv = l != 0.f ? 2.f / l : 0.f;
+#pragma unroll
+            for(int y = 0; y < 8; ++y) sum[y] *= inv;
+            // places 0 .. 7 are channels 0 4 1 5 2 6 3 7
+            if(row < u.rows)
+                *reinterpret_cast<v4i*>(a.out + (size_t)(u.token + row / per) * a.ldo
+                                        + (size_t)(u.head + row % per) * D + ch * 8)
+                    = v4i{(int)finite_halves(sum[0], sum[2]), (int)finite_halves(sum[4], sum[6]),
+                          (int)finite_halves(sum[1], sum[3]), (int)finite_halves(sum[5], sum[7])};
+        };
+        if(n <= kMany) {
+            clear();
+            const uint32_t in = min(in0 + way, u.rows - 1 - u.row0);
+            for(uint32_t i = 0; i < n; ++i) add(i, in);
+            write(in0 + way);
+            continue;
         }
+        for(uint32_t y = 0; y < kWays && u.row0 + in0 + y < u.rows; ++y) {
+            clear();
+            for(uint32_t i = way; i < n; i += kWays) add(i, in0 + y);
 #pragma unroll
-        for(uint32_t d = kLanes; d < kWave; d <<= 1) {
-            const float mo = __shfl_xor(m, d, kWave), lo = __shfl_xor(l, d, kWave);
-            float       vo[8];
+            for(uint32_t d = kLanes; d < kWave; d <<= 1) {
+                const float mo = __shfl_xor(m, d, kWave), lo = __shfl_xor(l, d, kWave);
+                float       vo[8];
 #pragma unroll
-            for(int y = 0; y < 8; ++y) vo[y] = __shfl_xor(sum[y], d, kWave);
-            take(mo, lo, vo);
+                for(int z = 0; z < 8; ++z) vo[z] = __shfl_xor(sum[z], d, kWave);
+                take(mo, lo, vo);
+            }
+            if(way == 0) write(in0 + y);
         }
-        if(way != 0) continue;
-        const float inv = l != 0.f ? 2.f / l : 0.f;
-#pragma unroll
-        for(int y = 0; y < 8; ++y) sum[y] *= inv;
-        // places 0 .. 7 are channels 0 4 1 5 2 6 3 7
-        *reinterpret_cast<v4i*>(a.out + (size_t)(u.token + row / per) * a.ldo
-                                + (size_t)(u.head + row % per) * D + ch * 8)
-            = v4i{(int)finite_halves(sum[0], sum[2]), (int)finite_halves(sum[4], sum[6]),
-                  (int)finite_halves(sum[1], sum[3]), (int)finite_halves(sum[5], sum[7])};
     }
 }
 
 // Runs of a launch: no more than steps at the most.
-uint32_t run_count(uint32_t seqs, uint32_t tokens, uint32_t heads, uint32_t kv_heads,
-                   uint32_t max_len)
+uint32_t run_count(uint64_t tiles, uint32_t kv_heads, uint32_t max_len)
 {
-    const uint64_t rows  = (uint64_t)tokens * (heads / kv_heads);
-    const uint64_t tiles = rows / kRows + std::min(seqs, tokens);
     return (uint32_t)std::min<uint64_t>(kBlocks, tiles * kv_heads * steps_of(max_len));
 }
 
 // Where everything lies in the workspace: the partials of this file's kernel, then what the
 // other one uses.
 struct Layout {
-    uint32_t       runs;
-    size_t         ml, cut, other, bytes;
+    uint32_t       few, more;  // runs
+    size_t         at[2][3];   // offsets of their sums, (maximum, sum) pairs, pieces
+    size_t         other, bytes;
     UnpackedLayout u;
 };
 
@@ -556,14 +620,25 @@ Layout layout(const w8a8_kv4_cache& c, uint32_t seqs, uint32_t tokens, uint32_t 
               uint32_t table_cols, uint32_t max_new)
 {
     Layout         w{};
-    const uint32_t max_len = table_cols * c.page_size;
-    w.runs                 = run_count(seqs, tokens, heads, c.kv_heads, max_len);
-    if(steps_of(max_len) > 1) { // else no unit is cut
-        const size_t slots = (size_t)w.runs * 2 * kRows;
-        w.ml               = slots * c.head_dim * 4;
-        w.cut              = w.ml + slots * 8;
-        w.other            = (w.cut + w.runs * sizeof(Piece) + 255) / 256 * 256;
-    }
+    const uint32_t max_len = table_cols * c.page_size, per = heads / c.kv_heads;
+    const uint32_t most    = std::min(seqs, tokens); // sequences with new tokens
+    w.few                  = run_count(most, c.kv_heads, max_len);
+    if((uint64_t)std::min(max_new, tokens) * per > 32)
+        w.more = run_count((uint64_t)tokens * per / 64 + most, c.kv_heads, max_len);
+    size_t     at   = 0;
+    const auto room = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    if(steps_of(max_len) > 1) // else no unit is cut
+        for(int i = 0; i < 2; ++i) {
+            const size_t runs = i == 0 ? w.few : w.more, rows = runs * 2 * (i == 0 ? 32 : 64);
+            w.at[i][0]        = room(rows * c.head_dim * 4);
+            w.at[i][1]        = room(rows * 8);
+            w.at[i][2]        = room(runs * sizeof(Piece));
+        }
+    w.other = at;
     w.u     = unpacked_layout(c, seqs, tokens, heads, table_cols, max_new);
     w.bytes = w.other + w.u.bytes;
     return w;
@@ -584,12 +659,15 @@ hipError_t launch_attention_kv4_chunks(const w8a8_kv4_cache& c, const ChunkArgs&
 {
     const Layout w  = layout(c, a.seqs, a.tokens, a.heads, a.table_cols, a.max_new);
     auto*        ws = static_cast<uint8_t*>(a.ws);
-    Runs         runs{};
-    runs.count = w.runs;
-    if(w.cut != 0) {
-        runs.o   = reinterpret_cast<float*>(ws);
-        runs.ml  = reinterpret_cast<float*>(ws + w.ml);
-        runs.cut = reinterpret_cast<Piece*>(ws + w.cut);
+    const bool   cut = w.other != 0;
+    Runs         runs[2]{};
+    for(int i = 0; i < 2; ++i) {
+        runs[i].count = i == 0 ? w.few : w.more;
+        if(cut) {
+            runs[i].o   = reinterpret_cast<float*>(ws + w.at[i][0]);
+            runs[i].ml  = reinterpret_cast<float*>(ws + w.at[i][1]);
+            runs[i].cut = reinterpret_cast<Piece*>(ws + w.at[i][2]);
+        }
     }
     const uint8_t* others = nullptr;
     if(w.u.bytes != 0) {
@@ -597,12 +675,16 @@ hipError_t launch_attention_kv4_chunks(const w8a8_kv4_cache& c, const ChunkArgs&
         others = ws + w.other + w.u.flags;
     }
     with_widths(c, [&](auto d, auto g) {
-        attention_kv4_chunks_kernel<d(), g()>
-            <<<runs.count, kThreads, 0, stream>>>(view(c), a, runs, others, c.pages);
-        if(runs.cut)
+        const auto kernel = w.more != 0 ? attention_kv4_chunks_kernel<d(), g(), true>
+                                        : attention_kv4_chunks_kernel<d(), g(), false>;
+        kernel<<<std::max(w.few, w.more), kThreads, 0, stream>>>(view(c), a, runs[0], runs[1],
+                                                                others, c.pages);
+        if(cut) {
+            const uint32_t tasks = (w.few * 32 + w.more * 64) / (kWave / (d() / 8));
             attention_kv4_chunks_join_kernel<d()>
-                <<<std::min(runs.count * kRows / kWaves, 1024u), kThreads, 0, stream>>>(
-                    a, runs, a.heads / c.kv_heads);
+                <<<std::min((tasks + kWaves - 1) / kWaves, 1024u), kThreads, 0, stream>>>(
+                    a, runs[0], runs[1], a.heads / c.kv_heads);
+        }
     });
     return hipGetLastError();
 }

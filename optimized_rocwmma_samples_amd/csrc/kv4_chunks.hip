@@ -123,9 +123,81 @@ struct Place {
     Chunk    c;
 };
 
+// A block's run: which steps of the line it takes, and where the first of them lies.
+struct Line {
+    uint32_t q, r;      // runs have q steps, the first r of them one more
+    uint32_t left, end; // its steps, and the place on the line behind the last
+    uint32_t seq, at;   // the first one's sequence, and place in it
+};
+
+// What the launch's blocks are given, and the sequences' ways.
+struct Ways {
+    const uint8_t* others; // [seqs] 1: unpacked first; or null
+    uint32_t       per, most;
+
+    // 32-row tiles a unit; 0: not this kernel's
+    __device__ uint32_t kind(const ChunkArgs& a, const Chunk& x, uint32_t i) const
+    {
+        if(x.fresh == 0 || (others != nullptr && others[i] != 0)) return 0;
+        return x.fresh * per > 32 ? 2 : 1;
+    }
+};
+
+__device__ __forceinline__ uint32_t unit_tiles(const Chunk& x, uint32_t per, uint32_t kind)
+{
+    return (x.fresh * per + 32 * kind - 1) / (32 * kind);
+}
+
+// Run `run` of `runs` on the line of the sequences whose units are T tiles of 32 rows.
+template <int T>
+__device__ __forceinline__ Line find_line(const ChunkArgs& a, const Ways& w, uint32_t kv_heads,
+                                          uint32_t run, uint32_t runs)
+{
+    const uint32_t lane = threadIdx.x % kWave;
+    uint32_t       n, s;
+    const auto     scan = [&](uint32_t i0) { // 64 sequences' steps
+        const uint32_t i = i0 + lane;
+        n                = 0;
+        if(i < a.seqs) {
+            const Chunk x = chunk_of(a, i, w.most);
+            if(w.kind(a, x, i) == T) n = unit_tiles(x, w.per, T) * kv_heads * steps_of(x.len);
+        }
+        s = lanes_sum(n);
+        return (uint32_t)__builtin_amdgcn_readlane((int)s, kWave - 1);
+    };
+    float    total = 0.f; // starts that do not ascend may count rows so often that sums wrap
+    uint32_t all   = 0;
+    for(uint32_t i = 0; i < a.seqs; i += kWave) {
+        all += scan(i);
+        total += wave_sum((float)n);
+    }
+    if(total > 2147483648.f) all = 0;
+    Line l;
+    l.q         = all / runs;
+    l.r         = all % runs;
+    uint32_t at = run * l.q + min(run, l.r);
+    l.left      = l.q + (run < l.r ? 1 : 0);
+    l.end       = at + l.left;
+    l.seq = l.at = 0;
+    if(l.left == 0) return l;
+    for(uint32_t i = 0; i < a.seqs; i += kWave) {
+        const uint32_t sum // (of up to 64 sequences it is still there)
+            = a.seqs > kWave ? scan(i) : (uint32_t)__builtin_amdgcn_readlane((int)s, kWave - 1);
+        if(at < sum) {
+            const int f = __builtin_ctzll(__ballot(s > at));
+            l.at = at - ((uint32_t)__builtin_amdgcn_readlane((int)s, f)
+                         - (uint32_t)__builtin_amdgcn_readlane((int)n, f));
+            l.seq = i + f;
+            break;
+        }
+        at -= sum;
+    }
+    return l;
+}
+
 template <int D, int G, int T>
 __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& a, const Runs& runs,
-                                           const uint8_t* others, uint32_t pages,
+                                           const Ways& ways, uint32_t run, uint32_t pages,
                                            uint8_t* lds, float* lds_ml)
 {
     using R = Raw<D, G>;
@@ -134,67 +206,27 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
     constexpr uint32_t kRows = 32 * T;             // rows of a unit
     const int      wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int      lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
-    const uint32_t run = blockIdx.x;
-    const uint32_t per = a.heads / c.kv_heads, most = a.table_cols << c.page_shift;
-    // LDS: the waves' values (at a unit's end two waves' results), then the queries
+    const uint32_t per = ways.per;
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds, tile = lds0 + wave * kTile;
     const uint32_t qat = lds0 + kWaves * kTile + lane * 16;
-    auto           chunk_at = [&](uint32_t i) { // without rows where they go another way
-        Chunk x = chunk_of(a, i, most);
-        if(others != nullptr && others[i] != 0) x.fresh = 0;
-        if((x.fresh * per > 32) != (T > 1)) x.fresh = 0;
-        return x;
-    };
-    auto           tiles_of = [&](const Chunk& s) { return (s.fresh * per + kRows - 1) / kRows; };
 
-    // ---- the block's run ---------------------------------------------------------------
-    // (in 64 bits: starts that do not ascend may count rows many times)
-    auto scan = [&](uint32_t i0, uint32_t& n, uint64_t& s) { // 64 sequences' steps
-        const uint32_t i = i0 + lane;
-        n                = 0;
-        if(i < a.seqs) {
-            const Chunk x = chunk_at(i);
-            n             = tiles_of(x) * c.kv_heads * steps_of(x.len);
-        }
-        s = n;
-#pragma unroll
-        for(int d = 1; d < kWave; d <<= 1) {
-            const uint64_t o = __shfl_up((unsigned long long)s, d, kWave);
-            if(lane >= d) s += o;
-        }
-        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)s, kWave - 1)
-               | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(s >> 32), kWave - 1)
-                     << 32;
-    };
-    uint32_t n;
-    uint64_t s, all = 0;
-    for(uint32_t i = 0; i < a.seqs; i += kWave) all += scan(i, n, s);
-    if(all > 0x7FFFFFFFull) all = 0;
-    const uint32_t q = (uint32_t)all / runs.count, r = (uint32_t)all % runs.count;
-    uint32_t       at = run * q + min(run, r), left = q + (run < r ? 1 : 0);
-    if(runs.cut && threadIdx.x == 0) runs.cut[run].last = 0;
-    if(left == 0) return;
-    const uint32_t end = at + left;
-    Place          here{};
-    for(uint32_t i = 0; i < a.seqs; i += kWave) {
-        const uint32_t sum = (uint32_t)scan(i, n, s);
-        if(at < sum) {
-            const int f = __builtin_ctzll(__ballot(s > at));
-            at -= (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)s, f)
-                  - (uint32_t)__builtin_amdgcn_readlane((int)n, f);
-            here.seq = i + f;
-            break;
-        }
-        at -= sum;
+    const Line line = find_line<T>(a, ways, c.kv_heads, run, runs.count);
+    uint32_t   tasks = 0; // that the join has with what this run cuts
+    if(line.left == 0) {
+        if(runs.cut && threadIdx.x == 0) runs.tasks[run] = 0;
+        return;
     }
-    auto enter = [&](Place& p) { // the sequence p.seq
-        p.c     = chunk_at(p.seq);
+    uint32_t   left  = line.left;
+    const auto enter = [&](Place& p) { // the sequence p.seq
+        p.c     = chunk_of(a, p.seq, ways.most);
         p.steps = steps_of(p.c.len);
-        p.tiles = tiles_of(p.c);
+        p.tiles = ways.kind(a, p.c, p.seq) == T ? unit_tiles(p.c, per, T) : 0;
     };
+    Place here{};
+    here.seq = line.seq;
     enter(here);
-    here.unit = at / here.steps;
-    here.step = at % here.steps;
+    here.unit = line.at / here.steps;
+    here.step = line.at % here.steps;
     auto advance = [&](Place& p) { // to the next step, whichever unit's; not past the run
         if(++p.step != p.steps) return;
         p.step = 0;
@@ -232,13 +264,13 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
 
     // ---- the queries, in LDS as the products take them: [32 rows][product][lane] ---------
     uint32_t   sees[T] = {}, least = 0; // keys the lane's rows see, and the unit's first row
-    const auto queries = [&](const Place& p) {
+    v8h        qv[T][kSteps / kWaves];  // this wave's share of them on their way
+    const auto fetch_queries = [&](const Place& p) {
         const uint32_t row0 = p.unit % p.tiles * kRows, rows = p.c.fresh * per;
         auto           seen = [&](uint32_t row) {
             return (uint32_t)max((int32_t)(p.c.len + row / per + 1 - p.c.fresh), 0);
         };
-        constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-        least                   = seen(row0);
+        least = seen(row0);
 #pragma unroll
         for(int t = 0; t < T; ++t) {
             const uint32_t row = min(row0 + 32 * t + col, rows - 1);
@@ -246,15 +278,23 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
             const uint16_t* from = a.q + (size_t)(p.c.begin + row / per) * a.ldq
                                    + (size_t)(p.unit / p.tiles * per + row % per) * D + 8 * half;
 #pragma unroll
-            for(int st = wave; st < kSteps; st += kWaves) {
-                const v8h v = *reinterpret_cast<const v8h*>(from + 16 * st);
-                v8h       u;
+            for(int i = 0; i < kSteps / kWaves; ++i)
+                qv[t][i] = *reinterpret_cast<const v8h*>(from + 16 * (wave + i * kWaves));
+        }
+    };
+    const auto keep_queries = [&] {
+        constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 #pragma unroll
-                for(int e = 0; e < 8; ++e) u[e] = v[kOrder[e]];
-                *(lds_v4i_t*)(uintptr_t)(qat + (t * kSteps + st) * kWave * 16)
+        for(int t = 0; t < T; ++t)
+#pragma unroll
+            for(int i = 0; i < kSteps / kWaves; ++i) {
+                v8h u;
+#pragma unroll
+                for(int e = 0; e < 8; ++e) u[e] = qv[t][i][kOrder[e]];
+                *(lds_v4i_t*)(uintptr_t)(qat + (t * kSteps + wave + i * kWaves) * kWave * 16)
                     = __builtin_bit_cast(v4i, u);
             }
-        }
+        __syncthreads();
     };
 
     const Unpack unpack;
@@ -282,7 +322,7 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
     Place next = here;
     {
         const int32_t page = page_at(here);
-        queries(here);
+        fetch_queries(here);
         fetch(x, here, page);
     }
     int32_t page_next = -1;
@@ -290,93 +330,87 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
         advance(next);
         page_next = page_at(next);
     }
-    __syncthreads(); // the queries are there
+    keep_queries();
 
-    // The waves' results of 32 rows joined and written, at the unit's end or the run's.
-    auto finish = [&](const int t, const Place& now, bool ends) {
-        const v2f ls = both_halves(l[t]);
-        const float lw = ls[0] + ls[1];
-        if(half == 0) {
-            lds_ml[(wave * 32 + col) * 2]     = m[t];
-            lds_ml[(wave * 32 + col) * 2 + 1] = lw;
-        }
-        __syncthreads();
-        float common = -INFINITY, sum = 0.f;
+    // The waves' results of 32 rows joined and written, at the unit's end or the run's: a half
+    // of them at a time is left in LDS, and each wave adds up a quarter of that.
+    auto finish = [&](const int t, bool ends) {
+        constexpr int kHalf = kBlk * 8, kMine = kBlk * 2; // registers
+        const v2f     ls = both_halves(l[t]);
+        const uint32_t row0 = here.unit % here.tiles * kRows + 32 * t, rows = here.c.fresh * per;
+        const uint32_t row = row0 + col, head0 = here.unit / here.tiles * per;
+        const size_t   slot = (size_t)(2 * run + (from_start ? 1 : 0)) * kRows + 32 * t + col;
+        const bool     done = ends && from_start;
 #pragma unroll
-        for(int w = 0; w < kWaves; ++w) common = fmaxf(common, lds_ml[(w * 32 + col) * 2]);
-        auto weight = [&](float mw) {
-            return mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - common) * c2);
-        };
+        for(int h = 0; h < 2; ++h) {
+            __syncthreads(); // all waves are done with what lies there
+            if(h == 0 && half == 0) {
+                lds_ml[(wave * 32 + col) * 2]     = m[t];
+                lds_ml[(wave * 32 + col) * 2 + 1] = ls[0] + ls[1];
+            }
 #pragma unroll
-        for(int w = 0; w < kWaves; ++w)
-            sum = fmaf(weight(lds_ml[(w * 32 + col) * 2]), lds_ml[(w * 32 + col) * 2 + 1], sum);
-        const float mine = weight(m[t]);
-#pragma unroll
-        for(int b = 0; b < kBlk; ++b) o[t][b] *= mine;
-        // the waves' results added up: 2 and 3 to 0 and 1, then 1 to 0
-#pragma unroll
-        for(int d = 2; d > 0; d /= 2) {
-            const uint32_t buf = lds0 + (wave % d) * (kBlk * 16 * kWave * 4) + lane * 16;
-            if(wave >= d && wave < 2 * d)
-#pragma unroll
-                for(int b = 0; b < kBlk; ++b)
-#pragma unroll
-                    for(int i = 0; i < 16; i += 4)
-                        *(lds_v4f_t*)(uintptr_t)(buf + (b * 4 + i / 4) * kWave * 16)
-                            = v4f{o[t][b][i], o[t][b][i + 1], o[t][b][i + 2], o[t][b][i + 3]};
+            for(int i = 0; i < kHalf; i += 4) {
+                const int at = h * kHalf + i;
+                *(lds_v4f_t*)(uintptr_t)(lds0 + wave * (kHalf * kWave * 4) + i * kWave * 4 + lane * 16)
+                    = v4f{o[t][at / 16][at % 16], o[t][at / 16][at % 16 + 1],
+                          o[t][at / 16][at % 16 + 2], o[t][at / 16][at % 16 + 3]};
+            }
             __syncthreads();
-            if(wave < d)
+            float common = -INFINITY, sum = 0.f;
 #pragma unroll
-                for(int b = 0; b < kBlk; ++b)
+            for(int w = 0; w < kWaves; ++w) common = fmaxf(common, lds_ml[(w * 32 + col) * 2]);
+            float r[kMine];
 #pragma unroll
-                    for(int i = 0; i < 16; i += 4) {
-                        const v4f u
-                            = *(lds_v4f_t*)(uintptr_t)(buf + (b * 4 + i / 4) * kWave * 16);
+            for(int w = 0; w < kWaves; ++w) {
+                const float mw = lds_ml[(w * 32 + col) * 2];
+                const float f
+                    = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - common) * c2);
+                sum = fmaf(f, lds_ml[(w * 32 + col) * 2 + 1], sum);
 #pragma unroll
-                        for(int e = 0; e < 4; ++e) o[t][b][i + e] += u[e];
-                    }
-            __syncthreads();
-        }
-        if(wave != 0) return;
-        const uint32_t row0 = now.unit % now.tiles * kRows + 32 * t, rows = now.c.fresh * per;
-        const uint32_t row = row0 + col, head0 = now.unit / now.tiles * per;
-        if(ends && from_start) {
-            const float inv = sum != 0.f ? 2.f / sum : 0.f;
-            uint16_t*   out = a.out + (size_t)(now.c.begin + row / per) * a.ldo
-                            + (size_t)(head0 + row % per) * D + 4 * half;
+                for(int i = 0; i < kMine; i += 4) {
+                    const v4f u = *(lds_v4f_t*)(uintptr_t)(lds0 + w * (kHalf * kWave * 4)
+                                                           + (wave * kMine + i) * kWave * 4
+                                                           + lane * 16);
 #pragma unroll
-            for(int b = 0; b < kBlk; ++b)
+                    for(int e = 0; e < 4; ++e)
+                        r[i + e] = w == 0 ? u[e] * f : fmaf(u[e], f, r[i + e]);
+                }
+            }
+            const uint32_t ch0 = 2 * (h * kHalf + wave * kMine) + 4 * half;
+            if(done) {
+                const float inv = sum != 0.f ? 2.f / sum : 0.f;
+                uint16_t*   out = a.out + (size_t)(here.c.begin + row / per) * a.ldo
+                                + (size_t)(head0 + row % per) * D + ch0;
 #pragma unroll
-                for(int i = 0; i < 16; i += 4) {
+                for(int i = 0; i < kMine; i += 4) {
                     // this half has channels 0 1, 4 5 (2 3, 6 7) of a chunk of 8
                     const auto w = __builtin_amdgcn_permlane32_swap(
-                        finite_halves(o[t][b][i] * inv, o[t][b][i + 2] * inv),
-                        finite_halves(o[t][b][i + 1] * inv, o[t][b][i + 3] * inv), false, false);
+                        finite_halves(r[i] * inv, r[i + 2] * inv),
+                        finite_halves(r[i + 1] * inv, r[i + 3] * inv), false, false);
                     if(row < rows)
-                        *reinterpret_cast<v2i*>(out + 32 * b + 8 * (i / 4))
-                            = v2i{(int)w[0], (int)w[1]};
+                        *reinterpret_cast<v2i*>(out + 2 * i) = v2i{(int)w[0], (int)w[1]};
                 }
-        } else if(row < rows) {
-            const size_t slot = (size_t)(2 * run + (from_start ? 1 : 0)) * kRows + 32 * t + col;
+            } else if(row < rows) {
 #pragma unroll
-            for(int b = 0; b < kBlk; ++b)
-#pragma unroll
-                for(int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<v4f*>(runs.o + slot * D + 32 * b + 2 * i + 4 * half)
-                        = v4f{o[t][b][i], o[t][b][i + 1], o[t][b][i + 2], o[t][b][i + 3]};
-            if(half == 0) *reinterpret_cast<v2f*>(runs.ml + slot * 2) = v2f{common * c2, sum};
+                for(int i = 0; i < kMine; i += 4)
+                    *reinterpret_cast<v4f*>(runs.o + slot * D + ch0 + 2 * i)
+                        = v4f{r[i], r[i + 1], r[i + 2], r[i + 3]};
+                if(h == 0 && half == 0 && wave == 0)
+                    *reinterpret_cast<v2f*>(runs.ml + slot * 2) = v2f{common * c2, sum};
+            }
         }
-        if(t == 0 && !ends && from_start && lane == 0) { // goes on behind the run: up to which
-            const uint32_t last = end - 1 + (now.steps - 1 - now.step); // its last step
-            runs.cut[run]       = {(last < r * (q + 1) ? last / (q + 1)
-                                                       : r + (last - r * (q + 1)) / q) + 1,
-                             now.c.begin, row0, rows, head0, {}};
+        if(t == 0 && !ends && from_start && threadIdx.x == 0) { // goes on behind the run
+            const uint32_t last = line.end - 1 + (here.steps - 1 - here.step); // its last step
+            const uint32_t q = line.q, r1 = line.r;
+            const uint32_t to
+                = last < r1 * (q + 1) ? last / (q + 1) : r1 + (last - r1 * (q + 1)) / q;
+            runs.cut[run] = {to + 1, here.c.begin, row0, rows, head0, {}};
+            tasks         = join_tasks<D>(to + 1 - run, min(kRows, rows - row0));
         }
     };
 
     for(; left > 0; --left) {
-        const Place    now  = here;
-        const uint32_t key0 = now.step * kStep + wave * kKeys;
+        const uint32_t key0 = here.step * kStep + wave * kKeys;
         const uint32_t live = (uint32_t)__ballot(x.ok); // keys that are there
         const bool     full = live == ~0u && key0 + kKeys <= least;
 
@@ -413,13 +447,7 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
                              sc[t]);
         }
         if(left > 1) { // the next step's loads, over the rest of this one
-            const int32_t page = page_next;
-            here               = next;
-            if(left > 2) {
-                advance(next);
-                page_next = page_at(next);
-            }
-            fetch(x, here, page);
+            fetch(x, next, page_next);
         }
         if(!full)
 #pragma unroll
@@ -491,112 +519,205 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
                 }
         }
 
-        const bool ends = now.step + 1 == now.steps;
-        if(!ends && left > 1) continue;
+        const bool ends = here.step + 1 == here.steps;
+        if(ends || left == 1) {
 #pragma unroll
-        for(int t = 0; t < T; ++t) finish(t, now, ends);
-        if(left > 1) { // the next unit
-            from_start = true;
-            begin_unit();
-            queries(here);
+            for(int t = 0; t < T; ++t) finish(t, ends);
             __syncthreads();
         }
+        if(left == 1) break;
+        here = next;
+        if(left > 2) {
+            advance(next);
+            page_next = page_at(next);
+        }
+        if(ends) { // the next unit
+            from_start = true;
+            begin_unit();
+            fetch_queries(here);
+            keep_queries();
+        }
     }
+    if(runs.cut && threadIdx.x == 0) runs.tasks[run] = tasks;
 }
 
-// Sequences of up to 32 rows a key head, then (MORE: there may be any) those of more, two
-// times 32 rows a unit, which unpacks its codes once for both.
+// Blocks for the sequences of more than 32 rows a key head (MORE: there may be any), two times
+// 32 rows a unit, which unpacks its codes once for both, then for those of up to 32.
 template <int D, int G, bool MORE>
 __global__ void __launch_bounds__(kThreads, 2)
     attention_kv4_chunks_kernel(CacheView c, ChunkArgs a, Runs few, Runs more,
                                 const uint8_t* others, uint32_t pages)
 {
+    // the waves' values (at a unit's end halves of their results), then the queries
     __shared__ alignas(256) uint8_t lds[kWaves * kKeys * D * 2 + (MORE ? 64 : 32) * D * 2];
     __shared__ float                ml[kWaves * 32 * 2];
-    if(blockIdx.x < few.count) chunks_run<D, G, 1>(c, a, few, others, pages, lds, ml);
-    if constexpr(MORE) {
-        __syncthreads();
-        if(blockIdx.x < more.count) chunks_run<D, G, 2>(c, a, more, others, pages, lds, ml);
-    }
+    const Ways     ways{others, a.heads / c.kv_heads, a.table_cols << c.page_shift};
+    if(!MORE || blockIdx.x >= more.count)
+        chunks_run<D, G, 1>(c, a, few, ways, blockIdx.x - (MORE ? more.count : 0), pages, lds, ml);
+    else if constexpr(MORE)
+        chunks_run<D, G, 2>(c, a, more, ways, blockIdx.x, pages, lds, ml);
 }
 
+// ---- the join ---------------------------------------------------------------------------
+// What the cut units of one kernel's runs look like: `members` blocks a run (else 1), each of
+// which has `rows` rows of a unit: of `heads` query heads and then of neighbouring rows.
+struct JoinSet {
+    Runs     runs;
+    uint32_t members, heads, rows;
+    uint32_t per;     // query heads that a sequence's rows go round
+    uint32_t first;   // entry of its first run
+    float    unit;    // of the sums of p v
+    bool     natural; // their channels in order, else in the codes' order
+};
+constexpr uint32_t kJoinMost = 2 * kBlocks + kUnpackedBlocks; // entries at the most
+
+struct JoinSets {
+    JoinSet         set[3];
+    const uint32_t* tasks; // of each entry
+    uint32_t        entries;
+};
+
 // Joins the partials of the cut units: the second slot of the run a unit begins in, then the
-// first ones of the runs after it.  A wave has 4 rows, lanes being 8 channels each.  Few
-// partials are taken by all four rows' lanes at once, each its own; of many a row at a time,
-// its lanes each every fourth, then the four are added up, in the same order always.
+// first ones of the runs after it.  Every block adds up by itself how many tasks the runs'
+// cut units make, and takes its share of them.  Lanes are 8 channels each.  Of few partials a
+// task is 32 (64) rows, two a group of lanes; of many one row, of which each group takes every
+// 16th (32nd) partial, and the groups are added up, always in the same order.
 template <int D>
-__global__ void __launch_bounds__(kThreads)
-    attention_kv4_chunks_join_kernel(ChunkArgs a, Runs few, Runs more, uint32_t per)
+__global__ void __launch_bounds__(kThreads) attention_kv4_chunks_join_kernel(ChunkArgs a, JoinSets j)
 {
-    constexpr uint32_t kLanes = D / 8, kWays = kWave / kLanes, kMany = 16;
-    const uint32_t     lane = threadIdx.x % kWave, ch = lane % kLanes, way = lane / kLanes;
-    const uint32_t     first = few.count * (32 / kWays), all = first + more.count * (64 / kWays);
-    for(uint32_t task = blockIdx.x * kWaves + threadIdx.x / kWave; task < all;
-        task += gridDim.x * kWaves) {
-        const bool     is_few = task < first;
-        const Runs&    runs   = is_few ? few : more;
-        const uint32_t rows = is_few ? 32 : 64, of = is_few ? task : task - first;
-        const uint32_t run  = __builtin_amdgcn_readfirstlane(of / (rows / kWays));
-        const uint32_t in0  = of % (rows / kWays) * kWays;
-        const Piece    u    = runs.cut[run];
-        if(u.last == 0 || u.row0 + in0 >= u.rows) continue;
-        const uint32_t n = u.last - run; // partials
-        float          m, l, sum[8];
-        auto           clear = [&] {
-            m = -INFINITY;
-            l = 0.f;
+    constexpr uint32_t kLanes = D / 8, kGroups = kThreads / kLanes;
+    constexpr uint32_t kEach = (kJoinMost + kThreads - 1) / kThreads;
+    static_assert(kJoinRows<D> == 2 * kGroups, "two rows a group");
+    __shared__ uint32_t  before[kEach * kThreads], part[kWaves];
+    __shared__ float     weights[kGroups][2];
+    __shared__ alignas(16) float sums[kGroups][kLanes][8];
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const uint32_t ch = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+
+    // ---- how many tasks come before each entry -----------------------------------------
+    uint32_t mine[kEach], all = 0;
 #pragma unroll
-            for(int y = 0; y < 8; ++y) sum[y] = 0.f;
-        };
-        auto take = [&](float mi, float li, const float* v) { // -inf: no key seen
-            const float now = fmaxf(m, mi);
-            const float al  = m == now ? 1.f : __builtin_amdgcn_exp2f(m - now);
-            const float e   = mi == -INFINITY ? 0.f : mi == now ? 1.f : __builtin_amdgcn_exp2f(mi - now);
-            m               = now;
-            l               = fmaf(l, al, mi == -INFINITY ? li : e * li); // 0, or NaN
-            if(e != 0.f)
+    for(uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t e = threadIdx.x * kEach + i;
+        mine[i]          = e < j.entries ? j.tasks[e] : 0;
+    }
 #pragma unroll
-                for(int y = 0; y < 8; ++y) sum[y] = fmaf(sum[y], al, e * v[y]);
-        };
-        auto add = [&](uint32_t i, uint32_t in) {
-            const size_t slot = (size_t)(2 * (run + i) + (i == 0 ? 1 : 0)) * rows + in;
-            const v2f    ml   = *reinterpret_cast<const v2f*>(runs.ml + slot * 2);
-            const v4f*   v    = reinterpret_cast<const v4f*>(runs.o + slot * D + ch * 8);
-            const v4f    v0 = v[0], v1 = v[1];
-            const float  both[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-            take(ml[0], ml[1], both);
-        };
-        auto write = [&](uint32_t in) {
-            const uint32_t row = u.row0 + in;
-            const float    inv = l != 0.f ? 2.f / l : 0.f;
+    for(uint32_t i = 0; i < kEach; ++i) all += mine[i];
+    const uint32_t s = lanes_sum(all);
+    if(lane == kWave - 1) part[wave] = s;
+    __syncthreads();
+    uint32_t at = s - all, total = 0;
 #pragma unroll
-            for(int y = 0; y < 8; ++y) sum[y] *= inv;
-            // places 0 .. 7 are channels 0 4 1 5 2 6 3 7
-            if(row < u.rows)
-                *reinterpret_cast<v4i*>(a.out + (size_t)(u.token + row / per) * a.ldo
-                                        + (size_t)(u.head + row % per) * D + ch * 8)
-                    = v4i{(int)finite_halves(sum[0], sum[2]), (int)finite_halves(sum[4], sum[6]),
-                          (int)finite_halves(sum[1], sum[3]), (int)finite_halves(sum[5], sum[7])};
-        };
-        if(n <= kMany) {
-            clear();
-            const uint32_t in = min(in0 + way, u.rows - 1 - u.row0);
-            for(uint32_t i = 0; i < n; ++i) add(i, in);
-            write(in0 + way);
-            continue;
+    for(uint32_t w = 0; w < kWaves; ++w) {
+        if(w < wave) at += part[w];
+        total += part[w];
+    }
+#pragma unroll
+    for(uint32_t i = 0; i < kEach; ++i) {
+        before[threadIdx.x * kEach + i] = at;
+        at += mine[i];
+    }
+    __syncthreads();
+
+    for(uint32_t task = blockIdx.x; task < total; task += gridDim.x) {
+        uint32_t lo = 0, hi = kEach * kThreads; // before[lo] <= task < before[hi]
+        while(hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if(before[mid] <= task)
+                lo = mid;
+            else
+                hi = mid;
         }
-        for(uint32_t y = 0; y < kWays && u.row0 + in0 + y < u.rows; ++y) {
-            clear();
-            for(uint32_t i = way; i < n; i += kWays) add(i, in0 + y);
+        lo                     = __builtin_amdgcn_readfirstlane(lo);
+        const uint32_t which   = lo < j.set[1].first ? 0 : lo < j.set[2].first ? 1 : 2;
+        const JoinSet& set     = j.set[which];
+        const uint32_t run     = (lo - set.first) / set.members;
+        const uint32_t member  = (lo - set.first) % set.members;
+        const Piece    p       = set.runs.cut[run];
+        const uint32_t row0    = p.row0 + member / set.heads * set.rows;
+        const uint32_t live    = min(set.rows, p.rows - row0);
+        const uint32_t n       = p.last - run; // partials
+        const bool     many    = n > kJoinMany;
+        const uint32_t of      = task - before[lo];
+        uint32_t       in[2]   = {many ? of : of * kJoinRows<D> + group, 0};
+        in[1]                  = many ? live : in[0] + kGroups; // its rows of the member's
+        float      m[2] = {-INFINITY, -INFINITY}, l[2] = {}, sum[2][8] = {};
+        const auto take = [&](int y, float mi, float li, const float* v) { // -inf: no key seen
+            const float now = fmaxf(m[y], mi);
+            const float al  = m[y] == now ? 1.f : __builtin_amdgcn_exp2f(m[y] - now);
+            const float w
+                = mi == -INFINITY ? 0.f : mi == now ? 1.f : __builtin_amdgcn_exp2f(mi - now);
+            m[y] = now;
+            l[y] = fmaf(l[y], al, mi == -INFINITY ? li : w * li); // 0, or NaN
+            if(mi != -INFINITY)
 #pragma unroll
-            for(uint32_t d = kLanes; d < kWave; d <<= 1) {
-                const float mo = __shfl_xor(m, d, kWave), lo = __shfl_xor(l, d, kWave);
-                float       vo[8];
+                for(int z = 0; z < 8; ++z) sum[y][z] = fmaf(sum[y][z], al, w * v[z]);
+        };
+        const uint32_t step = many ? kGroups : 1;
+        for(uint32_t i0 = many ? group : 0; i0 < n; i0 += 2 * step) {
+            v2f ml[2][2];
+            v4f v[2][2][2];
 #pragma unroll
-                for(int z = 0; z < 8; ++z) vo[z] = __shfl_xor(sum[z], d, kWave);
-                take(mo, lo, vo);
+            for(int x = 0; x < 2; ++x)
+#pragma unroll
+                for(int y = 0; y < 2; ++y) {
+                    const uint32_t i = min(i0 + x * step, n - 1);
+                    const size_t   slot
+                        = ((size_t)(2 * (run + i) + (i == 0 ? 1 : 0)) * set.members + member)
+                              * set.rows
+                          + min(in[y], live - 1);
+                    const v4f* from = reinterpret_cast<const v4f*>(set.runs.o + slot * D + ch * 8);
+                    ml[x][y]   = *reinterpret_cast<const v2f*>(set.runs.ml + slot * 2);
+                    v[x][y][0] = from[0];
+                    v[x][y][1] = from[1];
+                }
+#pragma unroll
+            for(int x = 0; x < 2; ++x) {
+                if(i0 + x * step >= n) continue;
+#pragma unroll
+                for(int y = 0; y < 2; ++y) {
+                    const v4f   u0 = v[x][y][0], u1 = v[x][y][1];
+                    const float w[8] = {u0[0], u0[1], u0[2], u0[3], u1[0], u1[1], u1[2], u1[3]};
+                    take(y, ml[x][y][0], ml[x][y][1], w);
+                }
             }
-            if(way == 0) write(in0 + y);
+        }
+        if(many) { // the groups' parts, one after the other
+            __syncthreads();
+            if(ch == 0) {
+                weights[group][0] = m[0];
+                weights[group][1] = l[0];
+            }
+#pragma unroll
+            for(int z = 0; z < 8; z += 4)
+                *reinterpret_cast<v4f*>(&sums[group][ch][z])
+                    = v4f{sum[0][z], sum[0][z + 1], sum[0][z + 2], sum[0][z + 3]};
+            __syncthreads();
+            if(group == 0)
+                for(uint32_t g = 1; g < kGroups; ++g)
+                    take(0, weights[g][0], weights[g][1], sums[g][ch]);
+            else
+                in[0] = live;
+        }
+#pragma unroll
+        for(int y = 0; y < 2; ++y) {
+            if(in[y] >= live) continue;
+            const float inv = l[y] != 0.f ? set.unit / l[y] : 0.f;
+            float       r[8];
+#pragma unroll
+            for(int z = 0; z < 8; ++z) r[z] = sum[y][z] * inv;
+            const uint32_t row = row0 + in[y];
+            // the codes' order: places 0 .. 7 are channels 0 4 1 5 2 6 3 7
+            const v4i w
+                = set.natural
+                      ? v4i{(int)finite_halves(r[0], r[1]), (int)finite_halves(r[2], r[3]),
+                            (int)finite_halves(r[4], r[5]), (int)finite_halves(r[6], r[7])}
+                      : v4i{(int)finite_halves(r[0], r[2]), (int)finite_halves(r[4], r[6]),
+                            (int)finite_halves(r[1], r[3]), (int)finite_halves(r[5], r[7])};
+            *reinterpret_cast<v4i*>(a.out + (size_t)(p.token + row / set.per) * a.ldo
+                                    + (size_t)(p.head + row % set.per + member % set.heads) * D
+                                    + ch * 8)
+                = w;
         }
     }
 }
@@ -612,7 +733,7 @@ uint32_t run_count(uint64_t tiles, uint32_t kv_heads, uint32_t max_len)
 struct Layout {
     uint32_t       few, more;  // runs
     size_t         at[2][3];   // offsets of their sums, (maximum, sum) pairs, pieces
-    size_t         other, bytes;
+    size_t         tasks, other, bytes;
     UnpackedLayout u;
 };
 
@@ -631,16 +752,18 @@ Layout layout(const w8a8_kv4_cache& c, uint32_t seqs, uint32_t tokens, uint32_t 
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    if(steps_of(max_len) > 1) // else no unit is cut
+    w.u = unpacked_layout(c, seqs, tokens, heads, table_cols, max_new);
+    if(steps_of(max_len) > 1 || w.u.bytes != 0) { // else no unit is cut
+        w.tasks = room(kJoinMost * 4);
         for(int i = 0; i < 2; ++i) {
             const size_t runs = i == 0 ? w.few : w.more, rows = runs * 2 * (i == 0 ? 32 : 64);
             w.at[i][0]        = room(rows * c.head_dim * 4);
             w.at[i][1]        = room(rows * 8);
             w.at[i][2]        = room(runs * sizeof(Piece));
         }
+    }
     w.other = at;
-    w.u     = unpacked_layout(c, seqs, tokens, heads, table_cols, max_new);
-    w.bytes = w.other + w.u.bytes;
+    w.bytes = at + w.u.bytes;
     return w;
 }
 
@@ -659,32 +782,42 @@ hipError_t launch_attention_kv4_chunks(const w8a8_kv4_cache& c, const ChunkArgs&
 {
     const Layout w  = layout(c, a.seqs, a.tokens, a.heads, a.table_cols, a.max_new);
     auto*        ws = static_cast<uint8_t*>(a.ws);
-    const bool   cut = w.other != 0;
-    Runs         runs[2]{};
+    const bool     cut   = w.other != 0;
+    const uint32_t per   = a.heads / c.kv_heads;
+    auto*          tasks = reinterpret_cast<uint32_t*>(ws + w.tasks);
+    Runs           runs[2]{};
     for(int i = 0; i < 2; ++i) {
         runs[i].count = i == 0 ? w.few : w.more;
         if(cut) {
-            runs[i].o   = reinterpret_cast<float*>(ws + w.at[i][0]);
-            runs[i].ml  = reinterpret_cast<float*>(ws + w.at[i][1]);
-            runs[i].cut = reinterpret_cast<Piece*>(ws + w.at[i][2]);
+            runs[i].o     = reinterpret_cast<float*>(ws + w.at[i][0]);
+            runs[i].ml    = reinterpret_cast<float*>(ws + w.at[i][1]);
+            runs[i].cut   = reinterpret_cast<Piece*>(ws + w.at[i][2]);
+            runs[i].tasks = tasks + i * w.few;
         }
     }
+    const uint32_t both = w.few + w.more;
+    JoinSets       sets{{{runs[0], 1, 1, 32, per, 0, 2.f, false},
+                   {runs[1], 1, 1, 64, per, w.few, 2.f, false},
+                   {{}, 1, 1, 1, 1, both, 1.f, true}},
+                  tasks,
+                  both};
     const uint8_t* others = nullptr;
     if(w.u.bytes != 0) {
-        launch_unpacked(c, a, w.u, ws + w.other, stream);
-        others = ws + w.other + w.u.flags;
+        const Runs r = unpacked_runs(w.u, ws + w.other, tasks + both);
+        launch_unpacked(c, a, w.u, r, ws + w.other, stream);
+        others      = ws + w.other + w.u.flags;
+        sets.set[2] = {r, w.u.members, w.u.heads, 128, 1, both, 1.f, true};
+        sets.entries += w.u.runs * w.u.members;
     }
+    // a task is at least a row, and mostly more
+    const uint32_t joins = (uint32_t)std::min<uint64_t>((uint64_t)a.tokens * a.heads, 1024);
     with_widths(c, [&](auto d, auto g) {
         const auto kernel = w.more != 0 ? attention_kv4_chunks_kernel<d(), g(), true>
                                         : attention_kv4_chunks_kernel<d(), g(), false>;
-        kernel<<<std::max(w.few, w.more), kThreads, 0, stream>>>(view(c), a, runs[0], runs[1],
-                                                                others, c.pages);
-        if(cut) {
-            const uint32_t tasks = (w.few * 32 + w.more * 64) / (kWave / (d() / 8));
-            attention_kv4_chunks_join_kernel<d()>
-                <<<std::min((tasks + kWaves - 1) / kWaves, 1024u), kThreads, 0, stream>>>(
-                    a, runs[0], runs[1], a.heads / c.kv_heads);
-        }
+        kernel<<<w.few + w.more, kThreads, 0, stream>>>(view(c), a, runs[0], runs[1], others,
+                                                       c.pages);
+        if(cut)
+            attention_kv4_chunks_join_kernel<d()><<<joins, kThreads, 0, stream>>>(a, sets);
     });
     return hipGetLastError();
 }

@@ -42,6 +42,25 @@ struct LongList {
     uint8_t*  flags; // [seqs] 1: in the list
 };
 
+} // namespace
+
+// v and the sum of v over the lanes before.
+__device__ __forceinline__ uint32_t lanes_sum(uint32_t v)
+{
+    const auto add = [&](auto ctrl, auto rows) {
+        v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value,
+                                                   decltype(rows)::value, 0xF, false);
+    };
+    using std::integral_constant;
+    add(integral_constant<int, 0x111>(), integral_constant<int, 0xF>()); // from 1, 2, 4, 8 lanes
+    add(integral_constant<int, 0x112>(), integral_constant<int, 0xF>()); // before, in rows of 16
+    add(integral_constant<int, 0x114>(), integral_constant<int, 0xF>());
+    add(integral_constant<int, 0x118>(), integral_constant<int, 0xF>());
+    add(integral_constant<int, 0x142>(), integral_constant<int, 0xA>()); // the row before's last
+    add(integral_constant<int, 0x143>(), integral_constant<int, 0xC>()); // lane 31's
+    return v;
+}
+
 // What the join needs of a unit that goes on behind the run it begins in.
 struct Piece {
     uint32_t last;  // run that has its last step, plus 1; 0: no such unit
@@ -51,6 +70,17 @@ struct Piece {
     uint32_t unused[3];
 };
 
+// Of so many partials a unit's rows are joined by a block each, else 32 (64) by a block.
+constexpr uint32_t kJoinMany = 16;
+template <int D>
+constexpr uint32_t kJoinRows = 2 * 256 / (D / 8);
+
+template <int D>
+__device__ __forceinline__ uint32_t join_tasks(uint32_t partials, uint32_t rows)
+{
+    return partials > kJoinMany ? rows : (rows + kJoinRows<D> - 1) / kJoinRows<D>;
+}
+
 // Partials: slot 2 r of run r holds a unit that began before it, 2 r + 1 one that begins in it
 // and goes on: fp32 [rows, head_dim], then (maximum, sum) of each row.
 struct Runs {
@@ -58,11 +88,11 @@ struct Runs {
     float*   o;
     float*   ml;
     Piece*   cut;
+    uint32_t* tasks; // the join's with each run's (and block's of it) cut unit
 };
 
-} // namespace
-
 // The kernels over unpacked keys and values (kv4_unpacked.hip).
+constexpr uint32_t kUnpackedBlocks = 3 * 256; // all resident: 3 a CU
 struct UnpackedLayout {
     uint32_t runs, members, heads, tiles; // members = heads x tiles blocks share a run's keys
     uint32_t room, rows;                  // of the list, of unpacked tokens; 0: none
@@ -70,7 +100,12 @@ struct UnpackedLayout {
 };
 UnpackedLayout unpacked_layout(const w8a8_kv4_cache& c, uint32_t seqs, uint32_t tokens,
                                uint32_t heads, uint32_t table_cols, uint32_t max_new);
+inline Runs unpacked_runs(const UnpackedLayout& u, uint8_t* ws, uint32_t* tasks)
+{
+    return {u.runs, reinterpret_cast<float*>(ws + u.o), reinterpret_cast<float*>(ws + u.ml),
+            reinterpret_cast<Piece*>(ws + u.cut), tasks};
+}
 void launch_unpacked(const w8a8_kv4_cache& c, const ChunkArgs& a, const UnpackedLayout& u,
-                     uint8_t* ws, hipStream_t stream);
+                     const Runs& runs, uint8_t* ws, hipStream_t stream);
 
 } // namespace w8a8

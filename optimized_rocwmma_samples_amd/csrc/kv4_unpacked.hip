@@ -20,7 +20,6 @@
 namespace w8a8 {
 namespace {
 
-constexpr uint32_t kResident = 3 * kCus;      // blocks: 3 a CU
 constexpr uint64_t kMostBytes = 1ull << 30;   // of unpacked keys and values
 
 template <int D>
@@ -185,9 +184,12 @@ __global__ void __launch_bounds__(kThreads, 3)
     for(uint32_t i = 0; i < count; i += kWave) all += scan(i, n, s);
     const uint32_t q = all / runs.count, r = all % runs.count;
     uint32_t       at = run * q + min(run, r), left = q + (run < r ? 1 : 0);
-    const bool     writer = member == 0 && threadIdx.x == 0;
-    if(writer) runs.cut[run].last = 0;
-    if(left == 0) return;
+    uint32_t*      tasks = runs.tasks + (size_t)run * gang.members + member;
+    uint32_t       mine  = 0; // the join's tasks with what this block's run cuts
+    if(left == 0) {
+        if(threadIdx.x == 0) *tasks = 0;
+        return;
+    }
     const uint32_t end = at + left;
     uint32_t       which = 0;
     for(uint32_t i = 0; i < count; i += kWave) {
@@ -260,10 +262,12 @@ __global__ void __launch_bounds__(kThreads, 3)
             }
         }
         left -= take;
-        if(writer && !ends && from_start) { // goes on behind the run: up to which one
+        if(!ends && from_start && threadIdx.x == 0) { // goes on behind the run: up to which one
             const uint32_t last = end - 1 + (keys - at - take); // its last key tile
-            runs.cut[run] = {(last < r * (q + 1) ? last / (q + 1) : r + (last - r * (q + 1)) / q) + 1,
-                             x.c.begin, tile * rows, x.c.fresh, head0, {}};
+            const uint32_t to = last < r * (q + 1) ? last / (q + 1) : r + (last - r * (q + 1)) / q;
+            if(member == 0) runs.cut[run] = {to + 1, x.c.begin, tile * rows, x.c.fresh, head0, {}};
+            if(row0 < x.c.fresh)
+                mine = join_tasks<D>(to + 1 - run, min((uint32_t)kRows, x.c.fresh - row0));
         }
         if(left == 0) break;
         at = 0;
@@ -276,54 +280,7 @@ __global__ void __launch_bounds__(kThreads, 3)
         }
         __syncthreads(); // all waves are done with the tiles in LDS
     }
-}
-
-// Joins the partials of the cut units: lanes are 8 channels of a few rows; a wave's rows are of
-// one member's 128.
-template <int D>
-__global__ void __launch_bounds__(kThreads)
-    attention_unpacked_join_kernel(ChunkArgs a, Runs runs, Gang gang)
-{
-    constexpr uint32_t kLanes = D / 8, kRowsWave = kWave / kLanes;
-    const uint32_t     lane = threadIdx.x % kWave, ch = lane % kLanes * 8;
-    const uint32_t     per_run = gang.members * (kRows / kRowsWave);
-    for(uint32_t task = blockIdx.x * kWaves + threadIdx.x / kWave; task < runs.count * per_run;
-        task += gridDim.x * kWaves) {
-        const uint32_t run    = __builtin_amdgcn_readfirstlane(task / per_run);
-        const uint32_t member = task % per_run / (kRows / kRowsWave);
-        const uint32_t row    = task % (kRows / kRowsWave) * kRowsWave + lane / kLanes;
-        const Piece    p      = runs.cut[run];
-        const uint32_t at     = p.row0 + member / gang.heads * kRows + row; // of the sequence's
-        if(p.last == 0 || at >= p.rows) continue;
-        float m = -INFINITY, l = 0.f, sum[8] = {};
-        for(uint32_t i = run; i < p.last; ++i) {
-            const size_t slot = ((size_t)(2 * i + (i == run ? 1 : 0)) * gang.members + member) * kRows
-                                + row;
-            const v2f  ml = *reinterpret_cast<const v2f*>(runs.ml + slot * 2);
-            const v4f* v  = reinterpret_cast<const v4f*>(runs.o + slot * D + ch);
-            const v4f  v0 = v[0], v1 = v[1];
-            // no key seen: its maximum is -inf and its sum 0, or NaN
-            const float now = fmaxf(m, ml[0]);
-            const float al  = m == now ? 1.f : __builtin_amdgcn_exp2f(m - now);
-            const float e   = ml[0] == -INFINITY ? 0.f
-                              : ml[0] == now     ? 1.f
-                                                 : __builtin_amdgcn_exp2f(ml[0] - now);
-            m               = now;
-            l               = fmaf(l, al, e * ml[1]);
-#pragma unroll
-            for(int y = 0; y < 4; ++y) {
-                sum[y]     = fmaf(sum[y], al, e * v0[y]);
-                sum[y + 4] = fmaf(sum[y + 4], al, e * v1[y]);
-            }
-        }
-        const float inv = l != 0.f ? 1.f / l : 0.f;
-        *reinterpret_cast<v4i*>(a.out + (size_t)(p.token + at) * a.ldo
-                                + (size_t)(p.head + member % gang.heads) * D + ch)
-            = v4i{(int)finite_halves(sum[0] * inv, sum[1] * inv),
-                  (int)finite_halves(sum[2] * inv, sum[3] * inv),
-                  (int)finite_halves(sum[4] * inv, sum[5] * inv),
-                  (int)finite_halves(sum[6] * inv, sum[7] * inv)};
-    }
+    if(threadIdx.x == 0) *tasks = mine;
 }
 
 } // namespace
@@ -347,7 +304,7 @@ UnpackedLayout unpacked_layout(const w8a8_kv4_cache& c, uint32_t seqs, uint32_t 
         if(per % h == 0) u.heads = h;
     u.tiles   = u.heads >= 4 ? 1 : 4 / u.heads;
     u.members = u.heads * u.tiles;
-    u.runs    = kResident / 8 / u.members * 8;
+    u.runs    = kUnpackedBlocks / 8 / u.members * 8;
     size_t at   = 0;
     auto   room = [&](size_t bytes) {
         const size_t here = at;
@@ -369,32 +326,23 @@ UnpackedLayout unpacked_layout(const w8a8_kv4_cache& c, uint32_t seqs, uint32_t 
 }
 
 void launch_unpacked(const w8a8_kv4_cache& c, const ChunkArgs& a, const UnpackedLayout& u,
-                     uint8_t* ws, hipStream_t stream)
+                     const Runs& runs, uint8_t* ws, hipStream_t stream)
 {
     const LongList list{u.room, u.rows, reinterpret_cast<uint32_t*>(ws + u.total),
                         reinterpret_cast<Long*>(ws + u.list), ws + u.flags};
     const Unpacked un{reinterpret_cast<uint16_t*>(ws + u.k), reinterpret_cast<uint16_t*>(ws + u.v),
                       reinterpret_cast<uint32_t*>(ws + u.missing)};
-    const Runs     runs{u.runs, reinterpret_cast<float*>(ws + u.o),
-                    reinterpret_cast<float*>(ws + u.ml), reinterpret_cast<Piece*>(ws + u.cut)};
     const Gang     gang{u.members, u.heads, u.tiles};
     const uint32_t keys = 4096 / c.head_dim;
     kv4_long_kernel<<<1, kWave, 0, stream>>>(a, list, a.heads / c.kv_heads,
                                              a.table_cols * c.page_size, keys);
     const uint32_t groups = (uint32_t)std::min<uint64_t>((uint64_t)u.rows / 32 * c.kv_heads, 4096);
-    const uint32_t joins  = std::min(u.runs * u.members * kRows / kWaves, 2048u);
     with_widths(c, [&](auto d, auto g) {
         kv4_unpack_kernel<d(), g()><<<groups, 256, 0, stream>>>(view(c), a, list, un, c.pages);
     });
-    if(c.head_dim == 64) {
-        attention_unpacked_kernel<64>
-            <<<u.runs * u.members, kThreads, 0, stream>>>(a, list, un, runs, gang, c.kv_heads);
-        attention_unpacked_join_kernel<64><<<joins, kThreads, 0, stream>>>(a, runs, gang);
-    } else {
-        attention_unpacked_kernel<128>
-            <<<u.runs * u.members, kThreads, 0, stream>>>(a, list, un, runs, gang, c.kv_heads);
-        attention_unpacked_join_kernel<128><<<joins, kThreads, 0, stream>>>(a, runs, gang);
-    }
+    const auto kernel
+        = c.head_dim == 64 ? attention_unpacked_kernel<64> : attention_unpacked_kernel<128>;
+    kernel<<<u.runs * u.members, kThreads, 0, stream>>>(a, list, un, runs, gang, c.kv_heads);
 }
 
 } // namespace w8a8

@@ -970,9 +970,13 @@ def kv4_load(cache: KV4Cache, slots, out=None):
     return k, v
 
 
-def _kv4_ints(name, t, count: int) -> None:
+def _kv4_ints(dev, name, t, count: int) -> int:
+    # the address of a list of whole numbers
+    if t.device != dev:
+        _require_on(dev, **{name: t})
     if t.dtype != _torch_module.int32 or t.shape != (count,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor [{count}]")
+    return t.data_ptr()
 
 
 def _kv4_table(block_table, seqs: int):
@@ -1021,7 +1025,7 @@ def attention_kv4(q, cache: KV4Cache, block_table, seq_lens, scale: float | None
     else:
         cols, table_ld = _kv4_table(block_table, seqs)
         tables = (cols, table_ld)
-    _kv4_ints("seq_lens", seq_lens, seqs)
+    _kv4_ints(dev, "seq_lens", seq_lens, seqs)
     out, ldo = _heads_out(out, q, seqs, heads, dim)
     _workspace_on(workspace, dev)
     ws, ws_bytes = _workspace(
@@ -1048,33 +1052,27 @@ def kv4_extend(new_tokens, seq_lens, block_table, free_pages, free_count, page_s
     its rows would pass `tokens`, its tokens the table's columns, or where the pages that
     the sequences before it leave are too few.  out: these four; the lengths and the
     count may be seq_lens and free_count themselves."""
-    torch = _torch()
+    _torch()
     _require_cuda(block_table)
     dev = block_table.device
-    _require_on(dev, new_tokens=new_tokens, seq_lens=seq_lens, free_pages=free_pages,
-                free_count=free_count)
     seqs = block_table.shape[0]
     cols, table_ld = _kv4_table(block_table, seqs)
-    _kv4_ints("new_tokens", new_tokens, seqs)
-    _kv4_ints("seq_lens", seq_lens, seqs)
-    _kv4_ints("free_pages", free_pages, free_pages.numel())
-    _kv4_ints("free_count", free_count, 1)
+    args = (_kv4_ints(dev, "new_tokens", new_tokens, seqs),
+            _kv4_ints(dev, "seq_lens", seq_lens, seqs), seqs, block_table.data_ptr(), cols,
+            table_ld, _kv4_ints(dev, "free_pages", free_pages, free_pages.numel()),
+            free_pages.numel(), _kv4_ints(dev, "free_count", free_count, 1), page_size)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
     if out is None:
         new = seq_lens.new_empty
-        slots, starts, lens, count = new(tokens), new(seqs + 1), new(seqs), new(1)
+        out = slots, starts, lens, count = new(tokens), new(seqs + 1), new(seqs), new(1)
+        at = slots.data_ptr(), tokens, starts.data_ptr(), lens.data_ptr(), count.data_ptr()
     else:
         slots, starts, lens, count = out
-        _require_on(dev, slots=slots, starts=starts, lens=lens, count=count)
-        _kv4_ints("slots", slots, tokens)
-        _kv4_ints("starts", starts, seqs + 1)
-        _kv4_ints("lens", lens, seqs)
-        _kv4_ints("count", count, 1)
-    _call_on(dev, "w8a8_kv4_extend", new_tokens.data_ptr(), seq_lens.data_ptr(), seqs,
-             block_table.data_ptr(), cols, table_ld, free_pages.data_ptr(), free_pages.numel(),
-             free_count.data_ptr(), page_size, slots.data_ptr(), tokens, starts.data_ptr(),
-             lens.data_ptr(), count.data_ptr(), _stream(dev))
+        at = (_kv4_ints(dev, "slots", slots, tokens), tokens,
+              _kv4_ints(dev, "starts", starts, seqs + 1), _kv4_ints(dev, "lens", lens, seqs),
+              _kv4_ints(dev, "count", count, 1))
+    _call_on(dev, "w8a8_kv4_extend", *args, *at, _stream(dev))
     return slots, starts, lens, count
 
 
@@ -1086,23 +1084,19 @@ def kv4_trim(keep, seq_lens, block_table, free_pages, free_count, page_size: int
     torch = _torch()
     _require_cuda(block_table)
     dev = block_table.device
-    _require_on(dev, keep=keep, seq_lens=seq_lens, free_pages=free_pages, free_count=free_count)
     seqs = block_table.shape[0]
     cols, table_ld = _kv4_table(block_table, seqs)
-    _kv4_ints("keep", keep, seqs)
-    _kv4_ints("seq_lens", seq_lens, seqs)
-    _kv4_ints("free_pages", free_pages, free_pages.numel())
-    _kv4_ints("free_count", free_count, 1)
+    args = (_kv4_ints(dev, "keep", keep, seqs), _kv4_ints(dev, "seq_lens", seq_lens, seqs), seqs,
+            block_table.data_ptr(), cols, table_ld,
+            _kv4_ints(dev, "free_pages", free_pages, free_pages.numel()), free_pages.numel(),
+            _kv4_ints(dev, "free_count", free_count, 1), page_size)
     if out is None:
         lens, count = torch.empty_like(seq_lens), torch.empty_like(free_count)
+        at = lens.data_ptr(), count.data_ptr()
     else:
         lens, count = out
-        _require_on(dev, lens=lens, count=count)
-        _kv4_ints("lens", lens, seqs)
-        _kv4_ints("count", count, 1)
-    _call_on(dev, "w8a8_kv4_trim", keep.data_ptr(), seq_lens.data_ptr(), seqs,
-             block_table.data_ptr(), cols, table_ld, free_pages.data_ptr(), free_pages.numel(),
-             free_count.data_ptr(), page_size, lens.data_ptr(), count.data_ptr(), _stream(dev))
+        at = _kv4_ints(dev, "lens", lens, seqs), _kv4_ints(dev, "count", count, 1)
+    _call_on(dev, "w8a8_kv4_trim", *args, *at, _stream(dev))
     return lens, count
 
 
@@ -1136,15 +1130,15 @@ def attention_kv4_chunks(q, cache: KV4Cache, block_table, seq_lens, starts,
     new tensor).  max_new: the most new tokens a sequence has, where it is known.
     workspace: 'auto' (allocated here) or a device tensor of
     attention_kv4_chunks_workspace_size bytes, for the same max_new."""
-    torch = _torch()
+    _torch()
     dev = cache.device
-    _require_on(dev, q=q, block_table=block_table, seq_lens=seq_lens, starts=starts, out=out)
+    _require_on(dev, q=q, block_table=block_table, out=out)
     ldq = _heads3d("q", q, None, cache.head_dim)
     tokens, heads, dim = q.shape
     seqs = seq_lens.numel()
     cols, table_ld = _kv4_table(block_table, seqs)
-    _kv4_ints("seq_lens", seq_lens, seqs)
-    _kv4_ints("starts", starts, seqs + 1)
+    lens_at = _kv4_ints(dev, "seq_lens", seq_lens, seqs)
+    starts_at = _kv4_ints(dev, "starts", starts, seqs + 1)
     max_new = 0 if max_new is None else max_new
     if max_new < 0:
         raise ValueError("max_new must not be negative")
@@ -1155,9 +1149,9 @@ def attention_kv4_chunks(q, cache: KV4Cache, block_table, seq_lens, starts,
             cache.pages, cache.page_size, cache.kv_heads, dim, cache.group, seqs, tokens, heads,
             cols, max_new), dev)
     _call_on(dev, "w8a8_attention_kv4_chunks", q.data_ptr(), cache._descriptor(),
-             block_table.data_ptr(), cols, table_ld, seq_lens.data_ptr(), starts.data_ptr(),
-             out.data_ptr(), seqs, tokens, heads, max_new, ldq, ldo,
-             dim ** -0.5 if scale is None else float(scale), _ptr(ws), ws_bytes, _stream(dev))
+             block_table.data_ptr(), cols, table_ld, lens_at, starts_at, out.data_ptr(), seqs,
+             tokens, heads, max_new, ldq, ldo, dim ** -0.5 if scale is None else float(scale),
+             _ptr(ws), ws_bytes, _stream(dev))
     return out
 
 
@@ -1187,7 +1181,8 @@ class KV4PageKeys:
     scales = property(lambda self: self._scales)
 
     def _descriptor(self):
-        if tuple(where() for where in self._where) != self._at:
+        codes, scales = self._where
+        if (codes(), scales()) != self._at:
             raise ValueError("a tensor of the page keys was given other memory: make new "
                              "KV4PageKeys")
         return self._ref
@@ -1208,38 +1203,41 @@ def kv4_summarize(cache: KV4Cache, keys: KV4PageKeys, block_table, seq_lens, sta
     (starts int32 [seqs + 1], ascending; `tokens` rows in all)."""
     _torch()
     dev = cache.device
-    _require_on(dev, block_table=block_table, seq_lens=seq_lens, starts=starts, codes=keys._codes)
+    _require_on(dev, block_table=block_table, codes=keys._codes)
     seqs = seq_lens.numel()
     cols, table_ld = _kv4_table(block_table, seqs)
-    _kv4_ints("seq_lens", seq_lens, seqs)
-    _kv4_ints("starts", starts, seqs + 1)
+    lens_at = _kv4_ints(dev, "seq_lens", seq_lens, seqs)
+    starts_at = _kv4_ints(dev, "starts", starts, seqs + 1)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
     _call_on(dev, "w8a8_kv4_summarize", cache._descriptor(), keys._descriptor(),
-             block_table.data_ptr(), cols, table_ld, seq_lens.data_ptr(), starts.data_ptr(), seqs,
-             tokens, _stream(dev))
+             block_table.data_ptr(), cols, table_ld, lens_at, starts_at, seqs, tokens,
+             _stream(dev))
 
 
 def kv4_page_keys(keys: KV4PageKeys, pages, out=None):
     """Values of page keys: fp32 [n, kv_heads, head_dim] of pages int32 [n].  Rows of pages
     outside are left as they were in `out` (undefined in a new tensor)."""
     torch = _torch()
-    _require_on(keys.device, pages=pages, out=out)
-    n = pages.numel()
-    _kv4_ints("pages", pages, n)
+    dev, n = keys.device, pages.numel()
+    at = _kv4_ints(dev, "pages", pages, n)
     shape = (n, keys.kv_heads, keys.head_dim)
     if out is None:
         out = keys._scales.new_empty(shape)
     else:
+        _require_on(dev, out=out)
         _require("out", out, torch.float32, shape)
-    _call_on(keys.device, "w8a8_kv4_page_keys_load", keys._descriptor(), pages.data_ptr(), n,
-             out.data_ptr(), _stream(keys.device))
+    _call_on(dev, "w8a8_kv4_page_keys_load", keys._descriptor(), at, n, out.data_ptr(),
+             _stream(dev))
     return out
 
 
 def kv4_select_workspace_size(seqs: int, kv_heads: int, columns: int, keep: int) -> int:
     """Bytes of workspace kv4_select needs (0: none)."""
     return int(library().w8a8_kv4_select_workspace_size(seqs, kv_heads, columns, keep))
+
+
+_select_workspace_size = functools.lru_cache(maxsize=64)(kv4_select_workspace_size)
 
 
 def kv4_select(q, keys: KV4PageKeys, block_table, seq_lens, keep: int, page_size: int, out=None,
@@ -1254,11 +1252,11 @@ def kv4_select(q, keys: KV4PageKeys, block_table, seq_lens, keep: int, page_size
     two.  workspace: 'auto' or a device tensor of kv4_select_workspace_size bytes."""
     torch = _torch()
     dev = keys.device
-    _require_on(dev, q=q, block_table=block_table, seq_lens=seq_lens)
+    _require_on(dev, q=q, block_table=block_table)
     ldq = _heads3d("q", q, None, keys.head_dim)
     seqs, heads, _ = q.shape
     cols, table_ld = _kv4_table(block_table, seqs)
-    _kv4_ints("seq_lens", seq_lens, seqs)
+    lens_at = _kv4_ints(dev, "seq_lens", seq_lens, seqs)
     if keep <= 0:
         raise ValueError("keep must be > 0")
     shape = (seqs, keys.kv_heads, keep)
@@ -1266,13 +1264,12 @@ def kv4_select(q, keys: KV4PageKeys, block_table, seq_lens, keep: int, page_size
         chosen, lens = seq_lens.new_empty(shape), seq_lens.new_empty(seqs)
     else:
         chosen, lens = out
-        _require_on(dev, pages=chosen, lens=lens)
+        _require_on(dev, pages=chosen)
         _require("pages", chosen, torch.int32, shape)
-        _kv4_ints("lens", lens, seqs)
+        _kv4_ints(dev, "lens", lens, seqs)
     _workspace_on(workspace, dev)
     ws, ws_bytes = _workspace(
-        workspace, lambda: kv4_select_workspace_size(seqs, keys.kv_heads, cols, keep), dev)
+        workspace, lambda: _select_workspace_size(seqs, keys.kv_heads, cols, keep), dev)
     _call_on(dev, "w8a8_kv4_select", q.data_ptr(), keys._descriptor(), block_table.data_ptr(),
-             cols, table_ld, seq_lens.data_ptr(), page_size, chosen.data_ptr(), keep,
-             lens.data_ptr(), seqs, heads, ldq, _ptr(ws), ws_bytes, _stream(dev))
+             cols, table_ld, lens_at, page_size, chosen.data_ptr(), keep, lens.data_ptr(), seqs, heads, ldq, _ptr(ws), ws_bytes, _stream(dev))
     return chosen, lens

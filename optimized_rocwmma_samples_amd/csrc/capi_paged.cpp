@@ -182,10 +182,10 @@ int w8a8_kv4_select(const void* q, const w8a8_kv4_page_keys* keys, const int32_t
         return fail(W8A8_ERROR_INVALID_VALUE, "%s: null pointer argument", fn);
     if(ldq < (uint64_t)heads * keys->head_dim)
         return fail(W8A8_ERROR_INVALID_VALUE, "%s: ldq=%u smaller than heads * head_dim", fn, ldq);
-    // a block of 512 threads per sequence and key head, one of 256 per 256 pages of them,
+    // a block of 1024 threads per sequence and key head, one of 256 per 256 pages of them,
     // and a launch of fewer than 2^32 threads
     const uint64_t units = (uint64_t)seqs * keys->kv_heads;
-    if(units > 0x7FFFFFull || units * (table_cols / 256ull + 1) > 0xFFFFFFull
+    if(units > 0x3FFFFFull || units * (table_cols / 256ull + 1) > 0xFFFFFFull
        || units * keep > 0x7FFFFFFFull)
         return fail(W8A8_ERROR_NOT_SUPPORTED,
                     "%s: too many sequences, key heads or columns in one call", fn);

@@ -11,7 +11,7 @@ namespace {
 // and values unpacked to fp16 first, once, and then takes the prompts' kernel over them;
 // the others unpack the codes they use where they use them, which costs each 32 rows
 // twice what the products take.
-constexpr uint32_t kFewRows = 256;
+constexpr uint32_t kFewRows = 512;
 
 // One sequence of the call.
 struct Chunk {

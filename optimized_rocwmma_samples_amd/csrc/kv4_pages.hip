@@ -14,10 +14,9 @@ namespace {
 // Where a sequence's tokens and pages go follows from two running sums over the sequences
 // (new tokens, pages needed).  Every block computes them by itself, 1024 sequences at a
 // time, so that none waits for another, and then takes its share of the tokens and pages,
-// finding each one's sequence by halving among the 1024 sums in LDS.  A launch of one block
-// also writes the lengths and the count; with more blocks a second launch of one does,
-// since the caller may have them written over the lengths and the count that every block
-// reads.
+// finding each one's sequence by halving among the 1024 sums in LDS.  The lengths and the
+// count are written by the first block, or, with more than one, by a second launch of one
+// where the caller has them written over the lengths and the count that every block reads.
 // ---------------------------------------------------------------------------
 constexpr int kSeqs = 1024; // threads of a block, and sequences a step
 
@@ -100,7 +99,7 @@ __global__ void __launch_bounds__(kSeqs) kv4_extend_kernel(Kv4ExtendArgs a)
         begins[threadIdx.x]  = (uint32_t)min(begin, (uint64_t)a.tokens);
         bases[threadIdx.x]   = (uint32_t)base;
         lengths[threadIdx.x] = given ? len : 0xFFFFFFFFu;
-        if(COMMIT && is) {
+        if(COMMIT && blockIdx.x == 0 && is) {
             a.starts[i] = (int32_t)min(begin, (uint64_t)a.tokens);
             if(given && need != 0) atomicMax(&taken, (uint32_t)base + need);
             a.lens_out[i] = (int32_t)(given ? len + n : len);
@@ -139,7 +138,7 @@ __global__ void __launch_bounds__(kSeqs) kv4_extend_kernel(Kv4ExtendArgs a)
     if(PLACES) // rows behind the last sequence
         shares((uint32_t)min(rows, (uint64_t)a.tokens), a.tokens,
                [&](uint32_t t) { a.slots[t] = -1; });
-    if(COMMIT) {
+    if(COMMIT && blockIdx.x == 0) {
         __syncthreads();
         if(threadIdx.x == 0) {
             a.starts[a.seqs] = (int32_t)min(rows, (uint64_t)a.tokens);
@@ -173,7 +172,7 @@ __global__ void __launch_bounds__(kSeqs) kv4_trim_kernel(Kv4TrimArgs a)
         const uint64_t base  = pages + block_sum(n, part, sum);
         bases[threadIdx.x]  = (uint32_t)base;
         firsts[threadIdx.x] = first;
-        if(COMMIT && i < a.seqs) a.lens_out[i] = (int32_t)kept;
+        if(COMMIT && blockIdx.x == 0 && i < a.seqs) a.lens_out[i] = (int32_t)kept;
         __syncthreads();
         if(PLACES) {
             const uint32_t in = min((uint32_t)kSeqs, a.seqs - i0);
@@ -186,8 +185,7 @@ __global__ void __launch_bounds__(kSeqs) kv4_trim_kernel(Kv4TrimArgs a)
         }
         pages += sum;
     }
-    if(COMMIT) {
-        __syncthreads();
+    if(COMMIT && blockIdx.x == 0) {
         if(threadIdx.x == 0) a.count_out[0] = (int32_t)min(avail + all, (uint64_t)a.capacity);
     }
 }
@@ -342,48 +340,51 @@ __global__ void __launch_bounds__(kWaveThreads)
 // The pages that suit a query: score = scale of the page key * (its codes . the query's
 // codes), the query being the sum of the key head's query heads in 8 bits.  The dot
 // product is a whole number below 2^21 and the scale a power of two, so a score is exact
-// in fp32 and equal scores are equal everywhere.  Two launches: scores, lane = page, as
-// whole numbers in the scores' order; then the keep-th largest by its bytes, from counts of
-// their values, and the columns in order.
+// in fp32 and equal scores are equal everywhere.  A block takes one key head of a sequence:
+// scores, lane = page, as whole numbers in their order; then the keep-th largest by its
+// bytes, from counts of their values; then the columns in order.
+//
+// Up to kOneBlockPages columns the scores stay in LDS and one launch does it all; with more,
+// a launch before it computes the scores with a block for each 256 pages, since one block
+// reads page keys at some 100 GB/s.
 // ---------------------------------------------------------------------------
-template <int D>
-__global__ void __launch_bounds__(kWaveThreads)
-    kv4_score_kernel(Kv4SelectArgs a, uint32_t* __restrict__ order, uint32_t parts)
-{
-    __shared__ double  tops[kWaveThreads / kWave];
-    __shared__ alignas(16) uint32_t codes[D / 4];
-    const uint32_t unit = blockIdx.x / parts, part = blockIdx.x % parts; // (sequence, key head)
-    const uint32_t seq = unit / a.kv_heads, head = unit % a.kv_heads;
-    const uint32_t len  = clamped(a.lens[seq], a.table_cols << a.page_shift);
-    const uint32_t have = (len + (1u << a.page_shift) - 1) >> a.page_shift;
-    if(have <= a.keep || part * kWaveThreads >= have) return; // all of them, or none here
+constexpr int      kSelectThreads = 1024;
+constexpr uint32_t kOneBlockPages = 4096;
 
-    // ---- the query's codes ------------------------------------------------------------
+// The query's codes of one key head into LDS; all threads of the block.
+template <int D>
+__device__ __forceinline__ void query_codes(const Kv4SelectArgs& a, uint32_t seq, uint32_t head,
+                                            double* tops, uint32_t* codes)
+{
     const uint32_t per = a.heads / a.kv_heads;
     double         sum = 0.0;
-    if(threadIdx.x < D)
-        for(uint32_t h = 0; h < per; ++h)
-            sum += (double)half_bits_to_float(
-                a.q[(size_t)seq * a.ldq + (size_t)(head * per + h) * D + threadIdx.x]);
-    double top = fabs(sum);
-    if(!(top < (double)INFINITY)) top = INFINITY;
-#pragma unroll
-    for(int d = 1; d < kWave; d <<= 1) top = fmax(top, shfl_xor_f64(top, d));
-    if(threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
-    __syncthreads();
-    top = fmax(fmax(tops[0], tops[1]), fmax(tops[2], tops[3]));
     if(threadIdx.x < D) {
-        const bool some = top > 0.0 && top < (double)INFINITY;
-        const int  e2   = some ? power_for(top) : 0;
-        reinterpret_cast<int8_t*>(codes)[threadIdx.x] = some ? (int8_t)(int)rint(ldexp(sum, -e2)) : 0;
+        const uint16_t* q = a.q + (size_t)seq * a.ldq + (size_t)head * per * D + threadIdx.x;
+#pragma unroll 8
+        for(uint32_t h = 0; h < per; ++h) sum += (double)half_bits_to_float(q[(size_t)h * D]);
+        double top = fabs(sum);
+        if(!(top < (double)INFINITY)) top = INFINITY;
+#pragma unroll
+        for(int d = 1; d < kWave; d <<= 1) top = fmax(top, shfl_xor_f64(top, d));
+        if(threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
     }
     __syncthreads();
+    if(threadIdx.x < D) {
+        const double top  = D == 128 ? fmax(tops[0], tops[1]) : tops[0];
+        const bool   some = top > 0.0 && top < (double)INFINITY;
+        const int    e2   = some ? power_for(top) : 0;
+        reinterpret_cast<int8_t*>(codes)[threadIdx.x]
+            = some ? (int8_t)(int)rint(ldexp(sum, -e2)) : 0;
+    }
+    __syncthreads();
+}
 
-    // ---- one page a lane --------------------------------------------------------------
-    const uint32_t col = part * kWaveThreads + threadIdx.x;
-    if(col >= have) return;
-    const int32_t page  = a.table[(size_t)seq * a.table_ld + col];
-    float         score = -INFINITY;
+// The score of a page as a whole number in the scores' order.
+template <int D>
+__device__ __forceinline__ uint32_t page_order(const Kv4SelectArgs& a, int32_t page, uint32_t head,
+                                               bool last, const uint32_t* codes)
+{
+    float score = -INFINITY;
     if(page >= 0 && (uint32_t)page < a.pages) {
         const size_t at  = (size_t)page * a.kv_heads + head;
         int32_t      dot = 0;
@@ -399,25 +400,46 @@ __global__ void __launch_bounds__(kWaveThreads)
         score = (float)dot * s + 0.f; // no -0
         if(!(score == score)) score = -INFINITY;
     }
-    if(col + 1 == have) score = INFINITY; // the last page is always taken
+    if(last) score = INFINITY; // always taken
     const uint32_t u = __float_as_uint(score);
-    order[(size_t)unit * a.table_cols + col] = (u >> 31) != 0 ? ~u : u | 0x80000000u;
+    return (u >> 31) != 0 ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 512;
+template <int D>
+__global__ void __launch_bounds__(kWaveThreads)
+    kv4_score_kernel(Kv4SelectArgs a, uint32_t* __restrict__ order, uint32_t parts)
+{
+    __shared__ double  tops[2];
+    __shared__ alignas(16) uint32_t codes[D / 4];
+    const uint32_t unit = blockIdx.x / parts, part = blockIdx.x % parts; // (sequence, key head)
+    const uint32_t seq = unit / a.kv_heads, head = unit % a.kv_heads;
+    const uint32_t len  = clamped(a.lens[seq], a.table_cols << a.page_shift);
+    const uint32_t have = (len + (1u << a.page_shift) - 1) >> a.page_shift;
+    if(have <= a.keep || part * kWaveThreads >= have) return; // all of them, or none here
+    query_codes<D>(a, seq, head, tops, codes);
+    const uint32_t col = part * kWaveThreads + threadIdx.x;
+    if(col >= have) return;
+    const int32_t page = a.table[(size_t)seq * a.table_ld + col];
+    order[(size_t)unit * a.table_cols + col] = page_order<D>(a, page, head, col + 1 == have, codes);
+}
 
+// SCORED: `order` holds the scores.
+template <int D, bool SCORED>
 __global__ void __launch_bounds__(kSelectThreads)
     kv4_select_kernel(Kv4SelectArgs a, const uint32_t* __restrict__ order)
 {
     constexpr int       kWaves = kSelectThreads / kWave;
+    __shared__ uint32_t scores[SCORED ? 1 : kOneBlockPages];
+    __shared__ double   tops[2];
+    __shared__ alignas(16) uint32_t codes[D / 4];
     __shared__ uint32_t count[256], part[2][kWaves], bin, above;
     const int           lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const uint32_t      unit = blockIdx.x, seq = unit / a.kv_heads;
+    const uint32_t      unit = blockIdx.x, seq = unit / a.kv_heads, head = unit % a.kv_heads;
     const uint32_t      len  = clamped(a.lens[seq], a.table_cols << a.page_shift);
     const uint32_t      have = (len + (1u << a.page_shift) - 1) >> a.page_shift;
     const int32_t*      from = a.table + (size_t)seq * a.table_ld;
     int32_t*            to   = a.chosen + (size_t)unit * a.keep;
-    if(unit % a.kv_heads == 0 && threadIdx.x == 0)
+    if(head == 0 && threadIdx.x == 0)
         a.lens_out[seq]
             = (int32_t)(have > a.keep ? len - ((have - a.keep) << a.page_shift) : len);
     if(have <= a.keep) {
@@ -425,8 +447,13 @@ __global__ void __launch_bounds__(kSelectThreads)
             to[i] = i < have ? from[i] : -1;
         return;
     }
+    if constexpr(!SCORED) {
+        query_codes<D>(a, seq, head, tops, codes);
+        for(uint32_t i = threadIdx.x; i < have; i += kSelectThreads)
+            scores[i] = page_order<D>(a, from[i], head, i + 1 == have, codes);
+    }
+    const uint32_t* mine = SCORED ? order + (size_t)unit * a.table_cols : scores;
     // ---- the keep-th largest, byte by byte from the top -------------------------------
-    const uint32_t* mine = order + (size_t)unit * a.table_cols;
     uint32_t        least = 0, mask = 0, left = a.keep; // of those that begin like `least`
     for(int shift = 24; shift >= 0; shift -= 8) {
         for(uint32_t i = threadIdx.x; i < 256; i += kSelectThreads) count[i] = 0;
@@ -497,32 +524,36 @@ __global__ void __launch_bounds__(kSelectThreads)
     }
 }
 
-uint32_t blocks_for(uint64_t work, uint32_t most)
+// Blocks for so many tokens to place, or columns whose pages may come back: one for few, since
+// each finds the running sums by itself.
+uint32_t blocks_for(uint64_t items)
 {
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, (work + kSeqs - 1) / kSeqs));
+    if(items <= 8 * kSeqs) return 1;
+    return (uint32_t)std::min<uint64_t>(256, (items + kSeqs - 1) / kSeqs);
 }
 
 } // namespace
 
 hipError_t launch_kv4_extend(const Kv4ExtendArgs& a, hipStream_t stream)
 {
-    if(a.tokens <= kOneBlockItems) {
-        kv4_extend_kernel<true, true><<<1, kSeqs, 0, stream>>>(a);
+    const uint32_t blocks = blocks_for(a.tokens);
+    if(blocks == 1 || (a.lens_out != a.lens && a.count_out != a.count)) {
+        kv4_extend_kernel<true, true><<<blocks, kSeqs, 0, stream>>>(a);
         return hipGetLastError();
     }
-    kv4_extend_kernel<true, false><<<blocks_for(a.tokens, 256), kSeqs, 0, stream>>>(a);
+    kv4_extend_kernel<true, false><<<blocks, kSeqs, 0, stream>>>(a);
     kv4_extend_kernel<false, true><<<1, kSeqs, 0, stream>>>(a);
     return hipGetLastError();
 }
 
 hipError_t launch_kv4_trim(const Kv4TrimArgs& a, hipStream_t stream)
 {
-    const uint64_t pages = (uint64_t)a.seqs * a.table_cols;
-    if(pages <= kOneBlockItems) {
-        kv4_trim_kernel<true, true><<<1, kSeqs, 0, stream>>>(a);
+    const uint32_t blocks = blocks_for((uint64_t)a.seqs * a.table_cols);
+    if(blocks == 1 || (a.lens_out != a.lens && a.lens_out != a.keep && a.count_out != a.count)) {
+        kv4_trim_kernel<true, true><<<blocks, kSeqs, 0, stream>>>(a);
         return hipGetLastError();
     }
-    kv4_trim_kernel<true, false><<<blocks_for(pages, 256), kSeqs, 0, stream>>>(a);
+    kv4_trim_kernel<true, false><<<blocks, kSeqs, 0, stream>>>(a);
     kv4_trim_kernel<false, true><<<1, kSeqs, 0, stream>>>(a);
     return hipGetLastError();
 }
@@ -549,19 +580,25 @@ hipError_t launch_kv4_page_keys(const Kv4PageKeysArgs& a, hipStream_t stream)
 
 size_t kv4_select_workspace_bytes(uint32_t seqs, uint32_t kv_heads, uint32_t cols, uint32_t keep)
 {
-    return cols <= keep ? 0 : (size_t)seqs * kv_heads * cols * 4;
+    return cols <= keep || cols <= kOneBlockPages ? 0 : (size_t)seqs * kv_heads * cols * 4;
 }
 
 hipError_t launch_kv4_select(const Kv4SelectArgs& a, hipStream_t stream)
 {
     const uint32_t units = a.seqs * a.kv_heads;
     auto*          order = static_cast<uint32_t*>(a.ws);
-    if(a.table_cols > a.keep) {
-        const uint32_t parts  = (a.table_cols + kWaveThreads - 1) / kWaveThreads;
-        const auto     kernel = a.head_dim == 64 ? kv4_score_kernel<64> : kv4_score_kernel<128>;
-        kernel<<<units * parts, kWaveThreads, 0, stream>>>(a, order, parts);
-    }
-    kv4_select_kernel<<<units, kSelectThreads, 0, stream>>>(a, order);
+    const auto     run   = [&](auto d) {
+        if(a.table_cols > a.keep && a.table_cols > kOneBlockPages) {
+            const uint32_t parts = (a.table_cols + kWaveThreads - 1) / kWaveThreads;
+            kv4_score_kernel<d()><<<units * parts, kWaveThreads, 0, stream>>>(a, order, parts);
+            kv4_select_kernel<d(), true><<<units, kSelectThreads, 0, stream>>>(a, order);
+        } else
+            kv4_select_kernel<d(), false><<<units, kSelectThreads, 0, stream>>>(a, order);
+    };
+    if(a.head_dim == 64)
+        run(std::integral_constant<int, 64>());
+    else
+        run(std::integral_constant<int, 128>());
     return hipGetLastError();
 }
 

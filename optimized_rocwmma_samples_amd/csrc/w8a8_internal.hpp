@@ -337,8 +337,6 @@ struct Kv4TrimArgs {
     int32_t *      lens_out, *count_out;
     uint32_t       seqs, table_cols, table_ld, capacity, page_shift;
 };
-// Tokens to place, or pages to take back, that one block handles in one launch.
-constexpr uint32_t kOneBlockItems = 8192;
 hipError_t launch_kv4_extend(const Kv4ExtendArgs& a, hipStream_t stream);
 hipError_t launch_kv4_trim(const Kv4TrimArgs& a, hipStream_t stream);
 

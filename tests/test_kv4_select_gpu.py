@@ -178,8 +178,12 @@ def test_select_strides_out_and_graph(w8a8, gpu):
         torch.cuda.synchronize()
         want, left = check_select(w8a8, gpu, q, keys, table, lens, 9, 16)
         assert torch.equal(out[0], want) and torch.equal(out[1], left)
+    # tables of many columns need a workspace
+    wide = table[:1].expand(3, 60).repeat(1, 100)
+    assert w8a8.kv4_select_workspace_size(3, 2, 6000, 9) >= 3 * 2 * 6000 * 4
     with pytest.raises(w8a8.W8A8Error, match="workspace"):
-        w8a8.kv4_select(q, keys, table, n, 9, 16, workspace=None)
+        w8a8.kv4_select(q, keys, wide, n, 9, 16, workspace=None)
+    check_select(w8a8, gpu, q, keys, wide, [16 * 5999, 431, 16], 9, 16)
 
 
 def attention_by_head(q, c, tables, lens):

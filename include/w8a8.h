@@ -855,7 +855,7 @@ int w8a8_kv4_page_keys_load(const w8a8_kv4_page_keys* keys, const int32_t* pages
  *   chosen int32 [seqs, kv_heads, keep]: pages in the order of their columns, -1
  *     behind the last; lens_out int32 [seqs]: the tokens in them, the same for all
  *     key heads.  Both for w8a8_attention_kv4_selected; neither may overlap an input.
- * workspace: w8a8_kv4_select_workspace_size bytes (0 for tables of up to 4096 columns), 16-byte
+ * workspace: w8a8_kv4_select_workspace_size bytes (0 for tables of few columns), 16-byte
  * aligned, needs no clearing; calls that share one must be ordered on one stream.
  */
 size_t w8a8_kv4_select_workspace_size(uint32_t seqs, uint32_t kv_heads, uint32_t table_cols,

@@ -44,23 +44,6 @@ struct LongList {
 
 } // namespace
 
-// v and the sum of v over the lanes before.
-__device__ __forceinline__ uint32_t lanes_sum(uint32_t v)
-{
-    const auto add = [&](auto ctrl, auto rows) {
-        v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value,
-                                                   decltype(rows)::value, 0xF, false);
-    };
-    using std::integral_constant;
-    add(integral_constant<int, 0x111>(), integral_constant<int, 0xF>()); // from 1, 2, 4, 8 lanes
-    add(integral_constant<int, 0x112>(), integral_constant<int, 0xF>()); // before, in rows of 16
-    add(integral_constant<int, 0x114>(), integral_constant<int, 0xF>());
-    add(integral_constant<int, 0x118>(), integral_constant<int, 0xF>());
-    add(integral_constant<int, 0x142>(), integral_constant<int, 0xA>()); // the row before's last
-    add(integral_constant<int, 0x143>(), integral_constant<int, 0xC>()); // lane 31's
-    return v;
-}
-
 // What the join needs of a unit that goes on behind the run it begins in.
 struct Piece {
     uint32_t last;  // run that has its last step, plus 1; 0: no such unit

@@ -63,6 +63,23 @@ __device__ __forceinline__ void load_dwords(int32_t* r, const void* p)
         r[0] = *static_cast<const int32_t*>(p);
 }
 
+// v and the sum of v over the lanes before.
+__device__ __forceinline__ uint32_t lanes_sum(uint32_t v)
+{
+    const auto add = [&](auto ctrl, auto rows) {
+        v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value,
+                                                   decltype(rows)::value, 0xF, false);
+    };
+    using std::integral_constant;
+    add(integral_constant<int, 0x111>(), integral_constant<int, 0xF>()); // from 1, 2, 4, 8 lanes
+    add(integral_constant<int, 0x112>(), integral_constant<int, 0xF>()); // before, in rows of 16
+    add(integral_constant<int, 0x114>(), integral_constant<int, 0xF>());
+    add(integral_constant<int, 0x118>(), integral_constant<int, 0xF>());
+    add(integral_constant<int, 0x142>(), integral_constant<int, 0xA>()); // the row before's last
+    add(integral_constant<int, 0x143>(), integral_constant<int, 0xC>()); // lane 31's
+    return v;
+}
+
 // The instantiation for a cache's head width and group.
 template <class F>
 void with_widths(const w8a8_kv4_cache& c, F f)

@@ -202,21 +202,41 @@ __global__ void __launch_bounds__(kSeqs) kv4_trim_kernel(Kv4TrimArgs a)
 // ---------------------------------------------------------------------------
 constexpr int kWaveThreads = 256;
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int d)
+__device__ __forceinline__ double of_halves(uint32_t lo, uint32_t hi)
 {
-    const uint64_t u = __double_as_longlong(v);
-    const uint32_t lo = __shfl_xor((int)(uint32_t)u, d, kWave);
-    const uint32_t hi = __shfl_xor((int)(uint32_t)(u >> 32), d, kWave);
     return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
 
-// The least power of two 2^e with top <= 127 * 2^e, top > 0.
-__device__ __forceinline__ int power_for(double top)
+// v and the one D lanes away, added up: D = 8, 16 or 32.
+template <int D>
+__device__ __forceinline__ double add_across(double v)
+{
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+    if constexpr(D == 32) {
+        const auto l = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+        const auto h = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+        return of_halves(l[0], h[0]) + of_halves(l[1], h[1]);
+    } else if constexpr(D == 16) {
+        const auto l = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+        const auto h = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+        return of_halves(l[0], h[0]) + of_halves(l[1], h[1]);
+    } else
+        return v + of_halves((uint32_t)dpp_mov_i32<kDppRowRor8>((int)lo),
+                             (uint32_t)dpp_mov_i32<kDppRowRor8>((int)hi));
+}
+
+// The least e with |v| <= 127 * 2^e; kNoPower of 0.  It grows with |v|, so the largest of
+// several is that of the largest value.
+constexpr int kNoPower = -5000;
+__device__ __forceinline__ int power_for(double v)
 {
     int          e;
-    const double m = frexp(top, &e);
-    return m <= 127.0 / 128.0 ? e - 7 : e - 6;
+    const double m = frexp(fabs(v), &e);
+    return v == 0.0 ? kNoPower : m <= 127.0 / 128.0 ? e - 7 : e - 6;
 }
+
+__device__ __forceinline__ int wave_max_i32(int v) { return -wave_min_i32(-v); }
 
 template <int D, int G>
 __global__ void __launch_bounds__(kWaveThreads)
@@ -242,12 +262,7 @@ __global__ void __launch_bounds__(kWaveThreads)
             from                 = (l > fresh ? l - fresh : 0) >> c.page_shift;
             if(fresh != 0 && l != 0) n = ((l - 1) >> c.page_shift) + 1 - from;
         }
-        uint32_t s = n;
-#pragma unroll
-        for(int d = 1; d < kWave; d <<= 1) {
-            const uint32_t o = __shfl_up(s, d, kWave);
-            if(lane >= d) s += o;
-        }
+        const uint32_t s    = lanes_sum(n);
         const uint64_t past = __ballot(s > at);
         if(past != 0) {
             const int f = __builtin_ctzll(past);
@@ -290,23 +305,18 @@ __global__ void __launch_bounds__(kWaveThreads)
                 sum[e] += fma(step, (double)((int)(w[i] >> (4 * e) & 15u) - 8), mid);
         }
     }
-#pragma unroll
-    for(int d = kLanes; d < kWave; d <<= 1)
-#pragma unroll
-        for(int e = 0; e < 8; ++e) sum[e] += shfl_xor_f64(sum[e], d);
-    double top = 0.0;
-    bool   ok  = true;
+    int  e2 = kNoPower;
+    bool ok = true;
 #pragma unroll
     for(int e = 0; e < 8; ++e) {
-        sum[e] = sum[e] / (double)rows;
+        if constexpr(kLanes == 8) sum[e] = add_across<8>(sum[e]);
+        sum[e] = add_across<32>(add_across<16>(sum[e])) / (double)rows;
         ok     = ok && fabs(sum[e]) < (double)INFINITY;
-        top    = fmax(top, fabs(sum[e]));
+        e2     = max(e2, power_for(sum[e]));
     }
     ok = __ballot(!ok) == 0;
-#pragma unroll
-    for(int d = 1; d < kLanes; d <<= 1) top = fmax(top, shfl_xor_f64(top, d));
-    const bool some = ok && top > 0.0;
-    const int  e2   = some ? power_for(top) : 0;
+    e2 = wave_max_i32(e2); // (its rows' lanes all hold the same)
+    const bool some = ok && e2 != kNoPower;
     if(r0 != 0) return;
     uint32_t q[2] = {0, 0};
     if(some)
@@ -345,8 +355,10 @@ __global__ void __launch_bounds__(kWaveThreads)
 // bytes, from counts of their values; then the columns in order.
 //
 // Up to kOneBlockPages columns the scores stay in LDS and one launch does it all; with more,
-// a launch before it computes the scores with a block for each 256 pages, since one block
-// reads page keys at some 100 GB/s.
+// or with more than half as many and few blocks, a launch before it computes the scores with a
+// block for each 256 pages, since one block reads page keys at some 50 GB/s.  us in one launch
+// and in two, heads of 128, 8 key heads: one sequence of 2048 pages 10.5, 11; of 4096 15.8,
+// 12.4; 32 sequences of 4096 41, 45.
 // ---------------------------------------------------------------------------
 constexpr int      kSelectThreads = 1024;
 constexpr uint32_t kOneBlockPages = 4096;
@@ -354,73 +366,89 @@ constexpr uint32_t kOneBlockPages = 4096;
 // The query's codes of one key head into LDS; all threads of the block.
 template <int D>
 __device__ __forceinline__ void query_codes(const Kv4SelectArgs& a, uint32_t seq, uint32_t head,
-                                            double* tops, uint32_t* codes)
+                                            int* powers, uint32_t* codes)
 {
-    const uint32_t per = a.heads / a.kv_heads;
-    double         sum = 0.0;
+    constexpr int  kNotFinite = 5000;
+    const uint32_t per        = a.heads / a.kv_heads;
+    double         sum        = 0.0;
     if(threadIdx.x < D) {
         const uint16_t* q = a.q + (size_t)seq * a.ldq + (size_t)head * per * D + threadIdx.x;
 #pragma unroll 8
         for(uint32_t h = 0; h < per; ++h) sum += (double)half_bits_to_float(q[(size_t)h * D]);
-        double top = fabs(sum);
-        if(!(top < (double)INFINITY)) top = INFINITY;
-#pragma unroll
-        for(int d = 1; d < kWave; d <<= 1) top = fmax(top, shfl_xor_f64(top, d));
-        if(threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
+        const int e = wave_max_i32(fabs(sum) < (double)INFINITY ? power_for(sum) : kNotFinite);
+        if(threadIdx.x % kWave == 0) powers[threadIdx.x / kWave] = e;
     }
     __syncthreads();
     if(threadIdx.x < D) {
-        const double top  = D == 128 ? fmax(tops[0], tops[1]) : tops[0];
-        const bool   some = top > 0.0 && top < (double)INFINITY;
-        const int    e2   = some ? power_for(top) : 0;
+        const int  e2   = D == 128 ? max(powers[0], powers[1]) : powers[0];
+        const bool some = e2 != kNoPower && e2 != kNotFinite;
         reinterpret_cast<int8_t*>(codes)[threadIdx.x]
             = some ? (int8_t)(int)rint(ldexp(sum, -e2)) : 0;
     }
     __syncthreads();
 }
 
-// The score of a page as a whole number in the scores' order.
-template <int D>
-__device__ __forceinline__ uint32_t page_order(const Kv4SelectArgs& a, int32_t page, uint32_t head,
-                                               bool last, const uint32_t* codes)
+// Scores of columns first .. end - 1 of `have`, as whole numbers in the scores' order, into
+// `order`: D / 16 lanes a page, 16 bytes each, so that a wave reads whole lines (a lane a page
+// takes 10 us for 2048 pages and not 4), THREADS lanes in all, 8 pages of each on their way.
+template <int D, int THREADS>
+__device__ __forceinline__ void page_orders(const Kv4SelectArgs& a, const int32_t* from,
+                                            uint32_t head, uint32_t first, uint32_t end,
+                                            uint32_t have, const uint32_t* codes, uint32_t* order)
 {
-    float score = -INFINITY;
-    if(page >= 0 && (uint32_t)page < a.pages) {
-        const size_t at  = (size_t)page * a.kv_heads + head;
-        int32_t      dot = 0;
-        const v4i*   k   = reinterpret_cast<const v4i*>(a.codes + at * D);
-        const float  s   = a.scales[at];
+    constexpr uint32_t kLanes = D / 16, kGroups = THREADS / kLanes, kAhead = 8;
+    const uint32_t     sub = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    const v4i          q = reinterpret_cast<const v4i*>(codes)[sub];
+    for(uint32_t c0 = first + group; c0 < end; c0 += kGroups * kAhead) {
+        int32_t page[kAhead];
+        v4i     k[kAhead];
+        float   s[kAhead];
 #pragma unroll
-        for(int i = 0; i < D / 16; ++i) {
-            const v4i u = k[i];
-#pragma unroll
-            for(int e = 0; e < 4; ++e)
-                dot = __builtin_amdgcn_sdot4(u[e], (int)codes[4 * i + e], dot, false);
+        for(uint32_t x = 0; x < kAhead; ++x) {
+            const uint32_t c = c0 + x * kGroups;
+            page[x]          = c < end ? from[c] : -1;
         }
-        score = (float)dot * s + 0.f; // no -0
-        if(!(score == score)) score = -INFINITY;
+#pragma unroll
+        for(uint32_t x = 0; x < kAhead; ++x) {
+            if(page[x] < 0 || (uint32_t)page[x] >= a.pages) page[x] = -1;
+            const size_t at = (size_t)max(page[x], 0) * a.kv_heads + head;
+            k[x]            = reinterpret_cast<const v4i*>(a.codes + at * D)[sub];
+            s[x]            = a.scales[at];
+        }
+#pragma unroll
+        for(uint32_t x = 0; x < kAhead; ++x) {
+            int32_t dot = 0;
+#pragma unroll
+            for(int e = 0; e < 4; ++e) dot = __builtin_amdgcn_sdot4(k[x][e], q[e], dot, false);
+            dot += dpp_mov_i32<kDppQuadXor1>(dot);
+            dot += dpp_mov_i32<kDppQuadXor2>(dot);
+            if constexpr(kLanes == 8) dot += dpp_mov_i32<kDppRowHalfMirror>(dot);
+            float score = page[x] >= 0 ? (float)dot * s[x] + 0.f : -INFINITY; // no -0
+            if(!(score == score)) score = -INFINITY;
+            const uint32_t c = c0 + x * kGroups;
+            if(c + 1 == have) score = INFINITY; // the last page is always taken
+            const uint32_t u = __float_as_uint(score);
+            if(sub == 0 && c < end) order[c] = (u >> 31) != 0 ? ~u : u | 0x80000000u;
+        }
     }
-    if(last) score = INFINITY; // always taken
-    const uint32_t u = __float_as_uint(score);
-    return (u >> 31) != 0 ? ~u : u | 0x80000000u;
 }
 
 template <int D>
 __global__ void __launch_bounds__(kWaveThreads)
     kv4_score_kernel(Kv4SelectArgs a, uint32_t* __restrict__ order, uint32_t parts)
 {
-    __shared__ double  tops[2];
+    __shared__ int     powers[2];
     __shared__ alignas(16) uint32_t codes[D / 4];
     const uint32_t unit = blockIdx.x / parts, part = blockIdx.x % parts; // (sequence, key head)
     const uint32_t seq = unit / a.kv_heads, head = unit % a.kv_heads;
     const uint32_t len  = clamped(a.lens[seq], a.table_cols << a.page_shift);
     const uint32_t have = (len + (1u << a.page_shift) - 1) >> a.page_shift;
     if(have <= a.keep || part * kWaveThreads >= have) return; // all of them, or none here
-    query_codes<D>(a, seq, head, tops, codes);
-    const uint32_t col = part * kWaveThreads + threadIdx.x;
-    if(col >= have) return;
-    const int32_t page = a.table[(size_t)seq * a.table_ld + col];
-    order[(size_t)unit * a.table_cols + col] = page_order<D>(a, page, head, col + 1 == have, codes);
+    query_codes<D>(a, seq, head, powers, codes);
+    const uint32_t first = part * kWaveThreads;
+    page_orders<D, kWaveThreads>(a, a.table + (size_t)seq * a.table_ld, head, first,
+                                 min(first + kWaveThreads, have), have, codes,
+                                 order + (size_t)unit * a.table_cols);
 }
 
 // SCORED: `order` holds the scores.
@@ -430,9 +458,9 @@ __global__ void __launch_bounds__(kSelectThreads)
 {
     constexpr int       kWaves = kSelectThreads / kWave;
     __shared__ uint32_t scores[SCORED ? 1 : kOneBlockPages];
-    __shared__ double   tops[2];
+    __shared__ int      powers[2];
     __shared__ alignas(16) uint32_t codes[D / 4];
-    __shared__ uint32_t count[256], part[2][kWaves], bin, above;
+    __shared__ uint32_t count[256], part[kWaves], bin, above, same;
     const int           lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const uint32_t      unit = blockIdx.x, seq = unit / a.kv_heads, head = unit % a.kv_heads;
     const uint32_t      len  = clamped(a.lens[seq], a.table_cols << a.page_shift);
@@ -448,9 +476,8 @@ __global__ void __launch_bounds__(kSelectThreads)
         return;
     }
     if constexpr(!SCORED) {
-        query_codes<D>(a, seq, head, tops, codes);
-        for(uint32_t i = threadIdx.x; i < have; i += kSelectThreads)
-            scores[i] = page_order<D>(a, from[i], head, i + 1 == have, codes);
+        query_codes<D>(a, seq, head, powers, codes);
+        page_orders<D, kSelectThreads>(a, from, head, 0, have, have, codes, scores);
     }
     const uint32_t* mine = SCORED ? order + (size_t)unit * a.table_cols : scores;
     // ---- the keep-th largest, byte by byte from the top -------------------------------
@@ -467,19 +494,15 @@ __global__ void __launch_bounds__(kSelectThreads)
             uint32_t n[4], sum = 0;
 #pragma unroll
             for(int e = 0; e < 4; ++e) sum += n[e] = count[255 - 4 * lane - e];
-            uint32_t s = sum;
-#pragma unroll
-            for(int d = 1; d < kWave; d <<= 1) {
-                const uint32_t o = __shfl_up(s, d, kWave);
-                if(lane >= d) s += o;
-            }
-            uint32_t before = s - sum;
+            const uint32_t s      = lanes_sum(sum);
+            uint32_t       before = s - sum;
             if(before < left && s >= left) { // one lane
 #pragma unroll
                 for(int e = 0; e < 4; ++e) {
                     if(before < left && before + n[e] >= left) {
                         bin   = 255 - 4 * lane - e;
                         above = before;
+                        same  = n[e];
                     }
                     before += n[e];
                 }
@@ -489,38 +512,41 @@ __global__ void __launch_bounds__(kSelectThreads)
         least |= bin << shift;
         mask |= 255u << shift;
         left -= above;
+        if(same == left) break; // all that begin like it
     }
-    // ---- the columns above it, and the first `left` of those equal to it --------------
-    uint32_t equal = 0, out = 0; // up to here
-    for(uint32_t i0 = 0; i0 < have; i0 += kSelectThreads) {
-        const uint32_t i = i0 + threadIdx.x;
-        const uint32_t u = i < have ? mine[i] : 0;
-        const bool     same = i < have && u == least, more = i < have && u > least;
-        const uint64_t sames = __ballot(same), mores = __ballot(more);
-        __syncthreads();
-        if(lane == 0) {
-            part[0][wave] = __builtin_popcountll(sames);
-            part[1][wave] = __builtin_popcountll(mores);
+    // ---- the columns above it, and the first `left` of those that begin like it ---------
+    constexpr uint32_t kEach = 4; // columns a thread, one after the other
+    uint32_t           equal = 0, out = 0; // up to here
+    for(uint32_t i0 = 0; i0 < have; i0 += kSelectThreads * kEach) {
+        const uint32_t i = i0 + threadIdx.x * kEach;
+        uint32_t       u[kEach], eq = 0, gt = 0;
+#pragma unroll
+        for(uint32_t x = 0; x < kEach; ++x) {
+            u[x] = i + x < have ? mine[i + x] & mask : 0;
+            eq += i + x < have && u[x] == least ? 1u : 0u;
+            gt += u[x] > least ? 1u : 0u;
         }
+        const uint32_t own = gt << 16 | eq, s = lanes_sum(own); // at most 4096 of each
         __syncthreads();
-        uint32_t eq = equal, gt = 0, all_eq = 0, all_gt = 0;
+        if(lane == kWave - 1) part[wave] = s;
+        __syncthreads();
+        uint32_t before = s - own, all = 0;
 #pragma unroll
         for(int w = 0; w < kWaves; ++w) {
-            if(w < wave) {
-                eq += part[0][w];
-                gt += part[1][w];
-            }
-            all_eq += part[0][w];
-            all_gt += part[1][w];
+            if(w < wave) before += part[w];
+            all += part[w];
         }
-        const uint64_t below = (1ull << lane) - 1;
-        eq += __builtin_popcountll(sames & below);
-        gt += __builtin_popcountll(mores & below);
+        uint32_t e = equal + (before & 0xFFFFu); // equals before the column
         // places: what is above, and the equals so far up to `left`
-        const uint32_t place = out + gt + (min(eq, left) - min(equal, left));
-        if(more || (same && eq < left)) to[place] = from[i];
-        out += all_gt + (min(equal + all_eq, left) - min(equal, left));
-        equal += all_eq;
+        uint32_t place = out + (before >> 16) + min(e, left) - min(equal, left);
+#pragma unroll
+        for(uint32_t x = 0; x < kEach; ++x) {
+            const bool is = i + x < have && u[x] == least;
+            if(u[x] > least || (is && e < left)) to[place++] = from[i + x];
+            e += is ? 1u : 0u;
+        }
+        out += (all >> 16) + min(equal + (all & 0xFFFFu), left) - min(equal, left);
+        equal += all & 0xFFFFu;
     }
 }
 
@@ -580,7 +606,10 @@ hipError_t launch_kv4_page_keys(const Kv4PageKeysArgs& a, hipStream_t stream)
 
 size_t kv4_select_workspace_bytes(uint32_t seqs, uint32_t kv_heads, uint32_t cols, uint32_t keep)
 {
-    return cols <= keep || cols <= kOneBlockPages ? 0 : (size_t)seqs * kv_heads * cols * 4;
+    const uint64_t units = (uint64_t)seqs * kv_heads;
+    if(cols <= keep || cols <= kOneBlockPages / 2 || (cols <= kOneBlockPages && units >= 128))
+        return 0; // one launch
+    return units * cols * 4;
 }
 
 hipError_t launch_kv4_select(const Kv4SelectArgs& a, hipStream_t stream)
@@ -588,7 +617,7 @@ hipError_t launch_kv4_select(const Kv4SelectArgs& a, hipStream_t stream)
     const uint32_t units = a.seqs * a.kv_heads;
     auto*          order = static_cast<uint32_t*>(a.ws);
     const auto     run   = [&](auto d) {
-        if(a.table_cols > a.keep && a.table_cols > kOneBlockPages) {
+        if(kv4_select_workspace_bytes(a.seqs, a.kv_heads, a.table_cols, a.keep) != 0) {
             const uint32_t parts = (a.table_cols + kWaveThreads - 1) / kWaveThreads;
             kv4_score_kernel<d()><<<units * parts, kWaveThreads, 0, stream>>>(a, order, parts);
             kv4_select_kernel<d(), true><<<units, kSelectThreads, 0, stream>>>(a, order);

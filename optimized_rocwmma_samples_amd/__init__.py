@@ -1052,7 +1052,7 @@ def kv4_extend(new_tokens, seq_lens, block_table, free_pages, free_count, page_s
     its rows would pass `tokens`, its tokens the table's columns, or where the pages that
     the sequences before it leave are too few.  out: these four; the lengths and the
     count may be seq_lens and free_count themselves."""
-    _torch()
+    torch = _torch()
     _require_cuda(block_table)
     dev = block_table.device
     seqs = block_table.shape[0]
@@ -1064,9 +1064,12 @@ def kv4_extend(new_tokens, seq_lens, block_table, free_pages, free_count, page_s
     if tokens < 0:
         raise ValueError("tokens must not be negative")
     if out is None:
-        new = seq_lens.new_empty
-        out = slots, starts, lens, count = new(tokens), new(seqs + 1), new(seqs), new(1)
-        at = slots.data_ptr(), tokens, starts.data_ptr(), lens.data_ptr(), count.data_ptr()
+        # one allocation for the four (0.9 us each of a 10 us call)
+        both = seq_lens.new_empty(tokens + 2 * seqs + 2)
+        slots, starts, lens, count = torch.split_with_sizes(both, (tokens, seqs + 1, seqs, 1))
+        at = both.data_ptr()
+        at = (at, tokens, at + 4 * tokens, at + 4 * (tokens + seqs + 1),
+              at + 4 * (tokens + 2 * seqs + 1))
     else:
         slots, starts, lens, count = out
         at = (_kv4_ints(dev, "slots", slots, tokens), tokens,
@@ -1271,5 +1274,6 @@ def kv4_select(q, keys: KV4PageKeys, block_table, seq_lens, keep: int, page_size
     ws, ws_bytes = _workspace(
         workspace, lambda: _select_workspace_size(seqs, keys.kv_heads, cols, keep), dev)
     _call_on(dev, "w8a8_kv4_select", q.data_ptr(), keys._descriptor(), block_table.data_ptr(),
-             cols, table_ld, lens_at, page_size, chosen.data_ptr(), keep, lens.data_ptr(), seqs, heads, ldq, _ptr(ws), ws_bytes, _stream(dev))
+             cols, table_ld, lens_at, page_size, chosen.data_ptr(), keep, lens.data_ptr(), seqs,
+             heads, ldq, _ptr(ws), ws_bytes, _stream(dev))
     return chosen, lens

@@ -9,10 +9,14 @@
 
 namespace w8a8 {
 
-inline bool aligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+inline bool aligned(const void* p, uintptr_t bytes)
+{
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+}
 
 // The head counts and scale of an attention call; 0 where they are right.
-inline int check_heads(const char* fn, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, float scale)
+inline int check_heads(const char* fn, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                       float scale)
 {
     if(heads == 0 || kv_heads == 0 || heads % kv_heads != 0)
         return fail(W8A8_ERROR_INVALID_VALUE,

@@ -58,7 +58,8 @@ int w8a8_kv4_extend(const int32_t* new_tokens, const int32_t* seq_lens, uint32_t
     if(const int rc = check_table(fn, seqs, table_cols, table_ld, page_size)) return rc;
     if(!free_count || !seq_starts || !count_out || (!free_pages && free_capacity != 0)
        || (!slots && tokens != 0)
-       || (seqs != 0 && (!new_tokens || !seq_lens || !lens_out || (!block_table && table_cols != 0))))
+       || (seqs != 0
+           && (!new_tokens || !seq_lens || !lens_out || (!block_table && table_cols != 0))))
         return fail(W8A8_ERROR_INVALID_VALUE, "%s: null pointer argument", fn);
     if(tokens > 0x7FFFFFFEu || free_capacity > 0x7FFFFFFFu)
         return fail(W8A8_ERROR_NOT_SUPPORTED, "%s: needs tokens and free_capacity < 2^31 - 1", fn);
@@ -280,8 +281,8 @@ int w8a8_attention_kv4_chunks(const void* q, const w8a8_kv4_cache* cache,
         return fail(W8A8_ERROR_NOT_SUPPORTED,
                     "%s: needs 16-byte aligned q, out and row strides of multiples of 8", fn);
     // steps of 128 keys of 32 rows, counted in 31 bits; a sequence's rows likewise
-    const uint64_t tiles
-        = (uint64_t)tokens * heads / 32 + (uint64_t)(tokens < seqs ? tokens : seqs) * cache->kv_heads;
+    const uint64_t some  = tokens < seqs ? tokens : seqs;
+    const uint64_t tiles = (uint64_t)tokens * heads / 32 + some * cache->kv_heads;
     if(tokens > 0x7FFFFFFFu || (uint64_t)tokens * heads > 0x7FFFFFFFull
        || tiles * ((uint64_t)table_cols * cache->page_size / 128 + 1) > 0x7FFFFFFFull)
         return fail(W8A8_ERROR_NOT_SUPPORTED, "%s: too many tokens, heads or columns in one call",

@@ -134,12 +134,13 @@ struct Line {
 struct Ways {
     const uint8_t* others; // [seqs] 1: unpacked first; or null
     uint32_t       per, most;
+    bool           more; // there are blocks for units of two tiles
 
     // 32-row tiles a unit; 0: not this kernel's
     __device__ uint32_t kind(const ChunkArgs& a, const Chunk& x, uint32_t i) const
     {
         if(x.fresh == 0 || (others != nullptr && others[i] != 0)) return 0;
-        return x.fresh * per > 32 ? 2 : 1;
+        return more && x.fresh * per > 32 ? 2 : 1;
     }
 };
 
@@ -351,7 +352,7 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
 #pragma unroll
             for(int i = 0; i < kHalf; i += 4) {
                 const int at = h * kHalf + i;
-                *(lds_v4f_t*)(uintptr_t)(lds0 + wave * (kHalf * kWave * 4) + i * kWave * 4 + lane * 16)
+                *(lds_v4f_t*)(uintptr_t)(lds0 + (wave * kHalf + i) * kWave * 4 + lane * 16)
                     = v4f{o[t][at / 16][at % 16], o[t][at / 16][at % 16 + 1],
                           o[t][at / 16][at % 16 + 2], o[t][at / 16][at % 16 + 3]};
             }
@@ -484,7 +485,8 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
 #pragma unroll
                 for(int i = 0; i < 8; i += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[t][st * 8 + i], c2, -mc[t]));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[t][st * 8 + i + 1], c2, -mc[t]));
+                    const float p1
+                        = __builtin_amdgcn_exp2f(fmaf(sc[t][st * 8 + i + 1], c2, -mc[t]));
                     l[t] += p0;
                     l[t] += p1;
                     const v2h h = __builtin_convertvector((v2f{p0, p1}), v2h);
@@ -541,8 +543,8 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
     if(runs.cut && threadIdx.x == 0) runs.tasks[run] = tasks;
 }
 
-// Blocks for the sequences of more than 32 rows a key head (MORE: there may be any), two times
-// 32 rows a unit, which unpacks its codes once for both, then for those of up to 32.
+// Blocks for the sequences of more than 32 rows a key head (MORE: the caller expects some), two
+// times 32 rows a unit, which unpacks its codes once for both, then for those of up to 32.
 template <int D, int G, bool MORE>
 __global__ void __launch_bounds__(kThreads, 2)
     attention_kv4_chunks_kernel(CacheView c, ChunkArgs a, Runs few, Runs more,
@@ -551,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     // the waves' values (at a unit's end halves of their results), then the queries
     __shared__ alignas(256) uint8_t lds[kWaves * kKeys * D * 2 + (MORE ? 64 : 32) * D * 2];
     __shared__ float                ml[kWaves * 32 * 2];
-    const Ways     ways{others, a.heads / c.kv_heads, a.table_cols << c.page_shift};
+    const Ways     ways{others, a.heads / c.kv_heads, a.table_cols << c.page_shift, MORE};
     if(!MORE || blockIdx.x >= more.count)
         chunks_run<D, G, 1>(c, a, few, ways, blockIdx.x - (MORE ? more.count : 0), pages, lds, ml);
     else if constexpr(MORE)
@@ -583,7 +585,8 @@ struct JoinSets {
 // task is 32 (64) rows, two a group of lanes; of many one row, of which each group takes every
 // 16th (32nd) partial, and the groups are added up, always in the same order.
 template <int D>
-__global__ void __launch_bounds__(kThreads) attention_kv4_chunks_join_kernel(ChunkArgs a, JoinSets j)
+__global__ void __launch_bounds__(kThreads)
+    attention_kv4_chunks_join_kernel(ChunkArgs a, JoinSets j)
 {
     constexpr uint32_t kLanes = D / 8, kGroups = kThreads / kLanes;
     constexpr uint32_t kEach = (kJoinMost + kThreads - 1) / kThreads;

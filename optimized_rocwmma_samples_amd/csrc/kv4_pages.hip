@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(kSeqs) kv4_trim_kernel(Kv4TrimArgs a)
                 const uint32_t s  = last_not_above(bases, in, f);
                 const uint64_t to = avail + (all - 1 - f);
                 if(to < a.capacity)
-                    a.free[to] = a.table[(size_t)(i0 + s) * a.table_ld + firsts[s] + (f - bases[s])];
+                    a.free[to]
+                        = a.table[(size_t)(i0 + s) * a.table_ld + firsts[s] + (f - bases[s])];
             });
         }
         pages += sum;
@@ -256,7 +257,8 @@ __global__ void __launch_bounds__(kWaveThreads)
         const uint32_t i = i0 + lane;
         uint32_t       n = 0, from = 0, l = 0;
         if(i < a.seqs) {
-            const uint32_t b = clamped(a.starts[i], a.tokens), e = clamped(a.starts[i + 1], a.tokens);
+            const uint32_t b = clamped(a.starts[i], a.tokens);
+            const uint32_t e = clamped(a.starts[i + 1], a.tokens);
             const uint32_t fresh = e > b ? e - b : 0;
             l                    = clamped(a.lens[i], a.table_cols << c.page_shift);
             from                 = (l > fresh ? l - fresh : 0) >> c.page_shift;

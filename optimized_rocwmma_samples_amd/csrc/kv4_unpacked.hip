@@ -162,7 +162,8 @@ __global__ void __launch_bounds__(kThreads, 3)
     // A sequence's row tiles of a gang see more and more keys, the last one all of them.
     auto tiles_of = [&](const Long& x) { return (x.c.fresh + rows - 1) / rows; };
     auto keys_of  = [&](const Long& x, uint32_t tile) { // key tiles
-        return (x.c.len - x.c.fresh + x.pad + min((tile + 1) * rows, x.c.fresh) + kKeys - 1) / kKeys;
+        const uint32_t end = min((tile + 1) * rows, x.c.fresh); // of its rows
+        return (x.c.len - x.c.fresh + x.pad + end + kKeys - 1) / kKeys;
     };
     auto all_keys = [&](const Long& x) { // of all its row tiles
         const uint32_t n = tiles_of(x), before = (x.c.len - x.c.fresh + x.pad) / kKeys;
@@ -295,7 +296,8 @@ UnpackedLayout unpacked_layout(const w8a8_kv4_cache& c, uint32_t seqs, uint32_t 
     const uint64_t longs = std::min<uint64_t>(seqs, tokens / (kFewRows / per + 1));
     const uint64_t each  = ((uint64_t)table_cols * c.page_size + 2 * keys - 1) / keys * keys;
     u.room               = (uint32_t)longs;
-    u.rows = (uint32_t)std::min<uint64_t>(longs * each, kMostBytes / (4ull * c.kv_heads * d) / keys * keys);
+    const uint64_t cap   = kMostBytes / (4ull * c.kv_heads * d) / keys * keys;
+    u.rows               = (uint32_t)std::min(longs * each, cap);
     if(u.rows == 0 || table_cols == 0) return UnpackedLayout{};
     // the gang: as many of a key head's query heads as divide them, and neighbouring tiles
     // of rows up to four blocks

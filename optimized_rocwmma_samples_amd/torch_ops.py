@@ -16,11 +16,15 @@ them without a graph break.
     out = torch.ops.w8a8.attention(q, k, v, seq_starts)
     torch.ops.w8a8.kv4_store(k, v, slots, kc, vc, ks, vs)   # a KV4Cache's four tensors
     out = torch.ops.w8a8.attention_kv4(q, kc, vc, ks, vs, block_table, seq_lens)
+    slots, starts, lens, count = torch.ops.w8a8.kv4_extend(new, lens, table, free, count, 64, n)
+    out = torch.ops.w8a8.attention_kv4_chunks(q, kc, vc, ks, vs, table, lens, starts)
+    pages, left = torch.ops.w8a8.kv4_select(q, codes, scales, table, lens, 64, 64)
 
 The ops are functional (every output is a new tensor), as torch.library
-custom ops must be, but for kv4_store, which writes the cache it is given; the
-package functions keep the in-place and preallocated-output forms.  They run only on device tensors: a CPU tensor
-raises, as everywhere in the package (there is no CPU path).
+custom ops must be, but for those that write what they are given: kv4_store the
+cache, kv4_extend the block table, kv4_trim the stack of free pages, kv4_summarize the
+page keys; the package functions keep the in-place and preallocated-output forms.
+They run only on device tensors: a CPU tensor raises, as everywhere in the package (there is no CPU path).
 
 Reference kernels: smoothquant <- kernel_smoothquant
 (rocwmma_smoothquant.cpp:58-122); gemm <- gemm_quant_tensor_scale
@@ -38,16 +42,22 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import KV4Cache, PackedWeights
+from . import KV4Cache, KV4PageKeys, PackedWeights
 from . import add_rmsnorm_smoothquant as _add_rmsnorm_smoothquant
 from . import attention as _attention
 from . import attention_kv4 as _attention_kv4
+from . import attention_kv4_chunks as _attention_kv4_chunks
 from . import fused_sq_gemm as _fused_sq_gemm
 from . import fused_sq_gemm_packed as _fused_sq_gemm_packed
 from . import gemm as _gemm
 from . import gemm_packed as _gemm_packed
+from . import kv4_extend as _kv4_extend
 from . import kv4_load as _kv4_load
+from . import kv4_page_keys as _kv4_page_keys
+from . import kv4_select as _kv4_select
 from . import kv4_store as _kv4_store
+from . import kv4_summarize as _kv4_summarize
+from . import kv4_trim as _kv4_trim
 from . import moe_ffn as _moe_ffn
 from . import moe_ffn_decode as _moe_ffn_decode
 from . import smoothquant as _smoothquant
@@ -235,7 +245,8 @@ def _(slots, k_codes, v_codes, k_scales, v_scales):
 def attention_kv4(q: Tensor, k_codes: Tensor, v_codes: Tensor, k_scales: Tensor, v_scales: Tensor,
                   block_table: Tensor, seq_lens: Tensor, scale: Optional[float] = None) -> Tensor:
     """Attention of one token per sequence, q [seqs, heads, head_dim], over a KV4Cache's
-    tensors; workspace allocated for the table's columns."""
+    tensors, with one block table or one for each key head; workspace allocated for the
+    table's columns."""
     return _attention_kv4(q, KV4Cache(k_codes, v_codes, k_scales, v_scales), block_table, seq_lens,
                           scale)
 
@@ -243,3 +254,89 @@ def attention_kv4(q: Tensor, k_codes: Tensor, v_codes: Tensor, k_scales: Tensor,
 @attention_kv4.register_fake
 def _(q, k_codes, v_codes, k_scales, v_scales, block_table, seq_lens, scale=None):
     return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("w8a8::kv4_extend", mutates_args=("block_table",))
+def kv4_extend(new_tokens: Tensor, seq_lens: Tensor, block_table: Tensor, free_pages: Tensor,
+               free_count: Tensor, page_size: int,
+               tokens: int) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(slots, starts, lengths, free pages left) of the tokens to come; writes the table's new
+    columns."""
+    new, seqs = seq_lens.new_empty, seq_lens.shape[0]
+    return _kv4_extend(new_tokens, seq_lens, block_table, free_pages, free_count, page_size, tokens,
+                       out=(new(tokens), new(seqs + 1), new(seqs), new(1)))
+
+
+@kv4_extend.register_fake
+def _(new_tokens, seq_lens, block_table, free_pages, free_count, page_size, tokens):
+    new, seqs = seq_lens.new_empty, seq_lens.shape[0]
+    return new(tokens), new(seqs + 1), new(seqs), new(1)
+
+
+@torch.library.custom_op("w8a8::kv4_trim", mutates_args=("free_pages",))
+def kv4_trim(keep: Tensor, seq_lens: Tensor, block_table: Tensor, free_pages: Tensor,
+             free_count: Tensor, page_size: int) -> Tuple[Tensor, Tensor]:
+    """(lengths, free pages) after sequences gave up tokens; writes the stack."""
+    return _kv4_trim(keep, seq_lens, block_table, free_pages, free_count, page_size)
+
+
+@kv4_trim.register_fake
+def _(keep, seq_lens, block_table, free_pages, free_count, page_size):
+    return torch.empty_like(seq_lens), torch.empty_like(free_count)
+
+
+@torch.library.custom_op("w8a8::attention_kv4_chunks", mutates_args=())
+def attention_kv4_chunks(q: Tensor, k_codes: Tensor, v_codes: Tensor, k_scales: Tensor,
+                         v_scales: Tensor, block_table: Tensor, seq_lens: Tensor, starts: Tensor,
+                         scale: Optional[float] = None, max_new: int = 0) -> Tensor:
+    """Attention of each sequence's last tokens, q [tokens, heads, head_dim], over a
+    KV4Cache's tensors; rows of no sequence are undefined."""
+    return _attention_kv4_chunks(q, KV4Cache(k_codes, v_codes, k_scales, v_scales), block_table,
+                                 seq_lens, starts, scale, max_new=max_new)
+
+
+@attention_kv4_chunks.register_fake
+def _(q, k_codes, v_codes, k_scales, v_scales, block_table, seq_lens, starts, scale=None,
+      max_new=0):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("w8a8::kv4_summarize", mutates_args=("page_codes", "page_scales"))
+def kv4_summarize(k_codes: Tensor, v_codes: Tensor, k_scales: Tensor, v_scales: Tensor,
+                  page_codes: Tensor, page_scales: Tensor, block_table: Tensor, seq_lens: Tensor,
+                  starts: Tensor, tokens: int) -> None:
+    """Page keys of the pages that the last tokens of each sequence lie in, into the tensors
+    of KV4PageKeys."""
+    _kv4_summarize(KV4Cache(k_codes, v_codes, k_scales, v_scales),
+                   KV4PageKeys(page_codes, page_scales), block_table, seq_lens, starts, tokens)
+
+
+@kv4_summarize.register_fake
+def _(k_codes, v_codes, k_scales, v_scales, page_codes, page_scales, block_table, seq_lens, starts,
+      tokens):
+    return None
+
+
+@torch.library.custom_op("w8a8::kv4_page_keys", mutates_args=())
+def kv4_page_keys(page_codes: Tensor, page_scales: Tensor, pages: Tensor) -> Tensor:
+    """Values fp32 [n, kv_heads, head_dim] of page keys; undefined for pages outside."""
+    return _kv4_page_keys(KV4PageKeys(page_codes, page_scales), pages)
+
+
+@kv4_page_keys.register_fake
+def _(page_codes, page_scales, pages):
+    return page_scales.new_empty((pages.shape[0], page_codes.shape[1], page_codes.shape[2]))
+
+
+@torch.library.custom_op("w8a8::kv4_select", mutates_args=())
+def kv4_select(q: Tensor, page_codes: Tensor, page_scales: Tensor, block_table: Tensor,
+               seq_lens: Tensor, keep: int, page_size: int) -> Tuple[Tensor, Tensor]:
+    """(pages [seqs, kv_heads, keep], tokens in them [seqs]) for attention_kv4."""
+    return _kv4_select(q, KV4PageKeys(page_codes, page_scales), block_table, seq_lens, keep,
+                       page_size)
+
+
+@kv4_select.register_fake
+def _(q, page_codes, page_scales, block_table, seq_lens, keep, page_size):
+    return (seq_lens.new_empty((q.shape[0], page_codes.shape[1], keep)),
+            torch.empty_like(seq_lens))

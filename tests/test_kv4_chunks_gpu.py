@@ -16,7 +16,8 @@ def starts_of(news, first=0):
     return (np.concatenate([[0], np.cumsum(news)]) + first).tolist()
 
 
-def check(w8a8, gpu, c, table, lens, news, heads, seed, spread=2.0, first=0, behind=0, max_new=None):
+def check(w8a8, gpu, c, table, lens, news, heads, seed, spread=2.0, first=0, behind=0,
+          max_new=None):
     """The rows of the sequences against the formula, the others left as they were."""
     import attention_ref as R
     import torch
@@ -59,6 +60,20 @@ def test_chunks_long(w8a8, gpu, dim, group, heads, kv_heads, lens, news):
     table = _table(70, 64, len(lens), 5, gpu)
     check(w8a8, gpu, c, table, lens, news, heads, 6)
     check(w8a8, gpu, c, table, lens, news, heads, 6, max_new=max(news))
+    # a bound that does not hold costs time, not rows
+    check(w8a8, gpu, c, table, lens, news, heads, 6, max_new=1)
+    check(w8a8, gpu, c, table, lens, news, heads, 6, max_new=20)
+
+
+@pytest.mark.parametrize("dim,group", WIDTHS)
+@pytest.mark.parametrize("heads,kv_heads", [(8, 1), (10, 2), (16, 8), (34, 2), (3, 3)])
+@pytest.mark.parametrize("lens,news", [([600], [600]), ([701, 5, 900], [513, 5, 400]),
+                                       ([1000, 1000], [577, 260]), ([131, 650], [130, 519])])
+def test_chunks_of_many_rows(w8a8, gpu, dim, group, heads, kv_heads, lens, news):
+    # sequences of more than 512 rows a key head: first new tokens at any place of a key tile
+    c = _filled(w8a8, gpu, 70, kv_heads, dim, 16, group, dim + heads)
+    table = _table(70, 63, len(lens), heads, gpu)
+    check(w8a8, gpu, c, table, lens, news, heads, 3)
 
 
 def test_chunks_many_sequences(w8a8, gpu):
@@ -78,8 +93,8 @@ def test_chunks_rows_of_no_sequence(w8a8, gpu):
     # tokens than there are, whose first rows see nothing
     c = _filled(w8a8, gpu, 20, 2, 128, 16, 32, 5)
     table = _table(20, 6, 5, 8, gpu)
-    _, got = check(w8a8, gpu, c, table, [50, 0, -9, 2 ** 31 - 1, 4], [9, 3, 2, 7, 11], 4, 1, first=5,
-                   behind=6)
+    _, got = check(w8a8, gpu, c, table, [50, 0, -9, 2 ** 31 - 1, 4], [9, 3, 2, 7, 11], 4, 1,
+                   first=5, behind=6)
     starts = starts_of([9, 3, 2, 7, 11], 5)
     assert (got[starts[1]: starts[3]] == 0).all() and (got[starts[4]: starts[4] + 7] == 0).all()
 
@@ -89,7 +104,8 @@ def test_chunks_nothing(w8a8, gpu):
     c = _filled(w8a8, gpu, 3, 2, 64, 16, 32, 5)
     q = torch.ones((4, 4, 64), dtype=torch.float16, device=gpu)
     none = torch.empty((2, 0), dtype=torch.int32, device=gpu)
-    assert (w8a8.attention_kv4_chunks(q, c, none, ints([5, 5], gpu), ints([0, 3, 4], gpu)) == 0).all()
+    got = w8a8.attention_kv4_chunks(q, c, none, ints([5, 5], gpu), ints([0, 3, 4], gpu))
+    assert (got == 0).all()
     bad = torch.full((2, 9), -1, dtype=torch.int32, device=gpu)
     got = w8a8.attention_kv4_chunks(q, c, bad, ints([140, 144], gpu), ints([0, 3, 4], gpu))
     assert (got == 0).all()
@@ -116,7 +132,7 @@ def test_chunks_starts_out_of_order(w8a8, gpu):
     assert torch.equal(a[6:], d[6:])
 
 
-@pytest.mark.parametrize("news", [[6, 20], [40, 90]])
+@pytest.mark.parametrize("news", [[6, 20], [40, 90], [61, 140]])
 def test_chunks_what_is_masked_does_not_reach(w8a8, gpu, news):
     # NaN behind a row's position, in pages that are not its own and outside the cache
     import torch
@@ -135,7 +151,7 @@ def test_chunks_what_is_masked_does_not_reach(w8a8, gpu, news):
     for at in (lens[1] - news[1], lens[1] - news[1] // 2, lens[1] - 1, 33 if news[1] < 100 else 0):
         d = w8a8.KV4Cache(*(t.clone() for t in (c.k_codes, c.v_codes, c.k_scales, c.v_scales)))
         page = int(table[1, at // 16])
-        if page < 0:
+        if not 0 <= page < c.pages:
             continue
         d.v_scales[page, 1, at % 16, 2] = float("nan")
         got = w8a8.attention_kv4_chunks(q, d, table, ints(lens, gpu), ints(starts, gpu))

@@ -110,8 +110,8 @@ def random_keys(w8a8, gpu, pages, heads, dim, seed, levels=128):
 
 @pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (128, 8, 2), (128, 17, 1), (64, 6, 2)])
 @pytest.mark.parametrize("page,lens,keep", [(16, [0, 1, 16, 17, 160, 250], 4), (16, [900, 33], 1),
-                                            (32, [3000, 64, 97], 2), (64, [64 * 40, 64 * 39 + 1], 39),
-                                            (64, [5, 100], 300)])
+                                            (32, [3000, 64, 97], 2), (64, [5, 100], 300),
+                                            (64, [64 * 40, 64 * 39 + 1], 39)])
 def test_select(w8a8, gpu, dim, heads, kv_heads, page, lens, keep):
     from attention_ref import randn
     cols = P.ceil_div(max(lens), page)

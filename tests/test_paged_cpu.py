@@ -1,0 +1,167 @@
+"""What the calls of the paged 4-bit cache in service refuse, before any HIP call (no GPU
+needed), through the C ABI and through the package."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+import optimized_rocwmma_samples_amd as W
+from optimized_rocwmma_samples_amd import _lib
+from test_operators_cpu import BAD_CACHES, INV, NOT, P, _cache, _refused, _status
+
+EXTEND = dict(new=P, lens=P, seqs=3, table=P, cols=4, ld=4, free=P, capacity=9, count=P, page=16,
+              slots=P, tokens=5, starts=P, lens_out=P, count_out=P, stream=None)
+TRIM = dict(keep=P, lens=P, seqs=3, table=P, cols=4, ld=4, free=P, capacity=9, count=P, page=16,
+            lens_out=P, count_out=P, stream=None)
+
+TABLES = [(dict(ld=3), INV, "table_ld"), (dict(page=8), NOT, "page_size"),
+          (dict(page=48), NOT, "page_size"), (dict(page=2048), NOT, "page_size"),
+          (dict(cols=2 ** 27, ld=2 ** 27), NOT, "2^31"), (dict(seqs=2 ** 28), NOT, "2^27"),
+          (dict(table=None), INV, "null"), (dict(count=None), INV, "null"),
+          (dict(free=None), INV, "null"), (dict(lens=None), INV, "null"),
+          (dict(lens_out=None), INV, "null"), (dict(count_out=None), INV, "null"),
+          (dict(capacity=2 ** 31), NOT, "free_capacity")]
+
+
+@pytest.mark.parametrize("changes,code,needle", TABLES + [
+    (dict(new=None), INV, "null"), (dict(slots=None), INV, "null"), (dict(starts=None), INV, "null"),
+    (dict(tokens=2 ** 31 - 1), NOT, "tokens")])
+def test_extend_refusals(w8a8, changes, code, needle):
+    _refused("w8a8_kv4_extend", EXTEND, changes, code, needle)
+
+
+@pytest.mark.parametrize("changes,code,needle", TABLES + [
+    (dict(keep=None), INV, "null"),
+    (dict(seqs=2 ** 20, cols=2 ** 12, ld=2 ** 12), NOT, "seqs * table_cols")])
+def test_trim_refusals(w8a8, changes, code, needle):
+    _refused("w8a8_kv4_trim", TRIM, changes, code, needle)
+
+
+def _keys(**kw):
+    d = dict(codes=P, scales=P, pages=4, kv_heads=2, head_dim=128)
+    d.update(kw)
+    return _lib.Kv4PageKeys(*d.values())
+
+
+BAD_KEYS = [(dict(codes=None), INV, "null"), (dict(scales=None), INV, "null"),
+            (dict(pages=0), INV, "pages"), (dict(kv_heads=0), INV, "kv_heads"),
+            (dict(head_dim=96), NOT, "head_dim"), (dict(codes=P + 8), NOT, "aligned")]
+
+
+def _calls(cache, keys):
+    c, k = ctypes.byref(cache), ctypes.byref(keys)
+    return {
+        "chunks": ("w8a8_attention_kv4_chunks", dict(
+            q=P, cache=c, table=P, cols=4, ld=4, lens=P, starts=P, out=P, seqs=2, tokens=6, heads=8,
+            max_new=0, ldq=1024, ldo=1024, scale=0.1, ws=P, ws_bytes=1 << 30, stream=None)),
+        "selected": ("w8a8_attention_kv4_selected", dict(
+            q=P, cache=c, tables=P, cols=4, lens=P, out=P, seqs=2, heads=8, ldq=1024, ldo=1024,
+            scale=0.1, ws=None, ws_bytes=0, stream=None)),
+        "summarize": ("w8a8_kv4_summarize", dict(
+            cache=c, keys=k, table=P, cols=4, ld=4, lens=P, starts=P, seqs=2, tokens=6,
+            stream=None)),
+        "page_keys": ("w8a8_kv4_page_keys_load", dict(keys=k, pages=P, count=3, out=P, stream=None)),
+        "select": ("w8a8_kv4_select", dict(
+            q=P, keys=k, table=P, cols=4, ld=4, lens=P, page=16, chosen=P, keep=2, lens_out=P,
+            seqs=2, heads=8, ldq=1024, ws=None, ws_bytes=0, stream=None))}
+
+
+@pytest.mark.parametrize("kw,code,needle", BAD_CACHES)
+def test_cache_refusals(w8a8, kw, code, needle):
+    calls = _calls(_cache(**kw), _keys())
+    for which in ("chunks", "selected", "summarize"):
+        _refused(*calls[which], {}, code, needle)
+
+
+@pytest.mark.parametrize("kw,code,needle", BAD_KEYS)
+def test_page_keys_refusals(w8a8, kw, code, needle):
+    calls = _calls(_cache(), _keys(**kw))
+    for which in ("summarize", "page_keys", "select"):
+        _refused(*calls[which], {}, code, needle)
+
+
+@pytest.mark.parametrize("which,changes,code,needle", [
+    ("chunks", dict(q=None), INV, "null"), ("chunks", dict(starts=None), INV, "null"),
+    ("chunks", dict(table=None), INV, "null"), ("chunks", dict(heads=7), INV, "divide"),
+    ("chunks", dict(ldq=1016), INV, "ldq"), ("chunks", dict(ldo=1028), NOT, "aligned"),
+    ("chunks", dict(out=P + 8), NOT, "aligned"), ("chunks", dict(ld=3), INV, "table_ld"),
+    ("chunks", dict(scale=float("nan")), INV, "scale"), ("chunks", dict(ws=None), INV, "workspace"),
+    ("chunks", dict(ws=P + 16), INV, "256-byte"), ("chunks", dict(ws_bytes=1000), INV, "workspace"),
+    ("chunks", dict(tokens=2 ** 31), NOT, "too many"),
+    ("chunks", dict(tokens=2 ** 20, cols=2 ** 24, ld=2 ** 24), NOT, "too many"),
+    ("selected", dict(q=None), INV, "null"), ("selected", dict(tables=None), INV, "null"),
+    ("selected", dict(lens=None), INV, "null"), ("selected", dict(heads=5), INV, "divide"),
+    ("selected", dict(ldo=8), INV, "ldo"), ("selected", dict(q=P + 4), NOT, "aligned"),
+    ("selected", dict(cols=2 ** 26), NOT, "2^31"),
+    ("selected", dict(ws=P + 8, ws_bytes=1 << 20), INV, "workspace"),
+    ("summarize", dict(table=None), INV, "null"), ("summarize", dict(starts=None), INV, "null"),
+    ("summarize", dict(ld=2), INV, "table_ld"),
+    ("summarize", dict(tokens=2 ** 31 - 1, seqs=2 ** 26), NOT, "too many"),
+    ("page_keys", dict(pages=None), INV, "null"), ("page_keys", dict(out=None), INV, "null"),
+    ("page_keys", dict(out=P + 4), NOT, "aligned"),
+    ("page_keys", dict(count=2 ** 27), NOT, "too many"),
+    ("select", dict(q=None), INV, "null"), ("select", dict(chosen=None), INV, "null"),
+    ("select", dict(lens_out=None), INV, "null"), ("select", dict(keep=0), INV, "keep"),
+    ("select", dict(heads=9), INV, "divide"), ("select", dict(ldq=8), INV, "ldq"),
+    ("select", dict(page=17), NOT, "page_size"), ("select", dict(seqs=2 ** 23), NOT, "too many"),
+    ("select", dict(keep=2 ** 31 - 1), NOT, "too many"),
+    ("select", dict(cols=5000, ld=5000), INV, "workspace"),
+    ("select", dict(cols=5000, ld=5000, ws=P + 4, ws_bytes=1 << 30), INV, "workspace"),
+    ("select", dict(cols=5000, ld=5000, ws=P, ws_bytes=5000), INV, "workspace")])
+def test_refusals(w8a8, which, changes, code, needle):
+    _refused(*_calls(_cache(), _keys())[which], changes, code, needle)
+
+
+def test_page_keys_of_another_cache(w8a8):
+    for kw in (dict(pages=5), dict(kv_heads=1), dict(head_dim=64)):
+        _refused(*_calls(_cache(), _keys(**kw))["summarize"], {}, INV, "not this cache's")
+    rc, msg = _status("w8a8_kv4_page_keys_load", [None, P, 3, P, None])
+    assert rc == INV and "null" in msg
+
+
+def test_nothing_to_do(w8a8):
+    calls = _calls(_cache(), _keys())
+    for which, changes in (("chunks", dict(seqs=0, q=None)), ("chunks", dict(tokens=0, ws=None)),
+                           ("selected", dict(seqs=0, q=None)), ("summarize", dict(tokens=0)),
+                           ("summarize", dict(seqs=0, table=None)), ("page_keys", dict(count=0)),
+                           ("select", dict(seqs=0, q=None))):
+        name, args = calls[which]
+        assert _status(name, list(dict(args, **changes).values()))[0] == 0, which
+
+
+def test_workspace_sizes(w8a8):
+    def chunks(seqs, tokens, heads, cols, max_new=0, **kw):
+        c = _cache(**kw)
+        return W.library().w8a8_attention_kv4_chunks_workspace_size(
+            ctypes.byref(c), seqs, tokens, heads, cols, max_new)
+    assert chunks(0, 5, 8, 4) == chunks(5, 0, 8, 4) == chunks(5, 5, 7, 4) == 0
+    assert chunks(5, 5, 8, 2, page_size=64) == 0       # 128 keys at the most: nothing is cut
+    assert 0 < chunks(5, 5, 8, 3, page_size=64) < 1 << 28
+    few = chunks(8, 64, 8, 2048, max_new=8)
+    assert 0 < few < chunks(8, 4096, 8, 2048)           # the long ones' keys and values
+    for args in ((1, 2048, 32, 2048), (64, 65536, 64, 8192), (1024, 65536, 8, 8192)):
+        assert 0 < chunks(*args, kv_heads=8, pages=1000) < 2 << 30
+    assert W.kv4_select_workspace_size(3, 8, 100, 5) == 0
+    assert W.kv4_select_workspace_size(3, 8, 10000, 5) == 3 * 8 * 10000 * 4
+    assert W.kv4_select_workspace_size(3, 8, 10000, 10000) == 0
+
+
+def test_package_refuses(w8a8):
+    torch = pytest.importorskip("torch")
+    n = torch.zeros(3, dtype=torch.int32)
+    one, table = n[:1], torch.zeros((3, 4), dtype=torch.int32)
+    with pytest.raises(ValueError, match="CPU"):
+        W.kv4_extend(n, n, table, n, one, 16, 3)
+    with pytest.raises(ValueError, match="CPU"):
+        W.kv4_trim(n, n, table, n, one, 16)
+    with pytest.raises(ValueError, match="CPU"):
+        W.KV4PageKeys(torch.zeros((2, 2, 64), dtype=torch.int8), torch.zeros((2, 2)))
+    W._torch()
+    for t in (n.long(), n[None], n[::2], torch.zeros(4, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="contiguous int32"):
+            W._kv4_ints(n.device, "lens", t, 3)
+    for t in (table.long(), table[0], table.t(), table.expand(2, 3, 4)):
+        with pytest.raises(ValueError):
+            W._kv4_table(t, 3)
+    assert W._kv4_table(torch.zeros((3, 9), dtype=torch.int32)[:, 2:6], 3) == (4, 9)

@@ -4,14 +4,17 @@
 //   out[t, h] = sum_j p[j] v[j],  p = softmax of scale * (q[t, h] . k[j]) over the tokens j of
 //   t's sequence up to t itself; the rows of q are the sequence's last tokens.
 //
-// The rows of a unit of work are the (token, query head) pairs of one key head, 32 at a
-// time: row r is token r / per, head r % per, per query heads sharing the key head.  Units
-// are walked in steps of 128 keys, 32 a wave.  All units' steps lie in one line, which is
-// cut into as many equal runs as there are blocks; what a cut leaves of a unit is written as
+// Sequences of few rows are computed here, those of many in kv4_unpacked.hip (kFewRows in
+// kv4_chunks.hpp).  The rows of a unit of work are (token, query head) pairs of one key head:
+// row r is token r / per, head r % per, per query heads sharing the key head.  A unit has 32
+// of them, or 64 where the sequence has more than 32 (24 x 5 tokens of 32/8 heads: 78 us in
+// units of 32, 63 in units of 64, whose codes are unpacked once for both).  Units are walked
+// in steps of 128 keys, 32 a wave.  All units' steps lie in one line, which is cut into as many
+// equal runs as there are blocks, two a CU; what a cut leaves of a unit is written as
 // partials (sum of p v, maximum and sum of p of each row) and joined by a second launch.
 //   * S^T = K Q^T with v_mfma_f32_32x32x16_f16: srcA rows are keys, and a lane's operand is 8
 //     channels of one key, which is a dword of its codes: unpacked, scaled and used where
-//     it was loaded.
+//     it was loaded.  The queries lie in LDS in the order of the other operand.
 //   * The scores of one query row lie in a lane (and lane ^ 32), so softmax stays there, and
 //     the probabilities are the srcB operand of O^T += V^T P^T as they are.
 //   * V^T's rows are channels: a wave unpacks its 32 rows of values into a tile of its own in
@@ -20,7 +23,18 @@
 // A code n becomes 1024 + n by two bit operations a pair, n - 8 and then offset + scale *
 // (n - 8), rounded once: half of what kv4_load gives, since a group that reaches the ends of
 // fp16 may pass them by half a step (the halves go into the scale of the scores and of the
-// result).
+// result).  Three roundings of 2^-11 are left, of keys, values and probabilities, as in
+// attention over fp16 keys and values; the keys' is the largest part of the error (4.9e-4 of a
+// result's 4.5e-4 .. 6.7e-4 where a product of fp32 keys leaves 2.1e-4).  Codes that enter as
+// 1 + n / 16, exactly, with scales applied around the products, as for single tokens, would
+// take a product per group and query row and cost long chunks a quarter of their time.
+//
+// MI355X, 32 query and 8 key heads of 128, groups of 32: 24 sequences of 5 tokens behind up to
+// 8192 (90 MB of cache in use) take 61 us of this kernel and 9 of the join: 1.5 TB/s, bound by
+// its vector instructions (unpacking is about half of them) and, with two waves a SIMD, by what
+// they wait for LDS and for each other's products.  One token of 131072 takes 49 + 5 us.  Codes
+// staged through LDS by DMA (62, 57), a key-first order of the step (72), three blocks a CU
+// (spills) are not faster.
 #include "kv4_chunks.hpp"
 
 #include <algorithm>
@@ -40,7 +54,7 @@ constexpr int      kWaves   = 4;
 constexpr int      kThreads = kWaves * kWave;
 constexpr int      kKeys    = 32;              // a wave's a step
 constexpr int      kStep    = kWaves * kKeys;  // keys of a step
-constexpr uint32_t kBlocks  = 512;             // two a CU
+constexpr uint32_t kBlocks  = 512;             // runs: two a CU, all resident
 
 __host__ __device__ inline uint32_t steps_of(uint32_t len)
 {

@@ -7,10 +7,12 @@
 namespace w8a8 {
 namespace {
 
-// A sequence with more rows (new tokens x query heads a key head) than this has its keys
-// and values unpacked to fp16 first, once, and then takes the prompts' kernel over them;
-// the others unpack the codes they use where they use them, which costs each 32 rows
-// twice what the products take.
+// A sequence with more rows (new tokens x query heads a key head) than this has its keys and
+// values unpacked to fp16 first, once, and then takes the prompts' tiles over them; the others
+// unpack codes where they use them, each 64 rows again.  us, one sequence of 8192 tokens, 32/8
+// heads of 128, unpacked where used and unpacked first: 260 rows (65 tokens) 47 .. 59 and
+// 69 .. 73, 512 rows 50 .. 64 and 82 .. 88; 1024 rows take 90 unpacked first, twice the 512 rows'
+// work where used.
 constexpr uint32_t kFewRows = 512;
 
 // One sequence of the call.
@@ -40,6 +42,7 @@ struct LongList {
     uint32_t* total; // [0] sequences in the list, [1] their rows
     Long*     list;
     uint8_t*  flags; // [seqs] 1: in the list
+    uint32_t  per, most_len, keys; // query heads a key head, tokens at the most, keys of a tile
 };
 
 } // namespace

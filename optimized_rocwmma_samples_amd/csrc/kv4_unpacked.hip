@@ -2,8 +2,8 @@
 // sequences' keys and values are unpacked to fp16 once, and the tiles of attention.hip run
 // over them.
 //
-// Unpacking costs 4 bytes written and read again for each of the cache's, some 2 % of a chunk
-// of 2048 tokens' time with four query heads a key head; unpacked by each block where it is
+// Unpacking costs 4 bytes written and read again for each of the cache's, some 4 % of the time
+// of a chunk of 2048 tokens with four query heads a key head; unpacked by each block where it is
 // used it would be a fifth of every block's instructions.
 //
 // The work of a sequence is cut into units of 128 rows of one query head over their key
@@ -12,6 +12,12 @@
 // the first find them in their XCD's L2.  All gangs' key tiles lie in one line, which is cut
 // into equal runs, one a gang of blocks, all resident: any mix of chunks keeps the chip evenly
 // busy.  What a cut leaves of a unit is joined by another launch.
+//
+// MI355X, 2048 new of 18432 tokens, 32/8 heads of 128: unpacking 25 us (75 MB written at 3 to
+// 4 TB/s), attention 660 to 690 (585 GFLOP at 850 to 890 TFLOP/s, of the 1307 of a large
+// product; bound like the prompts' kernel by score products that wait for their key fragments
+// and by vector instructions beside the matrix unit), joining 20 (up to 100 MB of partials).
+// Without unpacking, by the kernel of few rows, the same chunk took 1190.
 #include "attention_tile.hpp"
 #include "kv4_chunks.hpp"
 
@@ -26,45 +32,49 @@ template <int D>
 constexpr int kKeysOf = 4096 / D;
 
 // ---- which sequences ------------------------------------------------------------------
-__global__ void __launch_bounds__(kWave)
-    kv4_long_kernel(ChunkArgs a, LongList l, uint32_t per, uint32_t most_len, uint32_t keys)
+struct Which {
+    uint32_t count, rows; // sequences that are unpacked, and their rows in all
+};
+
+// Finds them, one wave: emit(sequence, is one, place in the list, entry), lane = sequence.
+template <class E>
+__device__ __forceinline__ Which find_longs(const ChunkArgs& a, const LongList& l, E emit)
 {
-    const uint32_t lane = threadIdx.x;
-    uint32_t       count = 0;
-    uint64_t       rows = 0, fresh = 0; // unpacked rows and new tokens so far
+    const uint32_t lane = threadIdx.x % kWave;
+    Which          w{};
+    bool           full = false;
     for(uint32_t i0 = 0; i0 < a.seqs; i0 += kWave) {
         const uint32_t i = i0 + lane;
         Chunk          c{};
-        if(i < a.seqs) c = chunk_of(a, i, most_len);
-        const bool     want = (uint64_t)c.fresh * per > kFewRows && c.len >= c.fresh;
-        const uint32_t pad  = (keys - (c.len - c.fresh) % keys) % keys;
-        const uint32_t need = want ? (c.len + pad + keys - 1) / keys * keys : 0;
-        uint64_t       s = need, f = want ? c.fresh : 0;
-#pragma unroll
-        for(int d = 1; d < kWave; d <<= 1) {
-            const uint64_t so = __shfl_up((unsigned long long)s, d, kWave);
-            const uint64_t fo = __shfl_up((unsigned long long)f, d, kWave);
-            if(lane >= (uint32_t)d) {
-                s += so;
-                f += fo;
-            }
-        }
-        // (starts that ascend never have more new tokens than rows, nor more sequences than
-        // the list has room for)
-        bool           ok   = want && rows + s <= l.rows && fresh + f <= a.tokens;
-        const uint64_t oks  = __ballot(ok);
-        const uint32_t at   = count + __builtin_popcountll(oks & ((1ull << lane) - 1));
-        ok                  = ok && at < l.most;
-        if(ok) l.list[at] = {i, (uint32_t)(rows + s - need), need, pad, c, 0};
-        if(i < a.seqs) l.flags[i] = ok;
-        count = min(count + (uint32_t)__builtin_popcountll(oks), l.most);
-        rows += __shfl((unsigned long long)s, kWave - 1, kWave);
-        fresh += __shfl((unsigned long long)f, kWave - 1, kWave);
+        if(i < a.seqs) c = chunk_of(a, i, l.most_len);
+        const bool     want = (uint64_t)c.fresh * l.per > kFewRows && c.len >= c.fresh;
+        const uint32_t pad  = (l.keys - (c.len - c.fresh) % l.keys) % l.keys;
+        // (one row more than there is room for is as good as any number)
+        const uint32_t need
+            = want ? min((c.len + pad + l.keys - 1) / l.keys * l.keys, l.rows + 1) : 0;
+        const uint32_t s  = lanes_sum(need);
+        bool           ok = want && !full && s <= l.rows - w.rows;
+        const uint64_t in = __ballot(ok);
+        const uint32_t at = w.count + __builtin_popcountll(in & ((1ull << lane) - 1));
+        ok                = ok && at < l.most; // more only where starts do not ascend
+        if(i < a.seqs) emit(i, ok, at, Long{i, w.rows + s - need, need, pad, c, 0});
+        const uint64_t oks = __ballot(ok);
+        full               = full || oks != __ballot(want); // those behind it find no room
+        w.count += __builtin_popcountll(oks);
+        if(oks != 0) w.rows += __builtin_amdgcn_readlane((int)s, 63 - __builtin_clzll(oks));
     }
-    if(lane == 0) {
-        l.total[0] = count;
-        l.total[1] = count != 0 ? l.list[count - 1].base + l.list[count - 1].need : 0;
-    }
+    return w;
+}
+
+// The list of many sequences; of up to 64 the next kernel's blocks find them by themselves,
+// which saves 5 us.
+__global__ void __launch_bounds__(kWave) kv4_long_kernel(ChunkArgs a, LongList l)
+{
+    const Which w = find_longs(a, l, [&](uint32_t i, bool ok, uint32_t at, const Long& x) {
+        if(ok) l.list[at] = x;
+        l.flags[i] = ok;
+    });
+    if(threadIdx.x == 0) *reinterpret_cast<Which*>(l.total) = w;
 }
 
 // ---- unpacking ------------------------------------------------------------------------
@@ -92,17 +102,37 @@ __global__ void __launch_bounds__(256)
     kv4_unpack_kernel(CacheView c, ChunkArgs a, LongList l, Unpacked u, uint32_t pages)
 {
     constexpr uint32_t kPer = D / 8, kRound = 256 / kPer; // chunks of a row, rows a round
+    __shared__ Long    longs[kWave];
+    __shared__ Which   found;
     const uint32_t     lane = threadIdx.x % kWave;
-    const uint32_t     count = l.total[0], work = l.total[1] / 32 * c.kv_heads;
+    const bool         here = a.seqs <= kWave; // the list is made here
+    if(here) {
+        if(threadIdx.x < kWave) {
+            const bool  first = blockIdx.x == 0;
+            const Which w = find_longs(a, l, [&](uint32_t i, bool ok, uint32_t at, const Long& x) {
+                if(ok) longs[at] = x;
+                if(ok && first) l.list[at] = x;
+                if(first) l.flags[i] = ok;
+            });
+            if(lane == 0) {
+                found = w;
+                if(first) *reinterpret_cast<Which*>(l.total) = w;
+            }
+        }
+        __syncthreads();
+    }
+    const Which     w    = here ? found : *reinterpret_cast<const Which*>(l.total);
+    const Long*     list = here ? longs : l.list;
+    const uint32_t  count = w.count, work = w.rows / 32 * c.kv_heads;
     for(uint32_t at = blockIdx.x; at < work; at += gridDim.x) {
         const uint32_t row0 = at / c.kv_heads * 32, head = at % c.kv_heads;
         uint32_t       which = 0; // the last sequence that begins at or before row0
         for(uint32_t i0 = 0; i0 < count; i0 += kWave) {
             const uint64_t in
-                = __ballot(i0 + lane < count && l.list[min(i0 + lane, count - 1)].base <= row0);
+                = __ballot(i0 + lane < count && list[min(i0 + lane, count - 1)].base <= row0);
             which += __builtin_popcountll(in);
         }
-        const Long&    x = l.list[which - 1];
+        const Long&    x = list[which - 1];
         const uint32_t from = row0 - x.base; // of the sequence's rows
         auto           page_of = [&](uint32_t r) { // of the token in row r, or -1
             const uint32_t t = from + r - x.pad;
@@ -307,6 +337,11 @@ UnpackedLayout unpacked_layout(const w8a8_kv4_cache& c, uint32_t seqs, uint32_t 
     u.tiles   = u.heads >= 4 ? 1 : 4 / u.heads;
     u.members = u.heads * u.tiles;
     u.runs    = kUnpackedBlocks / 8 / u.members * 8;
+    // the line of key tiles is counted in 32 bits, whatever the starts are (only some ten
+    // thousand query heads on one key head could make it longer)
+    if((tokens / (u.tiles * kRows) + 1ull) * (u.rows / keys) * c.kv_heads * (per / u.heads)
+       > 0xFFFFFFFFull)
+        return UnpackedLayout{};
     size_t at   = 0;
     auto   room = [&](size_t bytes) {
         const size_t here = at;
@@ -331,13 +366,13 @@ void launch_unpacked(const w8a8_kv4_cache& c, const ChunkArgs& a, const Unpacked
                      const Runs& runs, uint8_t* ws, hipStream_t stream)
 {
     const LongList list{u.room, u.rows, reinterpret_cast<uint32_t*>(ws + u.total),
-                        reinterpret_cast<Long*>(ws + u.list), ws + u.flags};
+                        reinterpret_cast<Long*>(ws + u.list), ws + u.flags,
+                        a.heads / c.kv_heads, a.table_cols * c.page_size,
+                        4096 / c.head_dim};
     const Unpacked un{reinterpret_cast<uint16_t*>(ws + u.k), reinterpret_cast<uint16_t*>(ws + u.v),
                       reinterpret_cast<uint32_t*>(ws + u.missing)};
     const Gang     gang{u.members, u.heads, u.tiles};
-    const uint32_t keys = 4096 / c.head_dim;
-    kv4_long_kernel<<<1, kWave, 0, stream>>>(a, list, a.heads / c.kv_heads,
-                                             a.table_cols * c.page_size, keys);
+    if(a.seqs > kWave) kv4_long_kernel<<<1, kWave, 0, stream>>>(a, list);
     const uint32_t groups = (uint32_t)std::min<uint64_t>((uint64_t)u.rows / 32 * c.kv_heads, 4096);
     with_widths(c, [&](auto d, auto g) {
         kv4_unpack_kernel<d(), g()><<<groups, 256, 0, stream>>>(view(c), a, list, un, c.pages);

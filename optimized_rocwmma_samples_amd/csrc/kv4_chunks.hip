@@ -140,7 +140,7 @@ struct Place {
 // A block's run: which steps of the line it takes, and where the first of them lies.
 struct Line {
     uint32_t q, r;      // runs have q steps, the first r of them one more
-    uint32_t left, end; // its steps, and the place on the line behind the last
+    uint32_t left, end; // its steps, and the place on the line behind the last (of equal runs)
     uint32_t seq, at;   // the first one's sequence, and place in it
 };
 
@@ -163,46 +163,69 @@ __device__ __forceinline__ uint32_t unit_tiles(const Chunk& x, uint32_t per, uin
     return (x.fresh * per + 32 * kind - 1) / (32 * kind);
 }
 
-// Run `run` of `runs` on the line of the sequences whose units are T tiles of 32 rows.
+// Run `run` of `runs` on the line of the sequences whose units are T tiles of 32 rows: equal
+// runs, or one unit each.
 template <int T>
 __device__ __forceinline__ Line find_line(const ChunkArgs& a, const Ways& w, uint32_t kv_heads,
                                           uint32_t run, uint32_t runs)
 {
     const uint32_t lane = threadIdx.x % kWave;
-    uint32_t       n, s;
+    uint32_t       n, units, steps, s;
     const auto     scan = [&](uint32_t i0) { // 64 sequences' steps
         const uint32_t i = i0 + lane;
-        n                = 0;
+        units = steps = 0;
         if(i < a.seqs) {
             const Chunk x = chunk_of(a, i, w.most);
-            if(w.kind(a, x, i) == T) n = unit_tiles(x, w.per, T) * kv_heads * steps_of(x.len);
+            if(w.kind(a, x, i) == T) {
+                units = unit_tiles(x, w.per, T) * kv_heads;
+                steps = steps_of(x.len);
+            }
         }
+        n = units * steps;
         s = lanes_sum(n);
         return (uint32_t)__builtin_amdgcn_readlane((int)s, kWave - 1);
     };
     float    total = 0.f; // starts that do not ascend may count rows so often that sums wrap
-    uint32_t all   = 0;
+    uint32_t all = 0, most_steps = 0, all_units = 0;
     for(uint32_t i = 0; i < a.seqs; i += kWave) {
         all += scan(i);
         total += wave_sum((float)n);
+        most_steps = max(most_steps, (uint32_t)-wave_min_i32(-(int32_t)steps));
+        all_units += __builtin_amdgcn_readlane((int)lanes_sum(units), kWave - 1);
     }
     if(total > 2147483648.f) all = 0;
-    Line l;
-    l.q         = all / runs;
-    l.r         = all % runs;
+    // One unit each where no unit has many steps more than an equal run: what is cut costs its
+    // run's end and the join, some 5 to 10 us with many units, less with few; a step 2 to 3.
+    // us cut and whole: 24 sequences of 256 tokens, 4 new ones each of 64/8 heads (192 units of
+    // 2 steps) 17.9, 12.4, of 1024 (8 steps for 3) 27.1, 22.2; 4 of 768, 1 new of 32/8 (32 units
+    // of 6 steps for 1) 14.5, 16.6.
+    const bool whole
+        = all_units <= runs && most_steps <= (all + runs - 1) / runs + min(5u, 1 + all_units / 32);
+    Line l{};
+    if(whole) {
+        l.q    = 1;
+        l.left = run < all_units && all != 0 ? 1 : 0;
+    } else {
+        l.q    = all / runs;
+        l.r    = all % runs;
+        l.left = l.q + (run < l.r ? 1 : 0);
+    }
     uint32_t at = run * l.q + min(run, l.r);
-    l.left      = l.q + (run < l.r ? 1 : 0);
     l.end       = at + l.left;
-    l.seq = l.at = 0;
     if(l.left == 0) return l;
     for(uint32_t i = 0; i < a.seqs; i += kWave) {
-        const uint32_t sum // (of up to 64 sequences it is still there)
-            = a.seqs > kWave ? scan(i) : (uint32_t)__builtin_amdgcn_readlane((int)s, kWave - 1);
+        if(a.seqs > kWave) scan(i); // (of up to 64 sequences it is still there)
+        if(whole) s = lanes_sum(units);
+        const uint32_t sum = (uint32_t)__builtin_amdgcn_readlane((int)s, kWave - 1);
         if(at < sum) {
             const int f = __builtin_ctzll(__ballot(s > at));
             l.at = at - ((uint32_t)__builtin_amdgcn_readlane((int)s, f)
-                         - (uint32_t)__builtin_amdgcn_readlane((int)n, f));
+                         - (uint32_t)__builtin_amdgcn_readlane((int)(whole ? units : n), f));
             l.seq = i + f;
+            if(whole) {
+                l.left = __builtin_amdgcn_readlane((int)steps, f);
+                l.at *= l.left;
+            }
             break;
         }
         at -= sum;
@@ -597,9 +620,11 @@ struct JoinSets {
 // first ones of the runs after it.  Every block adds up by itself how many tasks the runs'
 // cut units make, and takes its share of them.  Lanes are 8 channels each.  Of few partials a
 // task is 32 (64) rows, two a group of lanes; of many one row, of which each group takes every
-// 16th (32nd) partial, and the groups are added up, always in the same order.
+// 16th (32nd) partial, and the groups are added up, always in the same order.  Bound by the
+// partials' latency (24 sequences of 5 tokens 9 us) and, behind long chunks, by memory (15 to
+// 20 us for up to 100 MB).
 template <int D>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
     attention_kv4_chunks_join_kernel(ChunkArgs a, JoinSets j)
 {
     constexpr uint32_t kLanes = D / 8, kGroups = kThreads / kLanes;
@@ -654,7 +679,7 @@ __global__ void __launch_bounds__(kThreads)
         const uint32_t row0    = p.row0 + member / set.heads * set.rows;
         const uint32_t live    = min(set.rows, p.rows - row0);
         const uint32_t n       = p.last - run; // partials
-        const bool     many    = n > kJoinMany;
+        const bool     many    = join_many(n, live);
         const uint32_t of      = task - before[lo];
         uint32_t       in[2]   = {many ? of : of * kJoinRows<D> + group, 0};
         in[1]                  = many ? live : in[0] + kGroups; // its rows of the member's
@@ -671,11 +696,12 @@ __global__ void __launch_bounds__(kThreads)
                 for(int z = 0; z < 8; ++z) sum[y][z] = fmaf(sum[y][z], al, w * v[z]);
         };
         const uint32_t step = many ? kGroups : 1;
-        for(uint32_t i0 = many ? group : 0; i0 < n; i0 += 2 * step) {
-            v2f ml[2][2];
-            v4f v[2][2][2];
+        const auto     pass = [&](uint32_t i0, auto ahead) { // so many partials of a row
+            constexpr int kAhead = decltype(ahead)::value;
+            v2f ml[kAhead][2];
+            v4f v[kAhead][2][2];
 #pragma unroll
-            for(int x = 0; x < 2; ++x)
+            for(int x = 0; x < kAhead; ++x)
 #pragma unroll
                 for(int y = 0; y < 2; ++y) {
                     const uint32_t i = min(i0 + x * step, n - 1);
@@ -689,7 +715,7 @@ __global__ void __launch_bounds__(kThreads)
                     v[x][y][1] = from[1];
                 }
 #pragma unroll
-            for(int x = 0; x < 2; ++x) {
+            for(int x = 0; x < kAhead; ++x) {
                 if(i0 + x * step >= n) continue;
 #pragma unroll
                 for(int y = 0; y < 2; ++y) {
@@ -698,7 +724,12 @@ __global__ void __launch_bounds__(kThreads)
                     take(y, ml[x][y][0], ml[x][y][1], w);
                 }
             }
-        }
+        };
+        if(many)
+            for(uint32_t i0 = group; i0 < n; i0 += 4 * kGroups)
+                pass(i0, std::integral_constant<int, 4>());
+        else
+            for(uint32_t i0 = 0; i0 < n; i0 += 2) pass(i0, std::integral_constant<int, 2>());
         if(many) { // the groups' parts, one after the other
             __syncthreads();
             if(ch == 0) {

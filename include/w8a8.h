@@ -788,7 +788,7 @@ int w8a8_kv4_trim(const int32_t* keep, const int32_t* seq_lens, uint32_t seqs,
  * its own; a row that sees none gives zeros.  Tokens of a page number outside
  * [0, pages) are left out, rows of no sequence left as they were.  What a row may
  * not see does not reach it, NaN included; a group whose scale or offset is an
- * infinity counts as NaN.
+ * infinity counts as NaN.  out may not overlap q.
  * Keys and values enter the matrix products as fp16 (half of what w8a8_kv4_load
  * gives, rounded once), probabilities as well; scores, softmax statistics and sums
  * are fp32.  Results past the range of fp16 are its ends.

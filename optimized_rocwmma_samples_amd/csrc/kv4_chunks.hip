@@ -7,7 +7,7 @@
 // Sequences of few rows are computed here, those of many in kv4_unpacked.hip (kFewRows in
 // kv4_chunks.hpp).  The rows of a unit of work are (token, query head) pairs of one key head:
 // row r is token r / per, head r % per, per query heads sharing the key head.  A unit has 32
-// of them, or 64 where the sequence has more than 32 (24 x 5 tokens of 32/8 heads: 78 us in
+// of them, or 64 where the sequence has more than 32 (24 x 5 tokens of 64/8 heads: 78 us in
 // units of 32, 63 in units of 64, whose codes are unpacked once for both).  Units are walked
 // in steps of 128 keys, 32 a wave.  All units' steps lie in one line, which is cut into as many
 // equal runs as there are blocks, two a CU; what a cut leaves of a unit is written as
@@ -29,12 +29,12 @@
 // 1 + n / 16, exactly, with scales applied around the products, as for single tokens, would
 // take a product per group and query row and cost long chunks a quarter of their time.
 //
-// MI355X, 32 query and 8 key heads of 128, groups of 32: 24 sequences of 5 tokens behind up to
-// 8192 (90 MB of cache in use) take 61 us of this kernel and 9 of the join: 1.5 TB/s, bound by
-// its vector instructions (unpacking is about half of them) and, with two waves a SIMD, by what
-// they wait for LDS and for each other's products.  One token of 131072 takes 49 + 5 us.  Codes
-// staged through LDS by DMA (62, 57), a key-first order of the step (72), three blocks a CU
-// (spills) are not faster.
+// MI355X, 64 query and 8 key heads of 128, groups of 32: the last 5 tokens of 24 sequences of
+// 978 to 7719 (137 MB of codes and scales) take 60 us of this kernel, 2.3 TB/s, and 9 of the join.
+// Vector instructions fill 43 % of the SIMDs' cycles, about half of them unpacking, matrix
+// instructions 18 %; the rest is what two waves a SIMD wait for LDS, loads and each other's
+// products.  One token of 131072 of 32/8 heads: 49 + 5 us.  Codes staged through LDS by DMA
+// (62, 57), keys unpacked ahead of values (72), three blocks a CU (spills) are not faster.
 #include "kv4_chunks.hpp"
 
 #include <algorithm>

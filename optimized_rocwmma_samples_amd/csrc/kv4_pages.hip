@@ -17,6 +17,10 @@ namespace {
 // finding each one's sequence by halving among the 1024 sums in LDS.  The lengths and the
 // count are written by the first block, or, with more than one, by a second launch of one
 // where the caller has them written over the lengths and the count that every block reads.
+//
+// Bound by latency: lengths, sums with two barriers, a page number, a write.  MI355X: a step of
+// 256 sequences 5.8 us in one block, 48 prompts of some 32000 rows 6.7 in 32; 24 sequences
+// trimmed 3.8, 512 of 262144 columns 6.  A second launch costs a call 3 us.
 // ---------------------------------------------------------------------------
 constexpr int kSeqs = 1024; // threads of a block, and sequences a step
 
@@ -199,7 +203,8 @@ __global__ void __launch_bounds__(kSeqs) kv4_trim_kernel(Kv4TrimArgs a)
 //
 // A wave takes one key head of one page: lane = 8 channels (a dword of codes) of every
 // 4th (8th) row.  Bound by the start and one read's latency: 64 rows are 16 dwords a lane,
-// all on their way together.
+// all on their way together.  MI355X, 8 key heads of 128: the 128 pages of 8192 tokens 6.1 us
+// (5.9 MB), a step of 48 sequences 5.
 // ---------------------------------------------------------------------------
 constexpr int kWaveThreads = 256;
 

@@ -165,3 +165,12 @@ def test_package_refuses(w8a8):
         with pytest.raises(ValueError):
             W._kv4_table(t, 3)
     assert W._kv4_table(torch.zeros((3, 9), dtype=torch.int32)[:, 2:6], 3) == (4, 9)
+
+
+def test_workspace_of_a_line_past_32_bits(w8a8):
+    # 65521 query heads on one key head: its key tiles are not counted, nothing is unpacked
+    def size(tokens):
+        c = _cache(kv_heads=1, head_dim=64, page_size=64, pages=5000)
+        return W.library().w8a8_attention_kv4_chunks_workspace_size(
+            ctypes.byref(c), 16, tokens, 65521, 4096, 0)
+    assert size(600) < 1 << 28 < 1 << 30 < size(400)

@@ -364,8 +364,8 @@ __global__ void __launch_bounds__(kWaveThreads)
 // Up to kOneBlockPages columns the scores stay in LDS and one launch does it all; with more,
 // or with more than half as many and few blocks, a launch before it computes the scores with a
 // block for each 256 pages, since one block reads page keys at some 50 GB/s.  us in one launch
-// and in two, heads of 128, 8 key heads: one sequence of 2048 pages 10.5, 11; of 4096 15.8,
-// 12.4; 32 sequences of 4096 41, 45.
+// and in two, heads of 128, 8 key heads: one sequence of 2048 pages 10.6, 11; of 4096 15.8,
+// 11.6; 32 sequences of 4096 40, 45.
 // ---------------------------------------------------------------------------
 constexpr int      kSelectThreads = 1024;
 constexpr uint32_t kOneBlockPages = 4096;
@@ -397,19 +397,23 @@ __device__ __forceinline__ void query_codes(const Kv4SelectArgs& a, uint32_t seq
 
 // Scores of columns first .. end - 1 of `have`, as whole numbers in the scores' order, into
 // `order`: D / 16 lanes a page, 16 bytes each, so that a wave reads whole lines (a lane a page
-// takes 10 us for 2048 pages and not 4), THREADS lanes in all, 8 pages of each on their way.
+// takes 10 us for 2048 pages and not 4), THREADS lanes in all, 8 pages of each on their way (16
+// gain nothing with 2048 pages and lose 2 us with few), the first ones while the query's codes
+// are made (32 sequences of up to 1000 pages 10.6 us, 8.5 .. 10).
 template <int D, int THREADS>
-__device__ __forceinline__ void page_orders(const Kv4SelectArgs& a, const int32_t* from,
-                                            uint32_t head, uint32_t first, uint32_t end,
-                                            uint32_t have, const uint32_t* codes, uint32_t* order)
+__device__ __forceinline__ void page_orders(const Kv4SelectArgs& a, uint32_t seq, uint32_t head,
+                                            uint32_t first, uint32_t end, uint32_t have,
+                                            int* powers, uint32_t* codes, uint32_t* order)
 {
     constexpr uint32_t kLanes = D / 16, kGroups = THREADS / kLanes, kAhead = 8;
     const uint32_t     sub = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    const v4i          q = reinterpret_cast<const v4i*>(codes)[sub];
-    for(uint32_t c0 = first + group; c0 < end; c0 += kGroups * kAhead) {
-        int32_t page[kAhead];
-        v4i     k[kAhead];
-        float   s[kAhead];
+    const int32_t*     from = a.table + (size_t)seq * a.table_ld;
+    v4i                q{};
+    for(uint32_t b0 = first; b0 < end; b0 += kGroups * kAhead) {
+        const uint32_t c0 = b0 + group;
+        int32_t        page[kAhead];
+        v4i            k[kAhead];
+        float          s[kAhead];
 #pragma unroll
         for(uint32_t x = 0; x < kAhead; ++x) {
             const uint32_t c = c0 + x * kGroups;
@@ -421,6 +425,10 @@ __device__ __forceinline__ void page_orders(const Kv4SelectArgs& a, const int32_
             const size_t at = (size_t)max(page[x], 0) * a.kv_heads + head;
             k[x]            = reinterpret_cast<const v4i*>(a.codes + at * D)[sub];
             s[x]            = a.scales[at];
+        }
+        if(b0 == first) {
+            query_codes<D>(a, seq, head, powers, codes);
+            q = reinterpret_cast<const v4i*>(codes)[sub];
         }
 #pragma unroll
         for(uint32_t x = 0; x < kAhead; ++x) {
@@ -451,11 +459,9 @@ __global__ void __launch_bounds__(kWaveThreads)
     const uint32_t len  = clamped(a.lens[seq], a.table_cols << a.page_shift);
     const uint32_t have = (len + (1u << a.page_shift) - 1) >> a.page_shift;
     if(have <= a.keep || part * kWaveThreads >= have) return; // all of them, or none here
-    query_codes<D>(a, seq, head, powers, codes);
     const uint32_t first = part * kWaveThreads;
-    page_orders<D, kWaveThreads>(a, a.table + (size_t)seq * a.table_ld, head, first,
-                                 min(first + kWaveThreads, have), have, codes,
-                                 order + (size_t)unit * a.table_cols);
+    page_orders<D, kWaveThreads>(a, seq, head, first, min(first + kWaveThreads, have), have,
+                                 powers, codes, order + (size_t)unit * a.table_cols);
 }
 
 // SCORED: `order` holds the scores.
@@ -482,10 +488,8 @@ __global__ void __launch_bounds__(kSelectThreads)
             to[i] = i < have ? from[i] : -1;
         return;
     }
-    if constexpr(!SCORED) {
-        query_codes<D>(a, seq, head, powers, codes);
-        page_orders<D, kSelectThreads>(a, from, head, 0, have, have, codes, scores);
-    }
+    if constexpr(!SCORED)
+        page_orders<D, kSelectThreads>(a, seq, head, 0, have, have, powers, codes, scores);
     const uint32_t* mine = SCORED ? order + (size_t)unit * a.table_cols : scores;
     // ---- the keep-th largest, byte by byte from the top -------------------------------
     uint32_t        least = 0, mask = 0, left = a.keep; // of those that begin like `least`

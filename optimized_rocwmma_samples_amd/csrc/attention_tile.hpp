@@ -18,6 +18,7 @@ typedef __fp16   v4fp16 __attribute__((ext_vector_type(4)));
 
 typedef __attribute__((address_space(3))) v4fp16 lds_v4h_t;
 typedef __attribute__((address_space(3))) v8h    lds_v8h_t;
+typedef __attribute__((address_space(4))) uint32_t constant_u32_t;
 
 constexpr int kBufferFlags = 0x00020000; // raw buffer, 32-bit data format
 constexpr int kRows        = 128;        // query rows a block
@@ -196,18 +197,22 @@ __device__ __forceinline__ void attend(const TileRows& t, float c, const uint32_
     const uint32_t vat
         = lds0 + kTileBytes + tok0 * D * 2 + value_chunk<D>(tok0, ch0 / 8) * 16 + ch0 % 8 * 2;
 
+    const uint64_t gaps_at = (uint64_t)missing; // uniform as well
+    const auto*    gaps    = (const constant_u32_t*)(
+        (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(gaps_at >> 32)) << 32
+        | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)gaps_at));
     for(uint32_t kt = t.to, stage = 0; kt-- > t.from; stage ^= 1) {
+        // (a scalar load: a vector one would be waited for along with the next tile)
+        uint32_t none[kSubs] = {};
+        if constexpr(MASKED)
+#pragma unroll
+            for(int sub = 0; sub < kSubs; ++sub)
+                none[sub] = gaps[__builtin_amdgcn_readfirstlane(kt * kSubs + sub)];
         wait_vmcnt<0>();   // this wave's part of the tile is there,
         wait_lgkmcnt0();   // and its reads of the tile before are done:
         __syncthreads();   // so are every wave's
         if(kt > t.from) issue(stage ^ 1, kt - 1);
         if(kt * kKeys > first + 31) continue; // all of the tile is later than the wave's rows
-
-        uint32_t none[kSubs] = {};
-        if constexpr(MASKED)
-#pragma unroll
-            for(int sub = 0; sub < kSubs; ++sub)
-                none[sub] = __builtin_amdgcn_readfirstlane(missing[kt * kSubs + sub]);
 
         const uint32_t off  = stage * 2 * kTileBytes;
         const bool     diag = (kt + 1) * kKeys > first; // some of it is later than some rows
@@ -222,12 +227,11 @@ __device__ __forceinline__ void attend(const TileRows& t, float c, const uint32_
         if constexpr(MASKED) {
 #pragma unroll
             for(int sub = 0; sub < kSubs; ++sub) {
-                const uint32_t gone = none[sub];
-                if(gone != 0)
+                if(none[sub] == 0) continue;
+                const uint32_t gone = none[sub] >> (4 * half);
 #pragma unroll
-                    for(int i = 0; i < 16; ++i)
-                        s[sub][i] = (gone >> (8 * (i / 4) + 4 * half + i % 4) & 1u) != 0 ? -INFINITY
-                                                                                         : s[sub][i];
+                for(int i = 0; i < 16; ++i)
+                    if((gone >> (8 * (i / 4) + i % 4) & 1u) != 0) s[sub][i] = -INFINITY;
             }
         }
         if(diag) {

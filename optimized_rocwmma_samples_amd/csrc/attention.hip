@@ -22,13 +22,13 @@
 //   * The tile on the diagonal comes first and is the only one that masks.
 // A tile of 32 keys of 128 channels is 512 cycles of products a wave and about as many of
 // exponentials (a quarter of the rate), sums, maxima and roundings, which 3 waves a SIMD
-// overlap in part.  8192 tokens, 32 query and 8 key heads of 128: 545 to 590 us by the
-// card's clock, 1010 to 930 TFLOP/s, the matrix unit busy in 54 % of the cycles, vector
-// instructions in 52 %, waves waiting for 31 % of their time; 16 heads of 64: 161 to 172 us.
-// Bound, where blocks are few, by the chain of a block's own steps: the score product's key
-// fragments come from LDS into one register quad (two for two chains), so that each product
-// waits for its own read.  A block alone on its CU takes 1.2 us for 64 keys, whose products
-// are half of that, which is what a prompt of 1024 tokens waits for (26 us).
+// overlap in part.  8192 tokens, 32 query and 8 key heads of 128: 535 to 580 us by the
+// card's clock, 1030 to 950 TFLOP/s, the matrix unit busy in 55 % of the cycles, vector
+// instructions in 53 %, waves waiting for 23 % of their time; 16 heads of 64: 161 to 172 us.
+// Bound, where blocks are few, by the chain of a block's own steps: key fragments come from LDS
+// four ahead of their products, fragments of values each just before its own.  A block alone
+// on its CU takes 1.2 us for 64 keys, whose products are half of that, which is what a prompt
+// of 1024 tokens waits for.
 #include "attention_tile.hpp"
 
 namespace w8a8 {

@@ -217,13 +217,24 @@ __device__ __forceinline__ void attend(const TileRows& t, float c, const uint32_
         const uint32_t off  = stage * 2 * kTileBytes;
         const bool     diag = (kt + 1) * kKeys > first; // some of it is later than some rows
         v16f           s[kSubs] = {};
+        // Four key fragments on their way, in this order: left alone the compiler reads each into
+        // the same registers and waits for it (8192 tokens 556 us for 545; two ahead 559, where
+        // four are 554; six spill in the kernel over unpacked keys: 668 us, 676).
+        constexpr int  kAhead = 4, kProducts = kSteps * kSubs;
+        auto           key    = [&](int i) {
+            return *(const lds_v8h_t*)(uintptr_t)(((kat + off) ^ (i / kSubs * 32))
+                                                  + i % kSubs * 32 * D * 2);
+        };
+        v8h kf[kAhead];
 #pragma unroll
-        for(int st = 0; st < kSteps; ++st)
+        for(int i = 0; i < kAhead; ++i) kf[i] = key(i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for(int sub = 0; sub < kSubs; ++sub)
-                s[sub] = mfma(*(const lds_v8h_t*)(uintptr_t)(((kat + off) ^ (st * 32))
-                                                             + sub * 32 * D * 2),
-                              qf[st], s[sub]);
+        for(int i = 0; i < kProducts; ++i) {
+            s[i % kSubs] = mfma(kf[i % kAhead], qf[i / kSubs], s[i % kSubs]);
+            if(i + kAhead < kProducts) kf[i % kAhead] = key(i + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if constexpr(MASKED) {
 #pragma unroll
             for(int sub = 0; sub < kSubs; ++sub) {

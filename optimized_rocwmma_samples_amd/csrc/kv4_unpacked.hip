@@ -13,11 +13,10 @@
 // into equal runs, one a gang of blocks, all resident: any mix of chunks keeps the chip evenly
 // busy.  What a cut leaves of a unit is joined by another launch.
 //
-// MI355X, 2048 new of 18432 tokens, 32/8 heads of 128: unpacking 24 us (75 MB written at 3 TB/s
-// beside 17 read), attention 660 to 750 by the card's clock (584 GFLOP, 780 to 880 TFLOP/s, of
-// the 1390 of a large product; matrix instructions fill 45 % of the cycles and vector
-// instructions 45 %, each score product waits for its own read of key fragments, as in the
-// prompts' kernel), joining 20 (up to 100 MB of partials).  By the kernel of few rows, which
+// MI355X, 2048 new of 18432 tokens, 32/8 heads of 128: unpacking 22 us (75 MB written at 3 TB/s
+// beside 17 read), attention 605 to 710 by the card's clock (584 GFLOP, 820 to 960 TFLOP/s, of
+// the 1390 of a large product; matrix instructions fill 49 % of the cycles and vector
+// instructions 49 %, waves wait for 35 % of their time), joining 20 (up to 100 MB of partials).  By the kernel of few rows, which
 // unpacks for every 64 rows anew, the same chunk took 1190.
 #include "attention_tile.hpp"
 #include "kv4_chunks.hpp"

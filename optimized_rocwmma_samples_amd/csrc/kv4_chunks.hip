@@ -33,8 +33,11 @@
 // 978 to 7719 (137 MB of codes and scales) take 60 us of this kernel, 2.3 TB/s, and 9 of the join.
 // Vector instructions fill 43 % of the SIMDs' cycles, about half of them unpacking, matrix
 // instructions 18 %; the rest is what two waves a SIMD wait for LDS, loads and each other's
-// products.  One token of 131072 of 32/8 heads: 49 + 5 us.  Codes staged through LDS by DMA
-// (62, 57), keys unpacked ahead of values (72), three blocks a CU (spills) are not faster.
+// products.  One token of 131072 of 32/8 heads: 49 + 5 us.  Of equal runs of
+// 13 steps those of the first 256 blocks end after 44 us and the others, whose waves a SIMD
+// serves second, after 54; a unit's end costs 5.  Not faster: codes staged through LDS by DMA
+// (62, 57), keys unpacked ahead of values (72), three blocks a CU (spills), queries and values
+// read one product ahead, longer runs for the first blocks, priorities that take turns.
 #include "kv4_chunks.hpp"
 
 #include <algorithm>
@@ -277,18 +280,15 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
     };
 
     // ---- steps on their way ------------------------------------------------------------
-    auto page_at = [&](const Place& p) { // of the lane's key
+    auto page_at = [&](const Place& p) { // of the lane's key, as it stands in the table
         const uint32_t t    = p.step * kStep + wave * kKeys + col;
         int32_t        page = -1;
-        if(t < p.c.len) {
-            page = a.table[(size_t)p.seq * a.table_ld + (t >> c.page_shift)];
-            if(page < 0 || (uint32_t)page >= pages) page = -1;
-        }
+        if(t < p.c.len) page = a.table[(size_t)p.seq * a.table_ld + (t >> c.page_shift)];
         return page;
     };
     auto fetch = [&](R& x, const Place& p, int32_t page) {
-        x.ok             = page >= 0; // without one page 0's rows are read, and masked
-        const size_t row = cache_row(c, page >= 0 ? page : 0, p.unit / p.tiles,
+        x.ok             = (uint32_t)page < pages; // else page 0's rows are read, and masked
+        const size_t row = cache_row(c, x.ok ? page : 0, p.unit / p.tiles,
                                      (p.step * kStep + wave * kKeys + col) & (c.page_size - 1));
         const uint8_t* k = c.codes[0] + row * (D / 2) + half * (D / 8);
         load_dwords<R::kKeyWords>(x.k[0], k);
@@ -357,13 +357,13 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
     bool from_start = here.step == 0; // of the unit
 
     R     x;
-    Place next = here;
+    Place next = here, after{};
     {
         const int32_t page = page_at(here);
         fetch_queries(here);
         fetch(x, here, page);
     }
-    int32_t page_next = -1;
+    int32_t page_next = -1, page_after = -1;
     if(left > 1) {
         advance(next);
         page_next = page_at(next);
@@ -484,7 +484,14 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
                                                          qat + (t * kSteps + st) * kWave * 16)),
                              sc[t]);
         }
-        if(left > 1) { // the next step's loads, over the rest of this one
+        // The next step's loads, over the rest of this one; before them the page numbers of the
+        // step after it, which would else be waited for together with those loads (1 to 2 %).
+        if(left > 1) {
+            if(left > 2) {
+                after = next;
+                advance(after);
+                page_after = page_at(after);
+            }
             fetch(x, next, page_next);
         }
         if(!full)
@@ -565,11 +572,9 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
             __syncthreads();
         }
         if(left == 1) break;
-        here = next;
-        if(left > 2) {
-            advance(next);
-            page_next = page_at(next);
-        }
+        here      = next;
+        next      = after;
+        page_next = page_after;
         if(ends) { // the next unit
             from_start = true;
             begin_unit();

@@ -699,7 +699,10 @@ def board_power(torch, dev, loads, secs=2.0, lead=1.0, every=0.02):
                 break
         if handle is None:
             return {"note": "no amdsmi handle with this GPU's PCI bus id"}
-        cap = amdsmi.amdsmi_get_power_cap_info(handle).get("power_cap")
+        try:
+            cap = amdsmi.amdsmi_get_power_cap_info(handle).get("power_cap")
+        except amdsmi.AmdSmiException:  # not every driver tells it
+            cap = None
         out = {"power_cap_W": cap / 1e6 if isinstance(cap, (int, float)) else None,
                "note": f"amdsmi current_socket_power and GFX clock sampled every {every * 1e3:.0f} ms "
                        f"over {secs:.1f} s, after each load had run {lead:.1f} s"}

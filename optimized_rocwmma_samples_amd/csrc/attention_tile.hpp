@@ -132,8 +132,8 @@ struct TileRows {
 // One pass over the tiles: on return the wave's lane has its row's maximum m (mc = m c, 0
 // while no score is finite), its own half of the sum l of probabilities and, of 32
 // channels a block, the sum of their products with the values.  Where `first` is a multiple
-// of KEYS each wave meets its diagonal in its first tile.  MASKED: bit i of missing[j] says
-// that there is no key 32 j + i (whose values are zeros).
+// of KEYS each wave meets its diagonal in its first tile.  MASKED: a chunk's rows; bit i of
+// missing[j] says that there is no key 32 j + i (whose values are zeros).
 template <int D, int KEYS, bool MASKED>
 __device__ __forceinline__ void attend(const TileRows& t, float c, const uint32_t* missing,
                                        uint8_t* lds, float& m, float& l, float& mc,
@@ -178,15 +178,23 @@ __device__ __forceinline__ void attend(const TileRows& t, float c, const uint32_
     issue(0, t.to - 1);
 
     // ---- the wave's query rows: lane = row, 8 channels from 16 step + 8 half ----
-    v8h qf[kSteps];
-    {
+    // Zeros behind the last row.  Rows of a chunk may lie any distance apart; those of a prompt
+    // no more than 2^24 values, which a buffer's 32-bit offsets hold.  The same us: chunks (2048
+    // of 18432 tokens) 643 by addresses and 648 by a buffer, prompts (8192) 547 and 544.
+    v8h            qf[kSteps] = {};
+    const uint32_t qrow       = wave * 32 + col;
+    if constexpr(MASKED) {
+        const uint16_t* from = t.q + (size_t)qrow * t.ldq + half * 8;
+        if(qrow < t.rows)
+#pragma unroll
+            for(int s = 0; s < kSteps; ++s) qf[s] = *reinterpret_cast<const v8h*>(from + s * 16);
+    } else {
         const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint16_t*>(t.q), 0, (int)((t.rows - 1) * t.ldq * 2 + D * 2), kBufferFlags);
 #pragma unroll
         for(int s = 0; s < kSteps; ++s)
-            qf[s] = __builtin_bit_cast(
-                v8h, __builtin_amdgcn_raw_buffer_load_b128(
-                         rq, (wave * 32 + col) * t.ldq * 2 + s * 32 + half * 16, 0, 0));
+            qf[s] = __builtin_bit_cast(v8h, __builtin_amdgcn_raw_buffer_load_b128(
+                                                rq, qrow * t.ldq * 2 + s * 32 + half * 16, 0, 0));
     }
 
     // LDS places of the lane's reads, in stage 0: of a key's first step and a value's first

@@ -112,9 +112,11 @@ struct Unpack {
     }
 };
 
+// Half of a (scale, offset) pair, x - x / 2: an infinity becomes NaN by it.
 __device__ __forceinline__ v2h halved(int32_t pair)
 {
-    return __builtin_bit_cast(v2h, pair) * v2h{(_Float16)0.5f, (_Float16)0.5f};
+    const v2h x = __builtin_bit_cast(v2h, pair);
+    return __builtin_elementwise_fma(x, v2h{(_Float16)-0.5f, (_Float16)-0.5f}, x);
 }
 
 // The 16-byte chunk position of chunk c of a row of a wave's tile of values: spreads both the

@@ -83,10 +83,12 @@ struct Unpacked {
     uint32_t* missing; // bit i of word j: row 32 j + i has no token
 };
 
-// 8 values of a dword of codes, what kv4_load gives.
+// 8 values of a dword of codes, what kv4_load gives, but NaN where the scale or the offset is
+// an infinity (whose product with 0 is NaN; added to the offset it reaches all codes).
 __device__ __forceinline__ v4i unpacked(uint32_t w, uint32_t pair)
 {
-    const float s = half_bits_to_float(pair & 0xFFFFu), mid = half_bits_to_float(pair >> 16);
+    const float s = half_bits_to_float(pair & 0xFFFFu);
+    const float o = half_bits_to_float(pair >> 16), mid = fmaf(o, 0.f, fmaf(s, 0.f, o));
     v4i         out;
 #pragma unroll
     for(int j = 0; j < 4; ++j)

@@ -789,9 +789,9 @@ int w8a8_kv4_trim(const int32_t* keep, const int32_t* seq_lens, uint32_t seqs,
  * [0, pages) are left out, rows of no sequence left as they were.  What a row may
  * not see does not reach it, NaN included; a group whose scale or offset is an
  * infinity counts as NaN.  out may not overlap q.
- * Keys and values enter the matrix products as fp16 (half of what w8a8_kv4_load
- * gives, rounded once), probabilities as well; scores, softmax statistics and sums
- * are fp32.  Results past the range of fp16 are its ends.
+ * Keys and values enter the matrix products as fp16, off from offset + scale *
+ * (n - 8) by no more than 2^-11 of it and 2^-23, probabilities as well; scores, softmax
+ * statistics and sums are fp32.  Results past the range of fp16 are its ends.
  * max_new: no sequence has more new tokens than this (0: not known); more of them are
  * computed all the same, more slowly.
  * workspace: 256-byte aligned, w8a8_attention_kv4_chunks_workspace_size bytes (for

@@ -20,10 +20,11 @@
 //   * V^T's rows are channels: a wave unpacks its 32 rows of values into a tile of its own in
 //     LDS and reads it transposed with ds_read_b64_tr_b16.  Nothing waits for other waves
 //     until the unit ends.
-// A code n becomes 1024 + n by two bit operations a pair, n - 8 and then offset + scale *
-// (n - 8), rounded once: half of what kv4_load gives, since a group that reaches the ends of
-// fp16 may pass them by half a step (the halves go into the scale of the scores and of the
-// result).  Three roundings of 2^-11 are left, of keys, values and probabilities, as in
+// A code n becomes 512 + n / 2 by two bit operations a pair, (n - 8) / 2 and then offset / 2 +
+// scale * (n - 8) / 2, rounded once: half of what kv4_load gives, since a group that reaches the
+// ends of fp16 may pass them by half a step (the halves go into the scale of the scores and of
+// the result).  Half of a subnormal offset is rounded as well, so that small values are off by
+// up to 2^-23.  Three roundings of 2^-11 are left, of keys, values and probabilities, as in
 // attention over fp16 keys and values; the keys' is the largest part of the error (4.9e-4 of a
 // result's 4.5e-4 .. 6.7e-4 where a product of fp32 keys leaves 2.1e-4).  Codes that enter as
 // 1 + n / 16, exactly, with scales applied around the products, as for single tokens, would
@@ -87,18 +88,18 @@ __device__ __forceinline__ bool finite_pair(uint32_t w)
     return (w & 0x7C00u) != 0x7C00u && (w & 0x7C000000u) != 0x7C000000u;
 }
 
-// The 8 codes of a dword as fp16 values offset + scale * (n - 8), in the order 0 4 1 5 2 6 3 7;
-// `pair` is (scale, offset).
+// The 8 codes of a dword as fp16 values (offset + scale * (n - 8)) / 2, in the order 0 4 1 5 2 6
+// 3 7; `pair` is (scale, offset / 2).
 struct Unpack {
     uint32_t mask, big;
     __device__ Unpack()
     {
         asm volatile("v_mov_b32 %0, 0x000f000f" : "=v"(mask));
-        asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(big)); // 1024, whose last bit is 1
+        asm volatile("v_mov_b32 %0, 0x60006000" : "=v"(big)); // 512, whose last bit is 1/2
     }
     __device__ v8h operator()(uint32_t w, v2h pair) const
     {
-        const v2h middle = {(_Float16)1032.f, (_Float16)1032.f};
+        const v2h middle = {(_Float16)516.f, (_Float16)516.f};
         const v2h s = {pair[0], pair[0]}, o = {pair[1], pair[1]};
         v8h       f;
 #pragma unroll
@@ -112,11 +113,12 @@ struct Unpack {
     }
 };
 
-// Half of a (scale, offset) pair, x - x / 2: an infinity becomes NaN by it.
-__device__ __forceinline__ v2h halved(int32_t pair)
+// The scale as it is and half of the offset, x - 0 and x - x / 2: infinities become NaN by it.
+// (Half a scale that is subnormal in fp16 would be off by up to half a step, times 8.)
+__device__ __forceinline__ v2h scale_and_half(int32_t pair)
 {
     const v2h x = __builtin_bit_cast(v2h, pair);
-    return __builtin_elementwise_fma(x, v2h{(_Float16)-0.5f, (_Float16)-0.5f}, x);
+    return __builtin_elementwise_fma(x, v2h{(_Float16)-0.f, (_Float16)-0.5f}, x);
 }
 
 // The 16-byte chunk position of chunk c of a row of a wave's tile of values: spreads both the
@@ -465,7 +467,7 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
                 bad[g]         = __ballot(nan);
                 if(nan) x.vs[g] = 0;
             }
-            vs[g] = halved(x.vs[g]);
+            vs[g] = scale_and_half(x.vs[g]);
         }
 #pragma unroll
         for(int i = 0; i < R::kValueWords; ++i) {
@@ -478,7 +480,7 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
         v16f sc[T] = {};
 #pragma unroll
         for(int st = 0; st < kSteps; ++st) {
-            const v8h k = unpack((uint32_t)x.k[st % 2][st / 2], halved(x.ks[st / 2 * 32 / G]));
+            const v8h k = unpack((uint32_t)x.k[st % 2][st / 2], scale_and_half(x.ks[st / 2 * 32 / G]));
 #pragma unroll
             for(int t = 0; t < T; ++t)
                 sc[t] = mfma(k,

@@ -979,6 +979,12 @@ def _kv4_ints(dev, name, t, count: int) -> int:
     return t.data_ptr()
 
 
+def _count(name, value: int, least: int = 0) -> int:
+    if not least <= value <= 0xFFFFFFFF:  # the library takes it in 32 bits
+        raise ValueError(f"{name} must be in {least} .. 2^32 - 1, got {value}")
+    return value
+
+
 def _kv4_table(block_table, seqs: int):
     # columns and row stride of a block table
     table = block_table.shape
@@ -1060,9 +1066,9 @@ def kv4_extend(new_tokens, seq_lens, block_table, free_pages, free_count, page_s
     args = (_kv4_ints(dev, "new_tokens", new_tokens, seqs),
             _kv4_ints(dev, "seq_lens", seq_lens, seqs), seqs, block_table.data_ptr(), cols,
             table_ld, _kv4_ints(dev, "free_pages", free_pages, free_pages.numel()),
-            free_pages.numel(), _kv4_ints(dev, "free_count", free_count, 1), page_size)
-    if tokens < 0:
-        raise ValueError("tokens must not be negative")
+            free_pages.numel(), _kv4_ints(dev, "free_count", free_count, 1),
+            _count("page_size", page_size))
+    _count("tokens", tokens)
     if out is None:
         # one allocation for the four (0.9 us each of a 10 us call)
         both = seq_lens.new_empty(tokens + 2 * seqs + 2)
@@ -1092,7 +1098,7 @@ def kv4_trim(keep, seq_lens, block_table, free_pages, free_count, page_size: int
     args = (_kv4_ints(dev, "keep", keep, seqs), _kv4_ints(dev, "seq_lens", seq_lens, seqs), seqs,
             block_table.data_ptr(), cols, table_ld,
             _kv4_ints(dev, "free_pages", free_pages, free_pages.numel()), free_pages.numel(),
-            _kv4_ints(dev, "free_count", free_count, 1), page_size)
+            _kv4_ints(dev, "free_count", free_count, 1), _count("page_size", page_size))
     if out is None:
         lens, count = torch.empty_like(seq_lens), torch.empty_like(free_count)
         at = lens.data_ptr(), count.data_ptr()
@@ -1116,7 +1122,8 @@ def attention_kv4_chunks_workspace_size(cache: KV4Cache, seqs: int, tokens: int,
                                         columns: int, max_new: int | None = None) -> int:
     """Bytes of workspace attention_kv4_chunks needs (0: none); columns of the block table."""
     return _kv4_chunks_workspace_size(cache.pages, cache.page_size, cache.kv_heads, cache.head_dim,
-                                      cache.group, seqs, tokens, heads, columns, max_new or 0)
+                                      cache.group, seqs, tokens, heads, columns,
+                                      min(max_new or 0, tokens))
 
 
 def attention_kv4_chunks(q, cache: KV4Cache, block_table, seq_lens, starts,
@@ -1142,7 +1149,7 @@ def attention_kv4_chunks(q, cache: KV4Cache, block_table, seq_lens, starts,
     cols, table_ld = _kv4_table(block_table, seqs)
     lens_at = _kv4_ints(dev, "seq_lens", seq_lens, seqs)
     starts_at = _kv4_ints(dev, "starts", starts, seqs + 1)
-    max_new = 0 if max_new is None else max_new
+    max_new = 0 if max_new is None else min(max_new, tokens)
     if max_new < 0:
         raise ValueError("max_new must not be negative")
     out, ldo = _heads_out(out, q, tokens, heads, dim)
@@ -1211,8 +1218,7 @@ def kv4_summarize(cache: KV4Cache, keys: KV4PageKeys, block_table, seq_lens, sta
     cols, table_ld = _kv4_table(block_table, seqs)
     lens_at = _kv4_ints(dev, "seq_lens", seq_lens, seqs)
     starts_at = _kv4_ints(dev, "starts", starts, seqs + 1)
-    if tokens < 0:
-        raise ValueError("tokens must not be negative")
+    _count("tokens", tokens)
     _call_on(dev, "w8a8_kv4_summarize", cache._descriptor(), keys._descriptor(),
              block_table.data_ptr(), cols, table_ld, lens_at, starts_at, seqs, tokens,
              _stream(dev))
@@ -1260,8 +1266,8 @@ def kv4_select(q, keys: KV4PageKeys, block_table, seq_lens, keep: int, page_size
     seqs, heads, _ = q.shape
     cols, table_ld = _kv4_table(block_table, seqs)
     lens_at = _kv4_ints(dev, "seq_lens", seq_lens, seqs)
-    if keep <= 0:
-        raise ValueError("keep must be > 0")
+    _count("keep", keep, 1)
+    _count("page_size", page_size)
     shape = (seqs, keys.kv_heads, keep)
     if out is None:
         chosen, lens = seq_lens.new_empty(shape), seq_lens.new_empty(seqs)

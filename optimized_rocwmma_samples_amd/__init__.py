@@ -1168,10 +1168,11 @@ def attention_kv4_chunks(q, cache: KV4Cache, block_table, seq_lens, starts,
 class KV4PageKeys:
     """A key for each page of a KV4Cache (w8a8_kv4_page_keys): codes int8 [pages, kv_heads,
     head_dim], the mean of the page's keys in units of scales fp32 [pages, kv_heads], powers
-    of two.  KV4PageKeys.empty allocates them for a cache.  They are not to be given other
-    memory, which the calls refuse."""
+    of two.  KV4PageKeys.empty allocates them for a cache.  page_size: the cache's, where it is
+    known; the calls refuse another one.  The tensors are not to be given other memory, which
+    the calls refuse as well."""
 
-    def __init__(self, codes, scales):
+    def __init__(self, codes, scales, page_size: int | None = None):
         torch = _torch()
         _require_cuda(codes)
         _require_on(codes.device, scales=scales)
@@ -1182,6 +1183,7 @@ class KV4PageKeys:
         self._codes, self._scales = codes, scales
         self.pages, self.kv_heads, self.head_dim = codes.shape
         self.device = codes.device
+        self.page_size = page_size
         self._where = (codes.data_ptr, scales.data_ptr)
         self._at = tuple(where() for where in self._where)
         self._desc = _lib.Kv4PageKeys(*self._at, *codes.shape)
@@ -1197,13 +1199,19 @@ class KV4PageKeys:
                              "KV4PageKeys")
         return self._ref
 
+    def _require_page_size(self, page_size) -> None:
+        if self.page_size is not None and page_size != self.page_size:
+            raise ValueError(f"these are keys of pages of {self.page_size} tokens, "
+                             f"got page_size={page_size}")
+
     @classmethod
     def empty(cls, cache: KV4Cache):
         """Page keys of a cache's pages (contents undefined until kv4_summarize)."""
         torch = _torch()
         shape = (cache.pages, cache.kv_heads, cache.head_dim)
         return cls(torch.empty(shape, dtype=torch.int8, device=cache.device),
-                   torch.empty(shape[:2], dtype=torch.float32, device=cache.device))
+                   torch.empty(shape[:2], dtype=torch.float32, device=cache.device),
+                   cache.page_size)
 
 
 def kv4_summarize(cache: KV4Cache, keys: KV4PageKeys, block_table, seq_lens, starts,
@@ -1214,6 +1222,7 @@ def kv4_summarize(cache: KV4Cache, keys: KV4PageKeys, block_table, seq_lens, sta
     _torch()
     dev = cache.device
     _require_on(dev, block_table=block_table, codes=keys._codes)
+    keys._require_page_size(cache.page_size)
     seqs = seq_lens.numel()
     cols, table_ld = _kv4_table(block_table, seqs)
     lens_at = _kv4_ints(dev, "seq_lens", seq_lens, seqs)
@@ -1268,6 +1277,7 @@ def kv4_select(q, keys: KV4PageKeys, block_table, seq_lens, keep: int, page_size
     lens_at = _kv4_ints(dev, "seq_lens", seq_lens, seqs)
     _count("keep", keep, 1)
     _count("page_size", page_size)
+    keys._require_page_size(page_size)
     shape = (seqs, keys.kv_heads, keep)
     if out is None:
         chosen, lens = seq_lens.new_empty(shape), seq_lens.new_empty(seqs)

@@ -83,3 +83,20 @@ def test_negative_bound(w8a8, called):
 def test_no_pages_are_none(w8a8, called):
     with pytest.raises(ValueError, match="keep"):
         CALLS["select"](keep=0)
+
+
+def test_page_size_of_page_keys(w8a8, called):
+    # the keys know whose pages they are; without a page size they take any
+    c = cache()
+    k = keys(c)
+    assert k.page_size == 16
+    with pytest.raises(ValueError, match="pages of 16"):
+        W.kv4_select(Q, k, ints(3, 4), ints(3), 2, 32, workspace=None)
+    with pytest.raises(ValueError, match="pages of 16"):
+        W.kv4_summarize(W.KV4Cache.empty(4, 2, 64, 32, 32, "cpu"), k, ints(3, 4), ints(3), ints(4), 5)
+    assert not called
+    for size in (16, 32):
+        W.kv4_select(Q, W.KV4PageKeys(k.codes, k.scales), ints(3, 4), ints(3), 2, size,
+                     workspace=None)
+    W.kv4_select(Q, W.KV4PageKeys(k.codes, k.scales, 32), ints(3, 4), ints(3), 2, 32, workspace=None)
+    assert len(called) == 3

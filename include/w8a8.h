@@ -753,7 +753,11 @@ int w8a8_attention_kv4(const void* q, const w8a8_kv4_cache* cache, const int32_t
  * gets all of its places or none: none where its rows would pass `tokens`, its
  * tokens the table's columns, or where the pages that are left behind the
  * sequences before it do not suffice (one that finds too few leaves none to those
- * behind it that need any).  Then its slots are -1 and its length stays.
+ * behind it that need any).  Then its slots are -1 and its length stays: it is one
+ * with new_tokens[i] > 0 and lens_out[i] == seq_lens[i] (lens_out with memory of its
+ * own).  Its rows stay in seq_starts, and of its length the attention and page keys of
+ * the step would take the last tokens for its new ones: they are given a length of 0
+ * for it, which makes its rows zeros and touches no page.
  * lens_out may be seq_lens and count_out free_count; other arguments may not
  * overlap.
  */
@@ -770,6 +774,10 @@ int w8a8_kv4_extend(const int32_t* new_tokens, const int32_t* seq_lens, uint32_t
  * them (so that trimming what was just handed out restores the stack); pages past
  * free_capacity are dropped.  The block table is left as it was.  lens_out may be
  * seq_lens and count_out free_count; other arguments may not overlap.
+ * A page that is given back stands in one sequence's columns only: one of two is
+ * stacked twice, and would be handed out twice.  Pages that sequences share (a cached
+ * prefix) are kept by keep[i] of at least their tokens, until the caller, which
+ * counts their users, puts them back once.
  */
 int w8a8_kv4_trim(const int32_t* keep, const int32_t* seq_lens, uint32_t seqs,
                   const int32_t* block_table, uint32_t table_cols, uint32_t table_ld,

@@ -1056,8 +1056,10 @@ def kv4_extend(new_tokens, seq_lens, block_table, free_pages, free_count, page_s
     [seqs + 1] of the sequences' rows, lengths [seqs], free pages left [1]), all int32.
     A sequence gets all of its places or none (slots of -1, its length stays): none where
     its rows would pass `tokens`, its tokens the table's columns, or where the pages that
-    the sequences before it leave are too few.  out: these four; the lengths and the
-    count may be seq_lens and free_count themselves."""
+    the sequences before it leave are too few.  Those are (new_tokens > 0) & (lengths ==
+    seq_lens); their rows stay, so the step's attention and page keys take lengths that are
+    0 for them.  out: these four; the lengths and the count may be seq_lens and free_count
+    themselves."""
     torch = _torch()
     _require_cuda(block_table)
     dev = block_table.device
@@ -1088,8 +1090,9 @@ def kv4_extend(new_tokens, seq_lens, block_table, free_pages, free_count, page_s
 def kv4_trim(keep, seq_lens, block_table, free_pages, free_count, page_size: int, out=None):
     """Takes tokens back: sequence i is left with min(keep[i], seq_lens[i]) tokens (0: it is
     done), and the pages that it no longer needs go back on the stack of kv4_extend, in the
-    reverse of the order in which that takes them.  Returns (lengths [seqs], free pages
-    [1]), int32; out: these two, which may be seq_lens and free_count themselves."""
+    reverse of the order in which that takes them.  A page is given back by one sequence
+    only: of shared ones (a cached prefix) keep the tokens.  Returns (lengths [seqs], free
+    pages [1]), int32; out: these two, which may be seq_lens and free_count themselves."""
     torch = _torch()
     _require_cuda(block_table)
     dev = block_table.device

@@ -113,12 +113,13 @@ struct Unpack {
     }
 };
 
-// The scale as it is and half of the offset, x - 0 and x - x / 2: infinities become NaN by it.
-// (Half a scale that is subnormal in fp16 would be off by up to half a step, times 8.)
+// The scale as it is and half of the offset, x + 0 x and x - x / 2: infinities become NaN by it.
+// (Half a scale that is subnormal in fp16 would be off by up to half a step, times 8.  The
+// factors 0 and -1/2 are one inline constant; -0 or 1, 1/2 take a register, which spills.)
 __device__ __forceinline__ v2h scale_and_half(int32_t pair)
 {
     const v2h x = __builtin_bit_cast(v2h, pair);
-    return __builtin_elementwise_fma(x, v2h{(_Float16)-0.f, (_Float16)-0.5f}, x);
+    return __builtin_elementwise_fma(x, v2h{(_Float16)0.f, (_Float16)-0.5f}, x);
 }
 
 // The 16-byte chunk position of chunk c of a row of a wave's tile of values: spreads both the

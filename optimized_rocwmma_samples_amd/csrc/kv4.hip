@@ -251,8 +251,6 @@ RowPlan row_plan(const w8a8_kv4_cache& c, const Kv4Rows& r)
 // products of C tiles add up in one accumulator.  A column is then a partial of its
 // own, with its own maximum, sum and part of the result, merged at the unit's end.
 // ---------------------------------------------------------------------------
-typedef float    v2f __attribute__((ext_vector_type(2)));
-
 typedef __attribute__((address_space(3))) v2i      lds_v2i_t;
 typedef __attribute__((address_space(3))) v4i      lds_v4i_t;
 typedef __attribute__((address_space(3))) uint32_t lds_u32_t;

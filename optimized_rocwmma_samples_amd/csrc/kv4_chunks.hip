@@ -9,8 +9,9 @@
 // row r is token r / per, head r % per, per query heads sharing the key head.  A unit has 32
 // of them, or 64 where the sequence has more than 32 (24 x 5 tokens of 64/8 heads: 78 us in
 // units of 32, 63 in units of 64, whose codes are unpacked once for both).  Units are walked
-// in steps of 128 keys, 32 a wave.  All units' steps lie in one line, which is cut into as many
-// equal runs as there are blocks, two a CU; what a cut leaves of a unit is written as
+// in steps of 128 keys, 32 a wave.  The steps of the units of 64 rows lie in one line, those of
+// 32 in another; each line is cut into up to 512 equal runs, a block each, two of which a CU
+// holds, and the blocks of the first line start first.  What a cut leaves of a unit is written as
 // partials (sum of p v, maximum and sum of p of each row) and joined by a second launch.
 //   * S^T = K Q^T with v_mfma_f32_32x32x16_f16: srcA rows are keys, and a lane's operand is 8
 //     channels of one key, which is a dword of its codes: unpacked, scaled and used where
@@ -25,20 +26,24 @@
 // ends of fp16 may pass them by half a step (the halves go into the scale of the scores and of
 // the result).  Half of a subnormal offset is rounded as well, so that small values are off by
 // up to 2^-23.  Three roundings of 2^-11 are left, of keys, values and probabilities, as in
-// attention over fp16 keys and values; the keys' is the largest part of the error (4.9e-4 of a
-// result's 4.5e-4 .. 6.7e-4 where a product of fp32 keys leaves 2.1e-4).  Codes that enter as
-// 1 + n / 16, exactly, with scales applied around the products, as for single tokens, would
-// take a product per group and query row and cost long chunks a quarter of their time.
+// attention over fp16 keys and values.  Relative to the results' norm, 5 tokens verified and one
+// decoded beside a prompt: keys 4.9e-4 and 3.0e-4, values 1.9e-4, probabilities 1.0e-4 and
+// 0.7e-4, the results' own rounding 2.1e-4 and 2.0e-4; all of them 5.8e-4 and 4.0e-4.  That one
+// token alone, by attention_kv4, is 2.0e-4 off: its codes enter as 1 + n / 16, exactly, with
+// scales applied around the products, which here would take a product per group and query row
+// and cost long chunks a quarter of their time; so a token that is decoded beside chunks is
+// computed as they are.
 //
 // MI355X, 64 query and 8 key heads of 128, groups of 32: the last 5 tokens of 24 sequences of
 // 978 to 7719 (137 MB of codes and scales) take 60 us of this kernel, 2.3 TB/s, and 9 of the join.
-// Vector instructions fill 43 % of the SIMDs' cycles, about half of them unpacking, matrix
-// instructions 18 %; the rest is what two waves a SIMD wait for LDS, loads and each other's
-// products.  One token of 131072 of 32/8 heads: 49 + 5 us.  Of equal runs of
-// 13 steps those of the first 256 blocks end after 44 us and the others, whose waves a SIMD
-// serves second, after 54; a unit's end costs 5.  Not faster: codes staged through LDS by DMA
-// (62, 57), keys unpacked ahead of values (72), three blocks a CU (spills), queries and values
-// read one product ahead, longer runs for the first blocks, priorities that take turns.
+// Vector instructions fill 43 % of the SIMDs' cycles from the launch's start to its end, about
+// half of them unpacking, matrix instructions 18 %; the rest is what two waves a SIMD wait for
+// LDS, loads and each other's products, and the blocks' starts, unit ends and unequal ends.  One
+// token of 131072 of 32/8 heads: 49 + 5 us.  Of equal runs of 13 steps those of the first 256
+// blocks end after 44 us and the others, whose waves a SIMD serves second, after 54; a unit's end
+// costs 5.  Not faster: codes staged through LDS by DMA (62, 57), keys unpacked ahead of values
+// (72), three blocks a CU (spills), queries and values read one product ahead, longer runs for
+// the first blocks, priorities that take turns.
 #include "kv4_chunks.hpp"
 
 #include <algorithm>
@@ -46,11 +51,6 @@
 namespace w8a8 {
 namespace {
 
-typedef float  v2f __attribute__((ext_vector_type(2)));
-typedef float  v16f __attribute__((ext_vector_type(16)));
-typedef __fp16 v4fp16 __attribute__((ext_vector_type(4)));
-
-typedef __attribute__((address_space(3))) v4fp16 lds_v4h_t;
 typedef __attribute__((address_space(3))) v4i    lds_v4i_t;
 typedef __attribute__((address_space(3))) v4f    lds_v4f_t;
 
@@ -58,29 +58,11 @@ constexpr int      kWaves   = 4;
 constexpr int      kThreads = kWaves * kWave;
 constexpr int      kKeys    = 32;              // a wave's a step
 constexpr int      kStep    = kWaves * kKeys;  // keys of a step
-constexpr uint32_t kBlocks  = 512;             // runs: two a CU, all resident
+constexpr uint32_t kBlocks  = 512;             // runs of a line at the most: two blocks a CU
 
 __host__ __device__ inline uint32_t steps_of(uint32_t len)
 {
     return len == 0 ? 1u : (len + kStep - 1) / kStep; // a sequence of no tokens is written too
-}
-
-__device__ __forceinline__ v16f mfma(v8h a, v8h b, v16f c)
-{
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
-// The value of the other half of the wave (lane ^ 32) and this one's.
-__device__ __forceinline__ v2f both_halves(float v)
-{
-    const uint32_t u = __float_as_uint(v);
-    const auto     r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return {__uint_as_float(r[0]), __uint_as_float(r[1])};
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c)
-{
-    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
 __device__ __forceinline__ bool finite_pair(uint32_t w)
@@ -159,7 +141,7 @@ struct Ways {
     bool           more; // there are blocks for units of two tiles
 
     // 32-row tiles a unit; 0: not this kernel's
-    __device__ uint32_t kind(const ChunkArgs& a, const Chunk& x, uint32_t i) const
+    __device__ uint32_t kind(const Chunk& x, uint32_t i) const
     {
         if(x.fresh == 0 || (others != nullptr && others[i] != 0)) return 0;
         return more && x.fresh * per > 32 ? 2 : 1;
@@ -184,7 +166,7 @@ __device__ __forceinline__ Line find_line(const ChunkArgs& a, const Ways& w, uin
         units = steps = 0;
         if(i < a.seqs) {
             const Chunk x = chunk_of(a, i, w.most);
-            if(w.kind(a, x, i) == T) {
+            if(w.kind(x, i) == T) {
                 units = unit_tiles(x, w.per, T) * kv_heads;
                 steps = steps_of(x.len);
             }
@@ -266,7 +248,7 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
     const auto enter = [&](Place& p) { // the sequence p.seq
         p.c     = chunk_of(a, p.seq, ways.most);
         p.steps = steps_of(p.c.len);
-        p.tiles = ways.kind(a, p.c, p.seq) == T ? unit_tiles(p.c, per, T) : 0;
+        p.tiles = ways.kind(p.c, p.seq) == T ? unit_tiles(p.c, per, T) : 0;
     };
     Place here{};
     here.seq = line.seq;

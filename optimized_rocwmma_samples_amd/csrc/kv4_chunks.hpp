@@ -32,7 +32,7 @@ __device__ __forceinline__ Chunk chunk_of(const ChunkArgs& a, uint32_t i, uint32
 struct Long {
     uint32_t seq, base, need, pad;
     Chunk    c;
-    uint32_t unused;
+    uint32_t unused; // 32 bytes, which no line of memory cuts
 };
 
 // Which sequences are unpacked; in the workspace.
@@ -47,13 +47,14 @@ struct LongList {
 
 } // namespace
 
-// What the join needs of a unit that goes on behind the run it begins in.
+// What the join needs of a unit that goes on behind the run it begins in: written, and read,
+// where the run's tasks are not 0.
 struct Piece {
-    uint32_t last;  // run that has its last step, plus 1; 0: no such unit
+    uint32_t last;  // run that has its last step, plus 1
     uint32_t token; // first row of q of its sequence
     uint32_t row0, rows; // its rows row0 .. of the sequence's `rows`
     uint32_t head;       // first query head
-    uint32_t unused[3];
+    uint32_t unused[3]; // 32 bytes, as above
 };
 
 // Whether the rows of a unit are joined by a block each, which takes all partials at a time, or

@@ -1,16 +1,13 @@
 // kv4_device.hpp -- what the kernels of the paged 4-bit cache share.
 #pragma once
 
-#include "w8a8_device.hpp"
+#include "matrix_f16.hpp"
 #include "w8a8_internal.hpp"
 
 #include <type_traits>
 
 namespace w8a8 {
 namespace {
-
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
 struct CacheView {
     uint8_t*  codes[2];  // keys, values

@@ -205,12 +205,7 @@ __global__ void __launch_bounds__(kThreads, 3)
     // ---- the gang's run ----------------------------------------------------------------
     auto scan = [&](uint32_t i0, uint32_t& n, uint32_t& s) { // 64 sequences' key tiles
         n = i0 + lane < count ? all_keys(l.list[i0 + lane]) * groups : 0;
-        s = n;
-#pragma unroll
-        for(int d = 1; d < kWave; d <<= 1) {
-            const uint32_t o = __shfl_up(s, d, kWave);
-            if(lane >= (uint32_t)d) s += o;
-        }
+        s = lanes_sum(n);
         return (uint32_t)__builtin_amdgcn_readlane(s, kWave - 1);
     };
     uint32_t n, s, all = 0;

@@ -799,9 +799,12 @@ int w8a8_kv4_trim(const int32_t* keep, const int32_t* seq_lens, uint32_t seqs,
  * infinity counts as NaN.  out may not overlap q.
  * Keys and values enter the matrix products as fp16, off from offset + scale *
  * (n - 8) by no more than 2^-11 of it and 2^-23, probabilities as well; scores, softmax
- * statistics and sums are fp32.  Results past the range of fp16 are its ends.
- * max_new: no sequence has more new tokens than this (0: not known); more of them are
- * computed all the same, more slowly.
+ * statistics and sums are fp32.  So are those of a sequence of one new token, which
+ * w8a8_attention_kv4 takes with less rounding.  Results past the range of fp16 are its
+ * ends; keys and values are to lie in it up to a rounding, as w8a8_kv4_store writes them.
+ * max_new: no sequence has more new tokens than this (0: not known, as good as `tokens`,
+ * which takes more workspace and launches); more of them are computed all the same,
+ * more slowly.
  * workspace: 256-byte aligned, w8a8_attention_kv4_chunks_workspace_size bytes (for
  * the same cache, seqs, tokens, heads, table_cols and max_new), needs no clearing;
  * calls that share one must be ordered on one stream.

@@ -796,7 +796,7 @@ int w8a8_kv4_trim(const int32_t* keep, const int32_t* seq_lens, uint32_t seqs,
  * its own; a row that sees none gives zeros.  Tokens of a page number outside
  * [0, pages) are left out, rows of no sequence left as they were.  What a row may
  * not see does not reach it, NaN included; a group whose scale or offset is an
- * infinity counts as NaN.  out may not overlap q.
+ * infinity counts as NaN, and so does an infinite query.  out may not overlap q.
  * Keys and values enter the matrix products as fp16, off from offset + scale *
  * (n - 8) by no more than 2^-11 of it and 2^-23, probabilities as well; scores, softmax
  * statistics and sums are fp32.  So are those of a sequence of one new token, which

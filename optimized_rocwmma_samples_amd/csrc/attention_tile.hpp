@@ -160,7 +160,8 @@ __device__ __forceinline__ void attend(const TileRows& t, float c, const uint32_
         const uint16_t* from = t.q + (size_t)qrow * t.ldq + half * 8;
         if(qrow < t.rows)
 #pragma unroll
-            for(int s = 0; s < kSteps; ++s) qf[s] = *reinterpret_cast<const v8h*>(from + s * 16);
+            for(int s = 0; s < kSteps; ++s)
+                qf[s] = infinite_to_nan(*reinterpret_cast<const v8h*>(from + s * 16));
     } else {
         const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint16_t*>(t.q), 0, (int)((t.rows - 1) * t.ldq * 2 + D * 2), kBufferFlags);

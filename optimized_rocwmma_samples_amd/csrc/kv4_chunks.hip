@@ -313,9 +313,10 @@ __device__ __forceinline__ void chunks_run(const CacheView& c, const ChunkArgs& 
         for(int t = 0; t < T; ++t)
 #pragma unroll
             for(int i = 0; i < kSteps / kWaves; ++i) {
-                v8h u;
+                const v8h q = infinite_to_nan(qv[t][i]);
+                v8h       u;
 #pragma unroll
-                for(int e = 0; e < 8; ++e) u[e] = qv[t][i][kOrder[e]];
+                for(int e = 0; e < 8; ++e) u[e] = q[kOrder[e]];
                 *(lds_v4i_t*)(uintptr_t)(qat + (t * kSteps + wave + i * kWaves) * kWave * 16)
                     = __builtin_bit_cast(v4i, u);
             }

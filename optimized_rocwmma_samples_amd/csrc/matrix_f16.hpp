@@ -34,5 +34,12 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
+// The values, infinities as NaN.  Scores of a query that holds an infinity are infinities and
+// NaN, and so its softmax is NaN; but -infinity is also what keys get that a row may not see.
+__device__ __forceinline__ v8h infinite_to_nan(v8h v)
+{
+    return __builtin_elementwise_fma(v, v8h{}, v);
+}
+
 } // namespace
 } // namespace w8a8

@@ -1,5 +1,6 @@
 """Attention of chunks over groups whose scale or offset is an infinity: they count as NaN, to the
-rows that see them, by each of the ways a sequence can go."""
+rows that see them, by each of the ways a sequence can go.  And of queries with infinities, whose
+softmax is NaN."""
 from __future__ import annotations
 
 import pytest
@@ -46,3 +47,32 @@ def test_infinite_groups_are_nan(w8a8, gpu, dim, group, news, part, value):
             got = run(d)
             assert torch.isnan(got[nan]).all(), (at, keys)
             assert torch.equal(got[~nan], want[~nan]), (at, keys)
+
+
+@pytest.mark.parametrize("news,lens", [([4, 3], [61, 2]), ([40, 90], [40, 700]), ([9, 140], [5, 140])])
+def test_infinite_queries_are_nan(w8a8, gpu, news, lens):
+    # all scores -infinity among them, which is what unseen keys have as well; a row that sees
+    # no key gives zeros all the same
+    import attention_ref as R
+    import torch
+    heads, kv_heads, dim = 8, 2, 128
+    c = w8a8.KV4Cache.empty(50, kv_heads, dim, 16, 32, gpu)
+    k = R.randn((800, kv_heads, dim), 1, gpu).abs() + 1
+    w8a8.kv4_store(k, R.randn(k.shape, 2, gpu), torch.arange(800, dtype=torch.int32, device=gpu), c)
+    table, starts = _table(50, 46, 2, 5, gpu), starts_of(news)
+    q = R.randn((starts[-1], heads, dim), 3, gpu)
+
+    def run(q):
+        return w8a8.attention_kv4_chunks(q, c, table, ints(lens, gpu), ints(starts, gpu))
+    want = run(q)
+    assert torch.isfinite(want).all()
+    bad, nan = q.clone(), torch.zeros(want.shape, dtype=torch.bool, device=gpu)
+    for i, (row, head, channel, value) in enumerate([
+            (0, 0, 0, float("-inf")), (1, 3, 127, float("inf")), (starts[1], 5, 64, float("-inf")),
+            (starts[1] + 1, 7, 31, float("-inf")), (starts[-1] - 1, 4, 9, float("-inf")),
+            (starts[-1] - 1, 2, 77, float("inf"))]):
+        bad[row, head, channel] = value
+        s = 0 if row < starts[1] else 1
+        nan[row, head] = lens[s] - news[s] + row - starts[s] >= 0
+    got = run(bad)
+    assert torch.isnan(got[nan]).all() and torch.equal(got[~nan], want[~nan])

@@ -1140,7 +1140,9 @@ def attention_kv4_chunks(q, cache: KV4Cache, block_table, seq_lens, starts,
     already stored; seq_lens int32 [seqs] counts them.  Each row sees the tokens of its
     sequence up to its own.  block_table as in attention_kv4.  Returns fp16 [tokens,
     heads, head_dim]; rows of no sequence are left as they were in `out` (undefined in a
-    new tensor).  max_new: the most new tokens a sequence has, where it is known.
+    new tensor).  max_new: the most new tokens a sequence has, where it is known (else they
+    may be all rows, which takes more workspace and launches).  Keys and values are rounded
+    to fp16, for sequences of one new token too, which attention_kv4 takes as they are.
     workspace: 'auto' (allocated here) or a device tensor of
     attention_kv4_chunks_workspace_size bytes, for the same max_new."""
     _torch()
